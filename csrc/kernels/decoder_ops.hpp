@@ -1,0 +1,48 @@
+/**
+ * Entry points of the operators of a decoder block (residual_norm.cu, rotary.cu, gated_linear.cu). All pointers are device
+ * memory of `device`, dtype is an ncclDataType_t (float16, float32 or bfloat16), and the work goes to `stream`. They return 0, or
+ * -1 after a message on stderr.
+ */
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+/** Which of the vectors of a norm are fp32 and not of the activations' type. */
+enum { DCCL_NORM_WEIGHT_F32 = 1, DCCL_NORM_POST_F32 = 2, DCCL_NORM_GATE_F32 = 4 };
+
+extern "C" {
+
+/**
+ * y = x + scale * gate .* p with p = branch, or rms_norm(branch) .* post where post is given; n = rms_norm(y) .* weight. rows x width,
+ * rows in a row. Row r uses row r / rows_per_gate of the gate. Without a branch, n = rms_norm(x) .* weight and y is not
+ * written. rstd and rstd_post (fp32, one per row) may be null, gate and post too.
+ */
+int dccl_residual_norm(int device, int dtype, size_t rows, size_t width, const void* x, const void* branch, const void* weight, const void* post,
+                       const void* gate, size_t rows_per_gate, int f32_vectors, double eps, double scale, void* y, void* n, void* rstd, void* rstd_post,
+                       void* stream);
+
+/** Bytes of workspace that the backward pass of `gates` rows of gates (0: without a gate) takes; 0 after an error. */
+size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t width, size_t gates, int has_post);
+
+/**
+ * Gradients of dccl_residual_norm: from dy and dn (either may be null) those of x and branch, and in the vectors' own types those of
+ * weight, post and gate. y is the forward pass's output, or x where there was no branch. dbranch may be null where it equals dx
+ * (scale 1, no post, no gate) or there was no branch. No atomics: the same inputs give the same gradients.
+ */
+int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* y, const void* branch,
+                                const void* weight, const void* post, const void* gate, size_t rows_per_gate, int f32_vectors, double scale,
+                                const void* rstd, const void* rstd_post, void* dx, void* dbranch, void* dweight, void* dpost, void* dgate,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/** A tensor [batch, seq, heads, head dim] by its strides in elements; the head dim is dense. */
+struct DcclHeads { const void* in; void* out; long long in_batch, in_seq, in_head, out_batch, out_seq, out_head; int heads; };
+
+/**
+ * Turns pair j of every head of q and k (heads 0: not given) by positions * freqs[j] radians, or back where `back`, and scales it; what
+ * lies behind the pairs is copied. Pair j is (j, pairs + j), or (2j, 2j + 1) where `interleaved`. positions: int64 or int32 with
+ * the strides pos_batch and pos_seq, or null for first + index in the sequence.
+ */
+int dccl_rotary(int device, int dtype, size_t batch, size_t seq, int head_dim, int pairs, int interleaved, int back, const DcclHeads* q, const DcclHeads* k,
+                const double* freqs, const void* positions, int positions64, long long pos_batch, long long pos_seq, long long first, double scale, void* stream);
+
+} // extern "C"

@@ -1,0 +1,98 @@
+/**
+ * What the kernels over rows of activations share: short runs of elements as one access, their conversion, sums over a CTA, and
+ * launches on a device that need not be the current one.
+ */
+#pragma once
+#include "../device/reduce_ops.cuh"
+#include <atomic>
+#include <cstdint>
+#include <cstdio>
+#include <initializer_list>
+
+namespace dccl {
+
+/** N elements moved by one access. */
+template <typename T, int N> struct alignas(sizeof(T) * N) Run { T e[N]; };
+
+template <typename T, int N> __device__ __forceinline__ Run<T, N> ld_run(const T* p) { return *reinterpret_cast<const Run<T, N>*>(p); }
+template <typename T, int N> __device__ __forceinline__ void st_run(T* p, const Run<T, N>& v) { *reinterpret_cast<Run<T, N>*>(p) = v; }
+
+/** Elements [i, i + N) of a vector that is of type T, or fp32. */
+template <typename T, int N> __device__ __forceinline__ void ld_vector(float (&f)[N], const void* p, bool f32, size_t i) {
+    if (f32) {
+        if constexpr (N * sizeof(float) <= 16) {
+            const Run<float, N> r = ld_run<float, N>(reinterpret_cast<const float*>(p) + i);
+#pragma unroll
+            for (int e = 0; e < N; e++) f[e] = r.e[e];
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k += 4) {
+                const Run<float, 4> r = ld_run<float, 4>(reinterpret_cast<const float*>(p) + i + k);
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[k + e] = r.e[e];
+            }
+        }
+    } else {
+        const Run<T, N> r = ld_run<T, N>(reinterpret_cast<const T*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < N; e++) f[e] = Traits<T>::up(r.e[e]);
+    }
+}
+
+/** The sum over the CTA, in every thread and in a fixed order. `parts`: 32 words of shared memory that no other call uses until
+ *  every thread has passed a barrier after this one. */
+__device__ __forceinline__ float cta_sum(float v, float* parts) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const unsigned warps = blockDim.x / 32;
+    if (warps == 1) return v;
+    if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = threadIdx.x % 32 < warps ? parts[threadIdx.x % 32] : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+/** Makes `device` current for as long as it lives. */
+class OnDevice {
+public:
+    explicit OnDevice(int device) : device_(device) {
+        e = cudaGetDevice(&prev_);
+        if (e == cudaSuccess && prev_ != device) e = cudaSetDevice(device);
+    }
+    ~OnDevice() { if (prev_ >= 0 && prev_ != device_) cudaSetDevice(prev_); }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+    cudaError_t e;
+
+private:
+    int device_, prev_ = -1;
+};
+
+/** SMs of a device, asked once; 0 after an error. */
+inline int sm_count(int device) {
+    static std::atomic<int> known[64];
+    if (device < 0 || device >= 64) return 0;
+    int n = known[device].load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return 0; }
+        known[device].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+inline int report(const char* who, cudaError_t e) {
+    if (e == cudaSuccess) return 0;
+    fprintf(stderr, "%s: %s\n", who, cudaGetErrorString(e));
+    cudaGetLastError();
+    return -1;
+}
+
+inline bool aligned_to(size_t bytes, std::initializer_list<const void*> ps) {
+    uintptr_t low = 0;
+    for (const void* p : ps) low |= reinterpret_cast<uintptr_t>(p);
+    return low % bytes == 0;
+}
+
+} // namespace dccl

@@ -108,6 +108,10 @@ def _declare(lib):
         "dccl_local_reduce": (i, [vp, vp, sz, i, i]),
         "dccl_local_reduce_device": (i, [vp, vp, sz, i, i, vp]),
         "dccl_adamw_flat": (i, [i, i, sz, vp, vp, vp, vp, vp, vp] + [c.c_double] * 7 + [vp]),
+        "dccl_residual_norm": (i, [i, i, sz, sz] + [vp] * 5 + [sz, i, c.c_double, c.c_double] + [vp] * 5),
+        "dccl_residual_norm_workspace": (sz, [i, i, sz, sz, sz, i]),
+        "dccl_residual_norm_backward": (i, [i, i, sz, sz] + [vp] * 7 + [sz, i, c.c_double] + [vp] * 8 + [sz, vp]),
+        "dccl_rotary": (i, [i, i, sz, sz, i, i, i, i, vp, vp, vp, vp, i, c.c_longlong, c.c_longlong, c.c_longlong, c.c_double, vp]),
         "dccl_emu_early_producer": (i, [vp, vp, sz, c.c_uint, vp, vp]),
         "dccl_emu_early_observer": (i, [vp, vp]),
         "dccl_debug_bounds_build": (i, []),

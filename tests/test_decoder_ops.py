@@ -1,0 +1,439 @@
+"""The operators of a decoder block (dccl_b200.ops.decoder) against their formulas in 64 bits.
+
+Tolerances count roundings. A result of type T is off by half a step of T, u = eps / 2 of its size; what is computed in fp32 before
+that is off by a few times 2^-24 of the terms that went into it. Where a backward pass starts from a stored result of type T, its
+u goes through the formula as well: each bound below says how.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from dccl_b200 import ops  # noqa: E402
+
+EPS = 1e-5
+F32 = 2.0 ** -20      # of the sum of a result's terms: up to sixteen fp32 operations on each
+SUMS = 2.0 ** -17     # of the sum of a column's terms: up to a hundred more additions in a row
+gpu = pytest.mark.gpu
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def check(name, got, want, bound):
+    assert got.shape == want.shape, name
+    # below the smallest normal number (6e-5 of float16) the steps get no smaller: half of one is tiny * eps / 2, 2^-25 of float16
+    bound = bound + torch.finfo(got.dtype).tiny * half_step(got.dtype)
+    got = got.detach().double().cpu()
+    off = (got - want).abs() - bound
+    assert bool((off <= 0).all()), "%s: %.3g over its bound %.3g at %s (%.6g, not %.6g)" % (
+        name, off.max(), bound.reshape(-1)[off.argmax()], off.argmax().item(), got.reshape(-1)[off.argmax()], want.reshape(-1)[off.argmax()])
+
+
+# ---------------------------------------------------------------------------------------------- norms
+
+def norm_case(shape, dtype, post, gate, wide, seed=0, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    w = shape[-1]
+    vec = torch.float32 if wide else dtype
+    t = {"x": torch.randn(shape, generator=g) * 3, "branch": torch.randn(shape, generator=g), "weight": 1 + 0.2 * torch.randn(w, generator=g)}
+    if post:
+        t["post"] = 1 + 0.2 * torch.randn(w, generator=g)
+    if gate:
+        t["gate"] = torch.randn(gate, generator=g)
+    t = {k: v.to(dtype if k in ("x", "branch") else vec).to(device).requires_grad_(True) for k, v in t.items()}
+    dy, dn = (torch.randn(shape, generator=g).to(dtype).to(device) for _ in range(2))
+    return t, dy, dn
+
+
+def norm_call(t, scale):
+    return ops.residual_norm(t["x"], t["branch"], t["weight"], eps=EPS, post_weight=t.get("post"), gate=t.get("gate"), scale=scale)
+
+
+def norm_check(t, dy, dn, scale, y, n, grads, dtype):
+    """Everything against the formulas, with the bounds that follow from them."""
+    u = half_step(dtype)
+    d = {k: v.detach().double().cpu() for k, v in t.items()}
+    dy, dn = (0 if v is None else v.double().cpu() for v in (dy, dn))
+    width = d["x"].shape[-1]
+    post, gate = d.get("post", torch.ones(width, dtype=torch.float64)), d.get("gate", torch.ones(width, dtype=torch.float64))
+    b = d["branch"]
+    rb = (b.pow(2).mean(-1, keepdim=True) + EPS).rsqrt() if "post" in d else torch.ones_like(b[..., :1])
+    p = b * rb * post
+    want_y = d["x"] + scale * gate * p
+    ry = (want_y.pow(2).mean(-1, keepdim=True) + EPS).rsqrt()
+    yh = want_y * ry
+    terms = d["x"].abs() + (scale * gate * p).abs()
+    check("y", y, want_y, u * want_y.abs() + F32 * terms)
+    check("n", n, yh * d["weight"], u * (yh * d["weight"]).abs() + F32 * d["weight"].abs() * (terms * ry + yh.abs()))
+    if grads is None:
+        return
+    # backward: yh comes from the stored y, which is off by u of itself, and so does mean(t yh)
+    e_yh = u * yh.abs() + F32 * terms * ry
+    tt = dn * d["weight"]
+    c = (tt * yh).mean(-1, keepdim=True) if torch.is_tensor(tt) else torch.zeros_like(ry)
+    c_abs, e_c = (tt * yh).abs().mean(-1, keepdim=True) if torch.is_tensor(tt) else c, (tt * e_yh).abs().mean(-1, keepdim=True) if torch.is_tensor(tt) else c
+    D = dy + ry * (tt - yh * c)
+    e_D = ry * (e_yh * c.abs() + yh.abs() * e_c) + F32 * (abs(dy) + ry * (abs(tt) + yh.abs() * c_abs))
+    check("dx", grads["x"], D, u * D.abs() + e_D)
+    rows = tuple(range(D.dim() - 1))
+    if torch.is_tensor(dn):
+        dw = (dn * yh).sum(rows)
+        check("dweight", grads["weight"], dw, half_step(t["weight"].dtype) * dw.abs() + (dn.abs() * e_yh).sum(rows) + SUMS * (dn * yh).abs().sum(rows))
+    dp, e_dp = scale * D, abs(scale) * e_D
+    if "gate" in d:
+        terms_g = dp * p
+        over = [i for i in range(D.dim()) if i < D.dim() - gate.dim() or gate.shape[i - (D.dim() - gate.dim())] != D.shape[i]]
+        dims = tuple(over) or ()
+        fold = (lambda v: v.sum(dims).reshape(gate.shape)) if dims else (lambda v: v)
+        check("dgate", grads["gate"], fold(terms_g), half_step(t["gate"].dtype) * fold(terms_g).abs() + fold((e_dp * p).abs()) + SUMS * fold(terms_g.abs()))
+        dp, e_dp = dp * gate, e_dp * gate.abs()
+    if "post" in d:
+        bh = b * rb
+        check("dpost", grads["post"], (dp * bh).sum(rows), half_step(t["post"].dtype) * (dp * bh).sum(rows).abs() + (e_dp * bh.abs()).sum(rows) + SUMS * (dp * bh).abs().sum(rows))
+        v, e_v = dp * post, e_dp * post.abs()
+        cb, cb_abs, e_cb = ((f).mean(-1, keepdim=True) for f in (v * bh, (v * bh).abs(), e_v * bh.abs()))
+        dp, e_dp = rb * (v - bh * cb), rb * (e_v + bh.abs() * e_cb) + F32 * rb * (v.abs() + bh.abs() * cb_abs)
+    check("dbranch", grads["branch"], dp, u * dp.abs() + e_dp + F32 * dp.abs())
+
+
+def norm_run(shape, dtype, post=False, gate=None, scale=1.0, wide=False, use_y=True, use_n=True, device="cuda"):
+    t, dy, dn = norm_case(shape, dtype, post, gate, wide, device=device)
+    with torch.no_grad():
+        y0, n0 = norm_call(t, scale)
+    y, n = norm_call(t, scale)
+    assert torch.equal(y0, y) and torch.equal(n0, n), "with and without a graph"
+    outs = [(y, dy)] * use_y + [(n, dn)] * use_n
+    names = [k for k in t if k != "weight" or use_n]
+    grads = dict(zip(names, torch.autograd.grad([o for o, _ in outs], [t[k] for k in names], [g for _, g in outs])))
+    norm_check(t, dy if use_y else None, dn if use_n else None, scale, y, n, grads, dtype)
+
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.mark.parametrize("post,gate", [(False, None), (True, None), (True, "row"), (False, "seq")])
+def test_norm_on_cpu(post, gate):
+    norm_run((2, 5, 24), torch.float32, post, {"row": (24,), "seq": (2, 1, 24)}.get(gate), 0.5, device="cpu")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 8), (3, 2, 33), (5, 96), (2, 3, 257), (7, 250), (300, 1451), (2, 300, 2048), (9, 2049), (40, 4096), (3, 5000), (700, 6152), (5, 8192),
+                                   (4, 8193), (3, 16384), (2, 32768)], ids=str)
+@pytest.mark.parametrize("form", ["sum", "all"])
+def test_norm_at_its_widths(dtype, shape, form):
+    if form == "sum":
+        norm_run(shape, dtype)
+    else:
+        norm_run(shape, dtype, post=True, gate=shape[-1:], scale=0.37, wide=shape[-1] % 2 == 0)
+
+
+@gpu
+@pytest.mark.parametrize("gate", [None, (96,), (1, 1, 1, 96), (3, 1, 1, 96), (3, 4, 1, 96), (3, 4, 5, 96)], ids=str)
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("use", [(True, True), (True, False), (False, True)])
+def test_norm_forms(gate, post, use):
+    norm_run((3, 4, 5, 96), torch.bfloat16, post, gate, 1.0, use_y=use[0], use_n=use[1])
+    norm_run((3, 4, 5, 96), torch.float32, post, gate, -2.0, use_y=use[0], use_n=use[1])
+
+
+@gpu
+def test_norm_with_more_gates_than_ctas():
+    norm_run((1500, 2, 64), torch.float16, True, (1500, 1, 64), 0.5)
+
+
+@gpu
+def test_norm_of_views():
+    """Rows that start between two accesses, and tensors that are not dense: transposed, expanded."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    base = torch.randn(6 * 512 + 3, device="cuda", generator=g).bfloat16()
+    x = base[3:].view(6, 512)
+    branch = torch.randn(512, 6, device="cuda", generator=g).bfloat16().t()
+    weight = torch.randn(512 + 1, device="cuda", generator=g)[1:]
+    t = {"x": x, "branch": branch, "weight": weight}
+    y, n = norm_call(t, 1.0)
+    norm_check(t, None, None, 1.0, y, n, None, torch.bfloat16)
+    t["branch"] = base[:512].expand(6, 512)
+    y, n = norm_call(t, 1.0)
+    norm_check(t, None, None, 1.0, y, n, None, torch.bfloat16)
+
+
+@gpu
+def test_norm_gate_that_was_broadcast_gets_the_sum():
+    t, dy, dn = norm_case((4, 3, 64), torch.float32, False, (1, 1, 64), False, device="cuda")
+    one = t["gate"]
+    t["gate"] = one.expand(4, 1, 64)
+    y, n = norm_call(t, 1.0)
+    got = torch.autograd.grad((y, n), one, (dy, dn))[0]
+    t["gate"] = one
+    y, n = norm_call(t, 1.0)
+    want = torch.autograd.grad((y, n), one, (dy, dn))[0]
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-5)      # fp32 sums of twelve terms of about 1, in two orders
+
+
+@gpu
+def test_norm_rows_do_not_touch_each_other():
+    t, _, _ = norm_case((4, 200), torch.float32, True, (200,), False, device="cuda")
+    with torch.no_grad():
+        y, n = norm_call(t, 1.0)
+        for bad, row in ((float("nan"), 0), (float("inf"), 2)):
+            t["branch"][row, 7] = bad
+        y2, n2 = norm_call(t, 1.0)
+    for row in (1, 3):
+        assert torch.equal(y[row], y2[row]) and torch.equal(n[row], n2[row])
+    assert bool(n2[0].isnan().all()) and bool(n2[2, 7].isnan())
+
+
+@gpu
+def test_norm_without_rows():
+    x = torch.zeros(0, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    y, n = ops.residual_norm(x, x, w)
+    (y.sum() + n.sum()).backward()
+    assert y.shape == n.shape == x.grad.shape and bool((w.grad == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rms_norm(dtype):
+    t, _, dn = norm_case((5, 7, 1024), dtype, False, None, False, device="cuda")
+    n = ops.rms_norm(t["x"], t["weight"], eps=EPS)
+    grads = dict(zip(("x", "weight"), torch.autograd.grad(n, (t["x"], t["weight"]), dn)))
+    assert torch.equal(n, ops.rms_norm(t["x"].detach(), t["weight"].detach(), eps=EPS))
+    # a branch of zeros makes residual_norm the same function
+    t["branch"] = torch.zeros_like(t["x"])
+    grads["branch"] = grads["x"]
+    norm_check(t, None, dn, 1.0, t["x"], n, grads, dtype)
+
+
+@gpu
+def test_norm_gradient_against_differences():
+    t, dy, dn = norm_case((2, 3, 32), torch.float32, True, (2, 1, 32), False, device="cuda")
+    def loss(vals):
+        y, n = norm_call(vals, 0.7)
+        return ((y * dy).sum(-1).double() + (n * dn).sum(-1).double()).sum()
+    grads = torch.autograd.grad(loss(t), list(t.values()))
+    for (k, v), g in zip(t.items(), grads):
+        way = torch.randn(v.shape, generator=torch.Generator().manual_seed(1)).cuda()
+        h = 2.0 ** -8
+        with torch.no_grad():
+            up, down = (loss({**t, k: v + s * h * way}) for s in (1, -1))
+        # the third derivative is of the size of the first for h = 1: h^2 of it, and fp32 roundings of the loss over 2 h
+        want, got = (up - down) / (2 * h), (g * way).sum()
+        assert abs(want - got) <= 40 * h * h * g.norm() * way.norm() / math.sqrt(g.numel()) + 2e-3, (k, want, got)
+
+
+@gpu
+def test_gradients_have_the_same_bits_twice():
+    t, dy, dn = norm_case((64, 9, 1000), torch.bfloat16, True, (64, 1, 1000), False, device="cuda")
+    runs = []
+    for _ in range(2):
+        y, n = norm_call(t, 0.5)
+        runs.append(torch.autograd.grad((y, n), list(t.values()), (dy, dn)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def norm_refusals(device):
+    x, w = torch.zeros(2, 3, 8, device=device), torch.ones(8, device=device)
+    with pytest.raises(TypeError):
+        ops.rms_norm(x.double(), w)
+    with pytest.raises(TypeError):
+        ops.rms_norm([1.0], w)
+    with pytest.raises(TypeError):
+        ops.rms_norm(x.bfloat16(), w.half())
+    with pytest.raises(ValueError):
+        ops.rms_norm(x, w[:4])
+    with pytest.raises(ValueError):
+        ops.rms_norm(torch.zeros(2, 0, device=device), w[:0])
+    with pytest.raises(ValueError):
+        ops.rms_norm(torch.zeros(1, 32769, device=device), torch.zeros(32769, device=device))
+    with pytest.raises(TypeError):
+        ops.residual_norm(x, None, w)
+    with pytest.raises(TypeError):
+        ops.residual_norm(x, x.half(), w)
+    with pytest.raises(ValueError):
+        ops.residual_norm(x, x[0], w)
+    for shape in ((2, 8), (1, 3, 8), (2, 3, 4), (2, 2, 8), (3,)):
+        with pytest.raises(ValueError):
+            ops.residual_norm(x, x, w, gate=torch.ones(shape, device=device))
+    with pytest.raises(ValueError):
+        ops.residual_norm(x, x, w, post_weight=torch.ones(7, device=device))
+
+
+def test_norm_refusals():
+    norm_refusals("cpu")
+
+
+@gpu
+def test_norm_refusals_on_the_gpu():
+    norm_refusals("cuda")
+    with pytest.raises(ValueError):
+        ops.rms_norm(torch.zeros(2, 8, device="cuda"), torch.ones(8))
+
+
+# ---------------------------------------------------------------------------------------------- rotary positions
+
+def turn(x, freqs, positions, interleaved, scale):
+    """In 64 bits, as complex numbers; positions [batch, seq] or [seq]."""
+    p = freqs.shape[0]
+    x = x.detach().double().cpu()
+    angle = positions.double().cpu().unsqueeze(-1) * freqs.cpu()
+    spin = torch.polar(torch.full_like(angle, scale), angle)
+    v = x[..., :2 * p]
+    z = torch.complex(v[..., 0::2], v[..., 1::2]) if interleaved else torch.complex(v[..., :p], v[..., p:])
+    z = z * spin.unsqueeze(-2)
+    out = torch.stack((z.real, z.imag), -1).flatten(-2) if interleaved else torch.cat((z.real, z.imag), -1)
+    a = z.abs()
+    size = torch.stack((a, a), -1).flatten(-2) if interleaved else torch.cat((a, a), -1)
+    rest = x[..., 2 * p:]
+    return torch.cat((out, rest), -1), torch.cat((size, torch.zeros_like(rest)), -1)
+
+
+def check_turned(name, got, x, freqs, positions, interleaved, scale=1.0):
+    """The part of a turn is off by 2^-25 of one in fp32, which is 2^-22 radians, and the sine and cosine and the products by as much
+    again; the whole turns are three products in 64 bits, the reference's own among them, each off by 2^-53 of the angle."""
+    want, size = turn(x, freqs, positions, interleaved, scale)
+    angle = positions.double().cpu().abs().unsqueeze(-1).unsqueeze(-1)
+    check(name, got, want, half_step(got.dtype) * want.abs() + (2.0 ** -20 + angle * 2.0 ** -51) * size)
+
+
+def rotary_run(batch, seq, heads, kv, dim, pairs, dtype, interleaved=False, scale=1.0, furthest=4000, per_sequence=True, int32=False, device="cuda", front=False):
+    g = torch.Generator().manual_seed(seq * dim + pairs)
+    q, k, dq, dk = (torch.randn(batch, seq, h, dim, generator=g).to(dtype).to(device) for h in (heads, kv, heads, kv))
+    if front:       # the heads in front in memory
+        q, k, dq, dk = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, dq, dk))
+    q.requires_grad_(True), k.requires_grad_(True)
+    freqs = ops.rotary_frequencies(2 * pairs, device=device)
+    pos = torch.randint(0, furthest, (batch, seq) if per_sequence else (seq,), generator=g)
+    at = pos.to(torch.int32 if int32 else torch.int64).to(device)
+    with torch.no_grad():
+        q0, k0 = ops.rotary(q, k, freqs, at, interleaved, scale)
+    q1, k1 = ops.rotary(q, k, freqs, at, interleaved, scale)
+    assert torch.equal(q0, q1) and torch.equal(k0, k1) and q0.stride() == q.stride()
+    gq, gk = torch.autograd.grad((q1, k1), (q, k), (dq, dk))
+    check_turned("q", q1, q, freqs, pos, interleaved, scale)
+    check_turned("k", k1, k, freqs, pos, interleaved, scale)
+    check_turned("dq", gq, dq, -freqs, pos, interleaved, scale)
+    check_turned("dk", gk, dk, -freqs, pos, interleaved, scale)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_on_cpu(interleaved):
+    rotary_run(2, 5, 4, 2, 12, 4, torch.float32, interleaved, 0.9, device="cpu")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("sizes", [(1, 1, 1, 1, 2, 1), (2, 3, 4, 2, 64, 32), (1, 300, 32, 4, 64, 32), (3, 7, 5, 1, 80, 17), (2, 9, 3, 3, 128, 64), (1, 5, 2, 2, 96, 24), (2, 4, 2, 1, 13, 3),
+                                   (1, 3, 1, 1, 2048, 1024), (16, 1, 32, 4, 64, 32), (2, 50, 8, 8, 256, 32), (1, 6, 3, 1, 20, 4), (1, 6, 3, 1, 36, 16)], ids=str)
+def test_rotary_at_its_sizes(dtype, interleaved, sizes):
+    rotary_run(*sizes, dtype, interleaved)
+
+
+@gpu
+@pytest.mark.parametrize("per_sequence,int32,front", [(True, True, False), (False, False, True), (False, True, False), (True, False, True)])
+def test_rotary_positions_and_layouts(per_sequence, int32, front):
+    rotary_run(3, 11, 4, 2, 64, 32, torch.bfloat16, False, 1.25, per_sequence=per_sequence, int32=int32, front=front)
+
+
+@gpu
+def test_rotary_far_positions():
+    rotary_run(2, 40, 4, 2, 64, 32, torch.float32, furthest=(1 << 31) - 1)
+    q = torch.randn(1, 3, 2, 64, device="cuda")
+    freqs = ops.rotary_frequencies(64, device="cuda")
+    far = (1 << 33) + 5         # a double holds the turns to 2^-23
+    check_turned("q", ops.rotary(q, None, freqs, far), q, freqs, torch.arange(far, far + 3), False)
+    check_turned("q", ops.rotary(q, None, freqs, -7), q, freqs, torch.arange(-7, -4), False)
+
+
+@gpu
+def test_rotary_of_views():
+    """q and k as parts of one product, at an odd offset, one of them expanded, three dimensions, a transposed gradient."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    freqs = ops.rotary_frequencies(64, device="cuda")
+    both = torch.randn(2, 9, 6 * 64 + 1, device="cuda", generator=g).half()
+    pos = torch.arange(9)
+    for off in (0, 1):
+        q, k = both[..., off:off + 4 * 64].unflatten(-1, (4, 64)), both[..., off + 4 * 64:off + 6 * 64 - off].unflatten(-1, (-1, 64)) if off == 0 else both[..., 5 * 64 + 1:].unflatten(-1, (1, 64))
+        qo, ko = ops.rotary(q, k, freqs)
+        check_turned("q", qo, q, freqs, pos, False)
+        check_turned("k", ko, k, freqs, pos, False)
+    wide = both[..., :64].unsqueeze(2).expand(2, 9, 3, 64)
+    check_turned("expanded", ops.rotary(wide, None, freqs), wide, freqs, pos, False)
+    last = torch.randn(9, 64, 2, device="cuda", generator=g).transpose(1, 2)        # the head dim is not the dense one
+    check_turned("three", ops.rotary(last, None, freqs, torch.arange(0, 18, 2, device="cuda")), last, freqs, torch.arange(0, 18, 2), False)
+    x = torch.randn(2, 9, 4, 64, device="cuda", generator=g, requires_grad=True)
+    out = ops.rotary(x, None, freqs)
+    grad = torch.randn(64, 4, 9, 2, device="cuda", generator=g).permute(3, 2, 1, 0)
+    check_turned("gradient", torch.autograd.grad(out, x, grad)[0], grad, -freqs, pos, False)
+    pos = torch.randint(0, 99, (9, 4), device="cuda", generator=g)
+    check_turned("strided positions", ops.rotary(x, None, freqs, pos[:, 1:3].t()), x, freqs, pos[:, 1:3].t(), False)
+
+
+@gpu
+def test_rotary_one_of_two_outputs_used():
+    freqs = ops.rotary_frequencies(16, device="cuda")
+    q, k = torch.randn(1, 3, 2, 16, device="cuda", requires_grad=True), torch.randn(1, 3, 1, 16, device="cuda", requires_grad=True)
+    ops.rotary(q, k, freqs)[1].sum().backward()
+    assert q.grad is None and k.grad is not None
+    assert ops.rotary(q[:, :0], k[:, :0], freqs)[0].shape == (1, 0, 2, 16)
+
+
+def test_frequencies():
+    f = ops.rotary_frequencies(64, theta=500000.0)
+    assert f.dtype is torch.float64 and torch.allclose(f, torch.tensor([500000.0 ** (-j / 32) for j in range(32)], dtype=torch.float64), rtol=1e-14)
+    assert torch.allclose(ops.rotary_frequencies(64, 500000.0, "linear", 4.0), f / 4, rtol=1e-14)
+    t = ops.rotary_frequencies(64, 500000.0, "theta", 8.0)
+    assert t[0] == 1 and math.isclose(t[-1], f[-1] / 8, rel_tol=1e-12) and bool((t <= f * (1 + 1e-12)).all())
+    for kind, slow, fast in (("turns", 1, 4), ("yarn", 1, 32)):
+        s = ops.rotary_frequencies(64, 500000.0, kind, 8.0, original_length=8192)
+        turns = f * 8192 / (2 * math.pi)
+        assert torch.allclose(s[turns > fast * 1.6], f[turns > fast * 1.6], rtol=1e-12)      # 1.6 is more than one pair further
+        assert torch.allclose(s[turns < slow / 1.6], f[turns < slow / 1.6] / 8, rtol=1e-12)
+        assert bool((s.diff() < 0).all())
+    for bad in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=64, factor=0.5), dict(rotary_dim=64, theta=1.0), dict(rotary_dim=2, scaling="theta", factor=2.0),
+                dict(rotary_dim=64, scaling="yarn", factor=2.0), dict(rotary_dim=64, scaling="other", factor=2.0), dict(rotary_dim=64, scaling="turns", original_length=8, slow=5.0)):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(**bad)
+
+
+def rotary_refusals(device):
+    q, f = torch.zeros(2, 3, 4, 8, device=device), ops.rotary_frequencies(8, device=device)
+    for bad in (f.float(), f.to(torch.int64)):
+        with pytest.raises(TypeError):
+            ops.rotary(q, None, bad)
+    for bad in (f[:0], torch.ones(5, dtype=torch.float64, device=device), f.view(2, 2)):
+        with pytest.raises(ValueError):
+            ops.rotary(q, None, bad)
+    with pytest.raises(TypeError):
+        ops.rotary(q.double(), None, f)
+    with pytest.raises(TypeError):
+        ops.rotary(q, q.half(), f)
+    for k in (q[:1], q[:, :2], q[..., :6], q[0]):
+        with pytest.raises(ValueError):
+            ops.rotary(q, k, f)
+    with pytest.raises(ValueError):
+        ops.rotary(q[0, 0], None, f)
+    for pos in (torch.zeros(4, dtype=torch.int64, device=device), torch.zeros(3, 3, dtype=torch.int64, device=device), torch.zeros(1, 3, dtype=torch.int64, device=device), 2 ** 63):
+        with pytest.raises(ValueError):
+            ops.rotary(q, None, f, pos)
+    for pos in (torch.zeros(3, device=device), 1.5, True):
+        with pytest.raises(TypeError):
+            ops.rotary(q, None, f, pos)
+    with pytest.raises(ValueError):
+        ops.rotary(torch.zeros(1, 1, 1, 4096, device=device), None, torch.ones(1025, dtype=torch.float64, device=device))
+
+
+def test_rotary_refusals():
+    rotary_refusals("cpu")
+
+
+@gpu
+def test_rotary_refusals_on_the_gpu():
+    rotary_refusals("cuda")
+    with pytest.raises(ValueError):
+        ops.rotary(torch.zeros(1, 2, 1, 8, device="cuda"), None, ops.rotary_frequencies(8))
