@@ -52,6 +52,7 @@ const DriverApi* driver_api(std::string* err) {
             vmm &= resolve("cuDeviceGetAttribute", &g_api.DeviceGetAttribute);
             resolve("cuGetErrorString", &g_api.GetErrorString);
             resolve("cuPointerGetAttribute", &g_api.PointerGetAttribute);
+            resolve("cuTensorMapEncodeTiled", &g_api.TensorMapEncodeTiled);
             mc &= resolve("cuMulticastCreate", &g_api.MulticastCreate);
             mc &= resolve("cuMulticastAddDevice", &g_api.MulticastAddDevice);
             mc &= resolve("cuMulticastBindMem", &g_api.MulticastBindMem);

@@ -32,6 +32,8 @@ struct DriverApi {
     CUresult (*DeviceGetAttribute)(int*, CUdevice_attribute, CUdevice);
     CUresult (*GetErrorString)(CUresult, const char**);
     CUresult (*PointerGetAttribute)(void*, CUpointer_attribute, CUdeviceptr);   // optional (lazy registration)
+    CUresult (*TensorMapEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                     CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);   // optional (tensor-core kernels)
     bool vmm_ok = false;         // all memory-management entry points resolved
     bool multicast_ok = false;   // all multicast entry points resolved
 };

@@ -45,4 +45,22 @@ struct DcclHeads { const void* in; void* out; long long in_batch, in_seq, in_hea
 int dccl_rotary(int device, int dtype, size_t batch, size_t seq, int head_dim, int pairs, int interleaved, int back, const DcclHeads* q, const DcclHeads* k,
                 const double* freqs, const void* positions, int positions64, long long pos_batch, long long pos_seq, long long first, double scale, void* stream);
 
+/** Activations of a gated linear layer. */
+enum { DCCL_ACT_SILU = 0, DCCL_ACT_GELU = 1, DCCL_ACT_GELU_TANH = 2 };
+
+/** Bytes of workspace that a call of these sizes takes (0 as well); -1 after an error. `aligned`: every operand starts on 16 bytes. */
+long long dccl_gated_linear_workspace(int device, size_t tokens, size_t width, size_t ffn, int aligned, int backward);
+
+/**
+ * h = act(x Wg^T) .* (x Wu^T): x [tokens][width], Wg and Wu [ffn][width], h [tokens][ffn], all dense and of dtype float16 or bfloat16.
+ * Where g and u are not null they receive the two products in fp32, in rows of pre_stride elements (a multiple of four).
+ */
+int dccl_gated_linear(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up, int act, void* h,
+                      float* g, float* u, size_t pre_stride, void* workspace, long long workspace_bytes, void* stream);
+
+/** Its gradients from dh and the products that it left. Each of dx, and dw_gate with dw_up, may be null. No atomics. */
+int dccl_gated_linear_backward(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* dh, const float* g, const float* u, size_t pre_stride,
+                               const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up, void* workspace,
+                               long long workspace_bytes, void* stream);
+
 } // extern "C"

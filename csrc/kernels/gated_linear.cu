@@ -1,0 +1,588 @@
+/**
+ * The gated half of a feed-forward layer, h = act(x Wg^T) .* (x Wu^T), and its gradients
+ *
+ *     dg = dh .* u .* act'(g)      dx  = dg Wg + du Wu
+ *     du = dh .* act(g)            dWg = dg^T x,  dWu = du^T x
+ *
+ * 4 T F H operations forward and 8 T F H backward for T tokens: the tensor cores bound it, for few tokens the reading of the weights.
+ * All products are one kernel in three forms. Operands keep the layout that they have in memory: whichever of their two
+ * dimensions is the contiguous one, a box of 64 of it fills the 128-byte rows of a swizzled tile, and the product is told the
+ * tile's orientation. Sums stay in tensor memory in fp32 until the end of a tile.
+ */
+#include "decoder_ops.hpp"
+#include "launch_early.cuh"
+#include "row_access.cuh"
+#include "../device/tcgen05.cuh"
+#include "../gpu/driver_api.hpp"
+
+namespace dccl {
+
+enum Form {
+    GATED,          // C = act(x Wg^T) .* (x Wu^T): both operands contiguous along k; the columns of a tile are half of Wg and half of Wu
+    INPUT_GRAD,     // dx = dg Wg + du Wu: k runs through ffn twice; W is contiguous along the columns
+    WEIGHT_GRAD,    // dW = dg^T x, du^T x: k are the tokens, both operands contiguous along rows and columns of the result
+};
+
+constexpr int kTileM = 128, kTileK = 64, kStages = 4;
+constexpr int kEpilogueWarps = 4, kGemmThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kStageRowsBytes = 128;                                // one row of a swizzled tile
+
+struct GemmArgs {
+    CUtensorMap a0, a1, b0, b1;
+    unsigned m, n;                  // rows and columns of the result
+    unsigned tiles_m, tiles_n, batch, splits, k_blocks;             // k_blocks: of one tile over all its k
+    unsigned k_half;                // INPUT_GRAD: blocks of ffn, after which the second pair of operands follows
+    unsigned descriptor;            // of one product
+    int act;
+    void *c0, *c1;                  // results (c1: second of the batch)
+    float *g, *u;                   // GATED: the products, or null
+    size_t pre_stride;
+    float* partial;                 // [split][batch or gate, up][m][partial_stride] where splits > 1
+    size_t partial_stride;
+    int* gave_up;                   // host memory: a wait that did not end
+};
+
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+
+constexpr float kTanhScale = 1.5957691216057308f, kTanhCubic = 0.044715f;      // 2 sqrt(2 / pi)
+
+/** 0.5 g (1 + tanh(z)) = g sigmoid(2 z). */
+__device__ __forceinline__ float activate(float g, int act) {
+    if (act == DCCL_ACT_SILU) return g * sigmoid(g);
+    if (act == DCCL_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    return g * sigmoid(kTanhScale * fmaf(kTanhCubic * g * g, g, g));
+}
+
+/** The activation and its derivative. */
+__device__ __forceinline__ void activate_grad(float g, int act, float& a, float& da) {
+    if (act == DCCL_ACT_SILU) {
+        const float s = sigmoid(g);
+        a = g * s;
+        da = s * fmaf(g, 1.0f - s, 1.0f);
+    } else if (act == DCCL_ACT_GELU) {
+        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        a = g * cdf;
+        da = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), cdf);
+    } else {
+        const float s = sigmoid(kTanhScale * fmaf(kTanhCubic * g * g, g, g));
+        a = g * s;
+        da = fmaf(g * s * (1.0f - s), kTanhScale * fmaf(3.0f * kTanhCubic * g, g, 1.0f), s);
+    }
+}
+
+/** Rows of a tile's 32 columns pass through shared memory, so that a warp stores whole rows and not one line per lane. `stage`: 4 KB of
+ *  this warp, 16-byte pieces of row r at piece ^ (r % 8). */
+__device__ __forceinline__ void stage_rows(char* stage, const float (&v)[32]) {
+    const int lane = threadIdx.x % 32;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+        *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+}
+/** Stores the staged 32 x 32 values as fp32 at `to` (row 0, column 0), rows < rows and columns < columns. Rows start on 16 bytes. */
+__device__ __forceinline__ void store_fp32(const char* stage, float* to, size_t stride, int rows, int columns) {
+    const int lane = threadIdx.x % 32, c = lane % 8;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = i * 4 + lane / 8;
+        const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((c ^ (r & 7)) * 16));
+        if (r < rows && 4 * c < columns) *reinterpret_cast<float4*>(to + (size_t)r * stride + 4 * c) = v;      // up to three of the padding
+    }
+}
+/** The same as T, whose rows may start anywhere. */
+template <typename T> __device__ __forceinline__ void store_as(const char* stage, T* to, size_t stride, int rows, int columns, bool vec) {
+    const int lane = threadIdx.x % 32;
+    if (vec) {
+        const int c = lane % 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + lane / 4;
+            const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + (((2 * c) ^ (r & 7)) * 16));
+            const float4 w = *reinterpret_cast<const float4*>(stage + r * 128 + (((2 * c + 1) ^ (r & 7)) * 16));
+            Run<T, 8> o = {Traits<T>::down(v.x), Traits<T>::down(v.y), Traits<T>::down(v.z), Traits<T>::down(v.w),
+                           Traits<T>::down(w.x), Traits<T>::down(w.y), Traits<T>::down(w.z), Traits<T>::down(w.w)};
+            if (r < rows && 8 * c < columns) st_run<T, 8>(to + (size_t)r * stride + 8 * c, o);
+        }
+    } else if (lane < columns) {
+#pragma unroll 4
+        for (int r = 0; r < rows && r < 32; r++)
+            to[(size_t)r * stride + lane] = Traits<T>::down(*reinterpret_cast<const float*>(stage + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
+    }
+}
+
+/** Tile number -> place. Groups of 16 rows of tiles are walked column by column, so that the tiles of one moment share operands in L2. */
+struct Place { unsigned m, n, batch, split; };
+__device__ __forceinline__ Place place_of(unsigned tile, const GemmArgs& a) {
+    Place p;
+    p.split = tile % a.splits;
+    tile /= a.splits;
+    const unsigned per_batch = a.tiles_m * a.tiles_n;
+    p.batch = tile / per_batch;
+    tile %= per_batch;
+    const unsigned group = tile / (16 * a.tiles_n), first = group * 16, rows = a.tiles_m - first < 16 ? a.tiles_m - first : 16;
+    tile -= first * a.tiles_n;
+    p.m = first + tile % rows;
+    p.n = tile / rows;
+    return p;
+}
+
+template <int FORM, int N> struct GemmShape {
+    static constexpr int kBytesA = kTileM * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB;
+    static constexpr int kShared = kStages * kBytes + kEpilogueWarps * 4096 + 1024;      // 1024: the tiles' alignment
+    static constexpr int kColumns = FORM == GATED ? N / 2 : N;                           // of the result
+};
+
+/**
+ * One CTA per SM walks over tiles of 128 rows; warp 4 loads, warp 5 multiplies, warps 0 to 3 store. The sums of two tiles fit into
+ * tensor memory, so that one is stored while the next is multiplied.
+ */
+template <typename T, int FORM, int N>
+__global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs a) {
+    using Shape = GemmShape<FORM, N>;
+    extern __shared__ char shared[];
+    __shared__ uint64_t bars[2 * kStages + 5];
+    __shared__ uint32_t tmem_base;
+    __shared__ int failed;
+    char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
+    char* const staging = tiles + kStages * Shape::kBytes;
+    const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16, drained = sums_empty + 16;
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (warp == 5) tmem_alloc(shared_addr(&tmem_base), 2 * N);
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
+        for (int i = 0; i < 2; i++) { bar_init(sums_full + 8 * i, 1); bar_init(sums_empty + 8 * i, kEpilogueWarps); }
+        bar_init(drained, 1);
+        bar_init_fence();
+    }
+    if (threadIdx.x == 32 * 4) {
+        prefetch_map(&a.a0);
+        prefetch_map(&a.b0);
+        if (FORM == GATED) prefetch_map(&a.b1);
+        if (FORM != GATED) prefetch_map(&a.a1);
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    const uint32_t sums = tmem_base;
+    wait_for_stream();
+    const unsigned total = a.tiles_m * a.tiles_n * a.batch * a.splits;
+    unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
+    if (warp == 4 && lane == 0) {
+        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const Place p = place_of(tile, a);
+            const unsigned from = (unsigned)((unsigned long long)a.k_blocks * p.split / a.splits), to = (unsigned)((unsigned long long)a.k_blocks * (p.split + 1) / a.splits);
+            const int row = p.m * kTileM, column = p.n * Shape::kColumns;
+            unsigned kb = from;
+            for (; kb < to; kb++, filled++) {
+                const unsigned s = filled % kStages;
+                if (!bar_wait(empty + 8 * s, (filled / kStages & 1) ^ 1, &failed)) break;
+                const uint32_t bar = full + 8 * s, to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA;
+                bar_expect(bar, Shape::kBytes);
+                if constexpr (FORM == GATED) {
+                    load_box(to_a, &a.a0, kb * kTileK, row, bar);
+                    load_box(to_b, &a.b0, kb * kTileK, column, bar);
+                    load_box(to_b + Shape::kBytesB / 2, &a.b1, kb * kTileK, column, bar);
+                } else if constexpr (FORM == INPUT_GRAD) {
+                    const bool second = kb >= a.k_half;
+                    const int k = (second ? kb - a.k_half : kb) * kTileK;
+                    load_box(to_a, second ? &a.a1 : &a.a0, k, row, bar);
+#pragma unroll
+                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * kStageRowsBytes, second ? &a.b1 : &a.b0, column + 64 * i, k, bar);
+                } else {
+                    const CUtensorMap* map = p.batch ? &a.a1 : &a.a0;
+#pragma unroll
+                    for (int i = 0; i < kTileM / 64; i++) load_box(to_a + i * 64 * kStageRowsBytes, map, row + 64 * i, kb * kTileK, bar);
+#pragma unroll
+                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * kStageRowsBytes, &a.b0, column + 64 * i, kb * kTileK, bar);
+                }
+            }
+            if (kb < to) break;
+        }
+    } else if (warp == 5 && lane == 0) {
+        unsigned done = 0;
+        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
+            const Place p = place_of(tile, a);
+            const unsigned from = (unsigned)((unsigned long long)a.k_blocks * p.split / a.splits), to = (unsigned)((unsigned long long)a.k_blocks * (p.split + 1) / a.splits);
+            const unsigned buffer = done & 1;
+            if (!bar_wait(sums_empty + 8 * buffer, (done / 2 & 1) ^ 1, &failed)) break;
+            tc_after_sync();
+            const uint32_t d = sums + buffer * N;
+            unsigned kb = from;
+            for (; kb < to; kb++, filled++) {
+                const unsigned s = filled % kStages;
+                if (!bar_wait(full + 8 * s, filled / kStages & 1, &failed)) break;
+                tc_after_sync();
+                const uint32_t at_a = shared_addr(tiles) + s * Shape::kBytes, at_b = at_a + Shape::kBytesA;
+#pragma unroll
+                for (int k = 0; k < kTileK / 16; k++) {
+                    // 16 k: 32 bytes further along K-major rows, or 16 rows of 128 bytes further
+                    const uint64_t da = FORM == WEIGHT_GRAD ? tile_descriptor(at_a + k * 2048, 64 * kStageRowsBytes) : tile_descriptor(at_a + k * 32, 16);
+                    const uint64_t db = FORM == GATED ? tile_descriptor(at_b + k * 32, 16) : tile_descriptor(at_b + k * 2048, 64 * kStageRowsBytes);
+                    product(d, da, db, a.descriptor, kb > from || k);
+                }
+                commit(empty + 8 * s);
+            }
+            if (kb < to) break;
+            commit(sums_full + 8 * buffer);
+        }
+    } else if (warp < kEpilogueWarps) {
+        char* const stage = staging + warp * 4096;
+        unsigned done = 0;
+        const bool vec = a.n % 8 == 0 && aligned16(a.c0) && aligned16(a.c1);
+        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
+            const Place p = place_of(tile, a);
+            const unsigned buffer = done & 1;
+            if (!bar_wait(sums_full + 8 * buffer, done / 2 & 1, &failed)) break;
+            __syncwarp();
+            tc_after_sync();
+            const uint32_t d = sums + buffer * N + (warp * 32u << 16);
+            const size_t row = (size_t)p.m * kTileM + warp * 32;
+            const int rows = row < a.m ? (int)(a.m - row < 32 ? a.m - row : 32) : 0;
+#pragma unroll 1
+            for (int c = 0; c < Shape::kColumns; c += 32) {
+                const size_t column = (size_t)p.n * Shape::kColumns + c;
+                if (column >= a.n || !rows) break;
+                const int columns = (int)(a.n - column < 32 ? a.n - column : 32);
+                uint32_t r[32];
+                tmem_load32(r, d + c);
+                if constexpr (FORM == GATED) {
+                    uint32_t r2[32];
+                    tmem_load32(r2, d + N / 2 + c);
+                    tmem_wait();
+                    float g[32], u[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) { g[e] = __uint_as_float(r[e]); u[e] = __uint_as_float(r2[e]); }
+                    float* gate_to = a.splits > 1 ? a.partial + ((size_t)p.split * 2 * a.m + row) * a.partial_stride + column : a.g ? a.g + row * a.pre_stride + column : nullptr;
+                    float* up_to = a.splits > 1 ? a.partial + (((size_t)p.split * 2 + 1) * a.m + row) * a.partial_stride + column : a.u ? a.u + row * a.pre_stride + column : nullptr;
+                    const size_t stride = a.splits > 1 ? a.partial_stride : a.pre_stride;
+                    if (gate_to) {
+                        stage_rows(stage, g);
+                        store_fp32(stage, gate_to, stride, rows, columns);
+                        stage_rows(stage, u);
+                        store_fp32(stage, up_to, stride, rows, columns);
+                    }
+                    if (a.splits == 1) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) g[e] = activate(g[e], a.act) * u[e];
+                        stage_rows(stage, g);
+                        store_as<T>(stage, reinterpret_cast<T*>(a.c0) + row * a.n + column, a.n, rows, columns, vec);
+                    }
+                } else {
+                    tmem_wait();
+                    float v[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = __uint_as_float(r[e]);
+                    stage_rows(stage, v);
+                    if (a.splits > 1) store_fp32(stage, a.partial + (((size_t)p.split * a.batch + p.batch) * a.m + row) * a.partial_stride + column, a.partial_stride, rows, columns);
+                    else store_as<T>(stage, reinterpret_cast<T*>(p.batch ? a.c1 : a.c0) + row * a.n + column, a.n, rows, columns, vec);
+                }
+            }
+            tc_before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(sums_empty + 8 * buffer);
+        }
+    }
+    __syncthreads();
+    if (failed) {       // no wait is expected to run out: copies in flight still have to land, and products to end, before the memory is given back
+        int late = 0;
+        if (warp == 4 && lane == 0)
+            for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
+        if (warp == 5 && lane == 0) {
+            commit(drained);
+            bar_wait(drained, 0, &late);
+        }
+        if (threadIdx.x == 0 && a.gave_up) *reinterpret_cast<volatile int*>(a.gave_up) = 1;
+        __syncthreads();
+    }
+    tc_after_sync();
+    if (warp == 5) tmem_free(sums, 2 * N);
+}
+
+struct JoinArgs {
+    const float* partial;
+    size_t m, stride;               // rows, and elements between rows of a partial result
+    unsigned n, splits, batch;
+    int act;
+    void *c0, *c1;
+    float *g, *u;
+    size_t pre_stride;
+};
+
+/** Adds the parts that splits of k left, in the order of k, and finishes: one thread per element. */
+template <typename T, bool GATE> __global__ void __launch_bounds__(256) k_join(const __grid_constant__ JoinArgs a) {
+    wait_for_stream();
+    const size_t plane = a.m * a.stride, count = a.m * a.n;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count * (GATE ? 1 : a.batch); i += (size_t)gridDim.x * 256) {
+        const size_t batch = i / count, at = i % count, row = at / a.n, column = at % a.n, from = row * a.stride + column;
+        if constexpr (GATE) {
+            float g = 0, u = 0;
+            for (unsigned s = 0; s < a.splits; s++) { g += a.partial[2 * s * plane + from]; u += a.partial[(2 * s + 1) * plane + from]; }
+            if (a.g) { a.g[row * a.pre_stride + column] = g; a.u[row * a.pre_stride + column] = u; }
+            reinterpret_cast<T*>(a.c0)[at] = Traits<T>::down(activate(g, a.act) * u);
+        } else {
+            float v = 0;
+            for (unsigned s = 0; s < a.splits; s++) v += a.partial[(s * a.batch + batch) * plane + from];
+            reinterpret_cast<T*>(batch ? a.c1 : a.c0)[at] = Traits<T>::down(v);
+        }
+    }
+}
+
+struct PadArgs { const void* from[3]; void* to[3]; size_t rows[3]; unsigned width, stride; };
+
+/** Rows that do not start on 16 bytes, copied to some that do, for the tiled loads. The elements behind a row are not read by anyone. */
+template <typename T> __global__ void __launch_bounds__(256) k_pad(const __grid_constant__ PadArgs a) {
+    wait_for_stream();
+    for (int w = 0; w < 3; w++) {
+        const T* from = reinterpret_cast<const T*>(a.from[w]);
+        T* to = reinterpret_cast<T*>(a.to[w]);
+        for (size_t row = blockIdx.x; row < a.rows[w]; row += gridDim.x)
+            for (unsigned i = threadIdx.x; i < a.width; i += 256) to[row * a.stride + i] = from[row * a.width + i];
+    }
+}
+
+struct GateGradArgs { const void* dh; const float *g, *u; void *dg, *du; size_t pre_stride, stride; unsigned rows, n; int act; };
+
+/** dg and du from dh and the saved products. V: elements per access. */
+template <typename T, int V> __global__ void __launch_bounds__(256) k_gate_grad(const __grid_constant__ GateGradArgs a) {
+    wait_for_stream();
+    const unsigned runs = a.n / V;
+    const size_t count = (size_t)a.rows * runs;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (size_t)gridDim.x * 256) {
+        const size_t row = i / runs, column = i % runs * V;
+        float g[V], u[V];
+        ld_vector<float, V>(g, a.g, true, row * a.pre_stride + column);
+        ld_vector<float, V>(u, a.u, true, row * a.pre_stride + column);
+        const Run<T, V> dh = ld_run<T, V>(reinterpret_cast<const T*>(a.dh) + row * a.n + column);
+        Run<T, V> dg, du;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float d = Traits<T>::up(dh.e[e]);
+            float act, slope;
+            activate_grad(g[e], a.act, act, slope);
+            dg.e[e] = Traits<T>::down(d * u[e] * slope);
+            du.e[e] = Traits<T>::down(d * act);
+        }
+        st_run<T, V>(reinterpret_cast<T*>(a.dg) + row * a.stride + column, dg);
+        st_run<T, V>(reinterpret_cast<T*>(a.du) + row * a.stride + column, du);
+    }
+}
+
+/* ------------------------------------------------------------------------------------------------ host side */
+
+/** Set by a kernel whose wait ran out; looked at by the next call. Host memory that the device writes, for the life of the process. */
+static int* gave_up_flag() {
+    static int* flag = [] {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);       // a first call may come while a stream is being captured
+        void* p = nullptr;
+        if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { cudaGetLastError(); p = nullptr; }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (p) *reinterpret_cast<int*>(p) = 0;
+        return reinterpret_cast<int*>(p);
+    }();
+    return flag;
+}
+
+/** The two dimensions of an operand by which one is contiguous, and the box of it. */
+static cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, size_t inner, size_t outer, size_t stride, unsigned box_outer) {
+    const DriverApi* d = driver_api(nullptr);
+    if (!d || !d->TensorMapEncodeTiled) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {inner, outer}, strides[1] = {stride * 2};
+    const cuuint32_t box[2] = {64, box_outer}, steps[2] = {1, 1};
+    const CUresult r = d->TensorMapEncodeTiled(map, dtype == 6 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
+                                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+static size_t up_to(size_t v, size_t step) { return (v + step - 1) / step * step; }
+static unsigned blocks_of(size_t v, size_t block) { return (unsigned)((v + block - 1) / block); }
+
+/** Tiles of a product and the parts that its k is cut into. */
+struct GemmPlan { unsigned tiles_m, tiles_n, batch, splits, k_blocks; size_t partial_bytes; };
+
+static GemmPlan plan_gemm(int sms, int form, size_t m, size_t n, size_t k) {
+    GemmPlan p;
+    p.tiles_m = blocks_of(m, kTileM);
+    p.tiles_n = blocks_of(n, form == GATED ? 128 : 256);
+    p.batch = form == WEIGHT_GRAD ? 2 : 1;
+    p.k_blocks = blocks_of(k, kTileK) * (form == INPUT_GRAD ? 2 : 1);
+    const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch;
+    size_t splits = (size_t)sms / (tiles ? tiles : 1);
+    if (splits > p.k_blocks / 4) splits = p.k_blocks / 4;
+    p.splits = splits > 1 ? (unsigned)splits : 1;
+    p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (form == INPUT_GRAD ? 1 : 2) * m * up_to(n, 4) * sizeof(float) : 0;
+    return p;
+}
+
+template <typename T, int FORM> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
+    using Shape = GemmShape<FORM, 256>;
+    static std::atomic<bool> ready[64];
+    if (!ready[device].load(std::memory_order_relaxed)) {
+        const cudaError_t e = cudaFuncSetAttribute(k_gemm<T, FORM, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+        if (e != cudaSuccess) return e;
+        ready[device].store(true, std::memory_order_relaxed);
+    }
+    a.tiles_m = p.tiles_m;
+    a.tiles_n = p.tiles_n;
+    a.batch = p.batch;
+    a.splits = p.splits;
+    a.k_blocks = p.k_blocks;
+    a.partial_stride = up_to(a.n, 4);
+    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == WEIGHT_GRAD, FORM != GATED, kTileM, 256);
+    a.gave_up = gave_up_flag();
+    const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch * p.splits, sms = (size_t)sm_count(device);
+    cudaError_t e = launch_early_shared(k_gemm<T, FORM, 256>, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, Shape::kShared, stream, a);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    const JoinArgs j = {a.partial, a.m, a.partial_stride, a.n, p.splits, p.batch, a.act, a.c0, a.c1, a.g, a.u, a.pre_stride};
+    const size_t elements = (size_t)a.m * a.n * p.batch, ctas = (elements + 255) / 256;
+    return launch_early(k_join<T, FORM == GATED>, (unsigned)(ctas < 8 * sms ? ctas : 8 * sms), 256, stream, j);
+}
+
+/** Where the parts of a call's workspace lie. */
+struct GatedLayout { size_t stride, x, gate, up, dg, du, d_stride, partial, total; GemmPlan forward, input, weight; bool ok; };
+
+static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn, bool aligned, bool backward) {
+    GatedLayout l = {};
+    const int sms = sm_count(device);
+    l.ok = sms > 0 && tokens < (1u << 30) && width < (1u << 30) && ffn < (1u << 30);
+    if (!l.ok) return l;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) { const size_t here = at; at += up_to(bytes, 256); return here; };
+    const bool pad = !aligned || width % 8;
+    l.stride = pad ? up_to(width, 8) : width;
+    if (pad) {
+        l.x = take(tokens * l.stride * 2);
+        l.gate = take(ffn * l.stride * 2);
+        l.up = take(ffn * l.stride * 2);
+    }
+    l.d_stride = up_to(ffn, 8);
+    size_t partial = 0;
+    if (backward) {
+        l.dg = take(tokens * l.d_stride * 2);
+        l.du = take(tokens * l.d_stride * 2);
+        l.input = plan_gemm(sms, INPUT_GRAD, tokens, width, ffn);
+        l.weight = plan_gemm(sms, WEIGHT_GRAD, ffn, width, tokens);
+        partial = l.input.partial_bytes > l.weight.partial_bytes ? l.input.partial_bytes : l.weight.partial_bytes;
+    } else {
+        l.forward = plan_gemm(sms, GATED, tokens, ffn, width);
+        partial = l.forward.partial_bytes;
+    }
+    l.partial = take(partial);
+    l.total = at;
+    return l;
+}
+
+/** x, Wg and Wu as the tiled loads take them: in place, or padded into the workspace. */
+static cudaError_t pad_operands(int device, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, bool with_weights, const void*& x, const void*& w_gate, const void*& w_up,
+                                char* workspace, cudaStream_t stream) {
+    if (l.stride == width && aligned_to(16, {x, w_gate, w_up})) return cudaSuccess;
+    PadArgs a = {{x, w_gate, w_up}, {workspace + l.x, workspace + l.gate, workspace + l.up}, {tokens, with_weights ? ffn : 0, with_weights ? ffn : 0}, (unsigned)width, (unsigned)l.stride};
+    x = a.to[0];
+    w_gate = a.to[1];
+    w_up = a.to[2];
+    return launch_early(k_pad<uint16_t>, (unsigned)(8 * sm_count(device)), 256, stream, a);
+}
+
+template <typename T> static cudaError_t gated_forward(int device, int dtype, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up,
+                                                       int act, void* h, float* g, float* u, size_t pre_stride, char* workspace, cudaStream_t stream) {
+    cudaError_t e = pad_operands(device, l, tokens, width, ffn, true, x, w_gate, w_up, workspace, stream);
+    GemmArgs a = {};
+    if (e == cudaSuccess) e = make_map(&a.a0, dtype, x, width, tokens, l.stride, kTileM);
+    if (e == cudaSuccess) e = make_map(&a.b0, dtype, w_gate, width, ffn, l.stride, 128);
+    if (e == cudaSuccess) e = make_map(&a.b1, dtype, w_up, width, ffn, l.stride, 128);
+    if (e != cudaSuccess) return e;
+    a.m = (unsigned)tokens;
+    a.n = (unsigned)ffn;
+    a.act = act;
+    a.c0 = a.c1 = h;
+    a.g = g;
+    a.u = u;
+    a.pre_stride = pre_stride;
+    a.partial = (float*)(workspace + l.partial);
+    return run_gemm<T, GATED>(device, l.forward, a, stream);
+}
+
+template <typename T> static cudaError_t gated_backward(int device, int dtype, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void* dh, const float* g, const float* u,
+                                                        size_t pre_stride, const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up,
+                                                        char* workspace, cudaStream_t stream) {
+    const GateGradArgs d = {dh, g, u, workspace + l.dg, workspace + l.du, pre_stride, l.d_stride, (unsigned)tokens, (unsigned)ffn, act};
+    const size_t sms = (size_t)sm_count(device);
+    const bool vec = ffn % 8 == 0 && aligned_to(16, {dh, g, u}) && pre_stride % 4 == 0;
+    const size_t runs = tokens * (vec ? ffn / 8 : ffn), ctas = (runs + 255) / 256;
+    cudaError_t e = launch_early(vec ? k_gate_grad<T, 8> : k_gate_grad<T, 1>, (unsigned)(ctas < 64 * sms ? ctas : 64 * sms), 256, stream, d);
+    if (e == cudaSuccess) e = pad_operands(device, l, tokens, width, ffn, dx != nullptr, x, w_gate, w_up, workspace, stream);
+    GemmArgs a = {};
+    a.partial = (float*)(workspace + l.partial);
+    if (e == cudaSuccess && dx) {
+        e = make_map(&a.a0, dtype, d.dg, ffn, tokens, l.d_stride, kTileM);
+        if (e == cudaSuccess) e = make_map(&a.a1, dtype, d.du, ffn, tokens, l.d_stride, kTileM);
+        if (e == cudaSuccess) e = make_map(&a.b0, dtype, w_gate, width, ffn, l.stride, kTileK);
+        if (e == cudaSuccess) e = make_map(&a.b1, dtype, w_up, width, ffn, l.stride, kTileK);
+        if (e != cudaSuccess) return e;
+        a.m = (unsigned)tokens;
+        a.n = (unsigned)width;
+        a.k_half = blocks_of(ffn, kTileK);
+        a.c0 = a.c1 = dx;
+        e = run_gemm<T, INPUT_GRAD>(device, l.input, a, stream);
+    }
+    if (e == cudaSuccess && dw_gate) {
+        e = make_map(&a.a0, dtype, d.dg, ffn, tokens, l.d_stride, kTileK);
+        if (e == cudaSuccess) e = make_map(&a.a1, dtype, d.du, ffn, tokens, l.d_stride, kTileK);
+        if (e == cudaSuccess) e = make_map(&a.b0, dtype, x, width, tokens, l.stride, kTileK);
+        if (e != cudaSuccess) return e;
+        a.m = (unsigned)ffn;
+        a.n = (unsigned)width;
+        a.c0 = dw_gate;
+        a.c1 = dw_up;
+        e = run_gemm<T, WEIGHT_GRAD>(device, l.weight, a, stream);
+    }
+    return e;
+}
+
+static bool gave_up(const char* who) {
+    const int* flag = gave_up_flag();
+    if (!flag || !*reinterpret_cast<const volatile int*>(flag)) return false;
+    fprintf(stderr, "%s: an earlier product on this machine did not end in time; its results are incomplete\n", who);
+    return true;
+}
+
+} // namespace dccl
+
+using namespace dccl;
+
+extern "C" long long dccl_gated_linear_workspace(int device, size_t tokens, size_t width, size_t ffn, int aligned, int backward) {
+    const GatedLayout l = layout_of(device, tokens, width, ffn, aligned != 0, backward != 0);
+    return l.ok ? (long long)l.total : -1;
+}
+
+extern "C" int dccl_gated_linear(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up, int act, void* h,
+                                 float* g, float* u, size_t pre_stride, void* workspace, long long workspace_bytes, void* stream) {
+    const char* who = "dccl_gated_linear";
+    if (!tokens || !ffn) return 0;
+    const GatedLayout l = layout_of(device, tokens, width, ffn, aligned_to(16, {x, w_gate, w_up}), false);
+    if (!l.ok || !width || workspace_bytes < (long long)l.total || (dtype != 6 && dtype != 9) || act < 0 || act > DCCL_ACT_GELU_TANH || (!g != !u) || (g && pre_stride < ffn)
+        || pre_stride % 4 || !aligned_to(16, {g, u, workspace}))
+        return report(who, cudaErrorInvalidValue);
+    if (gave_up(who)) return -1;
+    OnDevice on(device);
+    if (on.e != cudaSuccess) return report(who, on.e);
+    const auto run = dtype == 6 ? gated_forward<__half> : gated_forward<__nv_bfloat16>;
+    return report(who, run(device, dtype, l, tokens, width, ffn, x, w_gate, w_up, act, h, g, u, pre_stride, (char*)workspace, (cudaStream_t)stream));
+}
+
+extern "C" int dccl_gated_linear_backward(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* dh, const float* g, const float* u, size_t pre_stride,
+                                          const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up, void* workspace,
+                                          long long workspace_bytes, void* stream) {
+    const char* who = "dccl_gated_linear_backward";
+    const GatedLayout l = layout_of(device, tokens, width, ffn, aligned_to(16, {x, w_gate, w_up}), true);
+    if (!l.ok || !tokens || !width || !ffn || workspace_bytes < (long long)l.total || (dtype != 6 && dtype != 9) || act < 0 || act > DCCL_ACT_GELU_TANH || !g || !u
+        || pre_stride < ffn || pre_stride % 4 || !aligned_to(16, {g, u, workspace}) || (!dw_gate != !dw_up))
+        return report(who, cudaErrorInvalidValue);
+    if (gave_up(who)) return -1;
+    OnDevice on(device);
+    if (on.e != cudaSuccess) return report(who, on.e);
+    const auto run = dtype == 6 ? gated_backward<__half> : gated_backward<__nv_bfloat16>;
+    return report(who, run(device, dtype, l, tokens, width, ffn, dh, g, u, pre_stride, x, w_gate, w_up, act, dx, dw_gate, dw_up, (char*)workspace, (cudaStream_t)stream));
+}

@@ -27,7 +27,7 @@ constexpr bool launch_is_cheap(size_t parameter_bytes) { return parameter_bytes 
  * edge a programmatic one leaves in a graph carries data that not every user of the capture API expects.
  */
 template <typename... P, typename... A>
-inline cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, A... args) {
+inline cudaError_t launch_early_shared(void (*kernel)(P...), unsigned grid, unsigned block, size_t shared_bytes, cudaStream_t stream, const A&... args) {
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -35,10 +35,15 @@ inline cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned bl
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = shared_bytes;
     cfg.stream = stream;
     if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess) cudaGetLastError();      // the launch reports it
     else if (capturing == cudaStreamCaptureStatusNone) { cfg.attrs = &attr; cfg.numAttrs = 1; }
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, A... args) {
+    return launch_early_shared(kernel, grid, block, 0, stream, args...);
 }
 
 } // namespace dccl

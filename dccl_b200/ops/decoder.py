@@ -8,10 +8,11 @@
                           and the entry of the next, in one pass
     rotary                queries and keys turned by their positions
     rotary_frequencies    the frequencies it takes, also those stretched to longer contexts
+    gated_linear          act(x Wg^T) * (x Wu^T): the two projections of a gated feed-forward layer
     ====================  ==============================================================================
 
 All are differentiable. CUDA tensors run one kernel per call on the current stream of their device (csrc/kernels/residual_norm.cu,
-rotary.cu) in float16, bfloat16 or float32; sums and statistics are fp32 and every result is rounded once. CPU tensors take
+rotary.cu, gated_linear.cu) in float16, bfloat16 or float32 (gated_linear: not float32); sums and statistics are fp32 and every result is rounded once. CPU tensors take
 the same formulas in torch, so the same model code is tested without a GPU. Inputs may have any strides; what a kernel cannot
 read in place is copied first. A call allocates its outputs and its workspace from torch's allocator and nothing else, so it can be
 captured into a graph; a gradient has the same bits whenever its inputs do (no atomics).
@@ -381,3 +382,99 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling=None, factor=1.0, orig
         keep = 1 - (index - first) / max(last - first, 0.001)
     keep = keep.clamp(0, 1)
     return f * (keep + (1 - keep) / factor)
+
+
+# ---------------------------------------------------------------------------------------------- gated linear
+
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}        # csrc/kernels/decoder_ops.hpp
+
+
+def _gated_work(x, w_gate, w_up, backward):
+    """(workspace or None, its bytes) of a call."""
+    aligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
+    size = lib().dccl_gated_linear_workspace(x.get_device(), x.numel() // x.shape[-1], x.shape[-1], w_gate.shape[0], aligned, backward)
+    _done(-1 if size < 0 else 0, "gated_linear")
+    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
+
+
+def _gated_forward(x, w_gate, w_up, act, keep):
+    """(h, g, u): g and u are the two products in fp32, in rows of a multiple of four elements, or None unless `keep`."""
+    width, ffn = x.shape[-1], w_gate.shape[0]
+    tokens = x.numel() // width
+    h = torch.empty(x.shape[:-1] + (ffn,), dtype=x.dtype, device=x.device)
+    g = u = None
+    stride = -(-ffn // 4) * 4
+    if keep:
+        g, u = (torch.empty(tokens, stride, dtype=torch.float32, device=x.device) for _ in range(2))
+    if tokens:
+        device = x.get_device()
+        work, size = _gated_work(x, w_gate, w_up, False)
+        _done(lib().dccl_gated_linear(device, dtype_of(x), tokens, width, ffn, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), act, h.data_ptr(), _ptr(g), _ptr(u), stride,
+                                      _ptr(work), size, current_stream_handle(device)), "gated_linear")
+    return h, g, u
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, act):
+        h, g, u = _gated_forward(x, w_gate, w_up, act, True)
+        ctx.act = act
+        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w_gate, w_up, g, u = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dh = dh.contiguous()
+        dx = torch.empty_like(x) if need[0] else None
+        dw_gate, dw_up = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need[1] or need[2] else (None, None)
+        width, ffn = x.shape[-1], w_gate.shape[0]
+        tokens = x.numel() // width
+        if tokens:
+            device = x.get_device()
+            work, size = _gated_work(x, w_gate, w_up, True)
+            _done(lib().dccl_gated_linear_backward(device, dtype_of(x), tokens, width, ffn, dh.data_ptr(), g.data_ptr(), u.data_ptr(), g.shape[1], x.data_ptr(), w_gate.data_ptr(),
+                                                   w_up.data_ptr(), ctx.act, _ptr(dx), _ptr(dw_gate), _ptr(dw_up), _ptr(work), size, current_stream_handle(device)),
+                  "gated_linear backward")
+        elif dw_gate is not None:
+            dw_gate.zero_(), dw_up.zero_()
+        return dx, dw_gate if need[1] else None, dw_up if need[2] else None, None
+
+
+def _activate_on_cpu(g, activation):
+    if activation == "silu":
+        return torch.nn.functional.silu(g)
+    return torch.nn.functional.gelu(g, approximate="tanh" if activation == "gelu_tanh" else "none")
+
+
+def gated_linear(x, w_gate, w_up, activation="silu"):
+    """``act(x @ w_gate.T) * (x @ w_up.T)``: x [..., width], the weights [ffn, width], all of one type; `activation` is "silu", "gelu" or
+    "gelu_tanh". Both products stay in fp32 up to the one rounding of the result.
+
+    On the GPU x is float16 or bfloat16. For the backward pass the call keeps the two products in fp32 (8 bytes per element of the result):
+    from 16 bits their rounding would come on top of the one that their gradients need to be multiplied again."""
+    _check_activations("gated_linear", "x", x, range(1, 65))
+    width = x.shape[-1]
+    if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 2:
+        raise TypeError("gated_linear: w_gate must be a tensor [ffn, width]")
+    ffn = w_gate.shape[0]
+    for name, w in (("w_gate", w_gate), ("w_up", w_up)):
+        _check_like("gated_linear", name, w, (ffn, width), (x.dtype,), x.device)
+    if not width or not ffn:
+        raise ValueError("gated_linear: weights of shape %s" % ((ffn, width),))
+    if activation not in _ACTIVATIONS:
+        raise ValueError("gated_linear: activation %r is none of %s" % (activation, ", ".join(_ACTIVATIONS)))
+    if not x.is_cuda:
+        v = x.float()
+        return (_activate_on_cpu(v @ w_gate.float().t(), activation) * (v @ w_up.float().t())).to(x.dtype)
+    if x.dtype is torch.float32:
+        raise TypeError("gated_linear: float32 is taken on the CPU only; the tensor cores multiply float16 and bfloat16")
+    if max(x.numel() // width, width, ffn) >= 1 << 30:
+        raise ValueError("gated_linear: a dimension of 2^30 or more")
+    act = _ACTIVATIONS[activation]
+    x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+    if _records(x, w_gate, w_up):
+        return _GatedLinear.apply(x, w_gate, w_up, act)
+    return _gated_forward(x, w_gate, w_up, act, False)[0]

@@ -437,3 +437,167 @@ def test_rotary_refusals_on_the_gpu():
     rotary_refusals("cuda")
     with pytest.raises(ValueError):
         ops.rotary(torch.zeros(1, 2, 1, 8, device="cuda"), None, ops.rotary_frequencies(8))
+
+
+# ---------------------------------------------------------------------------------------------- gated linear
+
+ACTS = ["silu", "gelu", "gelu_tanh"]
+
+
+def act_of(g, name):
+    if name == "silu":
+        return g * torch.sigmoid(g)
+    if name == "gelu":
+        return g * torch.special.ndtr(g)
+    return g * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3))
+
+
+def gated_case(tokens, width, ffn, dtype, device, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, width, generator=g)
+    wg, wu = (torch.randn(ffn, width, generator=g) / math.sqrt(width) for _ in range(2))
+    dh = torch.randn(tokens, ffn, generator=g)
+    return [t.to(dtype).to(device) for t in (x, wg, wu, dh)]
+
+
+def gated_check(x, wg, wu, dh, act, h, grads, dtype):
+    """fp32 sums of k products are off by 2^-24 of every partial sum at most: k 2^-24 of the sum of sizes. The rounding of dg and du to
+    `dtype` goes through the products that take them."""
+    u = half_step(dtype)
+    x, wg, wu = (t.detach().double().cpu().requires_grad_(True) for t in (x, wg, wu))
+    with torch.no_grad():
+        g, up = x @ wg.t(), x @ wu.t()
+        size = x.abs() @ wg.abs().t(), x.abs() @ wu.abs().t()
+    k = x.shape[1] * 2.0 ** -24
+    g.requires_grad_(True)
+    a = act_of(g, act)
+    slope = torch.autograd.grad(a.sum(), g)[0]
+    g, a = g.detach(), a.detach()
+    # |act'| is at most 1.13; sixteen fp32 operations on the activation
+    e_a, e_u = 1.13 * k * size[0] + F32 * (a.abs() + g.abs()), k * size[1]
+    want = a * up
+    check("h", h, want, u * want.abs() + e_a * up.abs() + a.abs() * e_u + e_a * e_u)
+    if grads is None:
+        return
+    dh = dh.double().cpu()
+    # |act''| is at most 0.8
+    e_slope = 0.8 * k * size[0] + F32 * (1 + g.abs())
+    dg, du = dh * up * slope, dh * a
+    e_g = u * dg.abs() + dh.abs() * (e_u * slope.abs() + up.abs() * e_slope + e_u * e_slope)
+    e_d = u * du.abs() + dh.abs() * e_a
+    tiny = torch.finfo(dtype).tiny * u      # of dg and du, where they are below the normal numbers
+    e_g, e_d = e_g + tiny, e_d + tiny
+    x, wg, wu = x.detach(), wg.detach(), wu.detach()
+    for name, got, want, bound, n in (
+            ("dx", grads[0], dg @ wg + du @ wu, e_g @ wg.abs() + e_d @ wu.abs(), 2 * dg.shape[1]),
+            ("dw_gate", grads[1], dg.t() @ x, e_g.t() @ x.abs(), x.shape[0]),
+            ("dw_up", grads[2], du.t() @ x, e_d.t() @ x.abs(), x.shape[0])):
+        terms = {"dx": dg.abs() @ wg.abs() + du.abs() @ wu.abs(), "dw_gate": dg.abs().t() @ x.abs(), "dw_up": du.abs().t() @ x.abs()}[name]
+        check(name, got, want, u * want.abs() + bound + n * 2.0 ** -24 * terms)
+
+
+def gated_run(tokens, width, ffn, dtype, act="silu", device="cuda", backward=True):
+    x, wg, wu, dh = gated_case(tokens, width, ffn, dtype, device)
+    h = ops.gated_linear(x, wg, wu, act)
+    grads = None
+    if backward:
+        for t in (x, wg, wu):
+            t.requires_grad_(True)
+        h2 = ops.gated_linear(x, wg, wu, act)
+        assert torch.equal(h, h2), "with and without a graph"
+        grads = torch.autograd.grad(h2, (x, wg, wu), dh)
+    gated_check(x, wg, wu, dh, act, h, grads, dtype)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_gated_on_cpu(act):
+    gated_run(5, 24, 36, torch.float32, act, device="cpu")
+
+
+SIZES = [(1, 64, 64), (1, 8, 8), (2, 1, 1), (3, 5, 7), (40, 256, 512), (128, 64, 128), (129, 72, 136), (200, 1000, 384), (257, 333, 191), (64, 2048, 200), (1, 2048, 5632), (300, 65, 1033),
+         (1000, 40, 48), (520, 512, 1024), (17, 96, 2050)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("sizes", SIZES, ids=str)
+def test_gated_at_its_sizes(dtype, sizes):
+    gated_run(*sizes, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("act", ACTS)
+def test_gated_activations(act):
+    gated_run(150, 264, 320, torch.bfloat16, act)
+    gated_run(9, 33, 65, torch.float16, act)
+
+
+@gpu
+def test_gated_of_views():
+    """Operands that start between two accesses, a transposed weight, leading dimensions, a gradient that was expanded."""
+    base = torch.randn(70 * 256 + 3, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    _, wg, wu, _ = gated_case(1, 256, 96, torch.bfloat16, "cuda")
+    x = base[3:].view(70, 256)
+    gated_check(x, wg, wu, None, "silu", ops.gated_linear(x, wg, wu), None, torch.bfloat16)
+    wt = wg.t().contiguous().t()
+    x3 = x.view(7, 10, 256).transpose(0, 1)
+    h = ops.gated_linear(x3, wt, wu)
+    gated_check(x3.reshape(70, 256), wg, wu, None, "silu", h.reshape(70, 96), None, torch.bfloat16)
+    x = x.clone().requires_grad_(True)
+    h = ops.gated_linear(x, wg, wu)
+    one = torch.ones(1, 1, device="cuda").bfloat16().expand(70, 96)
+    dx, = torch.autograd.grad(h, x, one, retain_graph=True)
+    assert torch.equal(dx, torch.autograd.grad(h, x, torch.ones_like(h))[0])
+
+
+@gpu
+def test_gated_gradients_of_some_inputs():
+    x, wg, wu, dh = gated_case(33, 64, 72, torch.bfloat16, "cuda")
+    all_in = [t.clone().requires_grad_(True) for t in (x, wg, wu)]
+    want = torch.autograd.grad(ops.gated_linear(*all_in), all_in, dh)
+    for i in range(3):
+        some = [t.clone().requires_grad_(i == j) for j, t in enumerate((x, wg, wu))]
+        assert torch.equal(torch.autograd.grad(ops.gated_linear(*some), some[i], dh)[0], want[i])
+
+
+@gpu
+def test_gated_infinities_stay_in_their_rows():
+    x, wg, wu, _ = gated_case(140, 64, 72, torch.bfloat16, "cuda")
+    h = ops.gated_linear(x, wg, wu)
+    x[3, 5], x[130, 0] = float("nan"), float("inf")
+    bad = ops.gated_linear(x, wg, wu)
+    rows = [r for r in range(140) if r not in (3, 130)]
+    assert torch.equal(bad[rows], h[rows]) and bool(bad[3].isnan().all()) and not bool(bad[130].isfinite().any())
+
+
+@gpu
+def test_gated_without_tokens():
+    x, wg, wu, _ = (t.requires_grad_(True) for t in gated_case(0, 64, 72, torch.bfloat16, "cuda"))
+    ops.gated_linear(x, wg, wu).sum().backward()
+    assert x.grad.shape == x.shape and bool((wg.grad == 0).all()) and bool((wu.grad == 0).all())
+
+
+def gated_refusals(device, dtype):
+    x, w = torch.zeros(2, 8, device=device, dtype=dtype), torch.zeros(6, 8, device=device, dtype=dtype)
+    for bad in ((x.double(), w, w), (x.int(), w, w), (x, w.double(), w), (x, w, w.double()), (x, [1], w), (x, w, None), (x, w[0], w)):
+        with pytest.raises(TypeError):
+            ops.gated_linear(*bad)
+    for bad in ((x, w[:, :4], w), (x, w, w[:3]), (x[:, :4], w, w), (x, w[:0], w[:0]), (x[:, :0], w[:, :0], w[:, :0])):
+        with pytest.raises(ValueError):
+            ops.gated_linear(*bad)
+    for act in ("relu", None, "SILU"):
+        with pytest.raises(ValueError):
+            ops.gated_linear(x, w, w, act)
+
+
+def test_gated_refusals():
+    gated_refusals("cpu", torch.float32)
+
+
+@gpu
+def test_gated_refusals_on_the_gpu():
+    gated_refusals("cuda", torch.bfloat16)
+    with pytest.raises(TypeError):
+        ops.gated_linear(torch.zeros(2, 8, device="cuda"), torch.zeros(6, 8, device="cuda"), torch.zeros(6, 8, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.gated_linear(torch.zeros(2, 8, device="cuda").half(), torch.zeros(6, 8).half(), torch.zeros(6, 8, device="cuda").half())
