@@ -21,13 +21,14 @@ int dccl_residual_norm(int device, int dtype, size_t rows, size_t width, const v
                        const void* gate, size_t rows_per_gate, int f32_vectors, double eps, double scale, void* y, void* n, void* rstd, void* rstd_post,
                        void* stream);
 
-/** Bytes of workspace that the backward pass of `gates` rows of gates (0: without a gate) takes; 0 after an error. */
-size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t width, size_t gates, int has_post);
+/** Bytes of workspace that the backward pass of `gates` rows of gates (0: without a gate) takes; 0 after an error. full: with a branch. */
+size_t dccl_residual_norm_workspace(int device, size_t rows, size_t width, size_t gates, int has_post, int full);
 
 /**
  * Gradients of dccl_residual_norm: from dy and dn (either may be null) those of x and branch, and in the vectors' own types those of
- * weight, post and gate. y is the forward pass's output, or x where there was no branch. dbranch may be null where it equals dx
- * (scale 1, no post, no gate) or there was no branch. No atomics: the same inputs give the same gradients.
+ * weight, post and gate. With a branch (and dbranch), y is the x of the forward pass. Without both, y is the forward pass's y, whose
+ * gradient dx is that of branch as well (scale 1, no post, no gate), or x where there was no branch. No atomics: the same
+ * inputs give the same gradients.
  */
 int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* y, const void* branch,
                                 const void* weight, const void* post, const void* gate, size_t rows_per_gate, int f32_vectors, double scale,

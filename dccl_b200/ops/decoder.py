@@ -124,7 +124,9 @@ class _ResidualNorm(torch.autograd.Function):
         y, n, rstd, rstd_post = _norm_forward(x, branch, weight, post, gate, eps, scale, True)
         ctx.scale, ctx.has_branch = scale, branch is not None
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(y, branch if post is not None or gate is not None else None, weight, post, gate, rstd, rstd_post)
+        # of a plain sum y is enough; otherwise the branch is needed anyway, and with x it gives y before its rounding
+        full = branch is not None and (post is not None or gate is not None or scale != 1.0)
+        ctx.save_for_backward(x if full else y, branch if full else None, weight, post, gate, rstd, rstd_post)
         return (y, n) if branch is not None else n
 
     @staticmethod
@@ -139,19 +141,18 @@ class _ResidualNorm(torch.autograd.Function):
         width = y.shape[-1]
         rows = y.numel() // width
         dx = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        own_branch = ctx.has_branch and (post is not None or gate is not None or ctx.scale != 1.0)
-        dbranch = torch.empty_like(dx) if own_branch else dx if ctx.has_branch else None
+        dbranch = torch.empty_like(dx) if branch is not None else dx if ctx.has_branch else None
         dweight = torch.empty_like(weight) if need[2] and dn is not None else None
         dpost = torch.empty_like(post) if post is not None and need[3] else None
         dgate = torch.empty_like(gate) if gate is not None and need[4] else None
         if rows:
             device, gates = y.get_device(), _gates(y, gate)
             L, dtype = lib(), dtype_of(y)
-            size = L.dccl_residual_norm_workspace(device, dtype, rows, width, gates, post is not None)
+            size = L.dccl_residual_norm_workspace(device, rows, width, gates, post is not None, branch is not None)
             work = torch.empty(size // 4, dtype=torch.float32, device=y.device)
             _done(L.dccl_residual_norm_backward(device, dtype, rows, width, _ptr(dy), _ptr(dn), y.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate),
                                                 rows // gates if gates else 0, _f32_flags(y, weight, post, gate), ctx.scale, rstd.data_ptr(), _ptr(rstd_post), dx.data_ptr(),
-                                                dbranch.data_ptr() if own_branch else None, _ptr(dweight), _ptr(dpost), _ptr(dgate), work.data_ptr(), size,
+                                                _ptr(dbranch) if branch is not None else None, _ptr(dweight), _ptr(dpost), _ptr(dgate), work.data_ptr(), size,
                                                 current_stream_handle(device)), "residual_norm backward")
         else:
             for g in (dweight, dpost, dgate):
