@@ -25,25 +25,33 @@ import math
 import torch
 
 from .._lib import lib
-from ..comm import DcclError, current_stream_handle, dtype_of
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
-_WEIGHT_F32, _POST_F32, _GATE_F32 = 1, 2, 4          # csrc/kernels/decoder_ops.hpp
 _MAX_WIDTH, _MAX_PAIRS = 32768, 1024                 # kNormMaxWidth of csrc/kernels/residual_norm.cu, kRotaryPairs of rotary.cu
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+_ENTRIES = ("dccl_residual_norm", "dccl_residual_norm_workspace", "dccl_residual_norm_backward", "dccl_rotary", "dccl_gated_linear_workspace", "dccl_gated_linear",
+            "dccl_gated_linear_backward")
+_native = None
 
 
-def _done(rc, what):
-    if rc != 0:
-        raise DcclError(1, what)
+def _ext():
+    """The host side of the operators on CUDA tensors (csrc/torch/decoder_ops.cpp), compiled where that has not been done yet."""
+    global _native
+    if _native is None:
+        from ..parallel import backend_build
+        L = lib()
+        if not hasattr(L, "dccl_residual_norm"):
+            raise RuntimeError("libdccl.so was built without CUDA; the device kernels are missing")
+        ext = backend_build.load(compile=True)
+        ext.decoder_ops_bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in _ENTRIES))
+        _native = ext
+    return _native
 
 
-def _records(*tensors):
-    """Whether autograd has to see a call with these inputs."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _refuse(what):
+    """The tensors are of the right types and shapes, and still none that a kernel can read."""
+    raise TypeError("%s takes plain tensors: no subclass that replaces their operations, no functorch transform, no complex conjugate" % what)
 
 
 def _check_like(what, name, t, shape, dtypes, device):
@@ -70,17 +78,6 @@ def _check_activations(what, name, x, dims):
 
 # ---------------------------------------------------------------------------------------------- norms
 
-def _gates(x, gate):
-    """Rows of gates (0: none), each of which covers as many consecutive rows of x."""
-    if gate is None:
-        return 0
-    n = 1
-    if gate.dim() > 1:
-        for s in gate.shape[:-1]:
-            n *= s
-    return n
-
-
 def _check_gate(x, gate):
     """A gate of one row ([width], or ones in front of it), or one per entry of the first dimensions of x: x's own sizes and then ones."""
     width, shape = x.shape[-1], tuple(gate.shape)
@@ -93,72 +90,6 @@ def _check_gate(x, gate):
     if not ok:
         raise ValueError("residual_norm: gate has shape %s; for x of %s it is [%d], or has x's leading sizes followed by ones" % (shape, tuple(x.shape), width))
     _check_like("residual_norm", "gate", gate, gate.shape, (x.dtype, torch.float32), x.device)
-
-
-def _f32_flags(x, weight, post, gate):
-    if x.dtype is torch.float32:
-        return 0
-    return ((_WEIGHT_F32 if weight.dtype is torch.float32 else 0) | (_POST_F32 if post is not None and post.dtype is torch.float32 else 0)
-            | (_GATE_F32 if gate is not None and gate.dtype is torch.float32 else 0))
-
-
-def _norm_forward(x, branch, weight, post, gate, eps, scale, keep):
-    """(y, n, rstd, rstd_post); y is x where there is no branch, the last two are None unless `keep`."""
-    width = x.shape[-1]
-    rows = x.numel() // width
-    n = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty_like(n) if branch is not None else x
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
-    rstd_post = torch.empty(rows, dtype=torch.float32, device=x.device) if keep and post is not None else None
-    if rows:
-        device, gates = x.get_device(), _gates(x, gate)
-        _done(lib().dccl_residual_norm(device, dtype_of(x), rows, width, x.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate), rows // gates if gates else 0,
-                                       _f32_flags(x, weight, post, gate), eps, scale, y.data_ptr() if branch is not None else None, n.data_ptr(), _ptr(rstd), _ptr(rstd_post),
-                                       current_stream_handle(device)), "residual_norm")
-    return y, n, rstd, rstd_post
-
-
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, branch, weight, post, gate, eps, scale):
-        y, n, rstd, rstd_post = _norm_forward(x, branch, weight, post, gate, eps, scale, True)
-        ctx.scale, ctx.has_branch = scale, branch is not None
-        ctx.set_materialize_grads(False)
-        # of a plain sum y is enough; otherwise the branch is needed anyway, and with x it gives y before its rounding
-        full = branch is not None and (post is not None or gate is not None or scale != 1.0)
-        ctx.save_for_backward(x if full else y, branch if full else None, weight, post, gate, rstd, rstd_post)
-        return (y, n) if branch is not None else n
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        y, branch, weight, post, gate, rstd, rstd_post = ctx.saved_tensors
-        dy, dn = grads if ctx.has_branch else (None, grads[0])
-        if dy is None and dn is None:
-            return (None,) * 7
-        dy, dn = (None if g is None else g.contiguous() for g in (dy, dn))
-        need = ctx.needs_input_grad
-        width = y.shape[-1]
-        rows = y.numel() // width
-        dx = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        dbranch = torch.empty_like(dx) if branch is not None else dx if ctx.has_branch else None
-        dweight = torch.empty_like(weight) if need[2] and dn is not None else None
-        dpost = torch.empty_like(post) if post is not None and need[3] else None
-        dgate = torch.empty_like(gate) if gate is not None and need[4] else None
-        if rows:
-            device, gates = y.get_device(), _gates(y, gate)
-            L, dtype = lib(), dtype_of(y)
-            size = L.dccl_residual_norm_workspace(device, rows, width, gates, post is not None, branch is not None)
-            work = torch.empty(size // 4, dtype=torch.float32, device=y.device)
-            _done(L.dccl_residual_norm_backward(device, dtype, rows, width, _ptr(dy), _ptr(dn), y.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate),
-                                                rows // gates if gates else 0, _f32_flags(y, weight, post, gate), ctx.scale, rstd.data_ptr(), _ptr(rstd_post), dx.data_ptr(),
-                                                _ptr(dbranch) if branch is not None else None, _ptr(dweight), _ptr(dpost), _ptr(dgate), work.data_ptr(), size,
-                                                current_stream_handle(device)), "residual_norm backward")
-        else:
-            for g in (dweight, dpost, dgate):
-                if g is not None:
-                    g.zero_()
-        return dx, dbranch, dweight, dpost, dgate, None, None
 
 
 def _norm_on_cpu(x, branch, weight, post, gate, eps, scale):
@@ -177,6 +108,10 @@ def _norm_on_cpu(x, branch, weight, post, gate, eps, scale):
 
 
 def _norm(what, x, branch, weight, post, gate, eps, scale):
+    if isinstance(x, torch.Tensor) and x.is_cuda:
+        out = _ext().residual_norm(x, branch, weight, eps, post, gate, scale)
+        if out is not NotImplemented:
+            return out
     _check_activations(what, "x", x, range(1, 65))
     width = x.shape[-1]
     if not 0 < width <= _MAX_WIDTH:
@@ -190,13 +125,12 @@ def _norm(what, x, branch, weight, post, gate, eps, scale):
     if gate is not None:
         _check_gate(x, gate)
     eps, scale = float(eps), float(scale)
-    if not x.is_cuda:
-        y, n = _norm_on_cpu(x, branch, weight, post, gate, eps, scale)
-        return n if branch is None else (y, n)
-    x, branch, weight, post, gate = (None if t is None else t.contiguous() for t in (x, branch, weight, post, gate))
-    if _records(x, branch, weight, post, gate):
-        return _ResidualNorm.apply(x, branch, weight, post, gate, eps, scale)
-    y, n, _, _ = _norm_forward(x, branch, weight, post, gate, eps, scale, False)
+    if x.is_cuda:
+        if x.numel() // width >= 1 << 31:
+            raise ValueError("%s: %d rows; fewer than 2^31 are taken" % (what, x.numel() // width))
+        out = _ext().residual_norm(x, branch, weight, eps, post, gate, scale)
+        return out if out is not NotImplemented else _refuse(what)
+    y, n = _norm_on_cpu(x, branch, weight, post, gate, eps, scale)
     return n if branch is None else (y, n)
 
 
@@ -222,67 +156,6 @@ def residual_norm(x, branch, weight, eps=1e-5, post_weight=None, gate=None, scal
 
 # ---------------------------------------------------------------------------------------------- rotary positions
 
-class _Heads(ctypes.Structure):
-    """DcclHeads of csrc/kernels/decoder_ops.hpp."""
-    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)] + [(n, ctypes.c_longlong) for n in ("ib", "is_", "ih", "ob", "os", "oh")] + [("heads", ctypes.c_int)]
-
-
-_NO_HEADS = _Heads()
-
-
-def _heads(x, out):
-    """x and out as [batch, seq, heads, dim] by their strides; of three dimensions the batch is missing."""
-    if x is None:
-        return _NO_HEADS
-    i, o = x.stride(), out.stride()
-    if x.dim() == 3:
-        return _Heads(x.data_ptr(), out.data_ptr(), 0, i[0], i[1], 0, o[0], o[1], x.shape[1])
-    return _Heads(x.data_ptr(), out.data_ptr(), i[0], i[1], i[2], o[0], o[1], o[2], x.shape[2])
-
-
-def _turn(q, k, freqs, positions, interleaved, scale, back):
-    outs = []
-    for x in (q, k):
-        outs.append(None if x is None else torch.empty_like(x))
-    like = q if q is not None else k
-    batch, seq = (1, like.shape[0]) if like.dim() == 3 else like.shape[:2]
-    if batch and seq:
-        device = like.get_device()
-        at, wide, pb, ps, first = None, 0, 0, 0, 0
-        if isinstance(positions, torch.Tensor):
-            at, wide = positions.data_ptr(), positions.dtype is torch.int64
-            pb, ps = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-        else:
-            first = positions
-        _done(lib().dccl_rotary(device, dtype_of(like), batch, seq, like.shape[-1], freqs.shape[0], interleaved, back, ctypes.byref(_heads(q, outs[0])),
-                                ctypes.byref(_heads(k, outs[1])), freqs.data_ptr(), at, wide, pb, ps, first, scale, current_stream_handle(device)), "rotary")
-    return outs
-
-
-def _dense_head(x):
-    return x if x is None or x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, freqs, positions, interleaved, scale):
-        tensor = isinstance(positions, torch.Tensor)
-        ctx.save_for_backward(freqs, positions if tensor else None)
-        ctx.first, ctx.interleaved, ctx.scale = None if tensor else positions, interleaved, scale
-        ctx.set_materialize_grads(False)
-        q, k = _turn(q, k, freqs, positions, interleaved, scale, 0)
-        return q if k is None else (q, k)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk=None):
-        freqs, positions = ctx.saved_tensors
-        dq, dk = (None if not need else _dense_head(g) for g, need in zip((dq, dk), ctx.needs_input_grad))
-        if dq is not None or dk is not None:
-            dq, dk = _turn(dq, dk, freqs, ctx.first if positions is None else positions, ctx.interleaved, ctx.scale, 1)
-        return dq, dk, None, None, None, None
-
-
 def _turn_on_cpu(x, cos, sin, interleaved):
     pairs = cos.shape[-1]
     v, rest = x[..., :2 * pairs].float(), x[..., 2 * pairs:]
@@ -302,6 +175,10 @@ def rotary(q, k, freqs, positions=None, interleaved=False, scale=1.0):
     positions: None (0, 1, ...), the first position of every sequence as an integer, or an int32 or int64 tensor [seq] or [batch, seq].
     interleaved: pair j is (2j, 2j + 1) and not (j, pairs + j).
     scale: factor of the turned elements, as stretched contexts use it."""
+    if isinstance(q, torch.Tensor) and q.is_cuda:
+        out = _ext().rotary(q, k, freqs, 0 if positions is None else positions, interleaved, scale)
+        if out is not NotImplemented:
+            return out
     _check_activations("rotary", "q", q, (3, 4))
     dim = q.shape[-1]
     if k is not None:
@@ -332,13 +209,10 @@ def rotary(q, k, freqs, positions=None, interleaved=False, scale=1.0):
         cos, sin = (angle.cos() * scale).float(), (angle.sin() * scale).float()
         q = _turn_on_cpu(q, cos, sin, interleaved)
         return q if k is None else (q, _turn_on_cpu(k, cos, sin, interleaved))
-    if (q.shape[-2] + (0 if k is None else k.shape[-2])) * dim > 1 << 24:
-        raise ValueError("rotary: a token has more than 2^24 elements")
-    q, k, freqs = _dense_head(q), _dense_head(k), freqs.contiguous()
-    if _records(q, k):
-        return _Rotary.apply(q, k, freqs, positions, interleaved, scale)
-    q, k = _turn(q, k, freqs, positions, interleaved, scale, 0)
-    return q if k is None else (q, k)
+    if (q.shape[-2] + (0 if k is None else k.shape[-2])) * dim > 1 << 24 or seq >= 1 << 31:
+        raise ValueError("rotary: a token has more than 2^24 elements, or a sequence 2^31 tokens")
+    out = _ext().rotary(q, k, freqs, positions, interleaved, scale)
+    return out if out is not NotImplemented else _refuse("rotary")
 
 
 def rotary_frequencies(rotary_dim, theta=10000.0, scaling=None, factor=1.0, original_length=None, slow=1.0, fast=None, device=None):
@@ -390,60 +264,6 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling=None, factor=1.0, orig
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}        # csrc/kernels/decoder_ops.hpp
 
 
-def _gated_work(x, w_gate, w_up, backward):
-    """(workspace or None, its bytes) of a call."""
-    aligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
-    size = lib().dccl_gated_linear_workspace(x.get_device(), x.numel() // x.shape[-1], x.shape[-1], w_gate.shape[0], aligned, backward)
-    _done(-1 if size < 0 else 0, "gated_linear")
-    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
-
-
-def _gated_forward(x, w_gate, w_up, act, keep):
-    """(h, g, u): g and u are the two products in fp32, in rows of a multiple of four elements, or None unless `keep`."""
-    width, ffn = x.shape[-1], w_gate.shape[0]
-    tokens = x.numel() // width
-    h = torch.empty(x.shape[:-1] + (ffn,), dtype=x.dtype, device=x.device)
-    g = u = None
-    stride = -(-ffn // 4) * 4
-    if keep:
-        g, u = (torch.empty(tokens, stride, dtype=torch.float32, device=x.device) for _ in range(2))
-    if tokens:
-        device = x.get_device()
-        work, size = _gated_work(x, w_gate, w_up, False)
-        _done(lib().dccl_gated_linear(device, dtype_of(x), tokens, width, ffn, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), act, h.data_ptr(), _ptr(g), _ptr(u), stride,
-                                      _ptr(work), size, current_stream_handle(device)), "gated_linear")
-    return h, g, u
-
-
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, act):
-        h, g, u = _gated_forward(x, w_gate, w_up, act, True)
-        ctx.act = act
-        ctx.save_for_backward(x, w_gate, w_up, g, u)
-        return h
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh):
-        x, w_gate, w_up, g, u = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dh = dh.contiguous()
-        dx = torch.empty_like(x) if need[0] else None
-        dw_gate, dw_up = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need[1] or need[2] else (None, None)
-        width, ffn = x.shape[-1], w_gate.shape[0]
-        tokens = x.numel() // width
-        if tokens:
-            device = x.get_device()
-            work, size = _gated_work(x, w_gate, w_up, True)
-            _done(lib().dccl_gated_linear_backward(device, dtype_of(x), tokens, width, ffn, dh.data_ptr(), g.data_ptr(), u.data_ptr(), g.shape[1], x.data_ptr(), w_gate.data_ptr(),
-                                                   w_up.data_ptr(), ctx.act, _ptr(dx), _ptr(dw_gate), _ptr(dw_up), _ptr(work), size, current_stream_handle(device)),
-                  "gated_linear backward")
-        elif dw_gate is not None:
-            dw_gate.zero_(), dw_up.zero_()
-        return dx, dw_gate if need[1] else None, dw_up if need[2] else None, None
-
-
 def _activate_on_cpu(g, activation):
     if activation == "silu":
         return torch.nn.functional.silu(g)
@@ -456,6 +276,10 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
 
     On the GPU x is float16 or bfloat16. For the backward pass the call keeps the two products in fp32 (8 bytes per element of the result):
     from 16 bits their rounding would come on top of the one that their gradients need to be multiplied again."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(activation, str):
+        h = _ext().gated_linear(x, w_gate, w_up, _ACTIVATIONS.get(activation, -1))
+        if h is not NotImplemented:
+            return h
     _check_activations("gated_linear", "x", x, range(1, 65))
     width = x.shape[-1]
     if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 2:
@@ -465,7 +289,7 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
         _check_like("gated_linear", name, w, (ffn, width), (x.dtype,), x.device)
     if not width or not ffn:
         raise ValueError("gated_linear: weights of shape %s" % ((ffn, width),))
-    if activation not in _ACTIVATIONS:
+    if not isinstance(activation, str) or activation not in _ACTIVATIONS:
         raise ValueError("gated_linear: activation %r is none of %s" % (activation, ", ".join(_ACTIVATIONS)))
     if not x.is_cuda:
         v = x.float()
@@ -474,8 +298,4 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
         raise TypeError("gated_linear: float32 is taken on the CPU only; the tensor cores multiply float16 and bfloat16")
     if max(x.numel() // width, width, ffn) >= 1 << 30:
         raise ValueError("gated_linear: a dimension of 2^30 or more")
-    act = _ACTIVATIONS[activation]
-    x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
-    if _records(x, w_gate, w_up):
-        return _GatedLinear.apply(x, w_gate, w_up, act)
-    return _gated_forward(x, w_gate, w_up, act, False)[0]
+    _refuse("gated_linear")
