@@ -22,7 +22,7 @@ int dccl_residual_norm(int device, int dtype, size_t rows, size_t width, const v
                        void* stream);
 
 /** Bytes of workspace that the backward pass of `gates` rows of gates (0: without a gate) takes; 0 after an error. full: with a branch. */
-size_t dccl_residual_norm_workspace(int device, size_t rows, size_t width, size_t gates, int has_post, int full);
+size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t width, size_t gates, int has_post, int full);
 
 /**
  * Gradients of dccl_residual_norm: from dy and dn (either may be null) those of x and branch, and in the vectors' own types those of

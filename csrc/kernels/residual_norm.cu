@@ -43,67 +43,71 @@ struct NormGradArgs {
     float scale;
 };
 
+/** What a call has. The kernels are compiled for each: tests of pointers inside of the loops took a third of their instructions. */
+enum { BRANCH = 1, POST = 2, GATE = 4, SCALE = 8 };
+
 /** E elements per thread in runs of V, run k of thread t at (k * threads + t) * V. */
-template <typename T, int V, int E>
-__global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, 1) k_residual_norm(const __grid_constant__ NormArgs a) {
+template <typename T, int V, int E, int F>
+__global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ? 2 : 1) k_residual_norm(const __grid_constant__ NormArgs a) {
     wait_for_stream();
     constexpr int K = E / V;
-    __shared__ float parts[2][32];
+    __shared__ __align__(16) float parts[2][32];
     const unsigned runs = a.width / V, step = blockDim.x, t = threadIdx.x;
     const size_t row = blockIdx.x, at = row * a.width;
     const T *x = reinterpret_cast<const T*>(a.x) + at, *b = reinterpret_cast<const T*>(a.branch) + at;
-    const bool has_branch = a.branch != nullptr;
-    Run<T, V> xr[K], br[K];
+    Run<T, V> xr[K], br[F & BRANCH ? K : 1];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const unsigned i = t + k * step;
         if (i < runs) {
             xr[k] = ld_run<T, V>(x + (size_t)i * V);
-            if (has_branch) br[k] = ld_run<T, V>(b + (size_t)i * V);
+            if constexpr (F & BRANCH) br[k] = ld_run<T, V>(b + (size_t)i * V);
         }
     }
     float factor = a.scale;
-    if (a.post) {
+    if constexpr (F & POST) {
         float sum = 0;
 #pragma unroll
         for (int k = 0; k < K; k++)
             if (t + k * step < runs)
 #pragma unroll
                 for (int e = 0; e < V; e++) { const float v = Traits<T>::up(br[k].e[e]); sum = fmaf(v, v, sum); }
-        const float rb = rsqrtf(cta_sum(sum, parts[0]) / a.width + a.eps);
-        if (a.rstd_post && t == 0) a.rstd_post[row] = rb;
-        factor = rb;
+        factor = rsqrtf(cta_sum(sum, parts[0]) / a.width + a.eps);
+        if (a.rstd_post && t == 0) a.rstd_post[row] = factor;
+        factor *= a.scale;
     }
     float y[E], sum = 0;
-    const size_t gate_at = a.gate ? row / a.rows_per_gate * a.width : 0;
+    const size_t gate_at = F & GATE ? row / a.rows_per_gate * a.width : 0;
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const unsigned i = t + k * step;
         if (i >= runs) continue;
         float v[V];
 #pragma unroll
-        for (int e = 0; e < V; e++) v[e] = has_branch ? factor * Traits<T>::up(br[k].e[e]) : 0.0f;
-        if (a.post) {
-            float w[V];
-            ld_vector<T, V>(w, a.post, a.f32 & DCCL_NORM_POST_F32, (size_t)i * V);
+        for (int e = 0; e < V; e++) v[e] = Traits<T>::up(xr[k].e[e]);
+        if constexpr (F & BRANCH) {
+            float p[V], w[V];
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] *= w[e] * a.scale;
-        }
-        if (a.gate) {
-            float g[V];
-            ld_vector<T, V>(g, a.gate, a.f32 & DCCL_NORM_GATE_F32, gate_at + (size_t)i * V);
+            for (int e = 0; e < V; e++) p[e] = Traits<T>::up(br[k].e[e]);
+            if constexpr (F & POST) {
+                ld_vector<T, V>(w, a.post, a.f32 & DCCL_NORM_POST_F32, (size_t)i * V);
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] *= g[e];
+                for (int e = 0; e < V; e++) p[e] *= w[e];
+            }
+            if constexpr (F & GATE) {
+                ld_vector<T, V>(w, a.gate, a.f32 & DCCL_NORM_GATE_F32, gate_at + (size_t)i * V);
+#pragma unroll
+                for (int e = 0; e < V; e++) p[e] *= w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = F & (POST | SCALE) ? fmaf(factor, p[e], v[e]) : v[e] + p[e];
+            st_run<T, V>(reinterpret_cast<T*>(a.y) + at + (size_t)i * V, round_run<T, V>(v));
         }
-        Run<T, V> out;
 #pragma unroll
         for (int e = 0; e < V; e++) {
-            const float s = has_branch ? Traits<T>::up(xr[k].e[e]) + v[e] : Traits<T>::up(xr[k].e[e]);
-            y[k * V + e] = s;
-            sum = fmaf(s, s, sum);
-            out.e[e] = Traits<T>::down(s);
+            y[k * V + e] = v[e];
+            sum = fmaf(v[e], v[e], sum);
         }
-        if (has_branch) st_run<T, V>(reinterpret_cast<T*>(a.y) + at + (size_t)i * V, out);
     }
     const float ry = rsqrtf(cta_sum(sum, parts[1]) / a.width + a.eps);
     if (a.rstd && t == 0) a.rstd[row] = ry;
@@ -113,38 +117,42 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, 1) k_resi
         if (i >= runs) continue;
         float w[V];
         ld_vector<T, V>(w, a.weight, a.f32 & DCCL_NORM_WEIGHT_F32, (size_t)i * V);
-        Run<T, V> out;
 #pragma unroll
-        for (int e = 0; e < V; e++) out.e[e] = Traits<T>::down(y[k * V + e] * ry * w[e]);
-        st_run<T, V>(reinterpret_cast<T*>(a.n) + at + (size_t)i * V, out);
+        for (int e = 0; e < V; e++) w[e] *= y[k * V + e] * ry;
+        st_run<T, V>(reinterpret_cast<T*>(a.n) + at + (size_t)i * V, round_run<T, V>(w));
     }
 }
 
-/** The arrays that a row of the backward pass reads. SUM: y = x + branch (or x), taken as it was stored. FULL: with post, a gate or a
- *  scale the branch is read in any case, and y comes from x and branch again, exact. */
-enum NormForm { SUM, FULL };
-enum { DN, Y, DY, B };      // Y: x in the FULL form
+/** The arrays that a row of the backward pass reads. Y is the y = x + branch (or x) that was stored; with post, a gate or a scale (FULL) the
+ *  branch is read in any case, Y is x, and y comes from both again, exact. */
+enum { DN, Y, DY, B };
+enum { IN_WEIGHT, IN_POST, IN_GATE };   // the vectors, in shared memory as fp32
+constexpr int FULL = POST | GATE | SCALE;
 
-constexpr int kNormStages = 3;
-/** Whether three rows fit into shared memory: 16-bit rows of up to 8192 elements, fp32 rows of up to 2048. */
-template <typename T, int V, int E> constexpr bool kNormStaged = V * sizeof(T) == 16 && E * sizeof(T) <= 32;
+/** Rows in shared memory at a time, where accesses are 16 bytes wide: three of up to 2048 elements, two of up to 8192 16-bit ones. */
+template <typename T, int V, int E> constexpr int kNormStages = V * sizeof(T) != 16 ? 0 : E == 8 ? 3 : E == 16 && sizeof(T) == 2 ? 2 : 0;
+
+template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(unsigned threads) {
+    return (size_t)threads * E * (kNormStages<T, V, E> * (F & FULL ? 4 : 3) * sizeof(T) + (E <= 16 ? (F & FULL ? 3 : 1) * sizeof(float) : 0));
+}
 
 /**
  * Each CTA takes units of rows that share a row of the gate and keeps the columns' sums (dw, dw2, dg) in registers: dg leaves at
  * the end of a unit, dw and dw2 at the end of the CTA, for k_norm_columns to add. Where accesses are 16 bytes wide a thread copies
- * its own elements of the next two rows into shared memory of its own while it works on this one: no register holds them and
- * no barrier guards them.
+ * its own elements of the next rows into shared memory of its own while it works on this one, and it keeps its part of the vectors
+ * there in fp32: no register holds them and no barrier guards them.
  */
-template <typename T, int V, int E, NormForm F>
-__global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? (F == SUM ? 4 : 3) : 1) k_residual_norm_grad(const __grid_constant__ NormGradArgs a) {
+template <typename T, int V, int E, int F>
+__global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? (F & FULL ? 3 : 4) : 1) k_residual_norm_grad(const __grid_constant__ NormGradArgs a) {
     wait_for_stream();
-    constexpr int K = E / V, kArrays = F == SUM ? 3 : 4;
-    constexpr bool kStaged = kNormStaged<T, V, E>;
-    extern __shared__ uint4 staged[];                   // [stage][array][run][thread]
-    __shared__ float parts[2][2][32];
+    constexpr int K = E / V, kArrays = F & FULL ? 4 : 3, kStages = kNormStages<T, V, E>, kPiece = V < 4 ? V : 4;
+    constexpr bool kVectors = E <= 16;                  // in shared memory
+    extern __shared__ uint4 staged[];                   // [stage][array][run][thread], then [vector][run][piece][thread] of kPiece floats
+    __shared__ __align__(16) float parts[2][2][32];
     const unsigned runs = a.width / V, step = blockDim.x, t = threadIdx.x;
     const float inv_width = 1.0f / a.width;
     const T* const arrays[4] = {reinterpret_cast<const T*>(a.dn), reinterpret_cast<const T*>(a.y), reinterpret_cast<const T*>(a.dy), reinterpret_cast<const T*>(a.branch)};
+    Run<float, kPiece>* const vectors = reinterpret_cast<Run<float, kPiece>*>(staged + (size_t)kStages * kArrays * K * step);
     const auto fetch = [&](size_t row, unsigned stage) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -159,37 +167,77 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
     };
     const auto load = [&](int j, int k, size_t row, unsigned stage, float (&f)[V]) {
         Run<T, V> r;
-        if constexpr (kStaged) r = *reinterpret_cast<const Run<T, V>*>(staged + ((stage * kArrays + j) * K + k) * step + t);
+        if constexpr (kStages > 0) r = *reinterpret_cast<const Run<T, V>*>(staged + ((stage * kArrays + j) * K + k) * step + t);
         else r = ld_run<T, V>(arrays[j] + row * a.width + (size_t)(t + k * step) * V);
 #pragma unroll
         for (int e = 0; e < V; e++) f[e] = Traits<T>::up(r.e[e]);
     };
-    float sum_w[E], sum_p[F == FULL ? E : 1], sum_g[F == FULL ? E : 1];
+    const auto keep_vector = [&](int which, const void* from, int flag, size_t at) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const unsigned i = t + k * step;
+            if (i >= runs) continue;
+            float f[V];
+            ld_vector<T, V>(f, from, a.f32 & flag, at + (size_t)i * V);
+#pragma unroll
+            for (int q = 0; q < V / kPiece; q++) {
+                Run<float, kPiece> piece;
+#pragma unroll
+                for (int e = 0; e < kPiece; e++) piece.e[e] = f[q * kPiece + e];
+                vectors[((which * K + k) * (V / kPiece) + q) * step + t] = piece;
+            }
+        }
+    };
+    const auto vector = [&](int which, const void* from, int flag, size_t at, int k, float (&f)[V]) {
+        if constexpr (kVectors) {
+#pragma unroll
+            for (int q = 0; q < V / kPiece; q++) {
+                const Run<float, kPiece> piece = vectors[((which * K + k) * (V / kPiece) + q) * step + t];
+#pragma unroll
+                for (int e = 0; e < kPiece; e++) f[q * kPiece + e] = piece.e[e];
+            }
+        } else {
+            ld_vector<T, V>(f, from, a.f32 & flag, at + (size_t)(t + k * step) * V);
+        }
+    };
+    if constexpr (kVectors) {
+        keep_vector(IN_WEIGHT, a.weight, DCCL_NORM_WEIGHT_F32, 0);
+        if constexpr (F & POST) keep_vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0);
+    }
+    float sum_w[E], sum_p[F & POST ? E : 1], sum_g[F & GATE ? E : 1];
 #pragma unroll
     for (int e = 0; e < E; e++) {
         sum_w[e] = 0;
-        if constexpr (F == FULL) sum_p[e] = sum_g[e] = 0;
+        if constexpr (F & POST) sum_p[e] = 0;
+        if constexpr (F & GATE) sum_g[e] = 0;
     }
     unsigned turn = 0;
     for (size_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        const size_t gate = unit / a.chunks, chunk = unit % a.chunks;
+        const size_t gate = unit / a.chunks, chunk = unit % a.chunks, gate_at = gate * a.width;
         const size_t begin = gate * a.rows_per_gate + chunk * a.rows_per_gate / a.chunks, end = gate * a.rows_per_gate + (chunk + 1) * a.rows_per_gate / a.chunks;
         unsigned stage = 0;
-        if constexpr (kStaged) {
+        if constexpr (kStages > 0) {
 #pragma unroll
-            for (int s = 0; s < kNormStages - 1; s++) {
+            for (int s = 0; s < kStages - 1; s++) {
                 if (begin + s < end) fetch(begin + s, s);
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
         }
+        if constexpr ((F & GATE) && kVectors) keep_vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at);
+        float next_ry = a.dn && begin < end ? a.rstd[begin] : 0.0f, next_rb = 1.0f;
+        if constexpr (F & POST) next_rb = begin < end ? a.rstd_post[begin] : 0.0f;
         for (size_t row = begin; row < end; row++, turn ^= 1) {
-            if constexpr (kStaged) {
-                const unsigned ahead = stage == 0 ? kNormStages - 1 : stage - 1;
-                if (row + kNormStages - 1 < end) fetch(row + kNormStages - 1, ahead);
+            if constexpr (kStages > 0) {
+                const unsigned ahead = stage == 0 ? kStages - 1 : stage - 1;
+                if (row + kStages - 1 < end) fetch(row + kStages - 1, ahead);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                asm volatile("cp.async.wait_group %0;" ::"n"(kNormStages - 1) : "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             }
-            const float ry = a.dn ? a.rstd[row] : 0.0f, rb = F == FULL && a.post ? a.rstd_post[row] : 1.0f;
+            const float ry = next_ry, rb = next_rb;
+            if (row + 1 < end) {
+                next_ry = a.dn ? a.rstd[row + 1] : 0.0f;
+                if constexpr (F & POST) next_rb = a.rstd_post[row + 1];
+            }
             float d[E], yh[E], dot = 0;
             if (a.dn) {
 #pragma unroll
@@ -199,25 +247,23 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     float w[V], dn[V], y[V];
                     load(DN, k, row, stage, dn);
                     load(Y, k, row, stage, y);
-                    if constexpr (F == FULL) {
-                        float v[V], b[V];
-                        load(B, k, row, stage, b);
+                    if constexpr (F & FULL) {
+                        float p[V];
+                        load(B, k, row, stage, p);
+                        if constexpr (F & POST) {
+                            vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0, k, w);
 #pragma unroll
-                        for (int e = 0; e < V; e++) v[e] = (a.post ? rb : a.scale) * b[e];      // as the forward pass rounds
-                        if (a.post) {
-                            ld_vector<T, V>(w, a.post, a.f32 & DCCL_NORM_POST_F32, (size_t)i * V);
-#pragma unroll
-                            for (int e = 0; e < V; e++) v[e] *= w[e] * a.scale;
+                            for (int e = 0; e < V; e++) p[e] *= w[e];
                         }
-                        if (a.gate) {
-                            ld_vector<T, V>(w, a.gate, a.f32 & DCCL_NORM_GATE_F32, gate * a.width + (size_t)i * V);
+                        if constexpr (F & GATE) {
+                            vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at, k, w);
 #pragma unroll
-                            for (int e = 0; e < V; e++) v[e] *= w[e];
+                            for (int e = 0; e < V; e++) p[e] *= w[e];
                         }
 #pragma unroll
-                        for (int e = 0; e < V; e++) y[e] += v[e];
+                        for (int e = 0; e < V; e++) y[e] = fmaf(F & POST ? rb * a.scale : a.scale, p[e], y[e]);      // as the forward pass rounds
                     }
-                    ld_vector<T, V>(w, a.weight, a.f32 & DCCL_NORM_WEIGHT_F32, (size_t)i * V);
+                    vector(IN_WEIGHT, a.weight, DCCL_NORM_WEIGHT_F32, 0, k, w);
 #pragma unroll
                     for (int e = 0; e < V; e++) {
                         const int j = k * V + e;
@@ -239,58 +285,54 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                 if (i >= runs) continue;
                 float dy[V];
                 if (a.dy) load(DY, k, row, stage, dy);
-                Run<T, V> dx, db;
+                float out[V];
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     const int j = k * V + e;
                     d[j] = fmaf(ry, d[j] - yh[j] * c, a.dy ? dy[e] : 0.0f);
-                    dx.e[e] = Traits<T>::down(d[j]);
+                    out[e] = d[j];
                 }
-                st_run<T, V>(reinterpret_cast<T*>(a.dx) + row * a.width + (size_t)i * V, dx);
-                if constexpr (F == FULL) {
+                st_run<T, V>(reinterpret_cast<T*>(a.dx) + row * a.width + (size_t)i * V, round_run<T, V>(out));
+                if constexpr (F & FULL) {
                     float w2[V], g[V], b[V];
                     load(B, k, row, stage, b);
-                    if (a.post) ld_vector<T, V>(w2, a.post, a.f32 & DCCL_NORM_POST_F32, (size_t)i * V);
-                    if (a.gate) ld_vector<T, V>(g, a.gate, a.f32 & DCCL_NORM_GATE_F32, gate * a.width + (size_t)i * V);
+                    if constexpr (F & POST) vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0, k, w2);
+                    if constexpr (F & GATE) vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at, k, g);
 #pragma unroll
                     for (int e = 0; e < V; e++) {
                         const int j = k * V + e;
                         float v = d[j] * a.scale;
-                        const float bh = b[e] * rb;
-                        if (a.gate) {
-                            sum_g[j] = fmaf(v, a.post ? bh * w2[e] : bh, sum_g[j]);
+                        const float bh = F & POST ? b[e] * rb : b[e];
+                        if constexpr (F & GATE) {
+                            sum_g[j] = fmaf(v, F & POST ? bh * w2[e] : bh, sum_g[j]);
                             v *= g[e];
                         }
-                        if (a.post) {
+                        if constexpr (F & POST) {
                             sum_p[j] = fmaf(v, bh, sum_p[j]);
                             v *= w2[e];
                             dot_b = fmaf(v, bh, dot_b);
                         }
-                        d[j] = v;
-                        db.e[e] = Traits<T>::down(v);
+                        d[j] = out[e] = v;
                     }
-                    if (!a.post) st_run<T, V>(reinterpret_cast<T*>(a.dbranch) + row * a.width + (size_t)i * V, db);
+                    if constexpr (!(F & POST)) st_run<T, V>(reinterpret_cast<T*>(a.dbranch) + row * a.width + (size_t)i * V, round_run<T, V>(out));
                 }
             }
-            if constexpr (F == FULL) {
-                if (a.post) {
-                    const float cb = cta_sum(dot_b, parts[turn][1]) * inv_width;
+            if constexpr (F & POST) {
+                const float cb = cta_sum(dot_b, parts[turn][1]) * inv_width * rb;
 #pragma unroll
-                    for (int k = 0; k < K; k++) {
-                        const unsigned i = t + k * step;
-                        if (i >= runs) continue;
-                        float b[V];
-                        load(B, k, row, stage, b);
-                        Run<T, V> db;
+                for (int k = 0; k < K; k++) {
+                    const unsigned i = t + k * step;
+                    if (i >= runs) continue;
+                    float b[V];
+                    load(B, k, row, stage, b);
 #pragma unroll
-                        for (int e = 0; e < V; e++) db.e[e] = Traits<T>::down(rb * (d[k * V + e] - b[e] * rb * cb));
-                        st_run<T, V>(reinterpret_cast<T*>(a.dbranch) + row * a.width + (size_t)i * V, db);
-                    }
+                    for (int e = 0; e < V; e++) b[e] = rb * (d[k * V + e] - b[e] * cb);
+                    st_run<T, V>(reinterpret_cast<T*>(a.dbranch) + row * a.width + (size_t)i * V, round_run<T, V>(b));
                 }
             }
-            stage = stage == kNormStages - 1 ? 0 : stage + 1;
+            if constexpr (kStages > 0) stage = stage == kStages - 1 ? 0 : stage + 1;
         }
-        if constexpr (F == FULL) {
+        if constexpr (F & GATE) {
             if (a.gate_sums) {
 #pragma unroll
                 for (int k = 0; k < K; k++)
@@ -310,7 +352,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
             for (int e = 0; e < V; e++) {
                 const size_t j = (size_t)blockIdx.x * a.width + (size_t)(t + k * step) * V + e;
                 if (a.weight_sums) a.weight_sums[j] = sum_w[k * V + e];
-                if constexpr (F == FULL)
+                if constexpr (F & POST)
                     if (a.post_sums) a.post_sums[j] = sum_p[k * V + e];
             }
 }
@@ -322,14 +364,14 @@ struct NormColumnArgs {
     int f32;
 };
 
-constexpr int kColumnSlices = 16;
+constexpr int kColumnSlices = 32;
 
 template <typename T> __device__ __forceinline__ void st_vector(void* p, bool f32, size_t i, float v) {
     if (f32) reinterpret_cast<float*>(p)[i] = v;
     else reinterpret_cast<T*>(p)[i] = Traits<T>::down(v);
 }
 
-/** Adds up what the CTAs left: 32 columns per CTA, 16 threads per column. The first blocks take the weight, then post, then each row of the gate. */
+/** Adds up what the CTAs left: 32 columns per CTA, 32 threads per column. The first blocks take the weight, then post, then each row of the gate. */
 template <typename T> __global__ void __launch_bounds__(32 * kColumnSlices) k_norm_columns(const __grid_constant__ NormColumnArgs a) {
     wait_for_stream();
     __shared__ float parts[kColumnSlices][33];
@@ -341,6 +383,7 @@ template <typename T> __global__ void __launch_bounds__(32 * kColumnSlices) k_no
     const unsigned n = is_weight || is_post ? a.ctas : a.chunks;
     float sum = 0;
     if (column < a.width)
+#pragma unroll 8
         for (unsigned i = slice; i < n; i += kColumnSlices) sum += from[(size_t)i * a.width + column];
     parts[slice][lane] = sum;
     __syncthreads();
@@ -361,18 +404,24 @@ static NormShape norm_shape(size_t width) {
     return {e, (int)((width + e * 32 - 1) / (e * 32)) * 32};
 }
 
-/** Elements per access: 16 bytes, else a pair of 16-bit elements, else one. */
-static int norm_run(int dtype, size_t width, bool aligned16_all, bool aligned8_all) {
+/** Elements per access: 16 bytes, else one. */
+static int norm_run(int dtype, size_t width, bool aligned) {
     const int wide = dtype == 7 ? 4 : 8;
-    if (width % wide == 0 && aligned16_all) return wide;
-    return dtype != 7 && width % 2 == 0 && aligned8_all ? 2 : 1;
+    return width % wide == 0 && aligned ? wide : 1;
 }
 
 /** CTAs of the backward pass, all resident at once, and how the rows of a gate are cut among them. */
 struct NormCut { size_t chunks, units; unsigned ctas; };
-static NormCut norm_cut(int device, size_t rows, size_t width, size_t gates, bool full) {
+static NormCut norm_cut(int device, int dtype, size_t rows, size_t width, size_t gates, bool full) {
     const NormShape s = norm_shape(width);
-    const size_t per_sm = s.elements == 8 ? (full ? 768 : 1024) / s.threads : s.elements == 16 ? 512 / s.threads : 1;
+    const bool wide = dtype == 7;
+    const size_t shared = s.elements == 8    ? (full ? wide ? norm_grad_shared<float, 4, 8, FULL>(s.threads) : norm_grad_shared<__half, 8, 8, FULL>(s.threads)
+                                                     : wide ? norm_grad_shared<float, 4, 8, 0>(s.threads) : norm_grad_shared<__half, 8, 8, 0>(s.threads))
+                          : s.elements == 16 ? (full ? wide ? norm_grad_shared<float, 4, 16, FULL>(s.threads) : norm_grad_shared<__half, 8, 16, FULL>(s.threads)
+                                                     : wide ? norm_grad_shared<float, 4, 16, 0>(s.threads) : norm_grad_shared<__half, 8, 16, 0>(s.threads))
+                                             : 0;
+    size_t per_sm = s.elements == 8 ? (full ? 768 : 1024) / s.threads : s.elements == 16 ? 512 / s.threads : 1;      // by registers
+    if (per_sm * (shared + 1536) > 227 * 1024) per_sm = 227 * 1024 / (shared + 1536);
     const size_t want = (size_t)sm_count(device) * (per_sm ? per_sm : 1);
     if (!want) return {0, 0, 0};
     const size_t groups = gates ? gates : 1, rows_per = rows / groups;
@@ -382,11 +431,11 @@ static NormCut norm_cut(int device, size_t rows, size_t width, size_t gates, boo
     return {chunks, units, (unsigned)(units < want ? units : want)};
 }
 
-template <typename T, int V, int E> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormArgs& a, bool, int) {
-    return launch_early(k_residual_norm<T, V, E>, grid, block, stream, a);
+template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormArgs& a, int) {
+    return launch_early(k_residual_norm<T, V, E, F>, grid, block, stream, a);
 }
-template <typename T, int V, int E, NormForm F> static cudaError_t norm_grad_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, int device) {
-    const size_t shared = kNormStaged<T, V, E> ? (size_t)kNormStages * (F == SUM ? 3 : 4) * E * sizeof(T) * block : 0;
+template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, int device) {
+    const size_t shared = norm_grad_shared<T, V, E, F>(block);
     if (shared > 40 << 10) {        // 48 KB with the static part need no leave
         static std::atomic<bool> ready[64];
         if (!ready[device].load(std::memory_order_relaxed)) {
@@ -397,24 +446,37 @@ template <typename T, int V, int E, NormForm F> static cudaError_t norm_grad_lau
     }
     return launch_early_shared(k_residual_norm_grad<T, V, E, F>, grid, block, shared, stream, a);
 }
-template <typename T, int V, int E> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, bool full, int device) {
-    return full ? norm_grad_launch<T, V, E, FULL>(grid, block, stream, a, device) : norm_grad_launch<T, V, E, SUM>(grid, block, stream, a, device);
+template <typename T, int V, int E, typename Args> static cudaError_t norm_form(int form, unsigned grid, unsigned block, cudaStream_t stream, const Args& a, int device) {
+    switch (form) {
+        case BRANCH:
+            if constexpr (std::is_same<Args, NormArgs>::value) return norm_launch<T, V, E, BRANCH>(grid, block, stream, a, device);
+            return cudaErrorInvalidValue;
+        case BRANCH | SCALE: return norm_launch<T, V, E, BRANCH | SCALE>(grid, block, stream, a, device);
+        case BRANCH | POST: return norm_launch<T, V, E, BRANCH | POST>(grid, block, stream, a, device);
+        case BRANCH | GATE | SCALE: return norm_launch<T, V, E, BRANCH | GATE | SCALE>(grid, block, stream, a, device);
+        case BRANCH | POST | GATE: return norm_launch<T, V, E, BRANCH | POST | GATE>(grid, block, stream, a, device);
+        default: return norm_launch<T, V, E, 0>(grid, block, stream, a, device);
+    }
 }
-template <typename T, int V, typename Args> static cudaError_t norm_launch(int elements, unsigned grid, unsigned block, cudaStream_t stream, const Args& a, bool full, int device) {
-    return elements == 8 ? norm_launch<T, V, 8>(grid, block, stream, a, full, device) : elements == 16 ? norm_launch<T, V, 16>(grid, block, stream, a, full, device)
-                                                                                                       : norm_launch<T, V, 32>(grid, block, stream, a, full, device);
+/** BRANCH, POST, GATE and SCALE of a call; post takes the scale in. */
+static int norm_form_of(const void* branch, const void* post, const void* gate, double scale) {
+    if (!branch) return 0;
+    return BRANCH | (post ? POST : 0) | (gate ? GATE : 0) | (!post && (gate || scale != 1.0) ? SCALE : 0);
 }
 
-template <typename Args> static cudaError_t norm_dispatch(int device, int dtype, int run, int elements, unsigned grid, unsigned block, cudaStream_t stream, const Args& a, bool full) {
+template <typename T, int V, typename Args> static cudaError_t norm_elements(int elements, int form, unsigned grid, unsigned block, cudaStream_t stream, const Args& a, int device) {
+    return elements == 8 ? norm_form<T, V, 8>(form, grid, block, stream, a, device) : elements == 16 ? norm_form<T, V, 16>(form, grid, block, stream, a, device)
+                                                                                                     : norm_form<T, V, 32>(form, grid, block, stream, a, device);
+}
+
+template <typename Args> static cudaError_t norm_dispatch(int device, int dtype, int run, int elements, int form, unsigned grid, unsigned block, cudaStream_t stream, const Args& a) {
     switch (dtype * 16 + run) {
-        case 6 * 16 + 8: return norm_launch<__half, 8>(elements, grid, block, stream, a, full, device);
-        case 6 * 16 + 2: return norm_launch<__half, 2>(elements, grid, block, stream, a, full, device);
-        case 6 * 16 + 1: return norm_launch<__half, 1>(elements, grid, block, stream, a, full, device);
-        case 9 * 16 + 8: return norm_launch<__nv_bfloat16, 8>(elements, grid, block, stream, a, full, device);
-        case 9 * 16 + 2: return norm_launch<__nv_bfloat16, 2>(elements, grid, block, stream, a, full, device);
-        case 9 * 16 + 1: return norm_launch<__nv_bfloat16, 1>(elements, grid, block, stream, a, full, device);
-        case 7 * 16 + 4: return norm_launch<float, 4>(elements, grid, block, stream, a, full, device);
-        case 7 * 16 + 1: return norm_launch<float, 1>(elements, grid, block, stream, a, full, device);
+        case 6 * 16 + 8: return norm_elements<__half, 8>(elements, form, grid, block, stream, a, device);
+        case 6 * 16 + 1: return norm_elements<__half, 1>(elements, form, grid, block, stream, a, device);
+        case 9 * 16 + 8: return norm_elements<__nv_bfloat16, 8>(elements, form, grid, block, stream, a, device);
+        case 9 * 16 + 1: return norm_elements<__nv_bfloat16, 1>(elements, form, grid, block, stream, a, device);
+        case 7 * 16 + 4: return norm_elements<float, 4>(elements, form, grid, block, stream, a, device);
+        case 7 * 16 + 1: return norm_elements<float, 1>(elements, form, grid, block, stream, a, device);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -434,13 +496,13 @@ extern "C" int dccl_residual_norm(int device, int dtype, size_t rows, size_t wid
     const NormShape s = norm_shape(width);
     OnDevice on(device);
     if (on.e != cudaSuccess) return report("dccl_residual_norm", on.e);
-    return report("dccl_residual_norm", norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all), aligned_to(8, all)), s.elements, (unsigned)rows, (unsigned)s.threads,
-                                                      (cudaStream_t)stream, a, false));
+    return report("dccl_residual_norm", norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, norm_form_of(branch, post, gate, scale),
+                                                      (unsigned)rows, (unsigned)s.threads, (cudaStream_t)stream, a));
 }
 
-extern "C" size_t dccl_residual_norm_workspace(int device, size_t rows, size_t width, size_t gates, int has_post, int full) {
+extern "C" size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t width, size_t gates, int has_post, int full) {
     if (!rows || !width || (gates && rows % gates)) return 0;
-    const NormCut cut = norm_cut(device, rows, width, gates, full != 0);
+    const NormCut cut = norm_cut(device, dtype, rows, width, gates, full != 0);
     return ((size_t)cut.ctas * (has_post ? 2 : 1) + (gates ? cut.units : 0)) * width * sizeof(float);
 }
 
@@ -453,10 +515,11 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     if (!rows || !width || width > kNormMaxWidth || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
         || !branch != !dbranch)
         return report(who, cudaErrorInvalidValue);
-    const bool full = branch != nullptr;
-    const NormCut cut = norm_cut(device, rows, width, gates, full);
+    const bool full = branch != nullptr;      // a plain sum has no branch here
+    if (full && !post && !gate && scale == 1.0) return report(who, cudaErrorInvalidValue);
+    const NormCut cut = norm_cut(device, dtype, rows, width, gates, full);
     const size_t blocks = (width + 31) / 32, vectors = (dn && dweight ? 1 : 0) + (post && dpost ? 1 : 0) + (gate && dgate ? gates : 0);
-    if (!cut.units || blocks * vectors > 0x7fffffffu || workspace_bytes < dccl_residual_norm_workspace(device, rows, width, gates, post != nullptr, full))
+    if (!cut.units || blocks * vectors > 0x7fffffffu || workspace_bytes < dccl_residual_norm_workspace(device, dtype, rows, width, gates, post != nullptr, full))
         return report(who, cudaErrorInvalidValue);
     float* const weight_sums = (float*)workspace;
     float* const post_sums = post ? weight_sums + (size_t)cut.ctas * width : nullptr;
@@ -469,7 +532,8 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     cudaStream_t stream = (cudaStream_t)stream_v;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
-    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all), aligned_to(8, all)), s.elements, cut.ctas, (unsigned)s.threads, stream, a, full);
+    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, full ? norm_form_of(branch, post, gate, scale) : 0, cut.ctas,
+                                  (unsigned)s.threads, stream, a);
     if (e == cudaSuccess && vectors) {
         const NormColumnArgs c = {a.weight_sums, a.post_sums, a.gate_sums, dweight, dpost, dgate, cut.ctas, (unsigned)cut.chunks, (unsigned)width, (unsigned)blocks, f32_vectors};
         const unsigned grid = (unsigned)(blocks * vectors);

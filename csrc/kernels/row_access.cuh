@@ -39,7 +39,23 @@ template <typename T, int N> __device__ __forceinline__ void ld_vector(float (&f
     }
 }
 
-/** The sum over the CTA, in every thread and in a fixed order. `parts`: 32 words of shared memory that no other call uses until
+/** N fp32 values, rounded to T: 16-bit types two at a time. */
+template <typename T, int N> __device__ __forceinline__ Run<T, N> round_run(const float (&f)[N]) {
+    Run<T, N> r;
+    if constexpr (N % 2 == 0 && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) *reinterpret_cast<__nv_bfloat162*>(&r.e[e]) = __floats2bfloat162_rn(f[e], f[e + 1]);
+    } else if constexpr (N % 2 == 0 && std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) *reinterpret_cast<__half2*>(&r.e[e]) = __floats2half2_rn(f[e], f[e + 1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) r.e[e] = Traits<T>::down(f[e]);
+    }
+    return r;
+}
+
+/** The sum over the CTA, in every thread and in a fixed order. `parts`: 32 aligned words of shared memory that no other call uses until
  *  every thread has passed a barrier after this one. */
 __device__ __forceinline__ float cta_sum(float v, float* parts) {
 #pragma unroll
@@ -47,10 +63,13 @@ __device__ __forceinline__ float cta_sum(float v, float* parts) {
     const unsigned warps = blockDim.x / 32;
     if (warps == 1) return v;
     if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = v;
+    if (threadIdx.x < 4 && warps % 4 && threadIdx.x >= warps % 4) parts[warps / 4 * 4 + threadIdx.x] = 0.0f;      // up to a multiple of four
     __syncthreads();
-    v = threadIdx.x % 32 < warps ? parts[threadIdx.x % 32] : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v = 0;
+    for (unsigned w = 0; w < warps; w += 4) {
+        const float4 p = *reinterpret_cast<const float4*>(parts + w);
+        v += (p.x + p.y) + (p.z + p.w);
+    }
     return v;
 }
 

@@ -156,7 +156,7 @@ struct NormBackward : public Node {
         const Tensor dp = p.defined() && task_should_compute_output(3) ? fresh_like(p) : Tensor(), dg = g.defined() && task_should_compute_output(4) ? fresh_like(g) : Tensor();
         if (rows) {
             const int device = x_.device().index();
-            const size_t bytes = entry.norm_workspace(device, rows, width, gates, p.defined(), b.defined());
+            const size_t bytes = entry.norm_workspace(device, dtype_of(x_), rows, width, gates, p.defined(), b.defined());
             const Tensor work = fresh({(int64_t)bytes}, at::kByte, x_);
             const int rc = entry.norm_backward(device, dtype_of(x_), rows, width, ptr(dy), ptr(dn), ptr(x_), ptr(b), ptr(w), ptr(p), ptr(g), gates ? rows / gates : 0,
                                                f32_vectors(x_, w, p, g), scale, ptr(rstd), ptr(rstd_post), ptr(dx), b.defined() ? ptr(db) : nullptr, ptr(dw), ptr(dp), ptr(dg),

@@ -109,7 +109,7 @@ def _declare(lib):
         "dccl_local_reduce_device": (i, [vp, vp, sz, i, i, vp]),
         "dccl_adamw_flat": (i, [i, i, sz, vp, vp, vp, vp, vp, vp] + [c.c_double] * 7 + [vp]),
         "dccl_residual_norm": (i, [i, i, sz, sz] + [vp] * 5 + [sz, i, c.c_double, c.c_double] + [vp] * 5),
-        "dccl_residual_norm_workspace": (sz, [i, sz, sz, sz, i, i]),
+        "dccl_residual_norm_workspace": (sz, [i, i, sz, sz, sz, i, i]),
         "dccl_residual_norm_backward": (i, [i, i, sz, sz] + [vp] * 7 + [sz, i, c.c_double] + [vp] * 8 + [sz, vp]),
         "dccl_rotary": (i, [i, i, sz, sz, i, i, i, i, vp, vp, vp, vp, i, c.c_longlong, c.c_longlong, c.c_longlong, c.c_double, vp]),
         "dccl_gated_linear_workspace": (c.c_longlong, [i, sz, sz, sz, i, i]),
