@@ -73,6 +73,27 @@ __device__ __forceinline__ float cta_sum(float v, float* parts) {
     return v;
 }
 
+/**
+ * Division of n < 2^31 by a number that the host knows: n / d = (n m) >> (32 + s) with m = ceil(2^(32 + s) / d) and 2^s >= d > 2^(s - 1), which is
+ * right as n times the excess of m over the quotient (below d / d) stays under 2^31 (Granlund and Montgomery, "Division by Invariant Integers using
+ * Multiplication"). m takes 33 bits; its highest is added as n.
+ */
+struct Divisor {
+    unsigned d, m, s;
+    Divisor() = default;
+    explicit Divisor(unsigned divisor) : d(divisor), s(0) {
+        while (s < 31 && (1u << s) < d) s++;
+        m = (unsigned)((((uint64_t)1 << (32 + s)) + d - 1) / d - ((uint64_t)1 << 32));
+    }
+    __host__ __device__ __forceinline__ unsigned quotient(unsigned n) const {
+#ifdef __CUDA_ARCH__
+        return (__umulhi(n, m) + n) >> s;
+#else
+        return ((unsigned)((uint64_t)n * m >> 32) + n) >> s;
+#endif
+    }
+};
+
 /** Makes `device` current for as long as it lives. */
 class OnDevice {
 public:

@@ -375,6 +375,18 @@ def test_rotary_of_views():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_leaves_what_does_not_turn(dtype, interleaved):
+    """The elements behind the pairs are copied, next to whatever stands beside them."""
+    freqs = ops.rotary_frequencies(10, device="cuda")
+    q = torch.randn(2, 3, 2, 32, device="cuda").to(dtype)
+    q[..., 10::3], q[..., 11::3] = float("inf"), float("nan")
+    out = ops.rotary(q, None, freqs, 9)
+    assert torch.equal(out[..., 10:].nan_to_num(7.0), q[..., 10:].nan_to_num(7.0)) and bool(out[..., :10].isfinite().all())
+
+
+@gpu
 def test_rotary_one_of_two_outputs_used():
     freqs = ops.rotary_frequencies(16, device="cuda")
     q, k = torch.randn(1, 3, 2, 16, device="cuda", requires_grad=True), torch.randn(1, 3, 1, 16, device="cuda", requires_grad=True)
