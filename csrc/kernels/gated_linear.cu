@@ -47,19 +47,19 @@ __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f
 constexpr float kTanhScale = 1.5957691216057308f, kTanhCubic = 0.044715f;      // 2 sqrt(2 / pi)
 
 /** 0.5 g (1 + tanh(z)) = g sigmoid(2 z). */
-__device__ __forceinline__ float activate(float g, int act) {
-    if (act == DCCL_ACT_SILU) return g * sigmoid(g);
-    if (act == DCCL_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-    return g * sigmoid(kTanhScale * fmaf(kTanhCubic * g * g, g, g));
+template <int ACT> __device__ __forceinline__ float activate(float g) {
+    if constexpr (ACT == DCCL_ACT_SILU) return g * sigmoid(g);
+    else if constexpr (ACT == DCCL_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    else return g * sigmoid(kTanhScale * fmaf(kTanhCubic * g * g, g, g));
 }
 
 /** The activation and its derivative. */
-__device__ __forceinline__ void activate_grad(float g, int act, float& a, float& da) {
-    if (act == DCCL_ACT_SILU) {
+template <int ACT> __device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
+    if constexpr (ACT == DCCL_ACT_SILU) {
         const float s = sigmoid(g);
         a = g * s;
         da = s * fmaf(g, 1.0f - s, 1.0f);
-    } else if (act == DCCL_ACT_GELU) {
+    } else if constexpr (ACT == DCCL_ACT_GELU) {
         const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         a = g * cdf;
         da = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), cdf);
@@ -68,6 +68,13 @@ __device__ __forceinline__ void activate_grad(float g, int act, float& a, float&
         a = g * s;
         da = fmaf(g * s * (1.0f - s), kTanhScale * fmaf(3.0f * kTanhCubic * g, g, 1.0f), s);
     }
+}
+
+/** f with the activation as a constant: one choice for many elements. */
+template <typename F> __device__ __forceinline__ void with_activation(int act, F&& f) {
+    if (act == DCCL_ACT_SILU) f(std::integral_constant<int, DCCL_ACT_SILU>{});
+    else if (act == DCCL_ACT_GELU) f(std::integral_constant<int, DCCL_ACT_GELU>{});
+    else f(std::integral_constant<int, DCCL_ACT_GELU_TANH>{});
 }
 
 /** Rows of a tile's 32 columns pass through shared memory, so that a warp stores whole rows and not one line per lane. `stage`: 4 KB of
@@ -264,8 +271,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                         store_fp32(stage, up_to, stride, rows, columns);
                     }
                     if (a.splits == 1) {
+                        with_activation(a.act, [&](auto act) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) g[e] = activate(g[e], a.act) * u[e];
+                            for (int e = 0; e < 32; e++) g[e] = activate<decltype(act)::value>(g[e]) * u[e];
+                        });
                         stage_rows(stage, g);
                         store_as<T>(stage, reinterpret_cast<T*>(a.c0) + row * a.n + column, a.n, rows, columns, vec);
                     }
@@ -320,7 +329,7 @@ template <typename T, bool GATE> __global__ void __launch_bounds__(256) k_join(c
             float g = 0, u = 0;
             for (unsigned s = 0; s < a.splits; s++) { g += a.partial[2 * s * plane + from]; u += a.partial[(2 * s + 1) * plane + from]; }
             if (a.g) { a.g[row * a.pre_stride + column] = g; a.u[row * a.pre_stride + column] = u; }
-            reinterpret_cast<T*>(a.c0)[at] = Traits<T>::down(activate(g, a.act) * u);
+            with_activation(a.act, [&](auto act) { reinterpret_cast<T*>(a.c0)[at] = Traits<T>::down(activate<decltype(act)::value>(g) * u); });
         } else {
             float v = 0;
             for (unsigned s = 0; s < a.splits; s++) v += a.partial[(s * a.batch + batch) * plane + from];
@@ -355,17 +364,18 @@ template <typename T, int V> __global__ void __launch_bounds__(256) k_gate_grad(
         ld_vector<float, V>(g, a.g, true, row * a.pre_stride + column);
         ld_vector<float, V>(u, a.u, true, row * a.pre_stride + column);
         const Run<T, V> dh = ld_run<T, V>(reinterpret_cast<const T*>(a.dh) + row * a.n + column);
-        Run<T, V> dg, du;
+        with_activation(a.act, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float d = Traits<T>::up(dh.e[e]);
-            float act, slope;
-            activate_grad(g[e], a.act, act, slope);
-            dg.e[e] = Traits<T>::down(d * u[e] * slope);
-            du.e[e] = Traits<T>::down(d * act);
-        }
-        st_run<T, V>(reinterpret_cast<T*>(a.dg) + row * a.stride + column, dg);
-        st_run<T, V>(reinterpret_cast<T*>(a.du) + row * a.stride + column, du);
+            for (int e = 0; e < V; e++) {
+                const float d = Traits<T>::up(dh.e[e]);
+                float value, slope;
+                activate_grad<decltype(act)::value>(g[e], value, slope);
+                g[e] = d * u[e] * slope;
+                u[e] = d * value;
+            }
+        });
+        st_run<T, V>(reinterpret_cast<T*>(a.dg) + row * a.stride + column, round_run<T, V>(g));
+        st_run<T, V>(reinterpret_cast<T*>(a.du) + row * a.stride + column, round_run<T, V>(u));
     }
 }
 
