@@ -38,6 +38,9 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     return true;
 }
 
+/** The same for a whole warp, which goes on as one. */
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* failed) { return __all_sync(0xffffffffu, bar_wait(bar, parity, failed)); }
+
 /* ---- tensor-map loads ---- */
 
 /** One box into shared memory; the barrier counts its bytes, those outside of the tensor (zeros) among them. x * element size is a

@@ -24,7 +24,8 @@ enum Form {
 };
 
 constexpr int kTileM = 128, kTileK = 64, kStages = 4;
-constexpr int kEpilogueWarps = 4, kGemmThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kEpilogueWarps = 8, kGemmThreads = 32 * (kEpilogueWarps + 2);
+constexpr unsigned kLoader = kEpilogueWarps, kMultiplier = kEpilogueWarps + 1;
 constexpr int kStageRowsBytes = 128;                                // one row of a swizzled tile
 
 struct GemmArgs {
@@ -141,7 +142,8 @@ template <int FORM, int N> struct GemmShape {
 };
 
 /**
- * One CTA per SM walks over tiles of 128 rows; warp 4 loads, warp 5 multiplies, warps 0 to 3 store. The sums of two tiles fit into
+ * One CTA per SM walks over tiles of 128 rows; one warp loads, one multiplies, eight store: a warp reaches the quarter of the tile's
+ * rows that its number gives, so two share one and take half of the columns each. The sums of two tiles fit into
  * tensor memory, so that one is stored while the next is multiplied.
  */
 template <typename T, int FORM, int N>
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     char* const staging = tiles + kStages * Shape::kBytes;
     const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16, drained = sums_empty + 16;
     const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (warp == 5) tmem_alloc(shared_addr(&tmem_base), 2 * N);
+    if (warp == kMultiplier) tmem_alloc(shared_addr(&tmem_base), 2 * N);
     if (threadIdx.x == 0) {
         failed = 0;
         for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         bar_init(drained, 1);
         bar_init_fence();
     }
-    if (threadIdx.x == 32 * 4) {
+    if (threadIdx.x == 32 * kLoader) {
         prefetch_map(&a.a0);
         prefetch_map(&a.b0);
         if (FORM == GATED) prefetch_map(&a.b1);
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     wait_for_stream();
     const unsigned total = a.tiles_m * a.tiles_n * a.batch * a.splits;
     unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
-    if (warp == 4 && lane == 0) {
+    if (warp == kLoader && lane == 0) {
         for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
             const Place p = place_of(tile, a);
             const unsigned from = (unsigned)((unsigned long long)a.k_blocks * p.split / a.splits), to = (unsigned)((unsigned long long)a.k_blocks * (p.split + 1) / a.splits);
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             }
             if (kb < to) break;
         }
-    } else if (warp == 5 && lane == 0) {
+    } else if (warp == kMultiplier && lane == 0) {
         unsigned done = 0;
         for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
             const Place p = place_of(tile, a);
@@ -241,14 +243,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
             const Place p = place_of(tile, a);
             const unsigned buffer = done & 1;
-            if (!bar_wait(sums_full + 8 * buffer, done / 2 & 1, &failed)) break;
-            __syncwarp();
+            if (!bar_wait_warp(sums_full + 8 * buffer, done / 2 & 1, &failed)) break;
             tc_after_sync();
-            const uint32_t d = sums + buffer * N + (warp * 32u << 16);
-            const size_t row = (size_t)p.m * kTileM + warp * 32;
+            const unsigned quarter = warp % 4, half = warp / 4;
+            const uint32_t d = sums + buffer * N + (quarter * 32u << 16);
+            const size_t row = (size_t)p.m * kTileM + quarter * 32;
             const int rows = row < a.m ? (int)(a.m - row < 32 ? a.m - row : 32) : 0;
 #pragma unroll 1
-            for (int c = 0; c < Shape::kColumns; c += 32) {
+            for (int c = half * (Shape::kColumns / 2); c < (int)(half + 1) * (Shape::kColumns / 2); c += 32) {
                 const size_t column = (size_t)p.n * Shape::kColumns + c;
                 if (column >= a.n || !rows) break;
                 const int columns = (int)(a.n - column < 32 ? a.n - column : 32);
@@ -296,9 +298,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     __syncthreads();
     if (failed) {       // no wait is expected to run out: copies in flight still have to land, and products to end, before the memory is given back
         int late = 0;
-        if (warp == 4 && lane == 0)
+        if (warp == kLoader && lane == 0)
             for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
-        if (warp == 5 && lane == 0) {
+        if (warp == kMultiplier && lane == 0) {
             commit(drained);
             bar_wait(drained, 0, &late);
         }
@@ -306,7 +308,129 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         __syncthreads();
     }
     tc_after_sync();
-    if (warp == 5) tmem_free(sums, 2 * N);
+    if (warp == kMultiplier) tmem_free(sums, 2 * N);
+}
+
+/* ---- few tokens ---- */
+
+constexpr int kFewRows = 32;            // of each weight, for one CTA
+
+template <int N> struct FewShape {
+    static constexpr int kBytesW = 2 * kFewRows * kTileK * 2, kBytes = kBytesW + N * kTileK * 2;
+    static constexpr int kStages = N == 16 ? 10 : N == 32 ? 8 : N == 64 ? 6 : 4;        // about 100 KB, so that two CTAs share an SM
+    static constexpr int kShared = kStages * kBytes + kBytesW + 1024;                  // kBytesW: rows 64 to 127 of the last stage's product
+};
+
+struct FewArgs {
+    CUtensorMap x, w_gate, w_up;
+    unsigned tokens, ffn, k_blocks, descriptor;
+    int act;
+    void* h;
+    float *g, *u;
+    size_t pre_stride;
+    int* gave_up;
+};
+
+/**
+ * Up to 128 tokens: reading the weights bounds it. Here they are the rows of the product and the tokens its columns, so that the work of the
+ * tensor cores shrinks with the tokens; each CTA takes 32 rows of both weights over all of k, which makes about one CTA per SM of an
+ * ordinary layer and leaves nothing to join. Rows 0 to 31 of a tile are of Wg and 32 to 63 of Wu. A product has 128 rows: the others
+ * are whatever lies behind in shared memory, and nobody reads what becomes of them.
+ */
+template <typename T, int N> __global__ void __launch_bounds__(128) k_gated_few(const __grid_constant__ FewArgs a) {
+    using Shape = FewShape<N>;
+    constexpr int kStages = Shape::kStages, kColumns = N < 32 ? 32 : N;
+    extern __shared__ char shared[];
+    __shared__ uint64_t bars[2 * kStages + 2];
+    __shared__ uint32_t tmem_base;
+    __shared__ int failed;
+    char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
+    const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, drained = sums_full + 8;
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x * kFewRows;
+    if (warp == 3) tmem_alloc(shared_addr(&tmem_base), kColumns);
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
+        bar_init(sums_full, 1);
+        bar_init(drained, 1);
+        bar_init_fence();
+    }
+    if (threadIdx.x == 32 * 2) {
+        prefetch_map(&a.x);
+        prefetch_map(&a.w_gate);
+        prefetch_map(&a.w_up);
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    const uint32_t sums = tmem_base;
+    wait_for_stream();
+    unsigned filled = 0;
+    if (warp == 2 && lane == 0) {
+        for (unsigned kb = 0; kb < a.k_blocks; kb++, filled++) {
+            const unsigned s = kb % kStages;
+            if (!bar_wait(empty + 8 * s, (kb / kStages & 1) ^ 1, &failed)) break;
+            const uint32_t bar = full + 8 * s, to = shared_addr(tiles) + s * Shape::kBytes;
+            bar_expect(bar, Shape::kBytes);
+            load_box(to, &a.w_gate, kb * kTileK, row, bar);
+            load_box(to + Shape::kBytesW / 2, &a.w_up, kb * kTileK, row, bar);
+            load_box(to + Shape::kBytesW, &a.x, kb * kTileK, 0, bar);
+        }
+    } else if (warp == 3 && lane == 0) {
+        for (unsigned kb = 0; kb < a.k_blocks; kb++) {
+            const unsigned s = kb % kStages;
+            if (!bar_wait(full + 8 * s, kb / kStages & 1, &failed)) break;
+            tc_after_sync();
+            const uint32_t at = shared_addr(tiles) + s * Shape::kBytes;
+#pragma unroll
+            for (int k = 0; k < kTileK / 16; k++)
+                product(sums, tile_descriptor(at + k * 32, 16), tile_descriptor(at + Shape::kBytesW + k * 32, 16), a.descriptor, kb || k);
+            commit(empty + 8 * s);
+        }
+        commit(sums_full);
+    }
+    __syncwarp();
+    // [gate, up][token][row]: the loads are over and the products done once the sums are
+    float* const values = reinterpret_cast<float*>(tiles);
+    if (warp < 2 && bar_wait_warp(sums_full, 0, &failed)) {
+        tc_after_sync();
+#pragma unroll 1
+        for (int c = 0; c < N; c += 32) {
+            uint32_t r[32];
+            tmem_load32(r, sums + (warp * 32u << 16) + c);
+            tmem_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+                if (c + e < N) values[(warp * N + c + e) * 32 + lane] = __uint_as_float(r[e]);
+        }
+        tc_before_sync();
+    }
+    __syncthreads();
+    if (failed) {       // as in k_gemm
+        int late = 0;
+        if (warp == 2 && lane == 0)
+            for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
+        if (warp == 3 && lane == 0) {
+            commit(drained);
+            bar_wait(drained, 0, &late);
+        }
+        if (threadIdx.x == 0 && a.gave_up) *reinterpret_cast<volatile int*>(a.gave_up) = 1;
+        __syncthreads();
+    } else if (row + lane < a.ffn) {
+        with_activation(a.act, [&](auto act) {
+            for (unsigned t = warp; t < a.tokens; t += 4) {
+                const float g = values[t * 32 + lane], u = values[(N + t) * 32 + lane];
+                if (a.g) {
+                    a.g[t * a.pre_stride + row + lane] = g;
+                    a.u[t * a.pre_stride + row + lane] = u;
+                }
+                reinterpret_cast<T*>(a.h)[(size_t)t * a.ffn + row + lane] = Traits<T>::down(activate<decltype(act)::value>(g) * u);
+            }
+        });
+    }
+    __syncwarp();
+    tc_after_sync();
+    if (warp == 3) tmem_free(sums, kColumns);
 }
 
 struct JoinArgs {
@@ -317,66 +441,109 @@ struct JoinArgs {
     void *c0, *c1;
     float *g, *u;
     size_t pre_stride;
+    bool vec;                       // rows of the results start on four elements
 };
 
-/** Adds the parts that splits of k left, in the order of k, and finishes: one thread per element. */
+/** Adds the parts that splits of k left, in the order of k, and finishes: four columns per thread. */
 template <typename T, bool GATE> __global__ void __launch_bounds__(256) k_join(const __grid_constant__ JoinArgs a) {
     wait_for_stream();
-    const size_t plane = a.m * a.stride, count = a.m * a.n;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count * (GATE ? 1 : a.batch); i += (size_t)gridDim.x * 256) {
-        const size_t batch = i / count, at = i % count, row = at / a.n, column = at % a.n, from = row * a.stride + column;
+    const size_t plane = a.m * a.stride;
+    const unsigned runs = (unsigned)(a.stride / 4);
+    const size_t index = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (index >= a.m * runs * (GATE ? 1 : a.batch)) return;
+    const size_t line = index / runs, row = GATE ? line : line % a.m, batch = GATE ? 0 : line / a.m;
+    const unsigned column = (unsigned)(index % runs) * 4;
+    const float* from = a.partial + batch * plane + row * a.stride + column;
+    const size_t next = plane * (GATE ? 2 : a.batch);
+    Run<float, 4> g = {}, u = {};
+#pragma unroll 4
+    for (unsigned s = 0; s < a.splits; s++) {
+        const Run<float, 4> p = ld_run<float, 4>(from + s * next);
+#pragma unroll
+        for (int e = 0; e < 4; e++) g.e[e] += p.e[e];
         if constexpr (GATE) {
-            float g = 0, u = 0;
-            for (unsigned s = 0; s < a.splits; s++) { g += a.partial[2 * s * plane + from]; u += a.partial[(2 * s + 1) * plane + from]; }
-            if (a.g) { a.g[row * a.pre_stride + column] = g; a.u[row * a.pre_stride + column] = u; }
-            with_activation(a.act, [&](auto act) { reinterpret_cast<T*>(a.c0)[at] = Traits<T>::down(activate<decltype(act)::value>(g) * u); });
-        } else {
-            float v = 0;
-            for (unsigned s = 0; s < a.splits; s++) v += a.partial[(s * a.batch + batch) * plane + from];
-            reinterpret_cast<T*>(batch ? a.c1 : a.c0)[at] = Traits<T>::down(v);
+            const Run<float, 4> q = ld_run<float, 4>(from + s * next + plane);
+#pragma unroll
+            for (int e = 0; e < 4; e++) u.e[e] += q.e[e];
         }
     }
+    if constexpr (GATE) {
+        if (a.g) {      // rows of these end on four elements as well
+            st_run<float, 4>(a.g + row * a.pre_stride + column, g);
+            st_run<float, 4>(a.u + row * a.pre_stride + column, u);
+        }
+        with_activation(a.act, [&](auto act) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) g.e[e] = activate<decltype(act)::value>(g.e[e]) * u.e[e];
+        });
+    }
+    T* to = reinterpret_cast<T*>(batch ? a.c1 : a.c0) + row * a.n + column;
+    if (a.vec) st_run<T, 4>(to, round_run<T, 4>(g.e));
+    else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (column + e < a.n) to[e] = Traits<T>::down(g.e[e]);
 }
 
 struct PadArgs { const void* from[3]; void* to[3]; size_t rows[3]; unsigned width, stride; };
 
-/** Rows that do not start on 16 bytes, copied to some that do, for the tiled loads. The elements behind a row are not read by anyone. */
-template <typename T> __global__ void __launch_bounds__(256) k_pad(const __grid_constant__ PadArgs a) {
+/** Rows that do not start on 16 bytes, copied to some that do, for the tiled loads: eight elements per thread. Nobody reads what is behind a row. */
+__global__ void __launch_bounds__(256) k_pad(const __grid_constant__ PadArgs a) {
     wait_for_stream();
-    for (int w = 0; w < 3; w++) {
-        const T* from = reinterpret_cast<const T*>(a.from[w]);
-        T* to = reinterpret_cast<T*>(a.to[w]);
-        for (size_t row = blockIdx.x; row < a.rows[w]; row += gridDim.x)
-            for (unsigned i = threadIdx.x; i < a.width; i += 256) to[row * a.stride + i] = from[row * a.width + i];
-    }
+    const unsigned runs = a.stride / 8;
+    size_t index = (size_t)blockIdx.x * 256 + threadIdx.x;
+    int w = 0;
+    while (w < 3 && index >= a.rows[w] * runs) index -= a.rows[w++] * runs;
+    if (w == 3) return;
+    const size_t row = index / runs;
+    const unsigned column = (unsigned)(index % runs) * 8;
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(a.from[w]) + row * a.width + column;
+    Run<uint16_t, 8> r = {};
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (column + e < a.width) r.e[e] = from[e];
+    st_run<uint16_t, 8>(reinterpret_cast<uint16_t*>(a.to[w]) + row * a.stride + column, r);
 }
 
 struct GateGradArgs { const void* dh; const float *g, *u; void *dg, *du; size_t pre_stride, stride; unsigned rows, n; int act; };
 
-/** dg and du from dh and the saved products. V: elements per access. */
-template <typename T, int V> __global__ void __launch_bounds__(256) k_gate_grad(const __grid_constant__ GateGradArgs a) {
+/** dg and du from dh and the saved products, eight elements per thread. Only the rows of dh may start anywhere (VEC: they do not). */
+template <typename T, bool VEC> __global__ void __launch_bounds__(256) k_gate_grad(const __grid_constant__ GateGradArgs a) {
     wait_for_stream();
-    const unsigned runs = a.n / V;
-    const size_t count = (size_t)a.rows * runs;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (size_t)gridDim.x * 256) {
-        const size_t row = i / runs, column = i % runs * V;
-        float g[V], u[V];
-        ld_vector<float, V>(g, a.g, true, row * a.pre_stride + column);
-        ld_vector<float, V>(u, a.u, true, row * a.pre_stride + column);
-        const Run<T, V> dh = ld_run<T, V>(reinterpret_cast<const T*>(a.dh) + row * a.n + column);
-        with_activation(a.act, [&](auto act) {
+    const unsigned runs = (a.n + 7) / 8;
+    const size_t index = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (index >= (size_t)a.rows * runs) return;
+    const size_t row = index / runs;
+    const unsigned column = (unsigned)(index % runs) * 8;
+    const bool second = column + 4 < a.n;       // rows of g and u end on four elements
+    float g[8], u[8], d[8];
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float d = Traits<T>::up(dh.e[e]);
-                float value, slope;
-                activate_grad<decltype(act)::value>(g[e], value, slope);
-                g[e] = d * u[e] * slope;
-                u[e] = d * value;
-            }
-        });
-        st_run<T, V>(reinterpret_cast<T*>(a.dg) + row * a.stride + column, round_run<T, V>(g));
-        st_run<T, V>(reinterpret_cast<T*>(a.du) + row * a.stride + column, round_run<T, V>(u));
+    for (int q = 0; q < 2; q++) {
+        if (q && !second) break;
+        const Run<float, 4> x = ld_run<float, 4>(a.g + row * a.pre_stride + column + 4 * q), y = ld_run<float, 4>(a.u + row * a.pre_stride + column + 4 * q);
+#pragma unroll
+        for (int e = 0; e < 4; e++) { g[4 * q + e] = x.e[e]; u[4 * q + e] = y.e[e]; }
     }
+    const T* dh = reinterpret_cast<const T*>(a.dh) + row * a.n + column;
+    if constexpr (VEC) {
+        const Run<T, 8> r = ld_run<T, 8>(dh);
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] = Traits<T>::up(r.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) d[e] = column + e < a.n ? Traits<T>::up(dh[e]) : 0.0f;
+    }
+    with_activation(a.act, [&](auto act) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float value, slope;
+            activate_grad<decltype(act)::value>(g[e], value, slope);
+            g[e] = d[e] * u[e] * slope;
+            u[e] = d[e] * value;
+        }
+    });
+    st_run<T, 8>(reinterpret_cast<T*>(a.dg) + row * a.stride + column, round_run<T, 8>(g));
+    st_run<T, 8>(reinterpret_cast<T*>(a.du) + row * a.stride + column, round_run<T, 8>(u));
 }
 
 /* ------------------------------------------------------------------------------------------------ host side */
@@ -445,9 +612,14 @@ template <typename T, int FORM> static cudaError_t run_gemm(int device, const Ge
     const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch * p.splits, sms = (size_t)sm_count(device);
     cudaError_t e = launch_early_shared(k_gemm<T, FORM, 256>, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, Shape::kShared, stream, a);
     if (e != cudaSuccess || p.splits == 1) return e;
-    const JoinArgs j = {a.partial, a.m, a.partial_stride, a.n, p.splits, p.batch, a.act, a.c0, a.c1, a.g, a.u, a.pre_stride};
-    const size_t elements = (size_t)a.m * a.n * p.batch, ctas = (elements + 255) / 256;
-    return launch_early(k_join<T, FORM == GATED>, (unsigned)(ctas < 8 * sms ? ctas : 8 * sms), 256, stream, j);
+    const JoinArgs j = {a.partial, a.m, a.partial_stride, a.n, p.splits, p.batch, a.act, a.c0, a.c1, a.g, a.u, a.pre_stride, a.n % 4 == 0 && aligned_to(8, {a.c0, a.c1})};
+    const size_t threads = (size_t)a.m * (a.partial_stride / 4) * p.batch;
+    return launch_early(k_join<T, FORM == GATED>, (unsigned)((threads + 255) / 256), 256, stream, j);
+}
+
+/** Whether k_gated_few takes a call: for wider layers than it has CTAs for, splits of k read the weights faster. */
+static bool few_tokens(int sms, size_t tokens, size_t width, size_t ffn) {
+    return tokens <= 128 && (width <= 4096 || 2 * blocks_of(ffn, kFewRows) >= (size_t)sms);
 }
 
 /** Where the parts of a call's workspace lie. */
@@ -477,7 +649,7 @@ static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn
         partial = l.input.partial_bytes > l.weight.partial_bytes ? l.input.partial_bytes : l.weight.partial_bytes;
     } else {
         l.forward = plan_gemm(sms, GATED, tokens, ffn, width);
-        partial = l.forward.partial_bytes;
+        if (!few_tokens(sms, tokens, width, ffn)) partial = l.forward.partial_bytes;
     }
     l.partial = take(partial);
     l.total = at;
@@ -485,19 +657,50 @@ static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn
 }
 
 /** x, Wg and Wu as the tiled loads take them: in place, or padded into the workspace. */
-static cudaError_t pad_operands(int device, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, bool with_weights, const void*& x, const void*& w_gate, const void*& w_up,
+static cudaError_t pad_operands(const GatedLayout& l, size_t tokens, size_t width, size_t ffn, bool with_weights, const void*& x, const void*& w_gate, const void*& w_up,
                                 char* workspace, cudaStream_t stream) {
     if (l.stride == width && aligned_to(16, {x, w_gate, w_up})) return cudaSuccess;
     PadArgs a = {{x, w_gate, w_up}, {workspace + l.x, workspace + l.gate, workspace + l.up}, {tokens, with_weights ? ffn : 0, with_weights ? ffn : 0}, (unsigned)width, (unsigned)l.stride};
     x = a.to[0];
     w_gate = a.to[1];
     w_up = a.to[2];
-    return launch_early(k_pad<uint16_t>, (unsigned)(8 * sm_count(device)), 256, stream, a);
+    const size_t threads = (a.rows[0] + a.rows[1] + a.rows[2]) * (l.stride / 8);
+    return launch_early(k_pad, (unsigned)((threads + 255) / 256), 256, stream, a);
+}
+
+template <typename T, int N> static cudaError_t run_few(int device, FewArgs& a, cudaStream_t stream) {
+    static std::atomic<bool> ready[64];
+    if (!ready[device].load(std::memory_order_relaxed)) {
+        const cudaError_t e = cudaFuncSetAttribute(k_gated_few<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<N>::kShared);
+        if (e != cudaSuccess) return e;
+        ready[device].store(true, std::memory_order_relaxed);
+    }
+    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, false, false, 128, N);
+    return launch_early_shared(k_gated_few<T, N>, blocks_of(a.ffn, kFewRows), 128, FewShape<N>::kShared, stream, a);
 }
 
 template <typename T> static cudaError_t gated_forward(int device, int dtype, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up,
                                                        int act, void* h, float* g, float* u, size_t pre_stride, char* workspace, cudaStream_t stream) {
-    cudaError_t e = pad_operands(device, l, tokens, width, ffn, true, x, w_gate, w_up, workspace, stream);
+    cudaError_t e = pad_operands(l, tokens, width, ffn, true, x, w_gate, w_up, workspace, stream);
+    if (few_tokens(sm_count(device), tokens, width, ffn)) {
+        const int columns = tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128;
+        FewArgs f = {};
+        if (e == cudaSuccess) e = make_map(&f.x, dtype, x, width, tokens, l.stride, columns);
+        if (e == cudaSuccess) e = make_map(&f.w_gate, dtype, w_gate, width, ffn, l.stride, kFewRows);
+        if (e == cudaSuccess) e = make_map(&f.w_up, dtype, w_up, width, ffn, l.stride, kFewRows);
+        if (e != cudaSuccess) return e;
+        f.tokens = (unsigned)tokens;
+        f.ffn = (unsigned)ffn;
+        f.k_blocks = blocks_of(width, kTileK);
+        f.act = act;
+        f.h = h;
+        f.g = g;
+        f.u = u;
+        f.pre_stride = pre_stride;
+        f.gave_up = gave_up_flag();
+        return columns == 16 ? run_few<T, 16>(device, f, stream) : columns == 32 ? run_few<T, 32>(device, f, stream) : columns == 64 ? run_few<T, 64>(device, f, stream)
+                                                                                                                                    : run_few<T, 128>(device, f, stream);
+    }
     GemmArgs a = {};
     if (e == cudaSuccess) e = make_map(&a.a0, dtype, x, width, tokens, l.stride, kTileM);
     if (e == cudaSuccess) e = make_map(&a.b0, dtype, w_gate, width, ffn, l.stride, 128);
@@ -518,11 +721,9 @@ template <typename T> static cudaError_t gated_backward(int device, int dtype, c
                                                         size_t pre_stride, const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up,
                                                         char* workspace, cudaStream_t stream) {
     const GateGradArgs d = {dh, g, u, workspace + l.dg, workspace + l.du, pre_stride, l.d_stride, (unsigned)tokens, (unsigned)ffn, act};
-    const size_t sms = (size_t)sm_count(device);
-    const bool vec = ffn % 8 == 0 && aligned_to(16, {dh, g, u}) && pre_stride % 4 == 0;
-    const size_t runs = tokens * (vec ? ffn / 8 : ffn), ctas = (runs + 255) / 256;
-    cudaError_t e = launch_early(vec ? k_gate_grad<T, 8> : k_gate_grad<T, 1>, (unsigned)(ctas < 64 * sms ? ctas : 64 * sms), 256, stream, d);
-    if (e == cudaSuccess) e = pad_operands(device, l, tokens, width, ffn, dx != nullptr, x, w_gate, w_up, workspace, stream);
+    const size_t threads = tokens * ((ffn + 7) / 8);
+    cudaError_t e = launch_early(ffn % 8 == 0 && aligned_to(16, {dh}) ? k_gate_grad<T, true> : k_gate_grad<T, false>, (unsigned)((threads + 255) / 256), 256, stream, d);
+    if (e == cudaSuccess) e = pad_operands(l, tokens, width, ffn, dx != nullptr, x, w_gate, w_up, workspace, stream);
     GemmArgs a = {};
     a.partial = (float*)(workspace + l.partial);
     if (e == cudaSuccess && dx) {

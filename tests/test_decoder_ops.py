@@ -527,7 +527,7 @@ def test_gated_on_cpu(act):
 
 
 SIZES = [(1, 64, 64), (1, 8, 8), (2, 1, 1), (3, 5, 7), (40, 256, 512), (128, 64, 128), (129, 72, 136), (200, 1000, 384), (257, 333, 191), (64, 2048, 200), (1, 2048, 5632), (300, 65, 1033),
-         (1000, 40, 48), (520, 512, 1024), (17, 96, 2050)]
+         (1000, 40, 48), (520, 512, 1024), (17, 96, 2050), (16, 4104, 96), (33, 4104, 2400), (65, 200, 31), (100, 136, 1000), (128, 129, 65)]
 
 
 @gpu
