@@ -313,17 +313,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 
 /* ---- few tokens ---- */
 
-constexpr int kFewRows = 32;            // of each weight, for one CTA
-
-template <int N> struct FewShape {
-    static constexpr int kBytesW = 2 * kFewRows * kTileK * 2, kBytes = kBytesW + N * kTileK * 2;
-    static constexpr int kStages = N == 16 ? 10 : N == 32 ? 8 : N == 64 ? 6 : 4;        // about 100 KB, so that two CTAs share an SM
-    static constexpr int kShared = kStages * kBytes + kBytesW + 1024;                  // kBytesW: rows 64 to 127 of the last stage's product
-};
+constexpr int kFewStages = 16;          // at most
+constexpr int kFewShared = 112 * 1024, kFewThreads = 192;
 
 struct FewArgs {
     CUtensorMap x, w_gate, w_up;
     unsigned tokens, ffn, k_blocks, descriptor;
+    unsigned rows, stages;              // rows of each weight for one CTA, a multiple of eight up to 64
     int act;
     void* h;
     float *g, *u;
@@ -333,29 +329,28 @@ struct FewArgs {
 
 /**
  * Up to 128 tokens: reading the weights bounds it. Here they are the rows of the product and the tokens its columns, so that the work of the
- * tensor cores shrinks with the tokens; each CTA takes 32 rows of both weights over all of k, which makes about one CTA per SM of an
- * ordinary layer and leaves nothing to join. Rows 0 to 31 of a tile are of Wg and 32 to 63 of Wu. A product has 128 rows: the others
- * are whatever lies behind in shared memory, and nobody reads what becomes of them.
+ * tensor cores shrinks with the tokens. Each CTA takes some rows of both weights over all of k, and nothing is left to join. The rows of Wg come first in a tile, then those of Wu. A product has 128 rows: the others are whatever lies behind in
+ * shared memory, and nobody reads what becomes of them.
  */
-template <typename T, int N> __global__ void __launch_bounds__(128) k_gated_few(const __grid_constant__ FewArgs a) {
-    using Shape = FewShape<N>;
-    constexpr int kStages = Shape::kStages, kColumns = N < 32 ? 32 : N;
+template <typename T, int N> __global__ void __launch_bounds__(kFewThreads, 2) k_gated_few(const __grid_constant__ FewArgs a) {
+    constexpr int kColumns = N < 32 ? 32 : N;
     extern __shared__ char shared[];
-    __shared__ uint64_t bars[2 * kStages + 2];
+    __shared__ uint64_t bars[2 * kFewStages + 2];
     __shared__ uint32_t tmem_base;
     __shared__ int failed;
     char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
-    const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, drained = sums_full + 8;
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = blockIdx.x * kFewRows;
-    if (warp == 3) tmem_alloc(shared_addr(&tmem_base), kColumns);
+    const uint32_t full = shared_addr(bars), empty = full + 8 * kFewStages, sums_full = empty + 8 * kFewStages, drained = sums_full + 8;
+    const uint32_t bytes_w = a.rows * 2 * kStageRowsBytes, bytes = bytes_w + N * kStageRowsBytes;
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, first = blockIdx.x * a.rows;
+    if (warp == 5) tmem_alloc(shared_addr(&tmem_base), kColumns);
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
+        for (unsigned i = 0; i < a.stages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
         bar_init(sums_full, 1);
         bar_init(drained, 1);
         bar_init_fence();
     }
-    if (threadIdx.x == 32 * 2) {
+    if (threadIdx.x == 32 * 4) {
         prefetch_map(&a.x);
         prefetch_map(&a.w_gate);
         prefetch_map(&a.w_up);
@@ -365,72 +360,78 @@ template <typename T, int N> __global__ void __launch_bounds__(128) k_gated_few(
     tc_after_sync();
     const uint32_t sums = tmem_base;
     wait_for_stream();
-    unsigned filled = 0;
-    if (warp == 2 && lane == 0) {
-        for (unsigned kb = 0; kb < a.k_blocks; kb++, filled++) {
-            const unsigned s = kb % kStages;
-            if (!bar_wait(empty + 8 * s, (kb / kStages & 1) ^ 1, &failed)) break;
-            const uint32_t bar = full + 8 * s, to = shared_addr(tiles) + s * Shape::kBytes;
-            bar_expect(bar, Shape::kBytes);
-            load_box(to, &a.w_gate, kb * kTileK, row, bar);
-            load_box(to + Shape::kBytesW / 2, &a.w_up, kb * kTileK, row, bar);
-            load_box(to + Shape::kBytesW, &a.x, kb * kTileK, 0, bar);
+    unsigned filled = 0, stage = 0, parity = 0;
+    if (warp == 4 && lane == 0) {
+        unsigned kb = blockIdx.x * 5 % a.k_blocks;
+        for (; filled < a.k_blocks; filled++) {
+            if (!bar_wait(empty + 8 * stage, parity ^ 1, &failed)) break;
+            const uint32_t bar = full + 8 * stage, to = shared_addr(tiles) + stage * bytes;
+            bar_expect(bar, bytes);
+            load_box(to, &a.w_gate, kb * kTileK, first, bar);
+            load_box(to + bytes_w / 2, &a.w_up, kb * kTileK, first, bar);
+            load_box(to + bytes_w, &a.x, kb * kTileK, 0, bar);
+            if (++kb == a.k_blocks) kb = 0;
+            if (++stage == a.stages) { stage = 0; parity ^= 1; }
         }
-    } else if (warp == 3 && lane == 0) {
+    } else if (warp == 5 && lane == 0) {
         for (unsigned kb = 0; kb < a.k_blocks; kb++) {
-            const unsigned s = kb % kStages;
-            if (!bar_wait(full + 8 * s, kb / kStages & 1, &failed)) break;
+            if (!bar_wait(full + 8 * stage, parity, &failed)) break;
             tc_after_sync();
-            const uint32_t at = shared_addr(tiles) + s * Shape::kBytes;
+            const uint32_t at = shared_addr(tiles) + stage * bytes;
 #pragma unroll
-            for (int k = 0; k < kTileK / 16; k++)
-                product(sums, tile_descriptor(at + k * 32, 16), tile_descriptor(at + Shape::kBytesW + k * 32, 16), a.descriptor, kb || k);
-            commit(empty + 8 * s);
+            for (int k = 0; k < kTileK / 16; k++) product(sums, tile_descriptor(at + k * 32, 16), tile_descriptor(at + bytes_w + k * 32, 16), a.descriptor, kb || k);
+            commit(empty + 8 * stage);
+            if (++stage == a.stages) { stage = 0; parity ^= 1; }
         }
         commit(sums_full);
     }
     __syncwarp();
     // [gate, up][token][row]: the loads are over and the products done once the sums are
     float* const values = reinterpret_cast<float*>(tiles);
-    if (warp < 2 && bar_wait_warp(sums_full, 0, &failed)) {
+    if (warp < 4 && warp * 32 < 2 * a.rows && bar_wait_warp(sums_full, 0, &failed)) {
         tc_after_sync();
 #pragma unroll 1
-        for (int c = 0; c < N; c += 32) {
+        for (int c = 0; c < N && c < (int)a.tokens; c += 32) {
             uint32_t r[32];
             tmem_load32(r, sums + (warp * 32u << 16) + c);
             tmem_wait();
+            if (threadIdx.x < 2 * a.rows) {
+                float* const to = values + (threadIdx.x < a.rows ? threadIdx.x : N * a.rows + threadIdx.x - a.rows) + c * a.rows;
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-                if (c + e < N) values[(warp * N + c + e) * 32 + lane] = __uint_as_float(r[e]);
+                for (int e = 0; e < 32; e++)
+                    if (c + e < (int)a.tokens) to[e * a.rows] = __uint_as_float(r[e]);
+            }
         }
         tc_before_sync();
     }
     __syncthreads();
     if (failed) {       // as in k_gemm
         int late = 0;
-        if (warp == 2 && lane == 0)
-            for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
-        if (warp == 3 && lane == 0) {
+        if (warp == 4 && lane == 0)
+            for (unsigned i = filled > a.stages ? filled - a.stages : 0; i < filled; i++) bar_wait(full + 8 * (i % a.stages), i / a.stages & 1, &late);
+        if (warp == 5 && lane == 0) {
             commit(drained);
             bar_wait(drained, 0, &late);
         }
         if (threadIdx.x == 0 && a.gave_up) *reinterpret_cast<volatile int*>(a.gave_up) = 1;
         __syncthreads();
-    } else if (row + lane < a.ffn) {
+    } else {
+        const unsigned rows = a.ffn - first < a.rows ? a.ffn - first : a.rows;
         with_activation(a.act, [&](auto act) {
-            for (unsigned t = warp; t < a.tokens; t += 4) {
-                const float g = values[t * 32 + lane], u = values[(N + t) * 32 + lane];
-                if (a.g) {
-                    a.g[t * a.pre_stride + row + lane] = g;
-                    a.u[t * a.pre_stride + row + lane] = u;
+            for (unsigned t = warp; t < a.tokens; t += kFewThreads / 32)
+                for (unsigned r = lane; r < rows; r += 32) {
+                    const float g = values[t * a.rows + r], u = values[(N + t) * a.rows + r];
+                    if (a.g) {
+                        a.g[t * a.pre_stride + first + r] = g;
+                        a.u[t * a.pre_stride + first + r] = u;
+                    }
+                    reinterpret_cast<T*>(a.h)[(size_t)t * a.ffn + first + r] = Traits<T>::down(activate<decltype(act)::value>(g) * u);
                 }
-                reinterpret_cast<T*>(a.h)[(size_t)t * a.ffn + row + lane] = Traits<T>::down(activate<decltype(act)::value>(g) * u);
-            }
         });
     }
     __syncwarp();
     tc_after_sync();
-    if (warp == 3) tmem_free(sums, kColumns);
+    if (warp == 5) tmem_free(sums, kColumns);
 }
 
 struct JoinArgs {
@@ -619,7 +620,16 @@ template <typename T, int FORM> static cudaError_t run_gemm(int device, const Ge
 
 /** Whether k_gated_few takes a call: for wider layers than it has CTAs for, splits of k read the weights faster. */
 static bool few_tokens(int sms, size_t tokens, size_t width, size_t ffn) {
-    return tokens <= 128 && (width <= 4096 || 2 * blocks_of(ffn, kFewRows) >= (size_t)sms);
+    return tokens <= 128 && (width <= 4096 || 2 * blocks_of(ffn, 8) >= (size_t)sms);
+}
+
+/** Rows of each weight for one CTA of k_gated_few, two of which share an SM: as many CTAs as there is room for, in as few rounds as it takes,
+ *  but not less than 32 rows while every SM has a CTA, since each CTA reads x as well (5632 rows: 32 take 13.7 us for one token and 16.9 for
+ *  64, 24 take 14.3 and 19.9, and one CTA of 40 rows per SM 13.8 and 19.0). */
+static unsigned few_rows(int sms, size_t ffn) {
+    const size_t room = 2 * (size_t)sms, rounds = (ffn + 64 * room - 1) / (64 * room);
+    const unsigned rows = (unsigned)up_to((ffn + room * rounds - 1) / (room * rounds), 8);
+    return rows < 32 && ffn >= 32 * (size_t)sms ? 32 : rows;
 }
 
 /** Where the parts of a call's workspace lie. */
@@ -671,12 +681,15 @@ static cudaError_t pad_operands(const GatedLayout& l, size_t tokens, size_t widt
 template <typename T, int N> static cudaError_t run_few(int device, FewArgs& a, cudaStream_t stream) {
     static std::atomic<bool> ready[64];
     if (!ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k_gated_few<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<N>::kShared);
+        const cudaError_t e = cudaFuncSetAttribute(k_gated_few<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_relaxed);
     }
     a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, false, false, 128, N);
-    return launch_early_shared(k_gated_few<T, N>, blocks_of(a.ffn, kFewRows), 128, FewShape<N>::kShared, stream, a);
+    // the product of the last stage reads 128 rows of it, and what behind them is inside of the allocation
+    const unsigned bytes = (2 * a.rows + N) * kStageRowsBytes, room = kFewShared - 1024 - 128 * kStageRowsBytes;
+    a.stages = room / bytes < (unsigned)kFewStages ? room / bytes : kFewStages;
+    return launch_early_shared(k_gated_few<T, N>, blocks_of(a.ffn, a.rows), kFewThreads, kFewShared, stream, a);
 }
 
 template <typename T> static cudaError_t gated_forward(int device, int dtype, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up,
@@ -686,8 +699,9 @@ template <typename T> static cudaError_t gated_forward(int device, int dtype, co
         const int columns = tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128;
         FewArgs f = {};
         if (e == cudaSuccess) e = make_map(&f.x, dtype, x, width, tokens, l.stride, columns);
-        if (e == cudaSuccess) e = make_map(&f.w_gate, dtype, w_gate, width, ffn, l.stride, kFewRows);
-        if (e == cudaSuccess) e = make_map(&f.w_up, dtype, w_up, width, ffn, l.stride, kFewRows);
+        f.rows = few_rows(sm_count(device), ffn);
+        if (e == cudaSuccess) e = make_map(&f.w_gate, dtype, w_gate, width, ffn, l.stride, f.rows);
+        if (e == cudaSuccess) e = make_map(&f.w_up, dtype, w_up, width, ffn, l.stride, f.rows);
         if (e != cudaSuccess) return e;
         f.tokens = (unsigned)tokens;
         f.ffn = (unsigned)ffn;
