@@ -59,9 +59,12 @@ long long dccl_gated_linear_workspace(int device, size_t tokens, size_t width, s
 int dccl_gated_linear(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up, int act, void* h,
                       float* g, float* u, size_t pre_stride, void* workspace, long long workspace_bytes, void* stream);
 
+/** Whether the backward pass of these operands needs the workspace of the forward pass, which holds copies of them in rows that start on 16 bytes. */
+int dccl_gated_linear_pads(size_t width, int aligned);
+
 /** Its gradients from dh and the products that it left. Each of dx, and dw_gate with dw_up, may be null. No atomics. */
 int dccl_gated_linear_backward(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* dh, const float* g, const float* u, size_t pre_stride,
-                               const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up, void* workspace,
-                               long long workspace_bytes, void* stream);
+                               const void* x, const void* w_gate, const void* w_up, const void* forward_workspace, int act, void* dx, void* dw_gate, void* dw_up,
+                               void* workspace, long long workspace_bytes, void* stream);
 
 } // extern "C"

@@ -23,7 +23,7 @@ enum Form {
     WEIGHT_GRAD,    // dW = dg^T x, du^T x: k are the tokens, both operands contiguous along rows and columns of the result
 };
 
-constexpr int kTileM = 128, kTileK = 64, kStages = 4;
+constexpr int kTileM = 128, kTileK = 64;
 constexpr int kEpilogueWarps = 8, kGemmThreads = 32 * (kEpilogueWarps + 2);
 constexpr unsigned kLoader = kEpilogueWarps, kMultiplier = kEpilogueWarps + 1;
 constexpr int kStageRowsBytes = 128;                                // one row of a swizzled tile
@@ -136,7 +136,7 @@ __device__ __forceinline__ Place place_of(unsigned tile, const GemmArgs& a) {
 }
 
 template <int FORM, int N> struct GemmShape {
-    static constexpr int kBytesA = kTileM * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB;
+    static constexpr int kBytesA = kTileM * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kBytes;
     static constexpr int kShared = kStages * kBytes + kEpilogueWarps * 4096 + 1024;      // 1024: the tiles' alignment
     static constexpr int kColumns = FORM == GATED ? N / 2 : N;                           // of the result
 };
@@ -149,6 +149,7 @@ template <int FORM, int N> struct GemmShape {
 template <typename T, int FORM, int N>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs a) {
     using Shape = GemmShape<FORM, N>;
+    constexpr int kStages = Shape::kStages;
     extern __shared__ char shared[];
     __shared__ uint64_t bars[2 * kStages + 5];
     __shared__ uint32_t tmem_base;
@@ -577,15 +578,19 @@ static cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, size_
 static size_t up_to(size_t v, size_t step) { return (v + step - 1) / step * step; }
 static unsigned blocks_of(size_t v, size_t block) { return (unsigned)((v + block - 1) / block); }
 
-/** Tiles of a product and the parts that its k is cut into. */
-struct GemmPlan { unsigned tiles_m, tiles_n, batch, splits, k_blocks; size_t partial_bytes; };
+/** Tiles of a product, 256 columns wide or 128, and the parts that its k is cut into. */
+struct GemmPlan { int columns; unsigned tiles_m, tiles_n, batch, splits, k_blocks; size_t partial_bytes; };
 
 static GemmPlan plan_gemm(int sms, int form, size_t m, size_t n, size_t k) {
     GemmPlan p;
     p.tiles_m = blocks_of(m, kTileM);
-    p.tiles_n = blocks_of(n, form == GATED ? 128 : 256);
     p.batch = form == WEIGHT_GRAD ? 2 : 1;
     p.k_blocks = blocks_of(k, kTileK) * (form == INPUT_GRAD ? 2 : 1);
+    // rounds of tiles, and what a round takes: half as wide a tile reads one operand twice as often
+    const auto tiles_n = [&](int columns) { return blocks_of(n, form == GATED ? columns / 2 : columns); };
+    const auto rounds = [&](int columns) { return ((size_t)p.tiles_m * tiles_n(columns) * p.batch + sms - 1) / sms; };
+    p.columns = rounds(128) * 15 < rounds(256) * 26 ? 128 : 256;
+    p.tiles_n = tiles_n(p.columns);
     const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch;
     size_t splits = (size_t)sms / (tiles ? tiles : 1);
     if (splits > p.k_blocks / 4) splits = p.k_blocks / 4;
@@ -594,11 +599,11 @@ static GemmPlan plan_gemm(int sms, int form, size_t m, size_t n, size_t k) {
     return p;
 }
 
-template <typename T, int FORM> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
-    using Shape = GemmShape<FORM, 256>;
+template <typename T, int FORM, int N> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
+    using Shape = GemmShape<FORM, N>;
     static std::atomic<bool> ready[64];
     if (!ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k_gemm<T, FORM, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+        const cudaError_t e = cudaFuncSetAttribute(k_gemm<T, FORM, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_relaxed);
     }
@@ -608,14 +613,18 @@ template <typename T, int FORM> static cudaError_t run_gemm(int device, const Ge
     a.splits = p.splits;
     a.k_blocks = p.k_blocks;
     a.partial_stride = up_to(a.n, 4);
-    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == WEIGHT_GRAD, FORM != GATED, kTileM, 256);
+    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == WEIGHT_GRAD, FORM != GATED, kTileM, N);
     a.gave_up = gave_up_flag();
     const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch * p.splits, sms = (size_t)sm_count(device);
-    cudaError_t e = launch_early_shared(k_gemm<T, FORM, 256>, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, Shape::kShared, stream, a);
+    cudaError_t e = launch_early_shared(k_gemm<T, FORM, N>, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, Shape::kShared, stream, a);
     if (e != cudaSuccess || p.splits == 1) return e;
     const JoinArgs j = {a.partial, a.m, a.partial_stride, a.n, p.splits, p.batch, a.act, a.c0, a.c1, a.g, a.u, a.pre_stride, a.n % 4 == 0 && aligned_to(8, {a.c0, a.c1})};
     const size_t threads = (size_t)a.m * (a.partial_stride / 4) * p.batch;
     return launch_early(k_join<T, FORM == GATED>, (unsigned)((threads + 255) / 256), 256, stream, j);
+}
+
+template <typename T, int FORM> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
+    return p.columns == 128 ? run_gemm<T, FORM, 128>(device, p, a, stream) : run_gemm<T, FORM, 256>(device, p, a, stream);
 }
 
 /** Whether k_gated_few takes a call: for wider layers than it has CTAs for, splits of k read the weights faster. */
@@ -633,7 +642,7 @@ static unsigned few_rows(int sms, size_t ffn) {
 }
 
 /** Where the parts of a call's workspace lie. */
-struct GatedLayout { size_t stride, x, gate, up, dg, du, d_stride, partial, total; GemmPlan forward, input, weight; bool ok; };
+struct GatedLayout { size_t stride, x, gate, up, padded, dg, du, d_stride, partial, total; GemmPlan forward, input, weight; bool ok; };
 
 static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn, bool aligned, bool backward) {
     GatedLayout l = {};
@@ -644,10 +653,12 @@ static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn
     const auto take = [&](size_t bytes) { const size_t here = at; at += up_to(bytes, 256); return here; };
     const bool pad = !aligned || width % 8;
     l.stride = pad ? up_to(width, 8) : width;
-    if (pad) {
+    if (pad) {      // at the same places in both directions: the backward pass finds them in what the forward pass left
         l.x = take(tokens * l.stride * 2);
         l.gate = take(ffn * l.stride * 2);
         l.up = take(ffn * l.stride * 2);
+        l.padded = at;
+        if (backward) at = 0;
     }
     l.d_stride = up_to(ffn, 8);
     size_t partial = 0;
@@ -667,10 +678,10 @@ static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn
 }
 
 /** x, Wg and Wu as the tiled loads take them: in place, or padded into the workspace. */
-static cudaError_t pad_operands(const GatedLayout& l, size_t tokens, size_t width, size_t ffn, bool with_weights, const void*& x, const void*& w_gate, const void*& w_up,
-                                char* workspace, cudaStream_t stream) {
-    if (l.stride == width && aligned_to(16, {x, w_gate, w_up})) return cudaSuccess;
-    PadArgs a = {{x, w_gate, w_up}, {workspace + l.x, workspace + l.gate, workspace + l.up}, {tokens, with_weights ? ffn : 0, with_weights ? ffn : 0}, (unsigned)width, (unsigned)l.stride};
+static cudaError_t pad_operands(const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void*& x, const void*& w_gate, const void*& w_up, char* workspace,
+                                cudaStream_t stream) {
+    if (!l.padded) return cudaSuccess;
+    const PadArgs a = {{x, w_gate, w_up}, {workspace + l.x, workspace + l.gate, workspace + l.up}, {tokens, ffn, ffn}, (unsigned)width, (unsigned)l.stride};
     x = a.to[0];
     w_gate = a.to[1];
     w_up = a.to[2];
@@ -694,7 +705,7 @@ template <typename T, int N> static cudaError_t run_few(int device, FewArgs& a, 
 
 template <typename T> static cudaError_t gated_forward(int device, int dtype, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up,
                                                        int act, void* h, float* g, float* u, size_t pre_stride, char* workspace, cudaStream_t stream) {
-    cudaError_t e = pad_operands(l, tokens, width, ffn, true, x, w_gate, w_up, workspace, stream);
+    cudaError_t e = pad_operands(l, tokens, width, ffn, x, w_gate, w_up, workspace, stream);
     if (few_tokens(sm_count(device), tokens, width, ffn)) {
         const int columns = tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128;
         FewArgs f = {};
@@ -717,8 +728,8 @@ template <typename T> static cudaError_t gated_forward(int device, int dtype, co
     }
     GemmArgs a = {};
     if (e == cudaSuccess) e = make_map(&a.a0, dtype, x, width, tokens, l.stride, kTileM);
-    if (e == cudaSuccess) e = make_map(&a.b0, dtype, w_gate, width, ffn, l.stride, 128);
-    if (e == cudaSuccess) e = make_map(&a.b1, dtype, w_up, width, ffn, l.stride, 128);
+    if (e == cudaSuccess) e = make_map(&a.b0, dtype, w_gate, width, ffn, l.stride, l.forward.columns / 2);
+    if (e == cudaSuccess) e = make_map(&a.b1, dtype, w_up, width, ffn, l.stride, l.forward.columns / 2);
     if (e != cudaSuccess) return e;
     a.m = (unsigned)tokens;
     a.n = (unsigned)ffn;
@@ -732,12 +743,16 @@ template <typename T> static cudaError_t gated_forward(int device, int dtype, co
 }
 
 template <typename T> static cudaError_t gated_backward(int device, int dtype, const GatedLayout& l, size_t tokens, size_t width, size_t ffn, const void* dh, const float* g, const float* u,
-                                                        size_t pre_stride, const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up,
-                                                        char* workspace, cudaStream_t stream) {
+                                                        size_t pre_stride, const void* x, const void* w_gate, const void* w_up, const char* padded, int act, void* dx, void* dw_gate,
+                                                        void* dw_up, char* workspace, cudaStream_t stream) {
     const GateGradArgs d = {dh, g, u, workspace + l.dg, workspace + l.du, pre_stride, l.d_stride, (unsigned)tokens, (unsigned)ffn, act};
     const size_t threads = tokens * ((ffn + 7) / 8);
     cudaError_t e = launch_early(ffn % 8 == 0 && aligned_to(16, {dh}) ? k_gate_grad<T, true> : k_gate_grad<T, false>, (unsigned)((threads + 255) / 256), 256, stream, d);
-    if (e == cudaSuccess) e = pad_operands(l, tokens, width, ffn, dx != nullptr, x, w_gate, w_up, workspace, stream);
+    if (l.padded) {
+        x = padded + l.x;
+        w_gate = padded + l.gate;
+        w_up = padded + l.up;
+    }
     GemmArgs a = {};
     a.partial = (float*)(workspace + l.partial);
     if (e == cudaSuccess && dx) {
@@ -777,6 +792,8 @@ static bool gave_up(const char* who) {
 
 using namespace dccl;
 
+extern "C" int dccl_gated_linear_pads(size_t width, int aligned) { return !aligned || width % 8; }
+
 extern "C" long long dccl_gated_linear_workspace(int device, size_t tokens, size_t width, size_t ffn, int aligned, int backward) {
     const GatedLayout l = layout_of(device, tokens, width, ffn, aligned != 0, backward != 0);
     return l.ok ? (long long)l.total : -1;
@@ -798,16 +815,18 @@ extern "C" int dccl_gated_linear(int device, int dtype, size_t tokens, size_t wi
 }
 
 extern "C" int dccl_gated_linear_backward(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* dh, const float* g, const float* u, size_t pre_stride,
-                                          const void* x, const void* w_gate, const void* w_up, int act, void* dx, void* dw_gate, void* dw_up, void* workspace,
-                                          long long workspace_bytes, void* stream) {
+                                          const void* x, const void* w_gate, const void* w_up, const void* forward_workspace, int act, void* dx, void* dw_gate,
+                                          void* dw_up, void* workspace, long long workspace_bytes, void* stream) {
     const char* who = "dccl_gated_linear_backward";
     const GatedLayout l = layout_of(device, tokens, width, ffn, aligned_to(16, {x, w_gate, w_up}), true);
     if (!l.ok || !tokens || !width || !ffn || workspace_bytes < (long long)l.total || (dtype != 6 && dtype != 9) || act < 0 || act > DCCL_ACT_GELU_TANH || !g || !u
-        || pre_stride < ffn || pre_stride % 4 || !aligned_to(16, {g, u, workspace}) || (!dw_gate != !dw_up))
+        || pre_stride < ffn || pre_stride % 4 || !aligned_to(16, {g, u, workspace, forward_workspace}) || (!dw_gate != !dw_up)
+        || (l.padded && !forward_workspace))
         return report(who, cudaErrorInvalidValue);
     if (gave_up(who)) return -1;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
     const auto run = dtype == 6 ? gated_backward<__half> : gated_backward<__nv_bfloat16>;
-    return report(who, run(device, dtype, l, tokens, width, ffn, dh, g, u, pre_stride, x, w_gate, w_up, act, dx, dw_gate, dw_up, (char*)workspace, (cudaStream_t)stream));
+    return report(who, run(device, dtype, l, tokens, width, ffn, dh, g, u, pre_stride, x, w_gate, w_up, (const char*)forward_workspace, act, dx, dw_gate, dw_up, (char*)workspace,
+                           (cudaStream_t)stream));
 }

@@ -33,6 +33,7 @@ struct Entries {
     decltype(&dccl_residual_norm_backward) norm_backward;
     decltype(&dccl_rotary) rotary;
     decltype(&dccl_gated_linear_workspace) gated_workspace;
+    decltype(&dccl_gated_linear_pads) gated_pads;
     decltype(&dccl_gated_linear) gated;
     decltype(&dccl_gated_linear_backward) gated_backward;
 } entry;
@@ -360,17 +361,20 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 /* ---------------------------------------------------------------------------------------------- gated linear */
 
+bool gated_aligned(const Tensor& x, const Tensor& w_gate, const Tensor& w_up) {
+    return ((uintptr_t)x.data_ptr() | (uintptr_t)w_gate.data_ptr() | (uintptr_t)w_up.data_ptr()) % 16 == 0;
+}
+
 /** The workspace of a call; undefined where it needs none. */
 Tensor gated_work(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, bool backward) {
-    const uintptr_t low = (uintptr_t)x.data_ptr() | (uintptr_t)w_gate.data_ptr() | (uintptr_t)w_up.data_ptr();
-    const long long bytes = entry.gated_workspace(x.device().index(), x.numel() / x.size(-1), x.size(-1), w_gate.size(0), low % 16 == 0, backward);
+    const long long bytes = entry.gated_workspace(x.device().index(), x.numel() / x.size(-1), x.size(-1), w_gate.size(0), gated_aligned(x, w_gate, w_up), backward);
     TORCH_CHECK(bytes >= 0, "gated_linear: sizes that it does not take");
     return bytes ? fresh({(int64_t)bytes}, at::kByte, x) : Tensor();
 }
 
 struct GatedBackward : public Node {
     SavedVariable x, w_gate, w_up;
-    Tensor g, u;
+    Tensor g, u, padded;
     int act = 0;
 
     variable_list apply(variable_list&& grads) override {
@@ -384,8 +388,8 @@ struct GatedBackward : public Node {
         const int64_t width = x_.size(-1), tokens = x_.numel() / width;
         if (tokens) {
             const Tensor work = gated_work(x_, wg, wu, true);
-            const int rc = entry.gated_backward(x_.device().index(), dtype_of(x_), tokens, width, wg.size(0), ptr(dh), ptr<float>(g), ptr<float>(u), g.size(1), ptr(x_), ptr(wg), ptr(wu), act,
-                                                ptr(dx), ptr(dg), ptr(du), ptr(work), work.defined() ? (long long)work.numel() : 0, stream_of(x_));
+            const int rc = entry.gated_backward(x_.device().index(), dtype_of(x_), tokens, width, wg.size(0), ptr(dh), ptr<float>(g), ptr<float>(u), g.size(1), ptr(x_), ptr(wg), ptr(wu),
+                                                ptr(padded), act, ptr(dx), ptr(dg), ptr(du), ptr(work), work.defined() ? (long long)work.numel() : 0, stream_of(x_));
             TORCH_CHECK(rc == 0, "gated_linear: the backward pass was not launched (see stderr)");
         } else if (weights) {
             dg.zero_();
@@ -397,8 +401,7 @@ struct GatedBackward : public Node {
     std::string name() const override { return "GatedLinearBackward"; }
     void release_variables() override {
         for (SavedVariable* v : {&x, &w_gate, &w_up}) v->reset_data();
-        g.reset();
-        u.reset();
+        for (Tensor* t : {&g, &u, &padded}) t->reset();
     }
 };
 
@@ -432,8 +435,9 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             g = fresh({tokens, stride}, at::kFloat, x);
             u = fresh({tokens, stride}, at::kFloat, x);
         }
+        Tensor work;
         if (tokens) {
-            const Tensor work = gated_work(x, wg, wu, false);
+            work = gated_work(x, wg, wu, false);
             const int rc = entry.gated(x.device().index(), dtype, tokens, width, ffn, ptr(x), ptr(wg), ptr(wu), act, ptr(h), ptr<float>(g), ptr<float>(u), stride, ptr(work),
                                        work.defined() ? (long long)work.numel() : 0, stream_of(x));
             TORCH_CHECK(rc == 0, "gated_linear was not launched (see stderr)");
@@ -446,6 +450,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             node->w_up = SavedVariable(wu, false);
             node->g = g;
             node->u = u;
+            if (entry.gated_pads(width, gated_aligned(x, wg, wu))) node->padded = work;
             node->act = act;
             torch::autograd::set_history(h, node);
         }
@@ -457,16 +462,16 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 /** decoder_ops_bind(addresses of the entry points, in the order of Entries). */
 PyObject* decoder_ops_bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    void* at[7];
-    TORCH_CHECK(nargs == 7, "decoder_ops_bind takes seven addresses");
-    for (int i = 0; i < 7; i++) {
+    void* at[8];
+    TORCH_CHECK(nargs == 8, "decoder_ops_bind takes eight addresses");
+    for (int i = 0; i < 8; i++) {
         at[i] = PyLong_AsVoidPtr(args[i]);
         if (PyErr_Occurred()) return nullptr;
         TORCH_CHECK(at[i], "decoder_ops_bind: an address is missing");
     }
     entry = {reinterpret_cast<decltype(entry.norm)>(at[0]), reinterpret_cast<decltype(entry.norm_workspace)>(at[1]), reinterpret_cast<decltype(entry.norm_backward)>(at[2]),
-             reinterpret_cast<decltype(entry.rotary)>(at[3]), reinterpret_cast<decltype(entry.gated_workspace)>(at[4]), reinterpret_cast<decltype(entry.gated)>(at[5]),
-             reinterpret_cast<decltype(entry.gated_backward)>(at[6])};
+             reinterpret_cast<decltype(entry.rotary)>(at[3]), reinterpret_cast<decltype(entry.gated_workspace)>(at[4]), reinterpret_cast<decltype(entry.gated_pads)>(at[5]),
+             reinterpret_cast<decltype(entry.gated)>(at[6]), reinterpret_cast<decltype(entry.gated_backward)>(at[7])};
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }

@@ -114,7 +114,8 @@ def _declare(lib):
         "dccl_rotary": (i, [i, i, sz, sz, i, i, i, i, vp, vp, vp, vp, i, c.c_longlong, c.c_longlong, c.c_longlong, c.c_double, vp]),
         "dccl_gated_linear_workspace": (c.c_longlong, [i, sz, sz, sz, i, i]),
         "dccl_gated_linear": (i, [i, i, sz, sz, sz, vp, vp, vp, i, vp, vp, vp, sz, vp, c.c_longlong, vp]),
-        "dccl_gated_linear_backward": (i, [i, i, sz, sz, sz, vp, vp, vp, sz, vp, vp, vp, i, vp, vp, vp, vp, c.c_longlong, vp]),
+        "dccl_gated_linear_pads": (i, [sz, i]),
+        "dccl_gated_linear_backward": (i, [i, i, sz, sz, sz, vp, vp, vp, sz, vp, vp, vp, vp, i, vp, vp, vp, vp, c.c_longlong, vp]),
         "dccl_emu_early_producer": (i, [vp, vp, sz, c.c_uint, vp, vp]),
         "dccl_emu_early_observer": (i, [vp, vp]),
         "dccl_debug_bounds_build": (i, []),

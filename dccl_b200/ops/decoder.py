@@ -30,8 +30,8 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MAX_WIDTH, _MAX_PAIRS = 32768, 1024                 # kNormMaxWidth of csrc/kernels/residual_norm.cu, kRotaryPairs of rotary.cu
 
 
-_ENTRIES = ("dccl_residual_norm", "dccl_residual_norm_workspace", "dccl_residual_norm_backward", "dccl_rotary", "dccl_gated_linear_workspace", "dccl_gated_linear",
-            "dccl_gated_linear_backward")
+_ENTRIES = ("dccl_residual_norm", "dccl_residual_norm_workspace", "dccl_residual_norm_backward", "dccl_rotary", "dccl_gated_linear_workspace", "dccl_gated_linear_pads",
+            "dccl_gated_linear", "dccl_gated_linear_backward")
 _native = None
 
 
