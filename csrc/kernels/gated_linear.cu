@@ -135,20 +135,20 @@ __device__ __forceinline__ Place place_of(unsigned tile, const GemmArgs& a) {
     return p;
 }
 
-template <int FORM, int N> struct GemmShape {
-    static constexpr int kBytesA = kTileM * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kBytes;
+template <int FORM, int N, bool PAIR> struct GemmShape {
+    static constexpr int kRows = PAIR ? 2 * kTileM : kTileM, kHeldN = PAIR ? N / 2 : N;      // rows of a tile; columns whose operand one CTA holds
+    static constexpr int kBytesA = kTileM * kTileK * 2, kBytesB = kHeldN * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kBytes;
     static constexpr int kShared = kStages * kBytes + kEpilogueWarps * 4096 + 1024;      // 1024: the tiles' alignment
     static constexpr int kColumns = FORM == GATED ? N / 2 : N;                           // of the result
 };
 
 /**
  * One CTA per SM walks over tiles of 128 rows; one warp loads, one multiplies, eight store: a warp reaches the quarter of the tile's
- * rows that its number gives, so two share one and take half of the columns each. The sums of two tiles fit into
- * tensor memory, so that one is stored while the next is multiplied.
+ * rows that its number gives, so two share one and take half of the columns each. The sums of two tiles fit into tensor memory, so that
+ * one is stored while the next is multiplied. As a PAIR, two CTAs share tiles of 256 rows, and each loads only half of the columns' operand.
  */
-template <typename T, int FORM, int N>
-__global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs a) {
-    using Shape = GemmShape<FORM, N>;
+template <typename T, int FORM, int N, bool PAIR> __device__ __forceinline__ void gemm(const GemmArgs& a) {
+    using Shape = GemmShape<FORM, N, PAIR>;
     constexpr int kStages = Shape::kStages;
     extern __shared__ char shared[];
     __shared__ uint64_t bars[2 * kStages + 5];
@@ -157,12 +157,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
     char* const staging = tiles + kStages * Shape::kBytes;
     const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16, drained = sums_empty + 16;
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (warp == kMultiplier) tmem_alloc(shared_addr(&tmem_base), 2 * N);
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = PAIR ? cluster_rank() : 0;
+    if (warp == kMultiplier) {
+        if constexpr (PAIR) pair_tmem_alloc(shared_addr(&tmem_base), 2 * N);
+        else tmem_alloc(shared_addr(&tmem_base), 2 * N);
+    }
     if (threadIdx.x == 0) {
         failed = 0;
         for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
-        for (int i = 0; i < 2; i++) { bar_init(sums_full + 8 * i, 1); bar_init(sums_empty + 8 * i, kEpilogueWarps); }
+        for (int i = 0; i < 2; i++) { bar_init(sums_full + 8 * i, 1); bar_init(sums_empty + 8 * i, (PAIR ? 2 : 1) * kEpilogueWarps); }
         bar_init(drained, 1);
         bar_init_fence();
     }
@@ -174,45 +177,53 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     }
     tc_before_sync();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();
     tc_after_sync();
     const uint32_t sums = tmem_base;
     wait_for_stream();
-    const unsigned total = a.tiles_m * a.tiles_n * a.batch * a.splits;
+    const unsigned total = a.tiles_m * a.tiles_n * a.batch * a.splits, first = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
     unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
     if (warp == kLoader && lane == 0) {
-        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+        const auto load = [&](uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
+            if constexpr (PAIR) pair_load_box(to, map, x, y, bar);
+            else load_box(to, map, x, y, bar);
+        };
+        for (unsigned tile = first; tile < total; tile += step) {
             const Place p = place_of(tile, a);
             const unsigned from = (unsigned)((unsigned long long)a.k_blocks * p.split / a.splits), to = (unsigned)((unsigned long long)a.k_blocks * (p.split + 1) / a.splits);
-            const int row = p.m * kTileM, column = p.n * Shape::kColumns;
+            const int row = p.m * Shape::kRows + rank * kTileM, column = p.n * Shape::kColumns + (FORM == GATED ? 0 : rank * Shape::kHeldN);
             unsigned kb = from;
             for (; kb < to; kb++, filled++) {
                 const unsigned s = filled % kStages;
                 if (!bar_wait(empty + 8 * s, (filled / kStages & 1) ^ 1, &failed)) break;
-                const uint32_t bar = full + 8 * s, to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA;
-                bar_expect(bar, Shape::kBytes);
+                const uint32_t to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA, bar = PAIR ? in_cta(full + 8 * s, 0) : full + 8 * s;
+                if (rank == 0) bar_expect(full + 8 * s, (PAIR ? 2 : 1) * Shape::kBytes);       // the leader counts both CTAs' bytes
                 if constexpr (FORM == GATED) {
-                    load_box(to_a, &a.a0, kb * kTileK, row, bar);
-                    load_box(to_b, &a.b0, kb * kTileK, column, bar);
-                    load_box(to_b + Shape::kBytesB / 2, &a.b1, kb * kTileK, column, bar);
+                    load(to_a, &a.a0, kb * kTileK, row, bar);
+                    if constexpr (PAIR) load(to_b, rank ? &a.b1 : &a.b0, kb * kTileK, column, bar);
+                    else {
+                        load(to_b, &a.b0, kb * kTileK, column, bar);
+                        load(to_b + Shape::kBytesB / 2, &a.b1, kb * kTileK, column, bar);
+                    }
                 } else if constexpr (FORM == INPUT_GRAD) {
                     const bool second = kb >= a.k_half;
                     const int k = (second ? kb - a.k_half : kb) * kTileK;
-                    load_box(to_a, second ? &a.a1 : &a.a0, k, row, bar);
+                    load(to_a, second ? &a.a1 : &a.a0, k, row, bar);
 #pragma unroll
-                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * kStageRowsBytes, second ? &a.b1 : &a.b0, column + 64 * i, k, bar);
+                    for (int i = 0; i < Shape::kHeldN / 64; i++) load(to_b + i * 64 * kStageRowsBytes, second ? &a.b1 : &a.b0, column + 64 * i, k, bar);
                 } else {
                     const CUtensorMap* map = p.batch ? &a.a1 : &a.a0;
 #pragma unroll
-                    for (int i = 0; i < kTileM / 64; i++) load_box(to_a + i * 64 * kStageRowsBytes, map, row + 64 * i, kb * kTileK, bar);
+                    for (int i = 0; i < kTileM / 64; i++) load(to_a + i * 64 * kStageRowsBytes, map, row + 64 * i, kb * kTileK, bar);
 #pragma unroll
-                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * kStageRowsBytes, &a.b0, column + 64 * i, kb * kTileK, bar);
+                    for (int i = 0; i < Shape::kHeldN / 64; i++) load(to_b + i * 64 * kStageRowsBytes, &a.b0, column + 64 * i, kb * kTileK, bar);
                 }
             }
             if (kb < to) break;
         }
-    } else if (warp == kMultiplier && lane == 0) {
+    } else if (warp == kMultiplier && lane == 0 && rank == 0) {
         unsigned done = 0;
-        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
+        for (unsigned tile = first; tile < total; tile += step, done++) {
             const Place p = place_of(tile, a);
             const unsigned from = (unsigned)((unsigned long long)a.k_blocks * p.split / a.splits), to = (unsigned)((unsigned long long)a.k_blocks * (p.split + 1) / a.splits);
             const unsigned buffer = done & 1;
@@ -230,25 +241,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                     // 16 k: 32 bytes further along K-major rows, or 16 rows of 128 bytes further
                     const uint64_t da = FORM == WEIGHT_GRAD ? tile_descriptor(at_a + k * 2048, 64 * kStageRowsBytes) : tile_descriptor(at_a + k * 32, 16);
                     const uint64_t db = FORM == GATED ? tile_descriptor(at_b + k * 32, 16) : tile_descriptor(at_b + k * 2048, 64 * kStageRowsBytes);
-                    product(d, da, db, a.descriptor, kb > from || k);
+                    if constexpr (PAIR) pair_product(d, da, db, a.descriptor, kb > from || k);
+                    else product(d, da, db, a.descriptor, kb > from || k);
                 }
-                commit(empty + 8 * s);
+                if constexpr (PAIR) pair_commit(empty + 8 * s);
+                else commit(empty + 8 * s);
             }
             if (kb < to) break;
-            commit(sums_full + 8 * buffer);
+            if constexpr (PAIR) pair_commit(sums_full + 8 * buffer);
+            else commit(sums_full + 8 * buffer);
         }
     } else if (warp < kEpilogueWarps) {
         char* const stage = staging + warp * 4096;
         unsigned done = 0;
         const bool vec = a.n % 8 == 0 && aligned16(a.c0) && aligned16(a.c1);
-        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
+        for (unsigned tile = first; tile < total; tile += step, done++) {
             const Place p = place_of(tile, a);
             const unsigned buffer = done & 1;
             if (!bar_wait_warp(sums_full + 8 * buffer, done / 2 & 1, &failed)) break;
             tc_after_sync();
             const unsigned quarter = warp % 4, half = warp / 4;
             const uint32_t d = sums + buffer * N + (quarter * 32u << 16);
-            const size_t row = (size_t)p.m * kTileM + quarter * 32;
+            const size_t row = (size_t)p.m * Shape::kRows + rank * kTileM + quarter * 32;
             const int rows = row < a.m ? (int)(a.m - row < 32 ? a.m - row : 32) : 0;
 #pragma unroll 1
             for (int c = half * (Shape::kColumns / 2); c < (int)(half + 1) * (Shape::kColumns / 2); c += 32) {
@@ -293,24 +307,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             }
             tc_before_sync();
             __syncwarp();
-            if (lane == 0) bar_arrive(sums_empty + 8 * buffer);
+            if (lane == 0) {
+                if constexpr (PAIR) bar_arrive_remote(in_cta(sums_empty + 8 * buffer, 0));
+                else bar_arrive(sums_empty + 8 * buffer);
+            }
         }
     }
     __syncthreads();
     if (failed) {       // no wait is expected to run out: copies in flight still have to land, and products to end, before the memory is given back
         int late = 0;
-        if (warp == kLoader && lane == 0)
+        if (warp == kLoader && lane == 0 && rank == 0)
             for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
-        if (warp == kMultiplier && lane == 0) {
-            commit(drained);
+        if (warp == kMultiplier && lane == 0 && rank == 0) {
+            if constexpr (PAIR) pair_commit(drained);
+            else commit(drained);
             bar_wait(drained, 0, &late);
         }
         if (threadIdx.x == 0 && a.gave_up) *reinterpret_cast<volatile int*>(a.gave_up) = 1;
         __syncthreads();
     }
+    if constexpr (PAIR) cluster_sync();      // neither CTA's memory goes before the other is done with it
     tc_after_sync();
-    if (warp == kMultiplier) tmem_free(sums, 2 * N);
+    if (warp == kMultiplier) {
+        if constexpr (PAIR) pair_tmem_free(sums, 2 * N);
+        else tmem_free(sums, 2 * N);
+    }
 }
+
+template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs a) { gemm<T, FORM, N, false>(a); }
+template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1) k_gemm_pair(const __grid_constant__ GemmArgs a) { gemm<T, FORM, N, true>(a); }
 
 /* ---- few tokens ---- */
 
@@ -579,31 +604,34 @@ static size_t up_to(size_t v, size_t step) { return (v + step - 1) / step * step
 static unsigned blocks_of(size_t v, size_t block) { return (unsigned)((v + block - 1) / block); }
 
 /** Tiles of a product, 256 columns wide or 128, and the parts that its k is cut into. */
-struct GemmPlan { int columns; unsigned tiles_m, tiles_n, batch, splits, k_blocks; size_t partial_bytes; };
+struct GemmPlan { bool pair; int columns; unsigned tiles_m, tiles_n, batch, splits, k_blocks; size_t partial_bytes; };
 
 static GemmPlan plan_gemm(int sms, int form, size_t m, size_t n, size_t k) {
     GemmPlan p;
-    p.tiles_m = blocks_of(m, kTileM);
+    p.pair = m > kTileM;
+    p.tiles_m = blocks_of(m, p.pair ? 2 * kTileM : kTileM);
     p.batch = form == WEIGHT_GRAD ? 2 : 1;
     p.k_blocks = blocks_of(k, kTileK) * (form == INPUT_GRAD ? 2 : 1);
+    const unsigned workers = p.pair ? sms / 2 : sms;
     // rounds of tiles, and what a round takes: half as wide a tile reads one operand twice as often
     const auto tiles_n = [&](int columns) { return blocks_of(n, form == GATED ? columns / 2 : columns); };
-    const auto rounds = [&](int columns) { return ((size_t)p.tiles_m * tiles_n(columns) * p.batch + sms - 1) / sms; };
+    const auto rounds = [&](int columns) { return ((size_t)p.tiles_m * tiles_n(columns) * p.batch + workers - 1) / workers; };
     p.columns = rounds(128) * 15 < rounds(256) * 26 ? 128 : 256;
     p.tiles_n = tiles_n(p.columns);
     const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch;
-    size_t splits = (size_t)sms / (tiles ? tiles : 1);
+    size_t splits = workers / (tiles ? tiles : 1);
     if (splits > p.k_blocks / 4) splits = p.k_blocks / 4;
     p.splits = splits > 1 ? (unsigned)splits : 1;
     p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (form == INPUT_GRAD ? 1 : 2) * m * up_to(n, 4) * sizeof(float) : 0;
     return p;
 }
 
-template <typename T, int FORM, int N> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
-    using Shape = GemmShape<FORM, N>;
+template <typename T, int FORM, int N, bool PAIR> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
+    using Shape = GemmShape<FORM, N, PAIR>;
+    void (*const kernel)(const GemmArgs) = PAIR ? k_gemm_pair<T, FORM, N> : k_gemm<T, FORM, N>;
     static std::atomic<bool> ready[64];
     if (!ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k_gemm<T, FORM, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_relaxed);
     }
@@ -613,10 +641,10 @@ template <typename T, int FORM, int N> static cudaError_t run_gemm(int device, c
     a.splits = p.splits;
     a.k_blocks = p.k_blocks;
     a.partial_stride = up_to(a.n, 4);
-    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == WEIGHT_GRAD, FORM != GATED, kTileM, N);
+    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == WEIGHT_GRAD, FORM != GATED, Shape::kRows, N);
     a.gave_up = gave_up_flag();
-    const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch * p.splits, sms = (size_t)sm_count(device);
-    cudaError_t e = launch_early_shared(k_gemm<T, FORM, N>, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, Shape::kShared, stream, a);
+    const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch * p.splits, workers = PAIR ? sm_count(device) / 2 : sm_count(device);
+    cudaError_t e = launch_early_shared(kernel, (unsigned)(tiles < workers ? tiles : workers) * (PAIR ? 2 : 1), kGemmThreads, Shape::kShared, stream, a);
     if (e != cudaSuccess || p.splits == 1) return e;
     const JoinArgs j = {a.partial, a.m, a.partial_stride, a.n, p.splits, p.batch, a.act, a.c0, a.c1, a.g, a.u, a.pre_stride, a.n % 4 == 0 && aligned_to(8, {a.c0, a.c1})};
     const size_t threads = (size_t)a.m * (a.partial_stride / 4) * p.batch;
@@ -624,7 +652,8 @@ template <typename T, int FORM, int N> static cudaError_t run_gemm(int device, c
 }
 
 template <typename T, int FORM> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
-    return p.columns == 128 ? run_gemm<T, FORM, 128>(device, p, a, stream) : run_gemm<T, FORM, 256>(device, p, a, stream);
+    if (p.pair) return p.columns == 128 ? run_gemm<T, FORM, 128, true>(device, p, a, stream) : run_gemm<T, FORM, 256, true>(device, p, a, stream);
+    return p.columns == 128 ? run_gemm<T, FORM, 128, false>(device, p, a, stream) : run_gemm<T, FORM, 256, false>(device, p, a, stream);
 }
 
 /** Whether k_gated_few takes a call: for wider layers than it has CTAs for, splits of k read the weights faster. */
