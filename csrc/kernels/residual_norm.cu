@@ -37,7 +37,7 @@ struct NormGradArgs {
     const float *rstd, *rstd_post;
     void *dx, *dbranch;
     float *weight_sums, *post_sums, *gate_sums;      // [CTA][width], [CTA][width], [unit][width]
-    size_t rows_per_gate, chunks, units;
+    size_t rows, rows_per_gate, chunks, units;
     unsigned width;
     int f32;
     float scale;
@@ -129,45 +129,71 @@ enum { DN, Y, DY, B };
 enum { IN_WEIGHT, IN_POST, IN_GATE };   // the vectors, in shared memory as fp32
 constexpr int FULL = POST | GATE | SCALE;
 
-/** Rows in shared memory at a time, where accesses are 16 bytes wide: three of up to 2048 elements, two of up to 8192 16-bit ones. */
-template <typename T, int V, int E> constexpr int kNormStages = V * sizeof(T) != 16 ? 0 : E == 8 ? 3 : E == 16 && sizeof(T) == 2 ? 2 : 0;
+/** Rows in shared memory at a time: three of up to 2048 elements, two of up to 8192 16-bit ones. */
+template <typename T, int E> constexpr int kNormStages = E == 8 ? 3 : E == 16 && sizeof(T) == 2 ? 2 : 0;
 
-template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(unsigned threads) {
-    return (size_t)threads * E * (kNormStages<T, V, E> * (F & FULL ? 4 : 3) * sizeof(T) + (E <= 16 ? (F & FULL ? 3 : 1) * sizeof(float) : 0));
+/** Bytes of an array's row there: a place for each thread's accesses, or, where rows start anywhere, the aligned 16 bytes that a row touches. */
+template <typename T, int V, int E> __host__ __device__ constexpr size_t norm_row_bytes(unsigned threads, unsigned width) {
+    return V * sizeof(T) == 16 ? (size_t)threads * E * sizeof(T) : (width * sizeof(T) + 15) / 16 * 16 + 16;
+}
+
+template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(unsigned threads, unsigned width) {
+    return kNormStages<T, E> * (F & FULL ? 4 : 3) * norm_row_bytes<T, V, E>(threads, width) + (E <= 16 ? (size_t)threads * E * (F & FULL ? 3 : 1) * sizeof(float) : 0);
 }
 
 /**
  * Each CTA takes units of rows that share a row of the gate and keeps the columns' sums (dw, dw2, dg) in registers: dg leaves at
- * the end of a unit, dw and dw2 at the end of the CTA, for k_norm_columns to add. Where accesses are 16 bytes wide a thread copies
- * its own elements of the next rows into shared memory of its own while it works on this one, and it keeps its part of the vectors
- * there in fp32: no register holds them and no barrier guards them.
+ * the end of a unit, dw and dw2 at the end of the CTA, for k_norm_columns to add. The next rows are copied into shared memory while
+ * the CTA works on this one: where accesses are 16 bytes wide, each thread's own elements by itself, with no barrier to guard them. Rows
+ * that start anywhere are copied in the aligned 16 bytes that they touch, which the threads share. (Read by element from global memory,
+ * rows of 1451 fp16 took 36 us out of L2 and 60 out of HBM for 1551 rows.) The vectors are kept there in fp32.
  */
 template <typename T, int V, int E, int F>
 __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? (F & FULL ? 3 : 4) : 1) k_residual_norm_grad(const __grid_constant__ NormGradArgs a) {
     wait_for_stream();
-    constexpr int K = E / V, kArrays = F & FULL ? 4 : 3, kStages = kNormStages<T, V, E>, kPiece = V < 4 ? V : 4;
+    constexpr int K = E / V, kArrays = F & FULL ? 4 : 3, kStages = kNormStages<T, E>, kPiece = V < 4 ? V : 4;
+    constexpr bool kOwn = V * sizeof(T) == 16;          // a thread's elements are its own matter
     constexpr bool kVectors = E <= 16;                  // in shared memory
     extern __shared__ uint4 staged[];                   // [stage][array][run][thread], then [vector][run][piece][thread] of kPiece floats
     __shared__ __align__(16) float parts[2][2][32];
     const unsigned runs = a.width / V, step = blockDim.x, t = threadIdx.x;
     const float inv_width = 1.0f / a.width;
     const T* const arrays[4] = {reinterpret_cast<const T*>(a.dn), reinterpret_cast<const T*>(a.y), reinterpret_cast<const T*>(a.dy), reinterpret_cast<const T*>(a.branch)};
-    Run<float, kPiece>* const vectors = reinterpret_cast<Run<float, kPiece>*>(staged + (size_t)kStages * kArrays * K * step);
+    const unsigned row_bytes = (unsigned)norm_row_bytes<T, V, E>(step, a.width);
+    Run<float, kPiece>* const vectors = reinterpret_cast<Run<float, kPiece>*>(reinterpret_cast<char*>(staged) + (size_t)kStages * kArrays * row_bytes);
     const auto fetch = [&](size_t row, unsigned stage) {
+        if constexpr (!kOwn) {
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const unsigned i = t + k * step;
-#pragma unroll
-            for (int j = 0; j < kArrays; j++)
-                if (i < runs && arrays[j]) {
-                    const uint32_t to = (uint32_t)__cvta_generic_to_shared(staged + ((stage * kArrays + j) * K + k) * step + t);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(arrays[j] + row * a.width + (size_t)i * V) : "memory");
+            for (int j = 0; j < kArrays; j++) {
+                if (!arrays[j]) continue;
+                const uintptr_t start = reinterpret_cast<uintptr_t>(arrays[j] + row * a.width), end = reinterpret_cast<uintptr_t>(arrays[j] + a.rows * a.width);
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(staged) + (stage * kArrays + j) * row_bytes;
+                const unsigned pieces = (unsigned)(((start & 15) + a.width * sizeof(T) + 15) / 16);
+                for (unsigned i = t; i < pieces; i += step) {
+                    const uintptr_t from = (start & ~(uintptr_t)15) + 16 * (size_t)i;
+                    const unsigned bytes = end - from < 16 ? (unsigned)(end - from) : 16;      // nothing is read behind the last row
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 16 * i), "l"(from), "r"(bytes) : "memory");
                 }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const unsigned i = t + k * step;
+#pragma unroll
+                for (int j = 0; j < kArrays; j++)
+                    if (i < runs && arrays[j]) {
+                        const uint32_t to = (uint32_t)__cvta_generic_to_shared(staged + ((stage * kArrays + j) * K + k) * step + t);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(arrays[j] + row * a.width + (size_t)i * V) : "memory");
+                    }
+            }
         }
     };
     const auto load = [&](int j, int k, size_t row, unsigned stage, float (&f)[V]) {
         Run<T, V> r;
-        if constexpr (kStages > 0) r = *reinterpret_cast<const Run<T, V>*>(staged + ((stage * kArrays + j) * K + k) * step + t);
+        if constexpr (kStages > 0 && !kOwn) {
+            const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(arrays[j] + row * a.width) & 15);
+            r = *reinterpret_cast<const Run<T, V>*>(reinterpret_cast<const char*>(staged) + (stage * kArrays + j) * row_bytes + shift + (t + k * step) * sizeof(T));
+        } else if constexpr (kStages > 0) r = *reinterpret_cast<const Run<T, V>*>(staged + ((stage * kArrays + j) * K + k) * step + t);
         else r = ld_run<T, V>(arrays[j] + row * a.width + (size_t)(t + k * step) * V);
 #pragma unroll
         for (int e = 0; e < V; e++) f[e] = Traits<T>::up(r.e[e]);
@@ -217,6 +243,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
         const size_t begin = gate * a.rows_per_gate + chunk * a.rows_per_gate / a.chunks, end = gate * a.rows_per_gate + (chunk + 1) * a.rows_per_gate / a.chunks;
         unsigned stage = 0;
         if constexpr (kStages > 0) {
+            if constexpr (!kOwn) __syncthreads();       // the last unit's rows
 #pragma unroll
             for (int s = 0; s < kStages - 1; s++) {
                 if (begin + s < end) fetch(begin + s, s);
@@ -229,9 +256,13 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
         for (size_t row = begin; row < end; row++, turn ^= 1) {
             if constexpr (kStages > 0) {
                 const unsigned ahead = stage == 0 ? kStages - 1 : stage - 1;
+                if constexpr (!kOwn) {      // this row is there, and every thread is done with the one before, whose place the next one takes
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                    __syncthreads();
+                }
                 if (row + kStages - 1 < end) fetch(row + kStages - 1, ahead);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+                if constexpr (kOwn) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             }
             const float ry = next_ry, rb = next_rb;
             if (row + 1 < end) {
@@ -415,10 +446,10 @@ struct NormCut { size_t chunks, units; unsigned ctas; };
 static NormCut norm_cut(int device, int dtype, size_t rows, size_t width, size_t gates, bool full) {
     const NormShape s = norm_shape(width);
     const bool wide = dtype == 7;
-    const size_t shared = s.elements == 8    ? (full ? wide ? norm_grad_shared<float, 4, 8, FULL>(s.threads) : norm_grad_shared<__half, 8, 8, FULL>(s.threads)
-                                                     : wide ? norm_grad_shared<float, 4, 8, 0>(s.threads) : norm_grad_shared<__half, 8, 8, 0>(s.threads))
-                          : s.elements == 16 ? (full ? wide ? norm_grad_shared<float, 4, 16, FULL>(s.threads) : norm_grad_shared<__half, 8, 16, FULL>(s.threads)
-                                                     : wide ? norm_grad_shared<float, 4, 16, 0>(s.threads) : norm_grad_shared<__half, 8, 16, 0>(s.threads))
+    const size_t shared = s.elements == 8    ? (full ? wide ? norm_grad_shared<float, 4, 8, FULL>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 8, FULL>(s.threads, (unsigned)width)
+                                                     : wide ? norm_grad_shared<float, 4, 8, 0>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 8, 0>(s.threads, (unsigned)width))
+                          : s.elements == 16 ? (full ? wide ? norm_grad_shared<float, 4, 16, FULL>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 16, FULL>(s.threads, (unsigned)width)
+                                                     : wide ? norm_grad_shared<float, 4, 16, 0>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 16, 0>(s.threads, (unsigned)width))
                                              : 0;
     size_t per_sm = s.elements == 8 ? (full ? 768 : 1024) / s.threads : s.elements == 16 ? 512 / s.threads : 1;      // by registers
     if (per_sm * (shared + 1536) > 227 * 1024) per_sm = 227 * 1024 / (shared + 1536);
@@ -435,7 +466,7 @@ template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsign
     return launch_early(k_residual_norm<T, V, E, F>, grid, block, stream, a);
 }
 template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, int device) {
-    const size_t shared = norm_grad_shared<T, V, E, F>(block);
+    const size_t shared = norm_grad_shared<T, V, E, F>(block, a.width);
     if (shared > 40 << 10) {        // 48 KB with the static part need no leave
         static std::atomic<bool> ready[64];
         if (!ready[device].load(std::memory_order_relaxed)) {
@@ -526,7 +557,7 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     float* const gate_sums = gate ? weight_sums + (size_t)cut.ctas * width * (post ? 2 : 1) : nullptr;
     const NormGradArgs a = {dy, dn, y, branch, weight, post, gate, (const float*)rstd, (const float*)rstd_post, dx, dbranch,
                             dn && dweight ? weight_sums : nullptr, post && dpost ? post_sums : nullptr, gate && dgate ? gate_sums : nullptr,
-                            gate ? rows_per_gate : rows, cut.chunks, cut.units, (unsigned)width, f32_vectors, (float)scale};
+                            rows, gate ? rows_per_gate : rows, cut.chunks, cut.units, (unsigned)width, f32_vectors, (float)scale};
     const auto all = {dy, dn, y, branch, weight, post, gate, (const void*)dx, (const void*)dbranch};
     const NormShape s = norm_shape(width);
     cudaStream_t stream = (cudaStream_t)stream_v;

@@ -162,6 +162,24 @@ def test_norm_of_views():
 
 
 @gpu
+@pytest.mark.parametrize("off", range(0, 8, 3))
+@pytest.mark.parametrize("width", [41, 2047, 2052, 6001])
+def test_norm_gradients_of_rows_that_start_anywhere(off, width):
+    """x, branch and the gradients at different distances from a 16-byte boundary, in the middle of larger buffers."""
+    dtype, rows = torch.bfloat16, 37
+    t, dy, dn = norm_case((rows, width), dtype, True, (width,), False, device="cuda")
+    def moved(v, o):
+        buf = torch.full((v.numel() + 16,), float("nan"), dtype=dtype, device="cuda")
+        buf[o:o + v.numel()] = v.detach().reshape(-1)
+        return buf[o:o + v.numel()].view(v.shape)
+    t["x"], t["branch"] = moved(t["x"], off).requires_grad_(True), moved(t["branch"], (off + 1) % 8).requires_grad_(True)
+    dy, dn = moved(dy, (off + 2) % 8), moved(dn, (off + 5) % 8)
+    y, n = norm_call(t, 0.5)
+    grads = dict(zip(t, torch.autograd.grad((y, n), list(t.values()), (dy, dn))))
+    norm_check(t, dy, dn, 0.5, y, n, grads, dtype)
+
+
+@gpu
 def test_norm_gate_that_was_broadcast_gets_the_sum():
     t, dy, dn = norm_case((4, 3, 64), torch.float32, False, (1, 1, 64), False, device="cuda")
     one = t["gate"]
