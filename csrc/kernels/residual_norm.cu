@@ -37,8 +37,9 @@ struct NormGradArgs {
     const float *rstd, *rstd_post;
     void *dx, *dbranch;
     float *weight_sums, *post_sums, *gate_sums;      // [CTA][width], [CTA][width], [unit][width]
-    size_t rows, rows_per_gate, chunks, units;
-    unsigned width;
+    size_t rows, rows_per_gate;
+    Divisor chunks;                                  // of the rows of a gate
+    unsigned chunk_rows, longer, units, width;
     int f32;
     float scale;
 };
@@ -188,13 +189,31 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
             }
         }
     };
-    const auto load = [&](int j, int k, size_t row, unsigned stage, float (&f)[V]) {
+    const T* here[4];                   // this thread's first run of the current row, unless it is in its own part of shared memory
+    T *dx_at, *db_at;
+    const auto find = [&](size_t row, unsigned stage) {
+        if constexpr (!kOwn || kStages == 0) {
+#pragma unroll
+            for (int j = 0; j < kArrays; j++) {
+                const T* const start = arrays[j] + row * a.width;
+                if constexpr (kStages > 0)
+                    here[j] = reinterpret_cast<const T*>(reinterpret_cast<const char*>(staged) + (stage * kArrays + j) * row_bytes + (reinterpret_cast<uintptr_t>(start) & 15)) + t * V;
+                else here[j] = start + t * V;
+            }
+            dx_at = reinterpret_cast<T*>(a.dx) + row * a.width + t * V;
+            db_at = reinterpret_cast<T*>(a.dbranch) + row * a.width + t * V;
+        }
+    };
+    const auto store = [&](bool branch, size_t row, int k, const float (&f)[V]) {
+        T* to;
+        if constexpr (!kOwn || kStages == 0) to = (branch ? db_at : dx_at) + k * step * V;
+        else to = reinterpret_cast<T*>(branch ? a.dbranch : a.dx) + row * a.width + (size_t)(t + k * step) * V;
+        st_run<T, V>(to, round_run<T, V>(f));
+    };
+    const auto load = [&](int j, int k, unsigned stage, float (&f)[V]) {
         Run<T, V> r;
-        if constexpr (kStages > 0 && !kOwn) {
-            const unsigned shift = (unsigned)(reinterpret_cast<uintptr_t>(arrays[j] + row * a.width) & 15);
-            r = *reinterpret_cast<const Run<T, V>*>(reinterpret_cast<const char*>(staged) + (stage * kArrays + j) * row_bytes + shift + (t + k * step) * sizeof(T));
-        } else if constexpr (kStages > 0) r = *reinterpret_cast<const Run<T, V>*>(staged + ((stage * kArrays + j) * K + k) * step + t);
-        else r = ld_run<T, V>(arrays[j] + row * a.width + (size_t)(t + k * step) * V);
+        if constexpr (kOwn && kStages > 0) r = *reinterpret_cast<const Run<T, V>*>(staged + ((stage * kArrays + j) * K + k) * step + t);
+        else r = ld_run<T, V>(here[j] + k * step * V);
 #pragma unroll
         for (int e = 0; e < V; e++) f[e] = Traits<T>::up(r.e[e]);
     };
@@ -238,9 +257,11 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
         if constexpr (F & GATE) sum_g[e] = 0;
     }
     unsigned turn = 0;
-    for (size_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        const size_t gate = unit / a.chunks, chunk = unit % a.chunks, gate_at = gate * a.width;
-        const size_t begin = gate * a.rows_per_gate + chunk * a.rows_per_gate / a.chunks, end = gate * a.rows_per_gate + (chunk + 1) * a.rows_per_gate / a.chunks;
+    for (unsigned unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const unsigned gate = a.chunks.quotient(unit), chunk = unit - gate * a.chunks.d;
+        const size_t gate_at = (size_t)gate * a.width;
+        // the first `longer` chunks have one row more than the others
+        const size_t begin = (size_t)gate * a.rows_per_gate + (size_t)chunk * a.chunk_rows + (chunk < a.longer ? chunk : a.longer), end = begin + a.chunk_rows + (chunk < a.longer);
         unsigned stage = 0;
         if constexpr (kStages > 0) {
             if constexpr (!kOwn) __syncthreads();       // the last unit's rows
@@ -269,6 +290,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                 next_ry = a.dn ? a.rstd[row + 1] : 0.0f;
                 if constexpr (F & POST) next_rb = a.rstd_post[row + 1];
             }
+            find(row, stage);
             float d[E], yh[E], dot = 0;
             if (a.dn) {
 #pragma unroll
@@ -276,11 +298,11 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     const unsigned i = t + k * step;
                     if (i >= runs) continue;
                     float w[V], dn[V], y[V];
-                    load(DN, k, row, stage, dn);
-                    load(Y, k, row, stage, y);
+                    load(DN, k, stage, dn);
+                    load(Y, k, stage, y);
                     if constexpr (F & FULL) {
                         float p[V];
-                        load(B, k, row, stage, p);
+                        load(B, k, stage, p);
                         if constexpr (F & POST) {
                             vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0, k, w);
 #pragma unroll
@@ -315,7 +337,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                 const unsigned i = t + k * step;
                 if (i >= runs) continue;
                 float dy[V];
-                if (a.dy) load(DY, k, row, stage, dy);
+                if (a.dy) load(DY, k, stage, dy);
                 float out[V];
 #pragma unroll
                 for (int e = 0; e < V; e++) {
@@ -323,10 +345,10 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     d[j] = fmaf(ry, d[j] - yh[j] * c, a.dy ? dy[e] : 0.0f);
                     out[e] = d[j];
                 }
-                st_run<T, V>(reinterpret_cast<T*>(a.dx) + row * a.width + (size_t)i * V, round_run<T, V>(out));
+                store(false, row, k, out);
                 if constexpr (F & FULL) {
                     float w2[V], g[V], b[V];
-                    load(B, k, row, stage, b);
+                    load(B, k, stage, b);
                     if constexpr (F & POST) vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0, k, w2);
                     if constexpr (F & GATE) vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at, k, g);
 #pragma unroll
@@ -345,7 +367,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                         }
                         d[j] = out[e] = v;
                     }
-                    if constexpr (!(F & POST)) st_run<T, V>(reinterpret_cast<T*>(a.dbranch) + row * a.width + (size_t)i * V, round_run<T, V>(out));
+                    if constexpr (!(F & POST)) store(true, row, k, out);
                 }
             }
             if constexpr (F & POST) {
@@ -355,10 +377,10 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     const unsigned i = t + k * step;
                     if (i >= runs) continue;
                     float b[V];
-                    load(B, k, row, stage, b);
+                    load(B, k, stage, b);
 #pragma unroll
                     for (int e = 0; e < V; e++) b[e] = rb * (d[k * V + e] - b[e] * cb);
-                    st_run<T, V>(reinterpret_cast<T*>(a.dbranch) + row * a.width + (size_t)i * V, round_run<T, V>(b));
+                    store(true, row, k, b);
                 }
             }
             if constexpr (kStages > 0) stage = stage == kStages - 1 ? 0 : stage + 1;
@@ -370,7 +392,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     if (t + k * step < runs)
 #pragma unroll
                         for (int e = 0; e < V; e++) {
-                            a.gate_sums[unit * a.width + (size_t)(t + k * step) * V + e] = sum_g[k * V + e];
+                            a.gate_sums[(size_t)unit * a.width + (t + k * step) * V + e] = sum_g[k * V + e];
                             sum_g[k * V + e] = 0;
                         }
             }
@@ -543,7 +565,7 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
                                            void* workspace, size_t workspace_bytes, void* stream_v) {
     const char* who = "dccl_residual_norm_backward";
     const size_t gates = gate && rows_per_gate ? rows / rows_per_gate : 0;
-    if (!rows || !width || width > kNormMaxWidth || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
+    if (!rows || rows > 0x7fffffffu || !width || width > kNormMaxWidth || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
         || !branch != !dbranch)
         return report(who, cudaErrorInvalidValue);
     const bool full = branch != nullptr;      // a plain sum has no branch here
@@ -557,7 +579,8 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     float* const gate_sums = gate ? weight_sums + (size_t)cut.ctas * width * (post ? 2 : 1) : nullptr;
     const NormGradArgs a = {dy, dn, y, branch, weight, post, gate, (const float*)rstd, (const float*)rstd_post, dx, dbranch,
                             dn && dweight ? weight_sums : nullptr, post && dpost ? post_sums : nullptr, gate && dgate ? gate_sums : nullptr,
-                            rows, gate ? rows_per_gate : rows, cut.chunks, cut.units, (unsigned)width, f32_vectors, (float)scale};
+                            rows, gate ? rows_per_gate : rows, Divisor((unsigned)cut.chunks), (unsigned)((gate ? rows_per_gate : rows) / cut.chunks),
+                            (unsigned)((gate ? rows_per_gate : rows) % cut.chunks), (unsigned)cut.units, (unsigned)width, f32_vectors, (float)scale};
     const auto all = {dy, dn, y, branch, weight, post, gate, (const void*)dx, (const void*)dbranch};
     const NormShape s = norm_shape(width);
     cudaStream_t stream = (cudaStream_t)stream_v;
