@@ -38,6 +38,7 @@ def main():
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--bucket-mb", type=int, default=25)
+    ap.add_argument("--fused", action="store_true", help="the decoder computes with the fused operators of dccl_b200.ops.decoder")
     ap.add_argument("--plain-buckets", action="store_true",
                     help="dccl_ddp: leave DDP's gradient buckets in ordinary memory (default: they come from a memory pool of symmetric memory)")
     args = ap.parse_args()
@@ -45,6 +46,7 @@ def main():
     torch.cuda.set_device(local)
     dev = torch.device("cuda", local)
     cfg = LlamaConfig.tinyllama_1b() if args.model == "1b" else LlamaConfig.tiny()
+    cfg.fused = args.fused
     seq = min(args.seq, cfg.max_seq)
     torch.manual_seed(0)
     model = LlamaDecoder(cfg).to(dev).to(torch.bfloat16)
@@ -155,7 +157,7 @@ def main():
             "data": "synthetic", "backend": args.backend, "gpu_launches": int(launches),
             "e2e": {"h2d_bytes_per_step": host_tokens.numel() * 8, "d2h_bytes_per_step": 4, "included": True},
             "config": {"model": "llama-1.1b" if args.model == "1b" else "llama-tiny", "params": cfg.num_params(), "global_batch": world * args.batch,
-                       "seq_len": seq, "parallelism": "dp%d" % world, "bucket_mb": args.bucket_mb, "optimizer": "AdamW fused, bf16 params"},
+                       "seq_len": seq, "parallelism": "dp%d" % world, "bucket_mb": args.bucket_mb, "fused_operators": bool(args.fused), "optimizer": "AdamW fused, bf16 params"},
             "final_loss": round(losses[-1], 4)}))
     if reducer is not None:
         reducer.close()

@@ -61,11 +61,13 @@ def main():
     ap.add_argument("--vocab-parallel", action="store_true", help="embedding, head and loss split over the vocabulary as well")
     ap.add_argument("--sequence-parallel", action="store_true",
                     help="activations between the blocks split along the sequence: all-gather + reduce-scatter instead of all-reduce")
+    ap.add_argument("--fused", action="store_true", help="the decoder computes with the fused operators of dccl_b200.ops.decoder")
     args = ap.parse_args()
     rank, world, local = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1)), int(os.environ.get("LOCAL_RANK", 0))
     torch.cuda.set_device(local)
     dev = torch.device("cuda", local)
     cfg = LlamaConfig.tinyllama_1b() if args.model == "1b" else LlamaConfig.tiny()
+    cfg.fused = args.fused
     if cfg.kv_heads % world:
         cfg.kv_heads = world if cfg.heads % world == 0 else cfg.kv_heads      # the default shape has 4 KV heads
     seq = min(args.seq, cfg.max_seq)
@@ -140,7 +142,7 @@ def main():
             "gpu_launches": int(launches), "in_place_reduce": bool(args.in_place_reduce and args.backend == "dccl"),
             "e2e": {"h2d_bytes_per_step": host_tokens.numel() * 8, "d2h_bytes_per_step": 4, "included": True},
             "config": {"model": "llama-1.1b" if args.model == "1b" else "llama-tiny", "params": cfg.num_params(), "global_batch": args.batch,
-                       "seq_len": seq, "parallelism": "tp%d" % world, "kv_heads": cfg.kv_heads, "vocab_parallel": bool(args.vocab_parallel), "sequence_parallel": bool(args.sequence_parallel), "optimizer": "AdamW fused, bf16 params"},
+                       "seq_len": seq, "parallelism": "tp%d" % world, "kv_heads": cfg.kv_heads, "vocab_parallel": bool(args.vocab_parallel), "sequence_parallel": bool(args.sequence_parallel), "fused_operators": bool(args.fused), "optimizer": "AdamW fused, bf16 params"},
             "final_loss": round(final_loss, 4), "final_loss_is_rank0_share": bool(args.sequence_parallel)}))
     model.close()
     dist.destroy_process_group()

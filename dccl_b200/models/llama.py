@@ -5,12 +5,18 @@ Plain PyTorch: RMSNorm, rotary position embedding, grouped-query attention throu
 the benchmark's shape: 22 layers, hidden 2048, 32 heads, 4 KV heads, FFN 5632, vocabulary 32000
 (about 1.1 B parameters). The model is only the workload whose gradients the library all-reduces;
 the "no library GEMM" rule of this project applies to the communication paths, not to it.
+
+With ``LlamaConfig(fused=True)`` the same modules compute with the operators of ``dccl_b200.ops.decoder``: each residual add in one pass with
+the norm after it, rotary positions of queries and keys in one launch, and the gated projections as one product (parameters and state
+dict stay the same; on the GPU the model is then float16 or bfloat16).
 """
 from dataclasses import dataclass
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops import decoder as ops
 
 
 @dataclass
@@ -24,6 +30,7 @@ class LlamaConfig:
     max_seq: int = 2048
     rope_theta: float = 10000.0
     eps: float = 1e-5
+    fused: bool = False
 
     @staticmethod
     def tinyllama_1b():
@@ -86,6 +93,18 @@ class Attention(nn.Module):
         return self.o(out.transpose(1, 2).reshape(b, s, self.h * self.hd))
 
 
+    def fused(self, x, freqs):
+        b, s, _ = x.shape
+        return self.o(attend(self.q(x).view(b, s, self.h, self.hd), self.k(x).view(b, s, self.kv, self.hd), self.v(x).view(b, s, self.kv, self.hd), freqs))
+
+
+def attend(q, k, v, freqs):
+    """Causal attention of [batch, seq, heads, head dim], whose queries and keys are turned by their positions first: [batch, seq, heads * head dim]."""
+    q, k = ops.rotary(q, k, freqs)
+    out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=q.shape[2] != k.shape[2])
+    return out.transpose(1, 2).flatten(2)
+
+
 class Block(nn.Module):
     def __init__(self, cfg):
         super().__init__()
@@ -99,6 +118,19 @@ class Block(nn.Module):
         x = x + self.attn(self.n1(x), cos, sin)
         h = self.n2(x)
         return x + self.down(F.silu(self.gate(h)) * self.up(h))
+
+    def fused(self, x, n, freqs, after):
+        """(x, n) after this block, from x and its norm n: n is the norm of x by `after`, which comes next."""
+        x, n = ops.residual_norm(x, self.attn.fused(n, freqs), self.n2.weight, eps=self.n2.eps)
+        return ops.residual_norm(x, self.down(ops.gated_linear(n, self.gate.weight, self.up.weight)), after.weight, eps=after.eps)
+
+
+def run_fused(x, blocks, last, freqs):
+    """The blocks and the last norm."""
+    n = ops.rms_norm(x, blocks[0].n1.weight, eps=blocks[0].n1.eps) if len(blocks) else ops.rms_norm(x, last.weight, eps=last.eps)
+    for i, blk in enumerate(blocks):
+        x, n = blk.fused(x, n, freqs, blocks[i + 1].n1 if i + 1 < len(blocks) else last)
+    return n
 
 
 class LlamaDecoder(nn.Module):
@@ -118,6 +150,9 @@ class LlamaDecoder(nn.Module):
 
     def forward(self, tokens):
         x = self.embed(tokens)
+        if self.cfg.fused:
+            freqs = ops.rotary_frequencies(self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, device=tokens.device)
+            return self.head(run_fused(x, self.blocks, self.norm, freqs))
         cos, sin = rope_tables(tokens.shape[1], self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, tokens.device)
         for blk in self.blocks:
             x = blk(x, cos, sin)

@@ -6,7 +6,8 @@ gate / up keep the rows of their own heads / columns, o and down keep the matchi
 block needs two all-reduces forward and two backward (``ops.copy_to_region`` at the entry of the attention and of
 the MLP, ``ops.reduce_from_region`` at their exits). Embedding, norms and the output head stay replicated; since
 every rank sees the same tokens their gradients come out identical on all ranks without further communication.
-Every rank starts from the same unsplit weights, so the sharded model computes what the unsplit one does.
+Every rank starts from the same unsplit weights, so the sharded model computes what the unsplit one does. A model made with
+``LlamaConfig(fused=True)`` stays fused: the residual add behind each collective and the norm after it are one pass.
 """
 import torch
 import torch.nn as nn
@@ -14,7 +15,8 @@ import torch.nn.functional as F
 
 from ..ops import functional as ops
 from ..parallel.tensor_parallel import SymmetricPool, column_linears_reduce_grad_in_place, row_linear_reduce_in_place
-from .llama import LlamaDecoder, apply_rope, rope_tables
+from ..ops.decoder import gated_linear, residual_norm, rotary_frequencies
+from .llama import LlamaDecoder, apply_rope, attend, rope_tables, run_fused
 
 
 def _rows(linear, lo, hi):
@@ -43,7 +45,8 @@ class ShardedAttention(nn.Module):
         self.v = _rows(attn.v, r * kw, (r + 1) * kw)
         self.o = _cols(attn.o, r * qw, (r + 1) * qw)
 
-    def forward(self, x, cos, sin):
+    def _project(self, x):
+        """q, k and v [batch, seq, heads of this rank, head dim] of the whole sequence."""
         if self.sp:      # the input is this rank's part of the sequence: gather it (backward: reduce-scatter)
             x = ops.all_gather(x, 1, self.comm)
         b, s, _ = x.shape
@@ -54,12 +57,18 @@ class ShardedAttention(nn.Module):
         else:
             x = ops.copy_to_region(x, self.comm)
             q, k, v = self.q(x), self.k(x), self.v(x)
-        q = q.view(b, s, self.h, self.hd).transpose(1, 2)
-        k = k.view(b, s, self.kv, self.hd).transpose(1, 2)
-        v = v.view(b, s, self.kv, self.hd).transpose(1, 2)
+        return q.view(b, s, self.h, self.hd), k.view(b, s, self.kv, self.hd), v.view(b, s, self.kv, self.hd)
+
+    def forward(self, x, cos, sin):
+        q, k, v = (t.transpose(1, 2) for t in self._project(x))
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.kv != self.h)
-        out = out.transpose(1, 2).reshape(b, s, self.h * self.hd)
+        return self._leave(out.transpose(1, 2).reshape(q.shape[0], q.shape[2], self.h * self.hd))
+
+    def fused(self, x, freqs):
+        return self._leave(attend(*self._project(x), freqs))
+
+    def _leave(self, out):
         if self.sp:      # sum the partial products and keep this rank's part of the sequence (backward: all-gather)
             return ops.reduce_scatter(self.o(out), 1, "sum", self.comm)
         if self.pool is not None:
@@ -93,6 +102,20 @@ class ShardedBlock(nn.Module):
             return x + row_linear_reduce_in_place(F.silu(g) * u, self.down.weight, self.comm, self.pool)
         h = ops.copy_to_region(self.n2(x), self.comm)
         return x + ops.reduce_from_region(self.down(F.silu(self.gate(h)) * self.up(h)), self.comm)
+
+    def fused(self, x, n, freqs, after):
+        """(x, n) after this block, as of the unsplit one. The pool takes the products at the exits and the input gradient of attention; that of
+        the gated product is a tensor of its own."""
+        x, n = residual_norm(x, self.attn.fused(n, freqs), self.n2.weight, eps=self.n2.eps)
+        h = ops.all_gather(n, 1, self.comm) if self.sp else ops.copy_to_region(n, self.comm)
+        h = gated_linear(h, self.gate.weight, self.up.weight)
+        if self.sp:
+            m = ops.reduce_scatter(self.down(h), 1, "sum", self.comm)
+        elif self.pool is not None:
+            m = row_linear_reduce_in_place(h, self.down.weight, self.comm, self.pool)
+        else:
+            m = ops.reduce_from_region(self.down(h), self.comm)
+        return residual_norm(x, m, after.weight, eps=after.eps)
 
 
 class VocabParallelEmbedding(nn.Module):
@@ -173,14 +196,18 @@ class ShardedLlamaDecoder(nn.Module):
 
     def forward(self, tokens):
         x = self.embed(tokens)
-        cos, sin = rope_tables(tokens.shape[1], self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, tokens.device)
         if self.sp:      # between the blocks every rank keeps 1 / world of the sequence; returns the logits of that part
             if tokens.shape[1] % self.comm.world:
                 raise ValueError("the sequence length (%d) must divide by the world size" % tokens.shape[1])
             x = self._my_part(x)
-        for blk in self.blocks:
-            x = blk(x, cos, sin)
-        x = self.norm(x)
+        head_dim = self.cfg.hidden // self.cfg.heads
+        if self.cfg.fused:
+            x = run_fused(x, self.blocks, self.norm, rotary_frequencies(head_dim, self.cfg.rope_theta, device=tokens.device))
+        else:
+            cos, sin = rope_tables(tokens.shape[1], head_dim, self.cfg.rope_theta, tokens.device)
+            for blk in self.blocks:
+                x = blk(x, cos, sin)
+            x = self.norm(x)
         if self.vocab_parallel:        # this rank's slice of the classes
             return self.head(ops.copy_to_region(x, self.comm))
         return self.head(x)

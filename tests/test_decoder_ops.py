@@ -631,3 +631,181 @@ def test_gated_refusals_on_the_gpu():
         ops.gated_linear(torch.zeros(2, 8, device="cuda"), torch.zeros(6, 8, device="cuda"), torch.zeros(6, 8, device="cuda"))
     with pytest.raises(ValueError):
         ops.gated_linear(torch.zeros(2, 8, device="cuda").half(), torch.zeros(6, 8).half(), torch.zeros(6, 8, device="cuda").half())
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+def decoders(device, dtype, **kw):
+    """The same decoder as a chain of torch's operations and fused, and tokens for it."""
+    import copy
+    from dccl_b200.models.llama import LlamaConfig, LlamaDecoder
+    torch.manual_seed(5)
+    plain = LlamaDecoder(LlamaConfig(vocab_size=192, hidden=128, layers=2, heads=4, kv_heads=2, ffn=200, max_seq=64, **kw)).to(dtype)
+    fused = copy.deepcopy(plain)
+    fused.cfg.fused = True
+    plain.cfg = copy.copy(plain.cfg)
+    plain.cfg.fused = False
+    tokens = torch.randint(0, 192, (3, 33), generator=torch.Generator().manual_seed(6))
+    return plain.to(device), fused.to(device), tokens.to(device)
+
+
+def test_the_fused_decoder_is_the_same_model():
+    """In fp32 on the CPU, where both are sums of the same terms in other orders: about fifty operations deep, each off by a few times 2^-24
+    (1e-5 of the largest gradient), and angles of the tables are off by 2^-24 of up to 33 radians."""
+    plain, fused, tokens = decoders("cpu", torch.float32)
+    assert list(plain.state_dict()) == list(fused.state_dict())
+    a, b = plain.loss(tokens), fused.loss(tokens)
+    a.backward()
+    b.backward()
+    assert abs(a - b) < 1e-5 * abs(a)
+    for (name, p), q in zip(plain.named_parameters(), fused.parameters()):
+        assert (p.grad - q.grad).abs().max() <= 3e-5 * p.grad.abs().max() + 1e-7, name
+
+
+@pytest.mark.parametrize("world", [1, 2])
+def test_the_fused_decoder_split_over_ranks(dccl_lib, world):
+    import os
+    from dccl_b200.utils.launch import python_ranks
+    res = python_ranks(os.path.join(os.path.dirname(os.path.abspath(__file__)), "workers", "llama_fused_worker.py"), [], world, timeout=300)
+    for r, p in enumerate(res):
+        assert p.returncode == 0, "rank %d:\n%s\n%s" % (r, p.stdout[-3000:], p.stderr[-3000:])
+        assert p.stdout.strip().splitlines()[-1].startswith("OK"), p.stdout
+
+
+@gpu
+def test_the_fused_decoder_on_the_gpu():
+    """bf16 on the GPU against the same operators on the CPU: about thirty bf16 results on the way to the loss and as many back, each off by
+    2^-9 in the root mean square at most, at random: 8 x 2^-9 = 1.6 % of the norm of a gradient, twice that allowed."""
+    import copy
+    _, fused, tokens = decoders("cpu", torch.bfloat16)
+    there = copy.deepcopy(fused).cuda()
+    a, b = fused.loss(tokens), there.loss(tokens.cuda())
+    a.backward()
+    b.backward()
+    assert abs(a.item() - b.item()) < 2.0 ** -7 * abs(a.item())
+    for (name, p), q in zip(fused.named_parameters(), there.parameters()):
+        off = (p.grad.double() - q.grad.double().cpu()).norm() / p.grad.double().norm()
+        assert off < 0.032, (name, off)
+
+
+@gpu
+def test_a_decoding_step_in_a_graph():
+    """One token of each sequence through norm, rotary and the gated layer, captured once and replayed with other inputs and positions; on a stream
+    of its own, next to a second graph with workspaces of its own."""
+    w = {k: torch.randn(s, device="cuda").bfloat16() * 0.05 for k, s in (("n", 256), ("g", (512, 256)), ("u", (512, 256)))}
+    freqs = ops.rotary_frequencies(64, device="cuda")
+    x, branch, q = (torch.randn(4, 1, 256, device="cuda").bfloat16() for _ in range(3))
+    at = torch.tensor([[5], [0], [70000], [12]], device="cuda")
+
+    def step():
+        with torch.no_grad():
+            y, n = ops.residual_norm(x, branch, w["n"])
+            return y, ops.gated_linear(n, w["g"], w["u"]), ops.rotary(q.view(4, 1, 4, 64), None, freqs, at)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(stream):
+        step()
+        for _ in range(2):
+            graphs.append((torch.cuda.CUDAGraph(),))
+            with torch.cuda.graph(graphs[-1][0], stream=stream):
+                graphs[-1] += step(),
+    torch.cuda.synchronize()
+    for turn_ in range(3):
+        for t in (x, branch, q):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(turn_)).bfloat16())
+        at.add_(turn_ * 1000)
+        want = step()
+        for graph, outs in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@gpu
+def test_a_training_step_in_a_graph():
+    """Forward and backward captured, replayed on new inputs."""
+    x, branch, weight = (t.cuda().bfloat16().requires_grad_(True) for t in (torch.randn(70, 96), torch.randn(70, 96), torch.ones(96)))
+    wg, wu = (torch.randn(80, 96).mul(0.1).cuda().bfloat16().requires_grad_(True) for _ in range(2))
+    dh = torch.randn(70, 80).cuda().bfloat16()
+
+    def step():
+        y, n = ops.residual_norm(x, branch, weight, post_weight=weight, scale=0.5)
+        return torch.autograd.grad((ops.gated_linear(n, wg, wu), y), (x, branch, weight, wg, wu), (dh, torch.ones_like(y)))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        outs = step()
+    for seed in range(2):
+        with torch.no_grad():
+            x.copy_(torch.randn(70, 96, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+
+
+@gpu
+def test_operators_of_two_streams_at_once():
+    x, wg, wu, _ = gated_case(300, 512, 640, torch.bfloat16, "cuda")
+    w = torch.ones(512, device="cuda").bfloat16()
+    want = ops.gated_linear(ops.rms_norm(x, w), wg, wu)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for s, o in zip(streams, outs):
+            with torch.cuda.stream(s):
+                o.append(ops.gated_linear(ops.rms_norm(x, w), wg, wu))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want) for o in outs for v in o)
+
+
+@gpu
+def test_autograd_of_the_operators():
+    """retain_graph, a second pass over a freed graph, inputs changed in place, gradients of gradients, forward mode."""
+    x, wg, wu, dh = gated_case(9, 64, 72, torch.bfloat16, "cuda")
+    w = torch.ones(64, device="cuda").bfloat16().requires_grad_(True)
+    freqs = ops.rotary_frequencies(16, device="cuda")
+    x.requires_grad_(True)
+    for make in (lambda v: ops.gated_linear(v, wg, wu), lambda v: ops.rms_norm(v, w), lambda v: ops.residual_norm(v, v, w)[1], lambda v: ops.rotary(v.view(1, 9, 4, 16), None, freqs)):
+        y = make(x)
+        first, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+        again, = torch.autograd.grad(y.sum(), x)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y.sum(), x)
+        g, = torch.autograd.grad(make(x).float().pow(2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+    v = x.detach().clone().requires_grad_(True)
+    z = v * 1
+    y = ops.gated_linear(z, wg, wu)
+    z.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            ops.rms_norm(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()), w.detach())
+    with torch.inference_mode():
+        assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(x.detach(), w.detach()))
+
+
+@gpu
+def test_operators_refuse_tensors_without_memory():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        x, w = torch.empty(4, 64, device="cuda"), torch.ones(64, device="cuda")
+        with pytest.raises(TypeError):
+            ops.rms_norm(x, w)
+    del mode
+
+
+@gpu
+def test_negated_views():
+    x, w = torch.randn(3, 64, device="cuda"), torch.ones(64, device="cuda")
+    assert torch.equal(ops.rms_norm(torch._neg_view(x), w), ops.rms_norm(-x, w))
