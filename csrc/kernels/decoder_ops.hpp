@@ -26,11 +26,10 @@ size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t w
 
 /**
  * Gradients of dccl_residual_norm: from dy and dn (either may be null) those of x and branch, and in the vectors' own types those of
- * weight, post and gate. With a branch (and dbranch), y is the x of the forward pass. Without both, y is the forward pass's y, whose
- * gradient dx is that of branch as well (scale 1, no post, no gate), or x where there was no branch. No atomics: the same
- * inputs give the same gradients.
+ * weight, post and gate. dbranch may be null where it equals dx (scale 1, no post, no gate). No atomics: the same inputs give the
+ * same gradients.
  */
-int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* y, const void* branch,
+int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* x, const void* branch,
                                 const void* weight, const void* post, const void* gate, size_t rows_per_gate, int f32_vectors, double scale,
                                 const void* rstd, const void* rstd_post, void* dx, void* dbranch, void* dweight, void* dpost, void* dgate,
                                 void* workspace, size_t workspace_bytes, void* stream);

@@ -12,9 +12,9 @@
  *     dw2 = sum s g .* D .* bh                  dg  = sum s D .* p
  *
  * A few operations per element that is moved: HBM bounds both. A CTA holds a row in registers, so that x, b (forward) and
- * dy, dn, y, b (backward) are read once and the sums of a row cost one barrier each. Rows are summed in fp32, and n comes from the
- * y of fp32 and not from the rounded one that is stored. The backward pass of a plain sum starts from the stored y, which saves it one of
- * five arrays; the rounding of y reaches the gradients only through yh.
+ * dy, dn, x, b (backward) are read once and the sums of a row cost one barrier each. Rows are summed in fp32, and n comes from the
+ * y of fp32 and not from the rounded one that is stored. The backward pass makes y again from x and b: from the stored y, which
+ * would save a plain sum one of five arrays, its rounding goes into every term of dw and makes that half again as inexact.
  */
 #include "decoder_ops.hpp"
 #include "launch_early.cuh"
@@ -33,7 +33,7 @@ struct NormArgs {
 };
 
 struct NormGradArgs {
-    const void *dy, *dn, *y, *branch, *weight, *post, *gate;
+    const void *dy, *dn, *x, *branch, *weight, *post, *gate;
     const float *rstd, *rstd_post;
     void *dx, *dbranch;
     float *weight_sums, *post_sums, *gate_sums;      // [CTA][width], [CTA][width], [unit][width]
@@ -124,11 +124,10 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ?
     }
 }
 
-/** The arrays that a row of the backward pass reads. Y is the y = x + branch (or x) that was stored; with post, a gate or a scale (FULL) the
- *  branch is read in any case, Y is x, and y comes from both again, exact. */
-enum { DN, Y, DY, B };
+/** The arrays that a row of the backward pass reads. */
+enum { DN, X, DY, B };
 enum { IN_WEIGHT, IN_POST, IN_GATE };   // the vectors, in shared memory as fp32
-constexpr int FULL = POST | GATE | SCALE;
+constexpr int FULL = POST | GATE | SCALE;      // any of them, and the branch has a gradient that is not x's
 
 /** Rows in shared memory at a time: three of up to 2048 elements, two of up to 8192 16-bit ones. */
 template <typename T, int E> constexpr int kNormStages = E == 8 ? 3 : E == 16 && sizeof(T) == 2 ? 2 : 0;
@@ -139,7 +138,7 @@ template <typename T, int V, int E> __host__ __device__ constexpr size_t norm_ro
 }
 
 template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(unsigned threads, unsigned width) {
-    return kNormStages<T, E> * (F & FULL ? 4 : 3) * norm_row_bytes<T, V, E>(threads, width) + (E <= 16 ? (size_t)threads * E * (F & FULL ? 3 : 1) * sizeof(float) : 0);
+    return kNormStages<T, E> * (F & BRANCH ? 4 : 3) * norm_row_bytes<T, V, E>(threads, width) + (E <= 16 ? (size_t)threads * E * (F & FULL ? 3 : 1) * sizeof(float) : 0);
 }
 
 /**
@@ -152,14 +151,14 @@ template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(uns
 template <typename T, int V, int E, int F>
 __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? (F & FULL ? 3 : 4) : 1) k_residual_norm_grad(const __grid_constant__ NormGradArgs a) {
     wait_for_stream();
-    constexpr int K = E / V, kArrays = F & FULL ? 4 : 3, kStages = kNormStages<T, E>, kPiece = V < 4 ? V : 4;
+    constexpr int K = E / V, kArrays = F & BRANCH ? 4 : 3, kStages = kNormStages<T, E>, kPiece = V < 4 ? V : 4;
     constexpr bool kOwn = V * sizeof(T) == 16;          // a thread's elements are its own matter
     constexpr bool kVectors = E <= 16;                  // in shared memory
     extern __shared__ uint4 staged[];                   // [stage][array][run][thread], then [vector][run][piece][thread] of kPiece floats
     __shared__ __align__(16) float parts[2][2][32];
     const unsigned runs = a.width / V, step = blockDim.x, t = threadIdx.x;
     const float inv_width = 1.0f / a.width;
-    const T* const arrays[4] = {reinterpret_cast<const T*>(a.dn), reinterpret_cast<const T*>(a.y), reinterpret_cast<const T*>(a.dy), reinterpret_cast<const T*>(a.branch)};
+    const T* const arrays[4] = {reinterpret_cast<const T*>(a.dn), reinterpret_cast<const T*>(a.x), reinterpret_cast<const T*>(a.dy), reinterpret_cast<const T*>(a.branch)};
     const unsigned row_bytes = (unsigned)norm_row_bytes<T, V, E>(step, a.width);
     Run<float, kPiece>* const vectors = reinterpret_cast<Run<float, kPiece>*>(reinterpret_cast<char*>(staged) + (size_t)kStages * kArrays * row_bytes);
     const auto fetch = [&](size_t row, unsigned stage) {
@@ -299,8 +298,8 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     if (i >= runs) continue;
                     float w[V], dn[V], y[V];
                     load(DN, k, stage, dn);
-                    load(Y, k, stage, y);
-                    if constexpr (F & FULL) {
+                    load(X, k, stage, y);
+                    if constexpr (F & BRANCH) {
                         float p[V];
                         load(B, k, stage, p);
                         if constexpr (F & POST) {
@@ -314,7 +313,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                             for (int e = 0; e < V; e++) p[e] *= w[e];
                         }
 #pragma unroll
-                        for (int e = 0; e < V; e++) y[e] = fmaf(F & POST ? rb * a.scale : a.scale, p[e], y[e]);      // as the forward pass rounds
+                        for (int e = 0; e < V; e++) y[e] = F & (POST | SCALE) ? fmaf(F & POST ? rb * a.scale : a.scale, p[e], y[e]) : y[e] + p[e];      // as the forward pass rounds
                     }
                     vector(IN_WEIGHT, a.weight, DCCL_NORM_WEIGHT_F32, 0, k, w);
 #pragma unroll
@@ -468,9 +467,9 @@ struct NormCut { size_t chunks, units; unsigned ctas; };
 static NormCut norm_cut(int device, int dtype, size_t rows, size_t width, size_t gates, bool full) {
     const NormShape s = norm_shape(width);
     const bool wide = dtype == 7;
-    const size_t shared = s.elements == 8    ? (full ? wide ? norm_grad_shared<float, 4, 8, FULL>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 8, FULL>(s.threads, (unsigned)width)
+    const size_t shared = s.elements == 8    ? (full ? wide ? norm_grad_shared<float, 4, 8, BRANCH | FULL>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 8, BRANCH | FULL>(s.threads, (unsigned)width)
                                                      : wide ? norm_grad_shared<float, 4, 8, 0>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 8, 0>(s.threads, (unsigned)width))
-                          : s.elements == 16 ? (full ? wide ? norm_grad_shared<float, 4, 16, FULL>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 16, FULL>(s.threads, (unsigned)width)
+                          : s.elements == 16 ? (full ? wide ? norm_grad_shared<float, 4, 16, BRANCH | FULL>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 16, BRANCH | FULL>(s.threads, (unsigned)width)
                                                      : wide ? norm_grad_shared<float, 4, 16, 0>(s.threads, (unsigned)width) : norm_grad_shared<__half, 8, 16, 0>(s.threads, (unsigned)width))
                                              : 0;
     size_t per_sm = s.elements == 8 ? (full ? 768 : 1024) / s.threads : s.elements == 16 ? 512 / s.threads : 1;      // by registers
@@ -501,9 +500,7 @@ template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsign
 }
 template <typename T, int V, int E, typename Args> static cudaError_t norm_form(int form, unsigned grid, unsigned block, cudaStream_t stream, const Args& a, int device) {
     switch (form) {
-        case BRANCH:
-            if constexpr (std::is_same<Args, NormArgs>::value) return norm_launch<T, V, E, BRANCH>(grid, block, stream, a, device);
-            return cudaErrorInvalidValue;
+        case BRANCH: return norm_launch<T, V, E, BRANCH>(grid, block, stream, a, device);
         case BRANCH | SCALE: return norm_launch<T, V, E, BRANCH | SCALE>(grid, block, stream, a, device);
         case BRANCH | POST: return norm_launch<T, V, E, BRANCH | POST>(grid, block, stream, a, device);
         case BRANCH | GATE | SCALE: return norm_launch<T, V, E, BRANCH | GATE | SCALE>(grid, block, stream, a, device);
@@ -559,17 +556,16 @@ extern "C" size_t dccl_residual_norm_workspace(int device, int dtype, size_t row
     return ((size_t)cut.ctas * (has_post ? 2 : 1) + (gates ? cut.units : 0)) * width * sizeof(float);
 }
 
-extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* y, const void* branch,
+extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* x, const void* branch,
                                            const void* weight, const void* post, const void* gate, size_t rows_per_gate, int f32_vectors, double scale,
                                            const void* rstd, const void* rstd_post, void* dx, void* dbranch, void* dweight, void* dpost, void* dgate,
                                            void* workspace, size_t workspace_bytes, void* stream_v) {
     const char* who = "dccl_residual_norm_backward";
     const size_t gates = gate && rows_per_gate ? rows / rows_per_gate : 0;
     if (!rows || rows > 0x7fffffffu || !width || width > kNormMaxWidth || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
-        || !branch != !dbranch)
+        || (dbranch && !branch) || (!dbranch && branch && (post || gate || scale != 1.0)))
         return report(who, cudaErrorInvalidValue);
-    const bool full = branch != nullptr;      // a plain sum has no branch here
-    if (full && !post && !gate && scale == 1.0) return report(who, cudaErrorInvalidValue);
+    const bool full = branch != nullptr;
     const NormCut cut = norm_cut(device, dtype, rows, width, gates, full);
     const size_t blocks = (width + 31) / 32, vectors = (dn && dweight ? 1 : 0) + (post && dpost ? 1 : 0) + (gate && dgate ? gates : 0);
     if (!cut.units || blocks * vectors > 0x7fffffffu || workspace_bytes < dccl_residual_norm_workspace(device, dtype, rows, width, gates, post != nullptr, full))
@@ -577,16 +573,16 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     float* const weight_sums = (float*)workspace;
     float* const post_sums = post ? weight_sums + (size_t)cut.ctas * width : nullptr;
     float* const gate_sums = gate ? weight_sums + (size_t)cut.ctas * width * (post ? 2 : 1) : nullptr;
-    const NormGradArgs a = {dy, dn, y, branch, weight, post, gate, (const float*)rstd, (const float*)rstd_post, dx, dbranch,
+    const NormGradArgs a = {dy, dn, x, branch, weight, post, gate, (const float*)rstd, (const float*)rstd_post, dx, dbranch,
                             dn && dweight ? weight_sums : nullptr, post && dpost ? post_sums : nullptr, gate && dgate ? gate_sums : nullptr,
                             rows, gate ? rows_per_gate : rows, Divisor((unsigned)cut.chunks), (unsigned)((gate ? rows_per_gate : rows) / cut.chunks),
                             (unsigned)((gate ? rows_per_gate : rows) % cut.chunks), (unsigned)cut.units, (unsigned)width, f32_vectors, (float)scale};
-    const auto all = {dy, dn, y, branch, weight, post, gate, (const void*)dx, (const void*)dbranch};
+    const auto all = {dy, dn, x, branch, weight, post, gate, (const void*)dx, (const void*)dbranch};
     const NormShape s = norm_shape(width);
     cudaStream_t stream = (cudaStream_t)stream_v;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
-    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, full ? norm_form_of(branch, post, gate, scale) : 0, cut.ctas,
+    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, norm_form_of(branch, post, gate, scale), cut.ctas,
                                   (unsigned)s.threads, stream, a);
     if (e == cudaSuccess && vectors) {
         const NormColumnArgs c = {a.weight_sums, a.post_sums, a.gate_sums, dweight, dpost, dgate, cut.ctas, (unsigned)cut.chunks, (unsigned)width, (unsigned)blocks, f32_vectors};

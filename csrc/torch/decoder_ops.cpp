@@ -144,15 +144,15 @@ struct NormBackward : public Node {
     Tensor rstd, rstd_post;
     double scale = 1;
     int64_t gates = 0;
-    bool x_is_y = false, has_branch = false;      // x holds y: an output of this node
+    bool has_branch = false, own_branch = false;      // own_branch: its gradient is not that of x
 
     variable_list apply(variable_list&& grads) override {
-        const Tensor x_ = x.unpack(x_is_y ? shared_from_this() : nullptr), b = branch.unpack(), w = weight.unpack(), p = post.unpack(), g = gate.unpack();
+        const Tensor x_ = x.unpack(), b = branch.unpack(), w = weight.unpack(), p = post.unpack(), g = gate.unpack();
         const Tensor dy = has_branch ? dense(grads[0]) : Tensor(), dn = dense(grads[has_branch ? 1 : 0]);
         variable_list out(5);
         if (!dy.defined() && !dn.defined()) return out;
         const int64_t width = x_.size(-1), rows = x_.numel() / width;
-        const Tensor dx = fresh_like(x_), db = b.defined() ? fresh_like(b) : has_branch ? dx : Tensor();
+        const Tensor dx = fresh_like(x_), db = own_branch ? fresh_like(b) : has_branch ? dx : Tensor();
         const Tensor dw = dn.defined() && task_should_compute_output(2) ? fresh_like(w) : Tensor();
         const Tensor dp = p.defined() && task_should_compute_output(3) ? fresh_like(p) : Tensor(), dg = g.defined() && task_should_compute_output(4) ? fresh_like(g) : Tensor();
         if (rows) {
@@ -160,7 +160,7 @@ struct NormBackward : public Node {
             const size_t bytes = entry.norm_workspace(device, dtype_of(x_), rows, width, gates, p.defined(), b.defined());
             const Tensor work = fresh({(int64_t)bytes}, at::kByte, x_);
             const int rc = entry.norm_backward(device, dtype_of(x_), rows, width, ptr(dy), ptr(dn), ptr(x_), ptr(b), ptr(w), ptr(p), ptr(g), gates ? rows / gates : 0,
-                                               f32_vectors(x_, w, p, g), scale, ptr(rstd), ptr(rstd_post), ptr(dx), b.defined() ? ptr(db) : nullptr, ptr(dw), ptr(dp), ptr(dg),
+                                               f32_vectors(x_, w, p, g), scale, ptr(rstd), ptr(rstd_post), ptr(dx), own_branch ? ptr(db) : nullptr, ptr(dw), ptr(dp), ptr(dg),
                                                ptr(work), bytes, stream_of(x_));
             TORCH_CHECK(rc == 0, "residual_norm: the backward pass was not launched (see stderr)");
         } else {
@@ -216,16 +216,14 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             TORCH_CHECK(rc == 0, "residual_norm was not launched (see stderr)");
         }
         if (keep) {
-            // of a plain sum y is enough; otherwise the branch is needed anyway, and with x it gives y before its rounding
-            const bool full = branch.defined() && (post.defined() || gate.defined() || scale != 1.0);
             std::shared_ptr<NormBackward> node(new NormBackward(), torch::autograd::deleteNode);
             node->set_next_edges(torch::autograd::collect_next_edges(x, branch, weight, post, gate));
             node->scale = scale;
             node->gates = gates;
             node->has_branch = branch.defined();
-            node->x_is_y = branch.defined() && !full;
-            if (!node->x_is_y) node->x = SavedVariable(x, false);
-            if (full) node->branch = SavedVariable(branch, false);
+            node->own_branch = branch.defined() && (post.defined() || gate.defined() || scale != 1.0);
+            node->x = SavedVariable(x, false);
+            node->branch = SavedVariable(branch, false);
             node->weight = SavedVariable(weight, false);
             node->post = SavedVariable(post, false);
             node->gate = SavedVariable(gate, false);
@@ -233,7 +231,6 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             node->rstd_post = rstd_post;
             if (branch.defined()) torch::autograd::set_history(y, node);
             torch::autograd::set_history(n, node);
-            if (node->x_is_y) node->x = SavedVariable(y, true);
         }
     }
     return branch.defined() ? wrap(std::move(y), std::move(n)) : wrap(std::move(n));

@@ -1,8 +1,8 @@
 """The operators of a decoder block (dccl_b200.ops.decoder) against their formulas in 64 bits.
 
 Tolerances count roundings. A result of type T is off by half a step of T, u = eps / 2 of its size; what is computed in fp32 before
-that is off by a few times 2^-24 of the terms that went into it. Where a backward pass starts from a stored result of type T, its
-u goes through the formula as well: each bound below says how.
+that is off by a few times 2^-24 of the terms that went into it. Where a value is rounded to T on the way, its u goes through
+the formula as well: each bound below says how.
 """
 import math
 
@@ -70,8 +70,8 @@ def norm_check(t, dy, dn, scale, y, n, grads, dtype):
     check("n", n, yh * d["weight"], u * (yh * d["weight"]).abs() + F32 * d["weight"].abs() * (terms * ry + yh.abs()))
     if grads is None:
         return
-    # backward: yh comes from the stored y, which is off by u of itself, and so does mean(t yh)
-    e_yh = u * yh.abs() + F32 * terms * ry
+    # backward: y is made again in fp32 from x and the branch
+    e_yh = F32 * (terms * ry + yh.abs())
     tt = dn * d["weight"]
     c = (tt * yh).mean(-1, keepdim=True) if torch.is_tensor(tt) else torch.zeros_like(ry)
     c_abs, e_c = (tt * yh).abs().mean(-1, keepdim=True) if torch.is_tensor(tt) else c, (tt * e_yh).abs().mean(-1, keepdim=True) if torch.is_tensor(tt) else c
