@@ -49,7 +49,7 @@ int dtype_of(const Tensor& t) {
 /** A tensor of values in CUDA memory, and none that stands for others (fake, functional, a subclass that takes over dispatch). */
 bool is_plain(const Tensor& t) {
     return t.is_cuda() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper)
-           && !t.key_set().has(c10::DispatchKey::FuncTorchBatched) && !t.key_set().has(c10::DispatchKey::Functionalize) && !t.is_conj();
+           && !t.key_set().has(c10::DispatchKey::FuncTorchBatched) && !t.key_set().has(c10::DispatchKey::Functionalize) && !t._is_zerotensor();
 }
 
 /** `o` as a tensor: false where it is none, or not plain. None leaves `t` undefined, if `optional`. */
@@ -140,14 +140,13 @@ int f32_vectors(const Tensor& x, const Tensor& weight, const Tensor& post, const
 }
 
 struct NormBackward : public Node {
-    SavedVariable x, branch, weight, post, gate;
-    Tensor rstd, rstd_post;
+    SavedVariable x, branch, weight, post, gate, rstd, rstd_post;       // saved like any, so that checkpointing and hooks see them
     double scale = 1;
     int64_t gates = 0;
     bool has_branch = false, own_branch = false;      // own_branch: its gradient is not that of x
 
     variable_list apply(variable_list&& grads) override {
-        const Tensor x_ = x.unpack(), b = branch.unpack(), w = weight.unpack(), p = post.unpack(), g = gate.unpack();
+        const Tensor x_ = x.unpack(), b = branch.unpack(), w = weight.unpack(), p = post.unpack(), g = gate.unpack(), ry = rstd.unpack(), rb = rstd_post.unpack();
         const Tensor dy = has_branch ? dense(grads[0]) : Tensor(), dn = dense(grads[has_branch ? 1 : 0]);
         variable_list out(5);
         if (!dy.defined() && !dn.defined()) return out;
@@ -160,7 +159,7 @@ struct NormBackward : public Node {
             const size_t bytes = entry.norm_workspace(device, dtype_of(x_), rows, width, gates, p.defined(), b.defined());
             const Tensor work = fresh({(int64_t)bytes}, at::kByte, x_);
             const int rc = entry.norm_backward(device, dtype_of(x_), rows, width, ptr(dy), ptr(dn), ptr(x_), ptr(b), ptr(w), ptr(p), ptr(g), gates ? rows / gates : 0,
-                                               f32_vectors(x_, w, p, g), scale, ptr(rstd), ptr(rstd_post), ptr(dx), own_branch ? ptr(db) : nullptr, ptr(dw), ptr(dp), ptr(dg),
+                                               f32_vectors(x_, w, p, g), scale, ptr(ry), ptr(rb), ptr(dx), own_branch ? ptr(db) : nullptr, ptr(dw), ptr(dp), ptr(dg),
                                                ptr(work), bytes, stream_of(x_));
             TORCH_CHECK(rc == 0, "residual_norm: the backward pass was not launched (see stderr)");
         } else {
@@ -172,9 +171,7 @@ struct NormBackward : public Node {
     }
     std::string name() const override { return "ResidualNormBackward"; }
     void release_variables() override {
-        for (SavedVariable* v : {&x, &branch, &weight, &post, &gate}) v->reset_data();
-        rstd.reset();
-        rstd_post.reset();
+        for (SavedVariable* v : {&x, &branch, &weight, &post, &gate, &rstd, &rstd_post}) v->reset_data();
     }
 };
 
@@ -227,8 +224,8 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             node->weight = SavedVariable(weight, false);
             node->post = SavedVariable(post, false);
             node->gate = SavedVariable(gate, false);
-            node->rstd = rstd;
-            node->rstd_post = rstd_post;
+            node->rstd = SavedVariable(rstd, false);
+            node->rstd_post = SavedVariable(rstd_post, false);
             if (branch.defined()) torch::autograd::set_history(y, node);
             torch::autograd::set_history(n, node);
         }
@@ -370,15 +367,13 @@ Tensor gated_work(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, boo
 }
 
 struct GatedBackward : public Node {
-    SavedVariable x, w_gate, w_up;
-    Tensor g, u, padded;
+    SavedVariable x, w_gate, w_up, gate, up, padded;
     int act = 0;
 
     variable_list apply(variable_list&& grads) override {
-        const Tensor x_ = x.unpack(), wg = w_gate.unpack(), wu = w_up.unpack(), dh = dense(grads[0]);
+        const Tensor x_ = x.unpack(), wg = w_gate.unpack(), wu = w_up.unpack(), g = gate.unpack(), u = up.unpack(), copies = padded.unpack(), dh = dense(grads[0]);
         variable_list out(3);
         if (!dh.defined()) return out;
-        TORCH_CHECK(g.defined(), "gated_linear: the graph was freed by an earlier backward pass (retain_graph=True keeps it)");
         const bool weights = task_should_compute_output(1) || task_should_compute_output(2);
         const Tensor dx = task_should_compute_output(0) ? fresh_like(x_) : Tensor();
         const Tensor dg = weights ? fresh_like(wg) : Tensor(), du = weights ? fresh_like(wu) : Tensor();
@@ -386,7 +381,7 @@ struct GatedBackward : public Node {
         if (tokens) {
             const Tensor work = gated_work(x_, wg, wu, true);
             const int rc = entry.gated_backward(x_.device().index(), dtype_of(x_), tokens, width, wg.size(0), ptr(dh), ptr<float>(g), ptr<float>(u), g.size(1), ptr(x_), ptr(wg), ptr(wu),
-                                                ptr(padded), act, ptr(dx), ptr(dg), ptr(du), ptr(work), work.defined() ? (long long)work.numel() : 0, stream_of(x_));
+                                                ptr(copies), act, ptr(dx), ptr(dg), ptr(du), ptr(work), work.defined() ? (long long)work.numel() : 0, stream_of(x_));
             TORCH_CHECK(rc == 0, "gated_linear: the backward pass was not launched (see stderr)");
         } else if (weights) {
             dg.zero_();
@@ -397,8 +392,7 @@ struct GatedBackward : public Node {
     }
     std::string name() const override { return "GatedLinearBackward"; }
     void release_variables() override {
-        for (SavedVariable* v : {&x, &w_gate, &w_up}) v->reset_data();
-        for (Tensor* t : {&g, &u, &padded}) t->reset();
+        for (SavedVariable* v : {&x, &w_gate, &w_up, &gate, &up, &padded}) v->reset_data();
     }
 };
 
@@ -445,9 +439,9 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             node->x = SavedVariable(x, false);
             node->w_gate = SavedVariable(wg, false);
             node->w_up = SavedVariable(wu, false);
-            node->g = g;
-            node->u = u;
-            if (entry.gated_pads(width, gated_aligned(x, wg, wu))) node->padded = work;
+            node->gate = SavedVariable(g, false);
+            node->up = SavedVariable(u, false);
+            node->padded = SavedVariable(entry.gated_pads(width, gated_aligned(x, wg, wu)) ? work : Tensor(), false);
             node->act = act;
             torch::autograd::set_history(h, node);
         }

@@ -809,3 +809,24 @@ def test_operators_refuse_tensors_without_memory():
 def test_negated_views():
     x, w = torch.randn(3, 64, device="cuda"), torch.ones(64, device="cuda")
     assert torch.equal(ops.rms_norm(torch._neg_view(x), w), ops.rms_norm(-x, w))
+
+
+@gpu
+def test_checkpointed_operators():
+    """What a backward pass needs is dropped and made again, also what no input or output is."""
+    from torch.utils.checkpoint import checkpoint
+    x, wg, wu, dh = gated_case(40, 65, 72, torch.bfloat16, "cuda")
+    w = torch.ones(65, device="cuda").bfloat16().requires_grad_(True)
+    for t in (x, wg, wu):
+        t.requires_grad_(True)
+
+    def part(v):
+        return ops.gated_linear(ops.residual_norm(v, v, w, post_weight=w)[1], wg, wu)
+
+    want = torch.autograd.grad(part(x), (x, w, wg, wu), dh)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(tuple(t.shape)) or t, lambda t: t):
+        part(x)
+    assert kept.count((40, 72)) == 2 and (40,) in kept          # the products and the rows' statistics
+    got = torch.autograd.grad(checkpoint(part, x, use_reentrant=False), (x, w, wg, wu), dh)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
