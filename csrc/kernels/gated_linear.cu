@@ -613,15 +613,16 @@ static GemmPlan plan_gemm(int sms, int form, size_t m, size_t n, size_t k) {
     p.batch = form == WEIGHT_GRAD ? 2 : 1;
     p.k_blocks = blocks_of(k, kTileK) * (form == INPUT_GRAD ? 2 : 1);
     const unsigned workers = p.pair ? sms / 2 : sms;
-    // rounds of tiles, and what a round takes: half as wide a tile reads one operand twice as often
-    const auto tiles_n = [&](int columns) { return blocks_of(n, form == GATED ? columns / 2 : columns); };
-    const auto rounds = [&](int columns) { return ((size_t)p.tiles_m * tiles_n(columns) * p.batch + workers - 1) / workers; };
-    p.columns = rounds(128) * 15 < rounds(256) * 26 ? 128 : 256;
-    p.tiles_n = tiles_n(p.columns);
-    const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch;
-    size_t splits = workers / (tiles ? tiles : 1);
-    if (splits > p.k_blocks / 4) splits = p.k_blocks / 4;
-    p.splits = splits > 1 ? (unsigned)splits : 1;
+    const auto tiles_of = [&](int columns) { return (size_t)p.tiles_m * blocks_of(n, form == GATED ? columns / 2 : columns) * p.batch; };
+    const auto splits_of = [&](int columns) {
+        const size_t tiles = tiles_of(columns), most = p.k_blocks / 4, s = workers / (tiles ? tiles : 1);
+        return s > most ? (most ? most : 1) : s ? s : 1;
+    };
+    // rounds of tiles, and what a round takes: a tile of half the width loads three quarters of the bytes, which is what these products wait for
+    const auto cost = [&](int columns) { return (columns == 128 ? 3 : 4) * 64 * ((tiles_of(columns) + workers - 1) / workers) / splits_of(columns); };
+    p.columns = cost(128) < cost(256) ? 128 : 256;
+    p.tiles_n = blocks_of(n, form == GATED ? p.columns / 2 : p.columns);
+    p.splits = (unsigned)splits_of(p.columns);
     p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (form == INPUT_GRAD ? 1 : 2) * m * up_to(n, 4) * sizeof(float) : 0;
     return p;
 }
