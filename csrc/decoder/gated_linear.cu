@@ -10,7 +10,7 @@
  * tile's orientation. Sums stay in tensor memory in fp32 until the end of a tile.
  */
 #include "decoder_ops.hpp"
-#include "launch_early.cuh"
+#include "../kernels/launch_early.cuh"
 #include "row_access.cuh"
 #include "../device/tcgen05.cuh"
 #include "../gpu/driver_api.hpp"

@@ -17,7 +17,7 @@
  * would save a plain sum one of five arrays, its rounding goes into every term of dw and makes that half again as inexact.
  */
 #include "decoder_ops.hpp"
-#include "launch_early.cuh"
+#include "../kernels/launch_early.cuh"
 #include "row_access.cuh"
 
 namespace dccl {
@@ -47,8 +47,9 @@ struct NormGradArgs {
 /** What a call has. The kernels are compiled for each: tests of pointers inside of the loops took a third of their instructions. */
 enum { BRANCH = 1, POST = 2, GATE = 4, SCALE = 8 };
 
-/** E elements per thread in runs of V, run k of thread t at (k * threads + t) * V. */
-template <typename T, int V, int E, int F>
+/** E elements per thread in runs of V, run k of thread t at (k * threads + t) * V. EXACT: rows fill the threads' elements, and no test stands between
+ *  the loads of one run and the arithmetic of another (backward, 8192 elements: 227 -> 203 us). */
+template <typename T, int V, int E, int F, bool EXACT>
 __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ? 2 : 1) k_residual_norm(const __grid_constant__ NormArgs a) {
     wait_for_stream();
     constexpr int K = E / V;
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ?
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const unsigned i = t + k * step;
-        if (i < runs) {
+        if (EXACT || i < runs) {
             xr[k] = ld_run<T, V>(x + (size_t)i * V);
             if constexpr (F & BRANCH) br[k] = ld_run<T, V>(b + (size_t)i * V);
         }
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ?
         float sum = 0;
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (t + k * step < runs)
+            if (EXACT || t + k * step < runs)
 #pragma unroll
                 for (int e = 0; e < V; e++) { const float v = Traits<T>::up(br[k].e[e]); sum = fmaf(v, v, sum); }
         factor = rsqrtf(cta_sum(sum, parts[0]) / a.width + a.eps);
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ?
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const unsigned i = t + k * step;
-        if (i >= runs) continue;
+        if (!EXACT && i >= runs) continue;
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; e++) v[e] = Traits<T>::up(xr[k].e[e]);
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ?
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const unsigned i = t + k * step;
-        if (i >= runs) continue;
+        if (!EXACT && i >= runs) continue;
         float w[V];
         ld_vector<T, V>(w, a.weight, a.f32 & DCCL_NORM_WEIGHT_F32, (size_t)i * V);
 #pragma unroll
@@ -148,7 +149,7 @@ template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(uns
  * that start anywhere are copied in the aligned 16 bytes that they touch, which the threads share. (Read by element from global memory,
  * rows of 1451 fp16 took 36 us out of L2 and 60 out of HBM for 1551 rows.) The vectors are kept there in fp32.
  */
-template <typename T, int V, int E, int F>
+template <typename T, int V, int E, int F, bool EXACT>
 __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? (F & FULL ? 3 : 4) : 1) k_residual_norm_grad(const __grid_constant__ NormGradArgs a) {
     wait_for_stream();
     constexpr int K = E / V, kArrays = F & BRANCH ? 4 : 3, kStages = kNormStages<T, E>, kPiece = V < 4 ? V : 4;
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                 const unsigned i = t + k * step;
 #pragma unroll
                 for (int j = 0; j < kArrays; j++)
-                    if (i < runs && arrays[j]) {
+                    if ((EXACT || i < runs) && arrays[j]) {
                         const uint32_t to = (uint32_t)__cvta_generic_to_shared(staged + ((stage * kArrays + j) * K + k) * step + t);
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(arrays[j] + row * a.width + (size_t)i * V) : "memory");
                     }
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const unsigned i = t + k * step;
-            if (i >= runs) continue;
+            if (!EXACT && i >= runs) continue;
             float f[V];
             ld_vector<T, V>(f, from, a.f32 & flag, at + (size_t)i * V);
 #pragma unroll
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
 #pragma unroll
                 for (int k = 0; k < K; k++) {
                     const unsigned i = t + k * step;
-                    if (i >= runs) continue;
+                    if (!EXACT && i >= runs) continue;
                     float w[V], dn[V], y[V];
                     load(DN, k, stage, dn);
                     load(X, k, stage, y);
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const unsigned i = t + k * step;
-                if (i >= runs) continue;
+                if (!EXACT && i >= runs) continue;
                 float dy[V];
                 if (a.dy) load(DY, k, stage, dy);
                 float out[V];
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
 #pragma unroll
                 for (int k = 0; k < K; k++) {
                     const unsigned i = t + k * step;
-                    if (i >= runs) continue;
+                    if (!EXACT && i >= runs) continue;
                     float b[V];
                     load(B, k, stage, b);
 #pragma unroll
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
             if (a.gate_sums) {
 #pragma unroll
                 for (int k = 0; k < K; k++)
-                    if (t + k * step < runs)
+                    if (EXACT || t + k * step < runs)
 #pragma unroll
                         for (int e = 0; e < V; e++) {
                             a.gate_sums[(size_t)unit * a.width + (t + k * step) * V + e] = sum_g[k * V + e];
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
     }
 #pragma unroll
     for (int k = 0; k < K; k++)
-        if (t + k * step < runs)
+        if (EXACT || t + k * step < runs)
 #pragma unroll
             for (int e = 0; e < V; e++) {
                 const size_t j = (size_t)blockIdx.x * a.width + (size_t)(t + k * step) * V + e;
@@ -484,19 +485,26 @@ static NormCut norm_cut(int device, int dtype, size_t rows, size_t width, size_t
 }
 
 template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormArgs& a, int) {
-    return launch_early(k_residual_norm<T, V, E, F>, grid, block, stream, a);
+    if constexpr (V * sizeof(T) == 16 && E == 16)       // with fewer elements it takes more registers, and 1 us longer at 16384 x 2048
+        if (a.width == block * E) return launch_early(k_residual_norm<T, V, E, F, true>, grid, block, stream, a);
+    return launch_early(k_residual_norm<T, V, E, F, false>, grid, block, stream, a);
 }
-template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, int device) {
+template <typename T, int V, int E, int F, bool EXACT> static cudaError_t norm_grad_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, int device) {
     const size_t shared = norm_grad_shared<T, V, E, F>(block, a.width);
     if (shared > 40 << 10) {        // 48 KB with the static part need no leave
         static std::atomic<bool> ready[64];
         if (!ready[device].load(std::memory_order_relaxed)) {
-            const cudaError_t e = cudaFuncSetAttribute(k_residual_norm_grad<T, V, E, F>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024);
+            const cudaError_t e = cudaFuncSetAttribute(k_residual_norm_grad<T, V, E, F, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024);
             if (e != cudaSuccess) return e;
             ready[device].store(true, std::memory_order_relaxed);
         }
     }
-    return launch_early_shared(k_residual_norm_grad<T, V, E, F>, grid, block, shared, stream, a);
+    return launch_early_shared(k_residual_norm_grad<T, V, E, F, EXACT>, grid, block, shared, stream, a);
+}
+template <typename T, int V, int E, int F> static cudaError_t norm_launch(unsigned grid, unsigned block, cudaStream_t stream, const NormGradArgs& a, int device) {
+    if constexpr (V * sizeof(T) == 16 && E <= 16)
+        if (a.width == block * E) return norm_grad_launch<T, V, E, F, true>(grid, block, stream, a, device);
+    return norm_grad_launch<T, V, E, F, false>(grid, block, stream, a, device);
 }
 template <typename T, int V, int E, typename Args> static cudaError_t norm_form(int form, unsigned grid, unsigned block, cudaStream_t stream, const Args& a, int device) {
     switch (form) {

@@ -10,7 +10,7 @@
  * element, as many instructions as to turn it, is paid once for all tokens.
  */
 #include "decoder_ops.hpp"
-#include "launch_early.cuh"
+#include "../kernels/launch_early.cuh"
 #include "row_access.cuh"
 
 namespace dccl {

@@ -1,5 +1,5 @@
 /**
- * Host side of the operators of a decoder block (csrc/kernels/decoder_ops.hpp) for dccl_b200/ops/decoder.py: their checks, outputs,
+ * Host side of the operators of a decoder block (csrc/decoder/decoder_ops.hpp) for dccl_b200/ops/decoder.py: their checks, outputs,
  * workspaces, launches on torch's current stream, and nodes of the autograd graph. The kernels of a decoding step take two to
  * three microseconds; from Python a call took 16 to 20, forward and backward together 130.
  *
@@ -7,7 +7,7 @@
  * says what is wrong. Plain CPython functions: their arguments are borrowed. Everything that could throw is caught at this border.
  */
 #include "decoder_ops.hpp"
-#include "../kernels/decoder_ops.hpp"
+#include "../decoder/decoder_ops.hpp"
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>

@@ -11,7 +11,7 @@
     gated_linear          act(x Wg^T) * (x Wu^T): the two projections of a gated feed-forward layer
     ====================  ==============================================================================
 
-All are differentiable. CUDA tensors run one kernel per call on the current stream of their device (csrc/kernels/residual_norm.cu,
+All are differentiable. CUDA tensors run one kernel per call on the current stream of their device (csrc/decoder/residual_norm.cu,
 rotary.cu, gated_linear.cu) in float16, bfloat16 or float32 (gated_linear: not float32); sums and statistics are fp32 and every result is rounded once. CPU tensors take
 the same formulas in torch, so the same model code is tested without a GPU. Inputs may have any strides; what a kernel cannot
 read in place is copied first. A call allocates its outputs and its workspace from torch's allocator and nothing else, so it can be
@@ -27,7 +27,7 @@ import torch
 from .._lib import lib
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
-_MAX_WIDTH, _MAX_PAIRS = 32768, 1024                 # kNormMaxWidth of csrc/kernels/residual_norm.cu, kRotaryPairs of rotary.cu
+_MAX_WIDTH, _MAX_PAIRS = 32768, 1024                 # kNormMaxWidth of csrc/decoder/residual_norm.cu, kRotaryPairs of rotary.cu
 
 
 _ENTRIES = ("dccl_residual_norm", "dccl_residual_norm_workspace", "dccl_residual_norm_backward", "dccl_rotary", "dccl_gated_linear_workspace", "dccl_gated_linear_pads",
@@ -261,7 +261,7 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling=None, factor=1.0, orig
 
 # ---------------------------------------------------------------------------------------------- gated linear
 
-_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}        # csrc/kernels/decoder_ops.hpp
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}        # csrc/decoder/decoder_ops.hpp
 
 
 def _activate_on_cpu(g, activation):

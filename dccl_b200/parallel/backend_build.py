@@ -22,7 +22,7 @@ _ROOT = os.path.dirname(_PKG)
 SRC_DIR = os.path.join(_ROOT, "csrc", "torch")
 SRCS = [os.path.join(SRC_DIR, name) for name in ("pg_dccl.cpp", "adamw_step.cpp", "decoder_ops.cpp")]
 HEADERS = [os.path.join(SRC_DIR, name) for name in ("adamw_step.hpp", "decoder_ops.hpp")]
-HEADERS += [os.path.join(_ROOT, "csrc", "kernels", name) for name in ("adamw.hpp", "decoder_ops.hpp")] + [os.path.join(_ROOT, "include", "dccl", "dccl.hpp")]
+HEADERS += [os.path.join(_ROOT, "csrc", "kernels", "adamw.hpp"), os.path.join(_ROOT, "csrc", "decoder", "decoder_ops.hpp")] + [os.path.join(_ROOT, "include", "dccl", "dccl.hpp")]
 OUT = os.path.join(_PKG, "lib", "_dccl_torch-%s-torch%s.so" % (sys.implementation.cache_tag, torch.__version__))
 
 

@@ -32,6 +32,24 @@ def check(name, got, want, bound):
         name, off.max(), bound.reshape(-1)[off.argmax()], off.argmax().item(), got.reshape(-1)[off.argmax()], want.reshape(-1)[off.argmax()])
 
 
+def test_early_launched_kernels_promise_nothing_about_their_inputs():
+    """As tests/test_local_calls.py asks of the kernels that it knows: they are launched before the one ahead of them has written, so every one
+    waits, and none declares what it reads read-only for as long as it runs."""
+    import os
+    folder, found = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc", "decoder"), set()
+    for name in sorted(os.listdir(folder)):
+        text = open(os.path.join(folder, name)).read()
+        assert "__restrict__" not in text and "__ldg" not in text, name
+        for part in text.split("__global__")[1:]:
+            signature, body = part.split("{", 1)
+            kernel = signature[:signature.rindex("(")].split("k_")[-1]
+            assert "wait_for_stream()" in body.split("\n}", 1)[0] or "gemm<" in body.split("\n", 1)[0], kernel
+            found.add(kernel.split("(")[0])
+    assert found == {"residual_norm", "residual_norm_grad", "norm_columns", "rotary", "gemm", "gemm_pair", "gated_few", "join", "pad", "gate_grad"}
+    gemm = open(os.path.join(folder, "gated_linear.cu")).read()
+    assert gemm.index("wait_for_stream()") < gemm.index("load(to_a")
+
+
 # ---------------------------------------------------------------------------------------------- norms
 
 def norm_case(shape, dtype, post, gate, wide, seed=0, device="cpu"):
