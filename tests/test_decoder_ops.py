@@ -742,11 +742,12 @@ def test_a_decoding_step_in_a_graph():
 
 
 @gpu
-def test_a_training_step_in_a_graph():
+@pytest.mark.parametrize("rows,width,ffn", [(70, 96, 80), (300, 264, 320), (130, 65, 131)])
+def test_a_training_step_in_a_graph(rows, width, ffn):
     """Forward and backward captured, replayed on new inputs."""
-    x, branch, weight = (t.cuda().bfloat16().requires_grad_(True) for t in (torch.randn(70, 96), torch.randn(70, 96), torch.ones(96)))
-    wg, wu = (torch.randn(80, 96).mul(0.1).cuda().bfloat16().requires_grad_(True) for _ in range(2))
-    dh = torch.randn(70, 80).cuda().bfloat16()
+    x, branch, weight = (t.cuda().bfloat16().requires_grad_(True) for t in (torch.randn(rows, width), torch.randn(rows, width), torch.ones(width)))
+    wg, wu = (torch.randn(ffn, width).mul(0.1).cuda().bfloat16().requires_grad_(True) for _ in range(2))
+    dh = torch.randn(rows, ffn).cuda().bfloat16()
 
     def step():
         y, n = ops.residual_norm(x, branch, weight, post_weight=weight, scale=0.5)
@@ -762,10 +763,52 @@ def test_a_training_step_in_a_graph():
         outs = step()
     for seed in range(2):
         with torch.no_grad():
-            x.copy_(torch.randn(70, 96, generator=torch.Generator().manual_seed(seed)))
+            x.copy_(torch.randn(rows, width, generator=torch.Generator().manual_seed(seed)))
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+
+
+FIRST = """
+import torch
+from dccl_b200 import ops
+x, w, wg, wu = (torch.randn(s, device="cuda").bfloat16() for s in ((200, 128), (128,), (256, 128), (256, 128)))
+freqs = ops.rotary_frequencies(32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+step = lambda: (ops.gated_linear(ops.rms_norm(x, w), wg, wu), ops.gated_linear(x[:1], wg, wu), ops.rotary(x.view(1, 200, 4, 32), None, freqs))
+with torch.cuda.graph(graph):
+    outs = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+print("OK")
+"""
+
+
+@gpu
+def test_the_first_call_of_a_process_can_be_captured():
+    import os
+    import subprocess
+    import sys
+    res = subprocess.run([sys.executable, "-c", FIRST], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip().endswith("OK"), res.stdout + res.stderr[-2000:]
+
+
+@gpu
+def test_operators_on_a_device_that_is_not_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    x, wg, wu, dh = gated_case(140, 64, 144, torch.bfloat16, "cuda:1")
+    for t in (x, wg, wu):
+        t.requires_grad_(True)
+    w = torch.ones(64, device="cuda:1").bfloat16()
+    h = ops.gated_linear(ops.rms_norm(x, w), wg, wu)
+    grads = torch.autograd.grad(h, (x, wg, wu), dh)
+    with torch.cuda.device(1):
+        again = ops.gated_linear(ops.rms_norm(x, w), wg, wu)
+        assert torch.equal(h, again) and all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(again, (x, wg, wu), dh)))
+    assert torch.cuda.current_device() == 0
 
 
 @gpu
