@@ -105,14 +105,15 @@ class ShardedBlock(nn.Module):
 
     def fused(self, x, n, freqs, after):
         """(x, n) after this block, as of the unsplit one. The pool takes the products at the exits and the input gradient of attention; that of
-        the gated product is a tensor of its own."""
-        x, n = residual_norm(x, self.attn.fused(n, freqs), self.n2.weight, eps=self.n2.eps)
+        the gated product is a tensor of its own. What a residual norm adds it keeps for the backward pass, so it gets a copy of a pool's buffer."""
+        a = self.attn.fused(n, freqs)
+        x, n = residual_norm(x, a if self.pool is None else a.clone(), self.n2.weight, eps=self.n2.eps)
         h = ops.all_gather(n, 1, self.comm) if self.sp else ops.copy_to_region(n, self.comm)
         h = gated_linear(h, self.gate.weight, self.up.weight)
         if self.sp:
             m = ops.reduce_scatter(self.down(h), 1, "sum", self.comm)
         elif self.pool is not None:
-            m = row_linear_reduce_in_place(h, self.down.weight, self.comm, self.pool)
+            m = row_linear_reduce_in_place(h, self.down.weight, self.comm, self.pool).clone()
         else:
             m = ops.reduce_from_region(self.down(h), self.comm)
         return residual_norm(x, m, after.weight, eps=after.eps)

@@ -147,7 +147,7 @@ def residual_norm(x, branch, weight, eps=1e-5, post_weight=None, gate=None, scal
 
     `branch` is what the sub-block computed, of x's shape and type. `gate` is one row ([width]), or one row per entry of x's leading
     dimensions ([batch, 1, width] for one gate per sequence). `weight`, `post_weight` and `gate` have x's type, or float32. n
-    comes from y before y is rounded. In backward an output that nothing used costs nothing; with scale 1 and neither gate
+    comes from y before y is rounded. x and branch are kept for the backward pass and must not be overwritten before it. In backward an output that nothing used costs nothing; with scale 1 and neither gate
     nor post_weight, x and branch get the same tensor as their gradient, as from a sum."""
     if branch is None:
         raise TypeError("residual_norm: branch must be a tensor (rms_norm has none)")
@@ -274,7 +274,8 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     """``act(x @ w_gate.T) * (x @ w_up.T)``: x [..., width], the weights [ffn, width], all of one type; `activation` is "silu", "gelu" or
     "gelu_tanh". Both products stay in fp32 up to the one rounding of the result.
 
-    On the GPU x is float16 or bfloat16. For the backward pass the call keeps the two products in fp32 (8 bytes per element of the result):
+    On the GPU x is float16 or bfloat16. The gradients of the two products are rounded to that type once, to be multiplied again: in float16
+    they overflow above 65504. For the backward pass the call keeps the two products in fp32 (8 bytes per element of the result):
     from 16 bits their rounding would come on top of the one that their gradients need to be multiplied again."""
     if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(activation, str):
         h = _ext().gated_linear(x, w_gate, w_up, _ACTIVATIONS.get(activation, -1))
