@@ -8,8 +8,8 @@
  * and its gradients. With yh = y ry, bh = b rb and t = dn .* w, the derivative of a row's norm is ry (t - yh mean(t .* yh)):
  *
  *     D = dy + ry (t - yh mean(t .* yh))        dx = D          dw  = sum over rows dn .* yh
- *     u = s g .* D .* w2                        db = rb (u - bh mean(u .* bh))
- *     dw2 = sum s g .* D .* bh                  dg  = sum s D .* p
+ *     u = s g .* w2 .* D                        db = rb (u - bh mean(u .* bh))
+ *     S   = sum over rows of a gate D .* bh     dg  = s w2 .* S,  dw2 = sum over gates s g .* S
  *
  * A few operations per element that is moved: HBM bounds both. A CTA holds a row in registers, so that x, b (forward) and
  * dy, dn, x, b (backward) are read once and the sums of a row cost one barrier each. Rows are summed in fp32, and n comes from the
@@ -40,7 +40,7 @@ struct NormGradArgs {
     const void *dy, *dn, *x, *branch, *weight, *post, *gate;
     const float *rstd, *rstd_post;
     void *dx, *dbranch;
-    float *weight_sums, *post_sums, *gate_sums;      // [CTA][width], [CTA][width], [unit][width]
+    float *weight_sums, *branch_sums;                // [CTA][width], [unit][width]
     size_t rows, rows_per_gate;
     Divisor chunks;                                  // of the rows of a gate
     unsigned chunk_rows, longer, units, width;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 16 ?
 
 /** The arrays that a row of the backward pass reads. */
 enum { DN, X, DY, B };
-enum { IN_WEIGHT, IN_POST, IN_GATE };   // the vectors, in shared memory as fp32
+enum { IN_WEIGHT, IN_BRANCH };          // the vectors, in shared memory as fp32: w, and s g .* w2, of which a row of the branch takes nothing else
 constexpr int FULL = POST | GATE | SCALE;      // any of them, and the branch has a gradient that is not x's
 
 /** Rows in shared memory at a time: three of up to 2048 elements, two of up to 8192 16-bit ones. */
@@ -143,12 +143,12 @@ template <typename T, int V, int E> __host__ __device__ constexpr size_t norm_ro
 }
 
 template <typename T, int V, int E, int F> constexpr size_t norm_grad_shared(unsigned threads, unsigned width) {
-    return kNormStages<T, E> * (F & BRANCH ? 4 : 3) * norm_row_bytes<T, V, E>(threads, width) + (E <= 16 ? (size_t)threads * E * (F & FULL ? 3 : 1) * sizeof(float) : 0);
+    return kNormStages<T, E> * (F & BRANCH ? 4 : 3) * norm_row_bytes<T, V, E>(threads, width) + (E <= 16 ? (size_t)threads * E * (F & FULL ? 2 : 1) * sizeof(float) : 0);
 }
 
 /**
- * Each CTA takes units of rows that share a row of the gate and keeps the columns' sums (dw, dw2, dg) in registers: dg leaves at
- * the end of a unit, dw and dw2 at the end of the CTA, for k_norm_columns to add. The next rows are copied into shared memory while
+ * Each CTA takes units of rows that share a row of the gate and keeps the columns' sums (dw, S) in registers: S leaves at
+ * the end of a unit, dw at the end of the CTA, for k_norm_columns to add. The next rows are copied into shared memory while
  * the CTA works on this one: where accesses are 16 bytes wide, each thread's own elements by itself, with no barrier to guard them. Rows
  * that start anywhere are copied in the aligned 16 bytes that they touch, which the threads share. (Read by element from global memory,
  * rows of 1451 fp16 took 36 us out of L2 and 60 out of HBM for 1551 rows.) The vectors are kept there in fp32.
@@ -221,23 +221,33 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
 #pragma unroll
         for (int e = 0; e < V; e++) f[e] = Traits<T>::up(r.e[e]);
     };
-    const auto keep_vector = [&](int which, const void* from, int flag, size_t at) {
+    const auto put = [&](int which, int k, const float (&f)[V]) {
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const unsigned i = t + k * step;
-            if (!EXACT && i >= runs) continue;
-            float f[V];
-            ld_vector<T, V>(f, from, a.f32 & flag, at + (size_t)i * V);
+        for (int q = 0; q < V / kPiece; q++) {
+            Run<float, kPiece> piece;
 #pragma unroll
-            for (int q = 0; q < V / kPiece; q++) {
-                Run<float, kPiece> piece;
-#pragma unroll
-                for (int e = 0; e < kPiece; e++) piece.e[e] = f[q * kPiece + e];
-                vectors[((which * K + k) * (V / kPiece) + q) * step + t] = piece;
-            }
+            for (int e = 0; e < kPiece; e++) piece.e[e] = f[q * kPiece + e];
+            vectors[((which * K + k) * (V / kPiece) + q) * step + t] = piece;
         }
     };
-    const auto vector = [&](int which, const void* from, int flag, size_t at, int k, float (&f)[V]) {
+    const auto weight_of = [&](int k, float (&f)[V]) { ld_vector<T, V>(f, a.weight, a.f32 & DCCL_NORM_WEIGHT_F32, (size_t)(t + k * step) * V); };
+    const auto branch_of = [&](size_t gate_at, int k, float (&f)[V]) {
+        const size_t i = (size_t)(t + k * step) * V;
+#pragma unroll
+        for (int e = 0; e < V; e++) f[e] = a.scale;
+        float w[V];
+        if constexpr (F & POST) {
+            ld_vector<T, V>(w, a.post, a.f32 & DCCL_NORM_POST_F32, i);
+#pragma unroll
+            for (int e = 0; e < V; e++) f[e] *= w[e];
+        }
+        if constexpr (F & GATE) {
+            ld_vector<T, V>(w, a.gate, a.f32 & DCCL_NORM_GATE_F32, gate_at + i);
+#pragma unroll
+            for (int e = 0; e < V; e++) f[e] *= w[e];
+        }
+    };
+    const auto vector = [&](int which, size_t gate_at, int k, float (&f)[V]) {
         if constexpr (kVectors) {
 #pragma unroll
             for (int q = 0; q < V / kPiece; q++) {
@@ -245,20 +255,23 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
 #pragma unroll
                 for (int e = 0; e < kPiece; e++) f[q * kPiece + e] = piece.e[e];
             }
-        } else {
-            ld_vector<T, V>(f, from, a.f32 & flag, at + (size_t)(t + k * step) * V);
-        }
+        } else if (which == IN_WEIGHT) weight_of(k, f);
+        else branch_of(gate_at, k, f);
     };
     if constexpr (kVectors) {
-        keep_vector(IN_WEIGHT, a.weight, DCCL_NORM_WEIGHT_F32, 0);
-        if constexpr (F & POST) keep_vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (!EXACT && t + k * step >= runs) continue;
+            float f[V];
+            weight_of(k, f);
+            put(IN_WEIGHT, k, f);
+        }
     }
-    float sum_w[E], sum_p[F & POST ? E : 1], sum_g[F & GATE ? E : 1];
+    float sum_w[E], sum_b[F & (POST | GATE) ? E : 1];
 #pragma unroll
     for (int e = 0; e < E; e++) {
         sum_w[e] = 0;
-        if constexpr (F & POST) sum_p[e] = 0;
-        if constexpr (F & GATE) sum_g[e] = 0;
+        if constexpr (F & (POST | GATE)) sum_b[e] = 0;
     }
     unsigned turn = 0;
     for (unsigned unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
@@ -275,7 +288,15 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
         }
-        if constexpr ((F & GATE) && kVectors) keep_vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at);
+        if constexpr ((F & FULL) && kVectors) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (!EXACT && t + k * step >= runs) continue;
+                float f[V];
+                branch_of(gate_at, k, f);
+                put(IN_BRANCH, k, f);
+            }
+        }
         float next_ry = a.dn && begin < end ? a.rstd[begin] : 0.0f, next_rb = 1.0f;
         if constexpr (F & POST) next_rb = begin < end ? a.rstd_post[begin] : 0.0f;
         for (size_t row = begin; row < end; row++, turn ^= 1) {
@@ -307,20 +328,15 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                     if constexpr (F & BRANCH) {
                         float p[V];
                         load(B, k, stage, p);
-                        if constexpr (F & POST) {
-                            vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0, k, w);
-#pragma unroll
-                            for (int e = 0; e < V; e++) p[e] *= w[e];
-                        }
-                        if constexpr (F & GATE) {
-                            vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at, k, w);
+                        if constexpr (F & FULL) {
+                            vector(IN_BRANCH, gate_at, k, w);
 #pragma unroll
                             for (int e = 0; e < V; e++) p[e] *= w[e];
                         }
 #pragma unroll
-                        for (int e = 0; e < V; e++) y[e] = F & (POST | SCALE) ? fmaf(F & POST ? rb * a.scale : a.scale, p[e], y[e]) : y[e] + p[e];      // as the forward pass rounds
+                        for (int e = 0; e < V; e++) y[e] = F & POST ? fmaf(rb, p[e], y[e]) : y[e] + p[e];
                     }
-                    vector(IN_WEIGHT, a.weight, DCCL_NORM_WEIGHT_F32, 0, k, w);
+                    vector(IN_WEIGHT, 0, k, w);
 #pragma unroll
                     for (int e = 0; e < V; e++) {
                         const int j = k * V + e;
@@ -351,25 +367,16 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
                 }
                 store(false, row, k, out);
                 if constexpr (F & FULL) {
-                    float w2[V], g[V], b[V];
+                    float w[V], b[V];
                     load(B, k, stage, b);
-                    if constexpr (F & POST) vector(IN_POST, a.post, DCCL_NORM_POST_F32, 0, k, w2);
-                    if constexpr (F & GATE) vector(IN_GATE, a.gate, DCCL_NORM_GATE_F32, gate_at, k, g);
+                    vector(IN_BRANCH, gate_at, k, w);
 #pragma unroll
                     for (int e = 0; e < V; e++) {
                         const int j = k * V + e;
-                        float v = d[j] * a.scale;
                         const float bh = F & POST ? b[e] * rb : b[e];
-                        if constexpr (F & GATE) {
-                            sum_g[j] = fmaf(v, F & POST ? bh * w2[e] : bh, sum_g[j]);
-                            v *= g[e];
-                        }
-                        if constexpr (F & POST) {
-                            sum_p[j] = fmaf(v, bh, sum_p[j]);
-                            v *= w2[e];
-                            dot_b = fmaf(v, bh, dot_b);
-                        }
-                        d[j] = out[e] = v;
+                        if constexpr (F & (POST | GATE)) sum_b[j] = fmaf(d[j], bh, sum_b[j]);
+                        d[j] = out[e] = d[j] * w[e];
+                        if constexpr (F & POST) dot_b = fmaf(d[j], bh, dot_b);
                     }
                     if constexpr (!(F & POST)) store(true, row, k, out);
                 }
@@ -389,40 +396,41 @@ __global__ void __launch_bounds__(E == 8 ? 256 : E == 16 ? 512 : 1024, E == 8 ? 
             }
             if constexpr (kStages > 0) stage = stage == kStages - 1 ? 0 : stage + 1;
         }
-        if constexpr (F & GATE) {
-            if (a.gate_sums) {
+        if constexpr (F & (POST | GATE)) {
+            if (a.branch_sums) {
 #pragma unroll
                 for (int k = 0; k < K; k++)
                     if (EXACT || t + k * step < runs)
 #pragma unroll
                         for (int e = 0; e < V; e++) {
-                            a.gate_sums[(size_t)unit * a.width + (t + k * step) * V + e] = sum_g[k * V + e];
-                            sum_g[k * V + e] = 0;
+                            a.branch_sums[(size_t)unit * a.width + (t + k * step) * V + e] = sum_b[k * V + e];
+                            sum_b[k * V + e] = 0;
                         }
             }
         }
     }
+    if (!a.weight_sums) return;
 #pragma unroll
     for (int k = 0; k < K; k++)
         if (EXACT || t + k * step < runs)
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const size_t j = (size_t)blockIdx.x * a.width + (size_t)(t + k * step) * V + e;
-                if (a.weight_sums) a.weight_sums[j] = sum_w[k * V + e];
-                if constexpr (F & POST)
-                    if (a.post_sums) a.post_sums[j] = sum_p[k * V + e];
-            }
+            for (int e = 0; e < V; e++) a.weight_sums[(size_t)blockIdx.x * a.width + (t + k * step) * V + e] = sum_w[k * V + e];
 }
 
 struct NormColumnArgs {
-    const float *weight_sums, *post_sums, *gate_sums;
+    const float *weight_sums, *branch_sums;
+    const void *post, *gate;
     void *dweight, *dpost, *dgate;
-    unsigned ctas, chunks, width, blocks;       // blocks: CTAs across the columns
+    unsigned ctas, chunks, units, width, blocks;       // blocks: CTAs across the columns
     int f32;
+    float scale;
 };
 
 constexpr int kColumnSlices = 32;
 
+template <typename T> __device__ __forceinline__ float ld_one(const void* p, bool f32, size_t i) {
+    return f32 ? reinterpret_cast<const float*>(p)[i] : Traits<T>::up(reinterpret_cast<const T*>(p)[i]);
+}
 template <typename T> __device__ __forceinline__ void st_vector(void* p, bool f32, size_t i, float v) {
     if (f32) reinterpret_cast<float*>(p)[i] = v;
     else reinterpret_cast<T*>(p)[i] = Traits<T>::down(v);
@@ -434,22 +442,32 @@ template <typename T> __global__ void __launch_bounds__(32 * kColumnSlices) k_no
     __shared__ float parts[kColumnSlices][33];
     const unsigned what = blockIdx.x / a.blocks, lane = threadIdx.x % 32, slice = threadIdx.x / 32;
     const size_t column = (size_t)(blockIdx.x % a.blocks) * 32 + lane;
-    const unsigned gate = what - (a.weight_sums != nullptr) - (a.post_sums != nullptr);
-    const bool is_weight = a.weight_sums && what == 0, is_post = !is_weight && a.post_sums && what == (a.weight_sums != nullptr);
-    const float* from = is_weight ? a.weight_sums : is_post ? a.post_sums : a.gate_sums + (size_t)gate * a.chunks * a.width;
-    const unsigned n = is_weight || is_post ? a.ctas : a.chunks;
+    const bool is_weight = a.dweight && what == 0, is_post = !is_weight && a.dpost && what == (a.dweight != nullptr);
+    const unsigned gate = what - (a.dweight != nullptr) - (a.dpost != nullptr);
+    const float* from = is_weight ? a.weight_sums : is_post ? a.branch_sums : a.branch_sums + (size_t)gate * a.chunks * a.width;
+    const unsigned n = is_weight ? a.ctas : is_post ? a.units : a.chunks;
     float sum = 0;
-    if (column < a.width)
+    if (column < a.width) {
+        if (is_post && a.gate) {
 #pragma unroll 8
-        for (unsigned i = slice; i < n; i += kColumnSlices) sum += from[(size_t)i * a.width + column];
+            for (unsigned i = slice; i < n; i += kColumnSlices)
+                sum = fmaf(from[(size_t)i * a.width + column], ld_one<T>(a.gate, a.f32 & DCCL_NORM_GATE_F32, (size_t)(i / a.chunks) * a.width + column), sum);
+        } else {
+#pragma unroll 8
+            for (unsigned i = slice; i < n; i += kColumnSlices) sum += from[(size_t)i * a.width + column];
+        }
+    }
     parts[slice][lane] = sum;
     __syncthreads();
     if (slice || column >= a.width) return;
 #pragma unroll
     for (int s = 1; s < kColumnSlices; s++) sum += parts[s][lane];
     if (is_weight) st_vector<T>(a.dweight, a.f32 & DCCL_NORM_WEIGHT_F32, column, sum);
-    else if (is_post) st_vector<T>(a.dpost, a.f32 & DCCL_NORM_POST_F32, column, sum);
-    else st_vector<T>(a.dgate, a.f32 & DCCL_NORM_GATE_F32, (size_t)gate * a.width + column, sum);
+    else if (is_post) st_vector<T>(a.dpost, a.f32 & DCCL_NORM_POST_F32, column, a.scale * sum);
+    else {
+        if (a.post) sum *= ld_one<T>(a.post, a.f32 & DCCL_NORM_POST_F32, column);
+        st_vector<T>(a.dgate, a.f32 & DCCL_NORM_GATE_F32, (size_t)gate * a.width + column, a.scale * sum);
+    }
 }
 
 constexpr size_t kNormMaxWidth = 32768;
@@ -565,7 +583,7 @@ extern "C" int dccl_residual_norm(int device, int dtype, size_t rows, size_t wid
 extern "C" size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t width, size_t gates, int has_post, int full) {
     if (!rows || !width || (gates && rows % gates)) return 0;
     const NormCut cut = norm_cut(device, dtype, rows, width, gates, full != 0);
-    return ((size_t)cut.ctas * (has_post ? 2 : 1) + (gates ? cut.units : 0)) * width * sizeof(float);
+    return (cut.ctas + (has_post || gates ? cut.units : 0)) * width * sizeof(float);
 }
 
 extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* x, const void* branch,
@@ -583,10 +601,9 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     if (!cut.units || blocks * vectors > 0x7fffffffu || workspace_bytes < dccl_residual_norm_workspace(device, dtype, rows, width, gates, post != nullptr, full))
         return report(who, cudaErrorInvalidValue);
     float* const weight_sums = (float*)workspace;
-    float* const post_sums = post ? weight_sums + (size_t)cut.ctas * width : nullptr;
-    float* const gate_sums = gate ? weight_sums + (size_t)cut.ctas * width * (post ? 2 : 1) : nullptr;
+    float* const branch_sums = (post && dpost) || (gate && dgate) ? weight_sums + (size_t)cut.ctas * width : nullptr;
     const NormGradArgs a = {dy, dn, x, branch, weight, post, gate, (const float*)rstd, (const float*)rstd_post, dx, dbranch,
-                            dn && dweight ? weight_sums : nullptr, post && dpost ? post_sums : nullptr, gate && dgate ? gate_sums : nullptr,
+                            dn && dweight ? weight_sums : nullptr, branch_sums,
                             rows, gate ? rows_per_gate : rows, Divisor((unsigned)cut.chunks), (unsigned)((gate ? rows_per_gate : rows) / cut.chunks),
                             (unsigned)((gate ? rows_per_gate : rows) % cut.chunks), (unsigned)cut.units, (unsigned)width, f32_vectors, (float)scale};
     const auto all = {dy, dn, x, branch, weight, post, gate, (const void*)dx, (const void*)dbranch};
@@ -597,7 +614,8 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, norm_form_of(branch, post, gate, scale), cut.ctas,
                                   (unsigned)s.threads, stream, a);
     if (e == cudaSuccess && vectors) {
-        const NormColumnArgs c = {a.weight_sums, a.post_sums, a.gate_sums, dweight, dpost, dgate, cut.ctas, (unsigned)cut.chunks, (unsigned)width, (unsigned)blocks, f32_vectors};
+        const NormColumnArgs c = {weight_sums, branch_sums, post, gate, dn ? dweight : nullptr, post ? dpost : nullptr, gate ? dgate : nullptr, cut.ctas, (unsigned)cut.chunks,
+                                  (unsigned)cut.units, (unsigned)width, (unsigned)blocks, f32_vectors, (float)scale};
         const unsigned grid = (unsigned)(blocks * vectors);
         e = dtype == 6 ? launch_early(k_norm_columns<__half>, grid, 32 * kColumnSlices, stream, c) : dtype == 7 ? launch_early(k_norm_columns<float>, grid, 32 * kColumnSlices, stream, c)
                                                                                                                : launch_early(k_norm_columns<__nv_bfloat16>, grid, 32 * kColumnSlices, stream, c);
