@@ -16,9 +16,8 @@
  * y of fp32 and not from the rounded one that is stored. The backward pass makes y again from x and b: from the stored y, which
  * would save a plain sum one of five arrays, its rounding goes into every term of dw and makes that half again as inexact.
  *
- * A plain sum of 16384 x 2048 bf16: forward 41 us (6.5 TB/s of four arrays), backward 57 (5.9 TB/s of five) and 4 for the columns' sums. 8192 x 8192
- * bf16 with every part: 108 us (5.0 TB/s), 203 (4.0 TB/s of six) and 10. The wide rows take sixteen warps with 128 registers each, which is
- * all of an SM, and wait for one another twice a row.
+ * A plain sum of 16384 x 2048 bf16: forward 41 us (6.5 TB/s of four arrays), backward 59 (5.7 TB/s of five) and 4 for the columns' sums. 8192 x 8192
+ * bf16 with every part: 106 us (5.1 TB/s), 148 (5.4 TB/s of six) and 6; there sixteen warps with 112 registers each are all of an SM.
  */
 #include "decoder_ops.hpp"
 #include "../kernels/launch_early.cuh"
@@ -421,12 +420,11 @@ struct NormColumnArgs {
     const float *weight_sums, *branch_sums;
     const void *post, *gate;
     void *dweight, *dpost, *dgate;
-    unsigned ctas, chunks, units, width, blocks;       // blocks: CTAs across the columns
+    Divisor chunks, blocks;         // blocks: CTAs across the columns
+    unsigned ctas, units, width;
     int f32;
     float scale;
 };
-
-constexpr int kColumnSlices = 32;
 
 template <typename T> __device__ __forceinline__ float ld_one(const void* p, bool f32, size_t i) {
     return f32 ? reinterpret_cast<const float*>(p)[i] : Traits<T>::up(reinterpret_cast<const T*>(p)[i]);
@@ -436,32 +434,32 @@ template <typename T> __device__ __forceinline__ void st_vector(void* p, bool f3
     else reinterpret_cast<T*>(p)[i] = Traits<T>::down(v);
 }
 
-/** Adds up what the CTAs left: 32 columns per CTA, 32 threads per column. The first blocks take the weight, then post, then each row of the gate. */
-template <typename T> __global__ void __launch_bounds__(32 * kColumnSlices) k_norm_columns(const __grid_constant__ NormColumnArgs a) {
+/** Adds up what the CTAs left: 32 columns per CTA, SLICES threads per column. The first blocks take the weight, then post, then each row of the gate. */
+template <typename T, int SLICES> __global__ void __launch_bounds__(32 * SLICES) k_norm_columns(const __grid_constant__ NormColumnArgs a) {
     wait_for_stream();
-    __shared__ float parts[kColumnSlices][33];
-    const unsigned what = blockIdx.x / a.blocks, lane = threadIdx.x % 32, slice = threadIdx.x / 32;
-    const size_t column = (size_t)(blockIdx.x % a.blocks) * 32 + lane;
+    __shared__ float parts[SLICES][33];
+    const unsigned what = a.blocks.quotient(blockIdx.x), lane = threadIdx.x % 32, slice = threadIdx.x / 32;
+    const size_t column = (size_t)(blockIdx.x - what * a.blocks.d) * 32 + lane;
     const bool is_weight = a.dweight && what == 0, is_post = !is_weight && a.dpost && what == (a.dweight != nullptr);
     const unsigned gate = what - (a.dweight != nullptr) - (a.dpost != nullptr);
-    const float* from = is_weight ? a.weight_sums : is_post ? a.branch_sums : a.branch_sums + (size_t)gate * a.chunks * a.width;
-    const unsigned n = is_weight ? a.ctas : is_post ? a.units : a.chunks;
+    const float* from = is_weight ? a.weight_sums : is_post ? a.branch_sums : a.branch_sums + (size_t)gate * a.chunks.d * a.width;
+    const unsigned n = is_weight ? a.ctas : is_post ? a.units : a.chunks.d;
     float sum = 0;
     if (column < a.width) {
         if (is_post && a.gate) {
 #pragma unroll 8
-            for (unsigned i = slice; i < n; i += kColumnSlices)
-                sum = fmaf(from[(size_t)i * a.width + column], ld_one<T>(a.gate, a.f32 & DCCL_NORM_GATE_F32, (size_t)(i / a.chunks) * a.width + column), sum);
+            for (unsigned i = slice; i < n; i += SLICES)
+                sum = fmaf(from[(size_t)i * a.width + column], ld_one<T>(a.gate, a.f32 & DCCL_NORM_GATE_F32, (size_t)a.chunks.quotient(i) * a.width + column), sum);
         } else {
 #pragma unroll 8
-            for (unsigned i = slice; i < n; i += kColumnSlices) sum += from[(size_t)i * a.width + column];
+            for (unsigned i = slice; i < n; i += SLICES) sum += from[(size_t)i * a.width + column];
         }
     }
     parts[slice][lane] = sum;
     __syncthreads();
     if (slice || column >= a.width) return;
 #pragma unroll
-    for (int s = 1; s < kColumnSlices; s++) sum += parts[s][lane];
+    for (int s = 1; s < SLICES; s++) sum += parts[s][lane];
     if (is_weight) st_vector<T>(a.dweight, a.f32 & DCCL_NORM_WEIGHT_F32, column, sum);
     else if (is_post) st_vector<T>(a.dpost, a.f32 & DCCL_NORM_POST_F32, column, a.scale * sum);
     else {
@@ -479,10 +477,11 @@ static NormShape norm_shape(size_t width) {
     return {e, (int)((width + e * 32 - 1) / (e * 32)) * 32};
 }
 
-/** Elements per access: 16 bytes, else one. */
-static int norm_run(int dtype, size_t width, bool aligned) {
+/** Elements per access: 16 bytes, else a pair of 16-bit elements, else one. */
+static int norm_run(int dtype, size_t width, std::initializer_list<const void*> all) {
     const int wide = dtype == 7 ? 4 : 8;
-    return width % wide == 0 && aligned ? wide : 1;
+    if (width % wide == 0 && aligned_to(16, all)) return wide;
+    return dtype != 7 && width % 2 == 0 && aligned_to(8, all) ? 2 : 1;
 }
 
 /** CTAs of the backward pass, all resident at once, and how the rows of a gate are cut among them. */
@@ -538,6 +537,11 @@ template <typename T, int V, int E, typename Args> static cudaError_t norm_form(
         default: return norm_launch<T, V, E, 0>(grid, block, stream, a, device);
     }
 }
+/** Few terms in many columns take small CTAs (148 terms of 3 x 8192 columns: 10.9 -> 6.4 us), many terms large ones. */
+template <typename T> static cudaError_t norm_columns(unsigned grid, cudaStream_t stream, const NormColumnArgs& c) {
+    return (c.ctas > c.units ? c.ctas : c.units) <= 256 ? launch_early(k_norm_columns<T, 8>, grid, 32 * 8, stream, c) : launch_early(k_norm_columns<T, 32>, grid, 32 * 32, stream, c);
+}
+
 /** BRANCH, POST, GATE and SCALE of a call; post takes the scale in. */
 static int norm_form_of(const void* branch, const void* post, const void* gate, double scale) {
     if (!branch) return 0;
@@ -552,8 +556,10 @@ template <typename T, int V, typename Args> static cudaError_t norm_elements(int
 template <typename Args> static cudaError_t norm_dispatch(int device, int dtype, int run, int elements, int form, unsigned grid, unsigned block, cudaStream_t stream, const Args& a) {
     switch (dtype * 16 + run) {
         case 6 * 16 + 8: return norm_elements<__half, 8>(elements, form, grid, block, stream, a, device);
+        case 6 * 16 + 2: return norm_elements<__half, 2>(elements, form, grid, block, stream, a, device);
         case 6 * 16 + 1: return norm_elements<__half, 1>(elements, form, grid, block, stream, a, device);
         case 9 * 16 + 8: return norm_elements<__nv_bfloat16, 8>(elements, form, grid, block, stream, a, device);
+        case 9 * 16 + 2: return norm_elements<__nv_bfloat16, 2>(elements, form, grid, block, stream, a, device);
         case 9 * 16 + 1: return norm_elements<__nv_bfloat16, 1>(elements, form, grid, block, stream, a, device);
         case 7 * 16 + 4: return norm_elements<float, 4>(elements, form, grid, block, stream, a, device);
         case 7 * 16 + 1: return norm_elements<float, 1>(elements, form, grid, block, stream, a, device);
@@ -576,7 +582,7 @@ extern "C" int dccl_residual_norm(int device, int dtype, size_t rows, size_t wid
     const NormShape s = norm_shape(width);
     OnDevice on(device);
     if (on.e != cudaSuccess) return report("dccl_residual_norm", on.e);
-    return report("dccl_residual_norm", norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, norm_form_of(branch, post, gate, scale),
+    return report("dccl_residual_norm", norm_dispatch(device, dtype, norm_run(dtype, width, all), s.elements, norm_form_of(branch, post, gate, scale),
                                                       (unsigned)rows, (unsigned)s.threads, (cudaStream_t)stream, a));
 }
 
@@ -611,14 +617,13 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     cudaStream_t stream = (cudaStream_t)stream_v;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
-    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, aligned_to(16, all)), s.elements, norm_form_of(branch, post, gate, scale), cut.ctas,
+    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, all), s.elements, norm_form_of(branch, post, gate, scale), cut.ctas,
                                   (unsigned)s.threads, stream, a);
     if (e == cudaSuccess && vectors) {
-        const NormColumnArgs c = {weight_sums, branch_sums, post, gate, dn ? dweight : nullptr, post ? dpost : nullptr, gate ? dgate : nullptr, cut.ctas, (unsigned)cut.chunks,
-                                  (unsigned)cut.units, (unsigned)width, (unsigned)blocks, f32_vectors, (float)scale};
+        const NormColumnArgs c = {weight_sums, branch_sums, post, gate, dn ? dweight : nullptr, post ? dpost : nullptr, gate ? dgate : nullptr, Divisor((unsigned)cut.chunks),
+                                  Divisor((unsigned)blocks), cut.ctas, (unsigned)cut.units, (unsigned)width, f32_vectors, (float)scale};
         const unsigned grid = (unsigned)(blocks * vectors);
-        e = dtype == 6 ? launch_early(k_norm_columns<__half>, grid, 32 * kColumnSlices, stream, c) : dtype == 7 ? launch_early(k_norm_columns<float>, grid, 32 * kColumnSlices, stream, c)
-                                                                                                               : launch_early(k_norm_columns<__nv_bfloat16>, grid, 32 * kColumnSlices, stream, c);
+        e = dtype == 6 ? norm_columns<__half>(grid, stream, c) : dtype == 7 ? norm_columns<float>(grid, stream, c) : norm_columns<__nv_bfloat16>(grid, stream, c);
     }
     return report(who, e);
 }
