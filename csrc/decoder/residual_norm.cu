@@ -477,7 +477,8 @@ static NormShape norm_shape(size_t width) {
     return {e, (int)((width + e * 32 - 1) / (e * 32)) * 32};
 }
 
-/** Elements per access: 16 bytes, else a pair of 16-bit elements, else one. */
+/** Elements per access: 16 bytes, else a pair of 16-bit elements, else one (both directions with every part, 16384 x 1450 fp16: pairs 164 us,
+ *  single elements 254; 4096 x 6002 bf16, a plain sum: 118 and 180). */
 static int norm_run(int dtype, size_t width, std::initializer_list<const void*> all) {
     const int wide = dtype == 7 ? 4 : 8;
     if (width % wide == 0 && aligned_to(16, all)) return wide;
