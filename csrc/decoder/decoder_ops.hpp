@@ -26,8 +26,8 @@ size_t dccl_residual_norm_workspace(int device, int dtype, size_t rows, size_t w
 
 /**
  * Gradients of dccl_residual_norm: from dy and dn (either may be null) those of x and branch, and in the vectors' own types those of
- * weight, post and gate. dbranch may be null where it equals dx (scale 1, no post, no gate). No atomics: the same inputs give the
- * same gradients.
+ * weight, post and gate. dbranch may be null where it equals dx (scale 1, no post, no gate), and is written wherever it is not. No atomics:
+ * the same inputs give the same gradients.
  */
 int dccl_residual_norm_backward(int device, int dtype, size_t rows, size_t width, const void* dy, const void* dn, const void* x, const void* branch,
                                 const void* weight, const void* post, const void* gate, size_t rows_per_gate, int f32_vectors, double scale,

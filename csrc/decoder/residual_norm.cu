@@ -576,7 +576,7 @@ extern "C" int dccl_residual_norm(int device, int dtype, size_t rows, size_t wid
                                   const void* gate, size_t rows_per_gate, int f32_vectors, double eps, double scale, void* y, void* n, void* rstd,
                                   void* rstd_post, void* stream) {
     if (!rows) return 0;
-    if (!width || width > kNormMaxWidth || rows > 0x7fffffffu || (gate && !rows_per_gate) || (post && !branch) || (gate && !branch))
+    if (!width || width > kNormMaxWidth || rows > 0x7fffffffu || !x || !weight || !n || (branch && !y) || (gate && !rows_per_gate) || (post && !branch) || (gate && !branch))
         return report("dccl_residual_norm", cudaErrorInvalidValue);
     const NormArgs a = {x, branch, weight, post, gate, y, n, (float*)rstd, (float*)rstd_post, rows_per_gate, (unsigned)width, f32_vectors, (float)eps, (float)scale};
     const auto all = {x, branch, weight, post, gate, (const void*)y, (const void*)n};
@@ -600,7 +600,7 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     const char* who = "dccl_residual_norm_backward";
     const size_t gates = gate && rows_per_gate ? rows / rows_per_gate : 0;
     if (!rows || rows > 0x7fffffffu || !width || width > kNormMaxWidth || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
-        || (dbranch && !branch) || (!dbranch && branch && (post || gate || scale != 1.0)))
+        || !x || !weight || !dx || !workspace || (dbranch && !branch) || (!dbranch && branch && (post || gate || scale != 1.0)))
         return report(who, cudaErrorInvalidValue);
     const bool full = branch != nullptr;
     const NormCut cut = norm_cut(device, dtype, rows, width, gates, full);
@@ -618,8 +618,8 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
     cudaStream_t stream = (cudaStream_t)stream_v;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
-    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, all), s.elements, norm_form_of(branch, post, gate, scale), cut.ctas,
-                                  (unsigned)s.threads, stream, a);
+    const int form = norm_form_of(branch, post, gate, scale) | (dbranch && !post ? SCALE : 0);       // a plain sum has no array of its own for the branch
+    cudaError_t e = norm_dispatch(device, dtype, norm_run(dtype, width, all), s.elements, form, cut.ctas, (unsigned)s.threads, stream, a);
     if (e == cudaSuccess && vectors) {
         const NormColumnArgs c = {weight_sums, branch_sums, post, gate, dn ? dweight : nullptr, post ? dpost : nullptr, gate ? dgate : nullptr, Divisor((unsigned)cut.chunks),
                                   Divisor((unsigned)blocks), cut.ctas, (unsigned)cut.units, (unsigned)width, f32_vectors, (float)scale};

@@ -272,6 +272,46 @@ def test_gradients_have_the_same_bits_twice():
     assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+@gpu
+@pytest.mark.parametrize("width", [64, 250, 257, 4096, 16384])
+def test_norm_entry_point_writes_each_gradient_that_it_gets_room_for(width):
+    """Of a plain sum the branch's gradient is x's: the entry point writes it all the same where a caller has a buffer for it."""
+    from dccl_b200._lib import lib
+    L, rows = lib(), 5
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x, branch, dy, dn = (torch.randn(rows, width, device="cuda", generator=g) for _ in range(4))
+    weight, rstd = torch.randn(width, device="cuda", generator=g), torch.empty(rows, device="cuda")
+    y, n = torch.empty_like(x), torch.empty_like(x)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert L.dccl_residual_norm(0, 7, rows, width, x.data_ptr(), branch.data_ptr(), weight.data_ptr(), None, None, 0, 0, EPS, 1.0, y.data_ptr(), n.data_ptr(), rstd.data_ptr(),
+                                None, stream) == 0
+    size = L.dccl_residual_norm_workspace(0, 7, rows, width, 0, 0, 1)
+    work = torch.empty(size, dtype=torch.uint8, device="cuda")
+    grads = []
+    for room in (True, False):
+        dx, dbranch, dweight = torch.full_like(x, math.nan), torch.full_like(x, math.nan), torch.full_like(weight, math.nan)
+        assert L.dccl_residual_norm_backward(0, 7, rows, width, dy.data_ptr(), dn.data_ptr(), x.data_ptr(), branch.data_ptr(), weight.data_ptr(), None, None, 0, 0, 1.0,
+                                             rstd.data_ptr(), None, dx.data_ptr(), dbranch.data_ptr() if room else None, dweight.data_ptr(), None, None, work.data_ptr(), size,
+                                             stream) == 0
+        grads.append((dx, dweight))
+        if room:
+            assert torch.equal(dbranch, dx)
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("missing", ["x", "weight", "y", "n"])
+def test_norm_entry_points_refuse_missing_buffers(missing, dccl_lib, capfd):
+    from dccl_b200._lib import lib
+    L = lib()
+    if not hasattr(L, "dccl_residual_norm"):
+        pytest.skip("built without CUDA")
+    at = {k: None if k == missing else 4096 for k in ("x", "weight", "y", "n")}      # never read: no call gets as far as a device
+    assert L.dccl_residual_norm(0, 7, 1, 8, at["x"], 4096, at["weight"], None, None, 0, 0, EPS, 1.0, at["y"], at["n"], None, None, None) == -1
+    assert L.dccl_residual_norm_backward(0, 7, 1, 8, 4096, 4096, at["x"], 4096, at["weight"], None, None, 0, 0, 1.0, 4096, None, at["y"], None, None, None, None,
+                                         at["n"], 1 << 30, None) == -1
+    assert capfd.readouterr().err.count("invalid argument") == 2
+
+
 def norm_refusals(device):
     x, w = torch.zeros(2, 3, 8, device=device), torch.ones(8, device=device)
     with pytest.raises(TypeError):
