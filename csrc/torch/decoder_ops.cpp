@@ -4,7 +4,9 @@
  * three microseconds; from Python a call took 16 to 20, forward and backward together 130.
  *
  * A function that finds anything but plain CUDA tensors of the right types and shapes returns NotImplemented: dccl_b200/ops/decoder.py then
- * says what is wrong. Plain CPython functions: their arguments are borrowed. Everything that could throw is caught at this border.
+ * says what is wrong. Where something follows torch's operations (a mode, a tracer, a subclass of Tensor) it returns None, and the same call
+ * comes back through an operator that torch knows. Plain CPython functions: their arguments are borrowed. Everything that could throw is
+ * caught at this border.
  */
 #include "decoder_ops.hpp"
 #include "../decoder/decoder_ops.hpp"
@@ -15,7 +17,11 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/PyInterpreterHooks.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -58,6 +64,42 @@ bool tensor_of(PyObject* o, bool optional, Tensor* t) {
     if (!THPVariable_Check(o)) return false;
     *t = THPVariable_Unpack(o);
     return is_plain(*t);
+}
+
+/** Python objects that calls are compared with, for the life of the process. An import may let other threads run, which a static's own guard would
+ *  keep from it: two of them find the same object instead. */
+struct Known {
+    const char *module, *name;
+    PyObject* object = nullptr;
+    PyObject* get() {
+        if (object) return object;
+        THPObjectPtr m(PyImport_ImportModule(module));
+        PyObject* o = m ? PyObject_GetAttrString(m.get(), name) : nullptr;
+        if (!o) throw python_error();
+        return object = o;
+    }
+} parameter{"torch.nn", "Parameter"}, disabled{"torch._C", "_disabled_torch_function_impl"}, device_context{"torch.utils._device", "DeviceContext"};
+
+/** Whether this is a tensor whose class takes torch's functions over. (Only what is left after the first lines costs anything.) */
+bool takes_functions_over(PyObject* o) {
+    PyObject* type = reinterpret_cast<PyObject*>(Py_TYPE(o));
+    if (type == THPVariableClass || o == Py_None || PyFloat_Check(o) || PyLong_Check(o) || type == parameter.get() || !THPVariable_Check(o)) return false;
+    THPObjectPtr f(PyObject_GetAttrString(type, "__torch_function__"));
+    if (!f) throw python_error();
+    return f.get() != disabled.get();
+}
+
+/** Whether something would see torch's operations of this call: a mode, a tracer, or a subclass of Tensor among the arguments. */
+bool observed(PyObject* const* args, Py_ssize_t nargs) {
+    using Functions = at::impl::PythonTorchFunctionTLS;
+    if (c10::impl::dispatch_mode_enabled() || at::tracer::impl::is_dispatch_enabled()) return true;
+    if (at::impl::torch_function_mode_enabled())        // the one behind torch.device and the default device only places new tensors
+        for (int64_t i = 0; i < Functions::stack_len(); i++)
+            if (reinterpret_cast<PyObject*>(Py_TYPE(Functions::get_stack_at(i)->ptr(c10::impl::getGlobalPyInterpreter()))) != device_context.get()) return true;
+    if (Functions::get_disabled_state() == at::impl::TorchFunctionDisabledState::ENABLED)
+        for (Py_ssize_t i = 0; i < nargs; i++)
+            if (takes_functions_over(args[i])) return true;
+    return false;
 }
 
 Tensor dense(const Tensor& t) {
@@ -196,6 +238,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if ((v->scalar_type() != x.scalar_type() && v->scalar_type() != at::kFloat) || v->device() != x.device()) Py_RETURN_NOTIMPLEMENTED;
         if (v != &gate && (v->dim() != 1 || v->size(0) != width)) Py_RETURN_NOTIMPLEMENTED;
     }
+    if (observed(args, nargs)) Py_RETURN_NONE;
     check_forward_mode("residual_norm", {&x, &branch, &weight, &post, &gate});
     Tensor y, n;
     {
@@ -329,6 +372,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const bool one = p.dim() == 1 && p.size(0) == seq, each = q.dim() == 4 && p.dim() == 2 && p.size(0) == batch && p.size(1) == seq;
         if ((!one && !each) || (p.scalar_type() != at::kLong && p.scalar_type() != at::kInt) || p.device() != q.device()) Py_RETURN_NOTIMPLEMENTED;
     }
+    if (observed(args, nargs)) Py_RETURN_NONE;
     check_forward_mode("rotary", {&q, &k});
     std::pair<Tensor, Tensor> out;
     {
@@ -411,6 +455,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         Py_RETURN_NOTIMPLEMENTED;
     const int64_t tokens = x.numel() / width;
     if (std::max({tokens, width, ffn}) >= kMaxDimension) Py_RETURN_NOTIMPLEMENTED;
+    if (observed(args, nargs)) Py_RETURN_NONE;
     check_forward_mode("gated_linear", {&x, &wg, &wu});
     Tensor h;
     {
@@ -468,9 +513,9 @@ PyObject* decoder_ops_bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyMethodDef methods[] = {
-    {"residual_norm", (PyCFunction)(void (*)())residual_norm, METH_FASTCALL, "(y, n), or n without a branch; NotImplemented where the arguments do not fit"},
-    {"rotary", (PyCFunction)(void (*)())rotary, METH_FASTCALL, "turned q and k; NotImplemented where the arguments do not fit"},
-    {"gated_linear", (PyCFunction)(void (*)())gated_linear, METH_FASTCALL, "act(x Wg^T) * (x Wu^T); NotImplemented where the arguments do not fit"},
+    {"residual_norm", (PyCFunction)(void (*)())residual_norm, METH_FASTCALL, "(y, n), or n without a branch; NotImplemented where the arguments do not fit, None where the call is observed"},
+    {"rotary", (PyCFunction)(void (*)())rotary, METH_FASTCALL, "turned q and k; NotImplemented and None likewise"},
+    {"gated_linear", (PyCFunction)(void (*)())gated_linear, METH_FASTCALL, "act(x Wg^T) * (x Wu^T); NotImplemented and None likewise"},
     {"decoder_ops_bind", (PyCFunction)(void (*)())decoder_ops_bind, METH_FASTCALL, "hands over the addresses of the library's entry points"},
     {nullptr, nullptr, 0, nullptr},
 };

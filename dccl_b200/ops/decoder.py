@@ -17,6 +17,9 @@ the same formulas in torch, so the same model code is tested without a GPU. Inpu
 read in place is copied first. A call allocates its outputs and its workspace from torch's allocator and nothing else, so it can be
 captured into a graph; a gradient has the same bits whenever its inputs do (no atomics).
 
+Under a mode of torch's (other than the one behind ``torch.device``), a tracer, or with a subclass of Tensor, the same kernels run as operators
+of torch's dispatcher (``torch.ops.dccl``), which those see and record. Fake and transformed tensors are refused.
+
 The original has no such operators: its API ends at the collectives (reference include/dccl/dccl.hpp:143-420).
 """
 import ctypes
@@ -47,6 +50,75 @@ def _ext():
         ext.decoder_ops_bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in _ENTRIES))
         _native = ext
     return _native
+
+
+# ---------------------------------------------------------------------------------------------- calls that something observes
+
+_SCHEMAS = {"residual_norm": "Tensor x, Tensor? branch, Tensor weight, float eps, Tensor? post_weight, Tensor? gate, float scale",
+            "rotary": "Tensor q, Tensor? k, Tensor freqs, Tensor? positions, int first, bool interleaved, float scale",
+            "gated_linear": "Tensor x, Tensor w_gate, Tensor w_up, int activation"}
+_registered = {}
+
+
+def _run(name, args):
+    """The kernels from inside of a registered operator, where nothing observes them any more."""
+    if name == "rotary":
+        q, k, freqs, positions, first, interleaved, scale = args
+        args = q, k, freqs, first if positions is None else positions, interleaved, scale
+    out = getattr(_ext(), name)(*args)
+    if out is None or out is NotImplemented:
+        raise RuntimeError("%s: a registered operator got tensors that are not plain" % name)
+    return list(out) if isinstance(out, tuple) else [out]
+
+
+def _register(name):
+    """`name` as an operator of torch's dispatcher, dccl::name, and its gradient as another, so that modes see them and tracers record them. The
+    gradient runs the forward pass again: what that keeps is not among the results that a tracer could hand over."""
+    def forward(*args):
+        with torch._C.DisableTorchFunction(), torch.no_grad():
+            return _run(name, args)
+
+    def backward(grads, *rest):
+        *args, needed = rest
+        with torch._C.DisableTorchFunction(), torch.enable_grad():
+            args = [a.detach().contiguous().requires_grad_(n) if isinstance(a, torch.Tensor) else a for a, n in zip(args, needed)]
+            outs = [(o, g) for o, g in zip(_run(name, args), grads) if g is not None]
+            leaves = [a for a, n in zip(args, needed) if n]
+            found, seen = torch.autograd.grad([o for o, _ in outs], leaves, [g for _, g in outs], allow_unused=True), []
+            for leaf, g in zip(leaves, found):      # results of an operator are tensors of their own
+                seen.append(torch.zeros_like(leaf) if g is None else g.clone() if any(g is s for s in seen) else g)
+            return seen
+
+    run = torch.library.custom_op("dccl::" + name, forward, mutates_args=(), device_types="cuda", schema="(%s) -> Tensor[]" % _SCHEMAS[name])
+    run_back = torch.library.custom_op("dccl::%s_backward" % name, backward, mutates_args=(), device_types="cuda",
+                                       schema="(Tensor?[] grads, %s, bool[] needed) -> Tensor[]" % _SCHEMAS[name])
+
+    def setup(ctx, inputs, output):
+        ctx.set_materialize_grads(False)
+        ctx.others = [None if isinstance(a, torch.Tensor) else (a,) for a in inputs]
+        ctx.save_for_backward(*(a for a in inputs if isinstance(a, torch.Tensor)))
+
+    def gradients(ctx, grads):
+        needed = list(ctx.needs_input_grad)
+        if all(g is None for g in grads) or not any(needed):
+            return (None,) * len(needed)
+        tensors = iter(ctx.saved_tensors)
+        found = iter(run_back(list(grads), *(next(tensors) if o is None else o[0] for o in ctx.others), needed))
+        return tuple(next(found) if n else None for n in needed)
+
+    run.register_autograd(gradients, setup_context=setup)
+    return run
+
+
+def _observed(name, *args):
+    """The call through torch's dispatcher, which tells whoever follows it."""
+    if name == "rotary":
+        q, k, freqs, positions, interleaved, scale = args
+        args = (q, k, freqs) + ((positions, 0) if isinstance(positions, torch.Tensor) else (None, positions)) + (interleaved, float(scale))
+    if name not in _registered:
+        _registered[name] = _register(name)
+    out = _registered[name](*args)
+    return out[0] if len(out) == 1 else tuple(out)
 
 
 def _refuse(what):
@@ -110,6 +182,8 @@ def _norm_on_cpu(x, branch, weight, post, gate, eps, scale):
 def _norm(what, x, branch, weight, post, gate, eps, scale):
     if isinstance(x, torch.Tensor) and x.is_cuda:
         out = _ext().residual_norm(x, branch, weight, eps, post, gate, scale)
+        if out is None:
+            return _observed("residual_norm", x, branch, weight, float(eps), post, gate, float(scale))
         if out is not NotImplemented:
             return out
     _check_activations(what, "x", x, range(1, 65))
@@ -129,6 +203,8 @@ def _norm(what, x, branch, weight, post, gate, eps, scale):
         if x.numel() // width >= 1 << 31:
             raise ValueError("%s: %d rows; fewer than 2^31 are taken" % (what, x.numel() // width))
         out = _ext().residual_norm(x, branch, weight, eps, post, gate, scale)
+        if out is None:
+            return _observed("residual_norm", x, branch, weight, eps, post, gate, scale)
         return out if out is not NotImplemented else _refuse(what)
     y, n = _norm_on_cpu(x, branch, weight, post, gate, eps, scale)
     return n if branch is None else (y, n)
@@ -177,6 +253,8 @@ def rotary(q, k, freqs, positions=None, interleaved=False, scale=1.0):
     scale: factor of the turned elements, as stretched contexts use it."""
     if isinstance(q, torch.Tensor) and q.is_cuda:
         out = _ext().rotary(q, k, freqs, 0 if positions is None else positions, interleaved, scale)
+        if out is None:
+            return _observed("rotary", q, k, freqs, 0 if positions is None else positions, interleaved, scale)
         if out is not NotImplemented:
             return out
     _check_activations("rotary", "q", q, (3, 4))
@@ -212,6 +290,8 @@ def rotary(q, k, freqs, positions=None, interleaved=False, scale=1.0):
     if (q.shape[-2] + (0 if k is None else k.shape[-2])) * dim > 1 << 24 or seq >= 1 << 31:
         raise ValueError("rotary: a token has more than 2^24 elements, or a sequence 2^31 tokens")
     out = _ext().rotary(q, k, freqs, positions, interleaved, scale)
+    if out is None:
+        return _observed("rotary", q, k, freqs, positions, interleaved, scale)
     return out if out is not NotImplemented else _refuse("rotary")
 
 
@@ -279,6 +359,8 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     from 16 bits their rounding would come on top of the one that their gradients need to be multiplied again."""
     if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(activation, str):
         h = _ext().gated_linear(x, w_gate, w_up, _ACTIVATIONS.get(activation, -1))
+        if h is None:
+            return _observed("gated_linear", x, w_gate, w_up, _ACTIVATIONS[activation])
         if h is not NotImplemented:
             return h
     _check_activations("gated_linear", "x", x, range(1, 65))

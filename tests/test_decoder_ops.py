@@ -9,6 +9,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
+import torch.utils._python_dispatch  # noqa: E402
 
 from dccl_b200 import ops  # noqa: E402
 
@@ -958,3 +959,136 @@ def test_checkpointed_operators():
     assert kept.count((40, 72)) == 2 and (40,) in kept          # the products and the rows' statistics
     got = torch.autograd.grad(checkpoint(part, x, use_reentrant=False), (x, w, wg, wu), dh)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------------------------- what follows torch's operations
+
+class SeesDispatch(torch.utils._python_dispatch.TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+class SeesFunctions(torch.overrides.TorchFunctionMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+def chain(device="cuda"):
+    """A function through every operator, each with what it may be given, and two inputs for it."""
+    g = torch.Generator().manual_seed(9)
+    t = [torch.randn(s, generator=g).to(device).bfloat16().requires_grad_(True) for s in ((2, 6, 64), (2, 6, 64), (64,), (64,), (2, 1, 64), (96, 64), (96, 64))]
+    _, branch, w, post, gate, wg, wu = t
+    freqs, at = ops.rotary_frequencies(16, device=device), torch.randint(0, 1000, (2, 6), generator=g).to(device)
+
+    def f(x):
+        y, n = ops.residual_norm(x, branch, w, post_weight=post, gate=gate, scale=0.5)
+        q, k = ops.rotary(n.view(2, 6, 4, 16), y[..., :32].view(2, 6, 2, 16), freqs, at, interleaved=True)
+        return ops.gated_linear(ops.rms_norm(q.flatten(2), w), wg, wu), ops.rotary(k, None, freqs, 7), y
+
+    return f, t, torch.randn(2, 6, 64, generator=g).to(device).bfloat16()
+
+
+def all_of(f, t, x):
+    """The outputs of f and the gradients of everything that goes into it."""
+    x = x.detach().requires_grad_(True)
+    outs = f(x)
+    return list(outs) + list(torch.autograd.grad(outs, [x] + t[1:], [torch.ones_like(o) for o in outs]))
+
+
+@gpu
+@pytest.mark.parametrize("mode", [SeesDispatch, SeesFunctions])
+def test_an_active_mode_sees_the_operators(mode):
+    f, t, x = chain()
+    want = all_of(f, t, x)
+    with mode() as m:
+        got = all_of(f, t, x)
+    seen = " ".join(m.seen)
+    for name in ("residual_norm", "rotary", "gated_linear"):
+        assert "dccl." + name in seen and (mode is SeesFunctions or "dccl.%s_backward" % name in seen), (name, m.seen)
+    # x gets a sum of two gradients, which the kernels of one call and of two add in one order
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_a_mode_that_places_new_tensors_changes_nothing(monkeypatch):
+    from dccl_b200.ops import decoder
+    f, t, x = chain()
+    want = all_of(f, t, x)
+    monkeypatch.setattr(decoder, "_observed", None)
+    with torch.device("cuda"):
+        assert all(torch.equal(a, b) for a, b in zip(all_of(f, t, x), want))
+
+
+@gpu
+@pytest.mark.parametrize("tracer", ["trace", "make_fx"])
+def test_tracers_record_the_operators(tracer):
+    """A recorded call computes from its inputs, and not what the inputs were when it was recorded."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, t, other = chain()
+    for v in t:
+        v.requires_grad_(tracer == "make_fx")       # torch.jit.trace takes no constants that do
+    with torch.no_grad():
+        recorded = torch.jit.trace(f, (t[0],)) if tracer == "trace" else make_fx(f)(t[0])
+        assert all(torch.equal(a, b) for a, b in zip(recorded(other), f(other)))
+    if tracer == "make_fx":
+        step = make_fx(lambda x: all_of(f, t, x))(t[0])
+        assert all(torch.equal(a, b) for a, b in zip(step(other), all_of(f, t, other)))
+
+
+@gpu
+def test_subclasses_of_tensor_see_the_operators():
+    class Plain(torch.Tensor):
+        pass
+
+    class Sees(torch.Tensor):
+        seen = []
+
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            cls.seen.append(str(func))
+            return super().__torch_function__(func, types, args, kwargs or {})
+
+    f, t, x = chain()
+    want = all_of(f, t, x)
+    for cls in (Plain, Sees):
+        with torch.no_grad():
+            outs = f(x.as_subclass(cls))
+        assert all(type(o) is cls for o in outs) and all(torch.equal(a.as_subclass(torch.Tensor), b) for a, b in zip(outs, want))
+        y = x.detach().as_subclass(cls).requires_grad_(True)
+        g, = torch.autograd.grad(f(y)[0].sum(), y)
+        assert torch.equal(g.as_subclass(torch.Tensor), torch.autograd.grad(f(x.requires_grad_(True))[0].sum(), x)[0])
+    assert any("dccl.gated_linear" in s for s in Sees.seen)
+
+
+@gpu
+def test_selective_checkpointing_of_the_operators():
+    """It follows a region by a mode, and takes what that sees again from its cache or makes it again."""
+    from functools import partial
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+    f, t, x = chain()
+    want = all_of(f, t, x)
+    for keep in (True, False):
+        def policy(ctx, op, *args, **kwargs):
+            return CheckpointPolicy.MUST_SAVE if keep and "dccl" in str(op) else CheckpointPolicy.PREFER_RECOMPUTE
+        got = all_of(lambda v: checkpoint(f, v, use_reentrant=False, context_fn=partial(create_selective_checkpoint_contexts, policy)), t, x)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_compiled_functions_stay_right():
+    """The compiler leaves the operators out of its graphs and calls them between."""
+    f, t, x = chain()
+    want = all_of(f, t, x)
+    compiled = torch.compile(f, backend="eager")
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(all_of(compiled, t, x), want))
