@@ -8,13 +8,16 @@ the "no library GEMM" rule of this project applies to the communication paths, n
 
 With ``LlamaConfig(fused=True)`` the same modules compute with the operators of ``dccl_b200.ops.decoder``: each residual add in one pass with
 the norm after it, rotary positions of queries and keys in one launch, and the gated projections as one product (parameters and state
-dict stay the same; on the GPU the model is then float16 or bfloat16).
+dict stay the same; on the GPU the model is then float16 or bfloat16). A module that is more than what stands here (another one put in its place, a
+bias, hooks) is called, and the others around it stay fused.
 """
+import functools
 from dataclasses import dataclass
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from ..ops import decoder as ops
 
@@ -92,10 +95,32 @@ class Attention(nn.Module):
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.kv != self.h)
         return self.o(out.transpose(1, 2).reshape(b, s, self.h * self.hd))
 
-
     def fused(self, x, freqs):
         b, s, _ = x.shape
         return self.o(attend(self.q(x).view(b, s, self.h, self.hd), self.k(x).view(b, s, self.kv, self.hd), self.v(x).view(b, s, self.kv, self.hd), freqs))
+
+
+# ---- the fused form. Every operator stands for modules that are then not called, so each use asks first whether calling them would do more.
+
+_OWN_FORWARD = {kind: kind.forward for kind in (nn.Linear, RMSNorm, Attention)}
+
+
+def untouched(module, kind):
+    """Whether a call of `module` computes what `kind` says and nothing else: of that very class, with neither a bias nor hooks nor another forward."""
+    return (type(module) is kind and kind.forward is _OWN_FORWARD[kind] and "forward" not in module.__dict__
+            and getattr(module, "bias", None) is None and module._compiled_call_impl is None and not _has_any_global_hook()
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+class Positions:
+    """The frequencies of the rotary positions, and their tables where a module has to be called that takes those."""
+
+    def __init__(self, seq, head_dim, theta, device):
+        self.freqs, self._tables = ops.rotary_frequencies(head_dim, theta, device=device), (seq, head_dim, theta, device)
+
+    @functools.cached_property
+    def tables(self):
+        return rope_tables(*self._tables)
 
 
 def attend(q, k, v, freqs):
@@ -103,6 +128,43 @@ def attend(q, k, v, freqs):
     q, k = ops.rotary(q, k, freqs)
     out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=q.shape[2] != k.shape[2])
     return out.transpose(1, 2).flatten(2)
+
+
+def attention(module, n, at, kind):
+    return module.fused(n, at.freqs) if untouched(module, kind) else module(n, *at.tables)
+
+
+def gated(n, gate, up):
+    if untouched(gate, nn.Linear) and untouched(up, nn.Linear):
+        return ops.gated_linear(n, gate.weight, up.weight)
+    return F.silu(gate(n)) * up(n)
+
+
+def norm_of(x, norm):
+    if norm is None:
+        return None
+    return ops.rms_norm(x, norm.weight, eps=norm.eps) if untouched(norm, RMSNorm) else norm(x)
+
+
+def add_norm(x, branch, norm):
+    """x + branch, and the norm of it; None where what comes next takes no norm."""
+    if norm is not None and untouched(norm, RMSNorm):
+        return ops.residual_norm(x, branch, norm.weight, eps=norm.eps)
+    x = x + branch
+    return x, norm_of(x, norm)
+
+
+def run_fused(x, blocks, last, at, kind):
+    """The blocks and the last norm. A block that is not an untouched one of its kind is called as a module."""
+    entries = [blk.n1 if untouched(blk, kind) else None for blk in blocks] + [last]
+    n = norm_of(x, entries[0])
+    for blk, entry, after in zip(blocks, entries, entries[1:]):
+        if entry is None:
+            x = blk(x, *at.tables)
+            n = norm_of(x, after)
+        else:
+            x, n = blk.fused(x, n, at, after)
+    return n
 
 
 class Block(nn.Module):
@@ -119,18 +181,13 @@ class Block(nn.Module):
         h = self.n2(x)
         return x + self.down(F.silu(self.gate(h)) * self.up(h))
 
-    def fused(self, x, n, freqs, after):
+    def fused(self, x, n, at, after):
         """(x, n) after this block, from x and its norm n: n is the norm of x by `after`, which comes next."""
-        x, n = ops.residual_norm(x, self.attn.fused(n, freqs), self.n2.weight, eps=self.n2.eps)
-        return ops.residual_norm(x, self.down(ops.gated_linear(n, self.gate.weight, self.up.weight)), after.weight, eps=after.eps)
+        x, n = add_norm(x, attention(self.attn, n, at, Attention), self.n2)
+        return add_norm(x, self.down(gated(n, self.gate, self.up)), after)
 
 
-def run_fused(x, blocks, last, freqs):
-    """The blocks and the last norm."""
-    n = ops.rms_norm(x, blocks[0].n1.weight, eps=blocks[0].n1.eps) if len(blocks) else ops.rms_norm(x, last.weight, eps=last.eps)
-    for i, blk in enumerate(blocks):
-        x, n = blk.fused(x, n, freqs, blocks[i + 1].n1 if i + 1 < len(blocks) else last)
-    return n
+_OWN_FORWARD[Block] = Block.forward
 
 
 class LlamaDecoder(nn.Module):
@@ -151,8 +208,8 @@ class LlamaDecoder(nn.Module):
     def forward(self, tokens):
         x = self.embed(tokens)
         if self.cfg.fused:
-            freqs = ops.rotary_frequencies(self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, device=tokens.device)
-            return self.head(run_fused(x, self.blocks, self.norm, freqs))
+            at = Positions(tokens.shape[1], self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, tokens.device)
+            return self.head(run_fused(x, self.blocks, self.norm, at, Block))
         cos, sin = rope_tables(tokens.shape[1], self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, tokens.device)
         for blk in self.blocks:
             x = blk(x, cos, sin)

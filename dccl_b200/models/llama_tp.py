@@ -15,8 +15,7 @@ import torch.nn.functional as F
 
 from ..ops import functional as ops
 from ..parallel.tensor_parallel import SymmetricPool, column_linears_reduce_grad_in_place, row_linear_reduce_in_place
-from ..ops.decoder import gated_linear, residual_norm, rotary_frequencies
-from .llama import LlamaDecoder, apply_rope, attend, rope_tables, run_fused
+from .llama import _OWN_FORWARD, LlamaDecoder, Positions, add_norm, apply_rope, attend, attention, gated, rope_tables, run_fused
 
 
 def _rows(linear, lo, hi):
@@ -103,20 +102,22 @@ class ShardedBlock(nn.Module):
         h = ops.copy_to_region(self.n2(x), self.comm)
         return x + ops.reduce_from_region(self.down(F.silu(self.gate(h)) * self.up(h)), self.comm)
 
-    def fused(self, x, n, freqs, after):
+    def fused(self, x, n, at, after):
         """(x, n) after this block, as of the unsplit one. The pool takes the products at the exits and the input gradient of attention; that of
         the gated product is a tensor of its own. What a residual norm adds it keeps for the backward pass, so it gets a copy of a pool's buffer."""
-        a = self.attn.fused(n, freqs)
-        x, n = residual_norm(x, a if self.pool is None else a.clone(), self.n2.weight, eps=self.n2.eps)
-        h = ops.all_gather(n, 1, self.comm) if self.sp else ops.copy_to_region(n, self.comm)
-        h = gated_linear(h, self.gate.weight, self.up.weight)
+        a = attention(self.attn, n, at, ShardedAttention)
+        x, n = add_norm(x, a if self.pool is None else a.clone(), self.n2)
+        h = gated(ops.all_gather(n, 1, self.comm) if self.sp else ops.copy_to_region(n, self.comm), self.gate, self.up)
         if self.sp:
             m = ops.reduce_scatter(self.down(h), 1, "sum", self.comm)
         elif self.pool is not None:
             m = row_linear_reduce_in_place(h, self.down.weight, self.comm, self.pool).clone()
         else:
             m = ops.reduce_from_region(self.down(h), self.comm)
-        return residual_norm(x, m, after.weight, eps=after.eps)
+        return add_norm(x, m, after)
+
+
+_OWN_FORWARD.update({kind: kind.forward for kind in (ShardedAttention, ShardedBlock)})
 
 
 class VocabParallelEmbedding(nn.Module):
@@ -201,11 +202,11 @@ class ShardedLlamaDecoder(nn.Module):
             if tokens.shape[1] % self.comm.world:
                 raise ValueError("the sequence length (%d) must divide by the world size" % tokens.shape[1])
             x = self._my_part(x)
-        head_dim = self.cfg.hidden // self.cfg.heads
+        place = tokens.shape[1], self.cfg.hidden // self.cfg.heads, self.cfg.rope_theta, tokens.device
         if self.cfg.fused:
-            x = run_fused(x, self.blocks, self.norm, rotary_frequencies(head_dim, self.cfg.rope_theta, device=tokens.device))
+            x = run_fused(x, self.blocks, self.norm, Positions(*place), ShardedBlock)
         else:
-            cos, sin = rope_tables(tokens.shape[1], head_dim, self.cfg.rope_theta, tokens.device)
+            cos, sin = rope_tables(*place)
             for blk in self.blocks:
                 x = blk(x, cos, sin)
             x = self.norm(x)

@@ -723,6 +723,112 @@ def test_the_fused_decoder_is_the_same_model():
         assert (p.grad - q.grad).abs().max() <= 3e-5 * p.grad.abs().max() + 1e-7, name
 
 
+class Doubled(torch.nn.Module):
+    """Stands in a module's place and does more."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, *args):
+        return 2 * self.inner(*args)
+
+
+def double(module, args, out):
+    return 2 * out
+
+
+def touch(model, how):
+    """Changes what modules of a decoder do. The same change to its plain and its fused form has to have the same effect."""
+    block, other = model.blocks[0], model.blocks[1]
+    linears = {"%s of %d" % (name, i): (b, name) for i, b in enumerate(model.blocks) for name in ("gate", "up")}
+    if how == "hooks on all":
+        calls = []
+        for name, m in model.named_modules():
+            m.register_forward_hook(lambda m, a, o, name=name: calls.append(name))
+        return calls
+    if how == "hooks that change":
+        for m in (block.n1, block.gate, other.n2, other.attn, other.up, model.norm):
+            m.register_forward_hook(double)
+    elif how == "hooks before":
+        for m in (block.n2, block.up, other.n1, model.norm):
+            m.register_forward_pre_hook(lambda m, args: (2 * args[0],))
+    elif how == "a block's hook":
+        block.register_forward_hook(double)
+    elif how == "the last block's hook":
+        other.register_forward_hook(double)
+    elif how == "other modules":
+        block.gate, block.n2, other.attn, other.n1, model.norm = (Doubled(m) for m in (block.gate, block.n2, other.attn, other.n1, model.norm))
+    elif how == "other blocks":
+        model.blocks[0], model.blocks[1] = Doubled(block), Doubled(other)
+    elif how == "other classes":
+        block.n2, other.n1 = (torch.nn.LayerNorm(model.cfg.hidden) for _ in range(2))
+    elif how == "biases":
+        for b, name in linears.values():
+            getattr(b, name).bias = torch.nn.Parameter(torch.linspace(-1, 1, getattr(b, name).out_features, dtype=getattr(b, name).weight.dtype))
+    elif how == "another forward":
+        for m in (block.up, other.n2, block.attn, other):
+            m.forward = lambda *args, f=m.forward: 2 * f(*args)
+    elif how == "parametrized":
+        torch.nn.utils.parametrizations.weight_norm(block.gate)
+        torch.nn.utils.parametrize.register_parametrization(other.n2, "weight", Doubled(torch.nn.Identity()))
+    elif how == "hooks backward":
+        for m in (block.n1, block.gate, other.attn, other, model.norm):
+            m.register_full_backward_hook(lambda m, gi, go: tuple(None if g is None else 2 * g for g in gi))
+    else:
+        raise ValueError(how)
+
+
+TOUCHES = ["hooks on all", "hooks that change", "hooks before", "a block's hook", "the last block's hook", "other modules", "other blocks", "other classes", "biases", "another forward",
+           "parametrized", "hooks backward"]
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("how", TOUCHES)
+def test_what_is_done_to_a_modules_call_is_done_to_the_fused_decoder(how, split):
+    """Bounds of test_the_fused_decoder_is_the_same_model, eight times as wide for what is doubled up to three times on the way."""
+    from dccl_b200 import Communicator
+    from dccl_b200.models.llama_tp import shard
+    models = decoders("cpu", torch.float32)
+    tokens = models[2]
+    comm = Communicator(rank=0, world=1) if split else None
+    try:
+        seen = []
+        pair = [shard(m, comm) if split else m for m in models[:2]]
+        for m in pair:
+            seen.append(touch(m, how))
+        losses = [m.loss(tokens) for m in pair]
+        for v in losses:
+            v.backward()
+        if how == "hooks on all":
+            assert sorted(seen[0]) == sorted(seen[1])
+        assert abs(losses[0] - losses[1]) < 8e-5 * abs(losses[0])
+        for (name, p), q in zip(pair[0].named_parameters(), pair[1].named_parameters()):
+            assert q[0] == name and (p.grad - q[1].grad).abs().max() <= 24e-5 * p.grad.abs().max() + 1e-6, name
+    finally:
+        if comm is not None:
+            comm.finalize()
+
+
+def test_a_hook_on_every_module_runs_in_the_fused_decoder():
+    plain, fused, tokens = decoders("cpu", torch.float32)
+    calls = []
+    with torch.no_grad():
+        want = fused(tokens)
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, o: calls.append(type(m).__name__))
+    try:
+        with torch.no_grad():
+            got = fused(tokens)
+        there, calls[:] = sorted(calls), []
+        with torch.no_grad():
+            plain(tokens)
+    finally:
+        handle.remove()
+    assert there == sorted(calls) and torch.allclose(got, want, rtol=1e-4, atol=1e-5)
+    with torch.no_grad():
+        assert torch.equal(fused(tokens), want)
+
+
 @pytest.mark.parametrize("world", [1, 2])
 def test_the_fused_decoder_split_over_ranks(dccl_lib, world):
     import os
