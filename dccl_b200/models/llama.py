@@ -8,8 +8,8 @@ the "no library GEMM" rule of this project applies to the communication paths, n
 
 With ``LlamaConfig(fused=True)`` the same modules compute with the operators of ``dccl_b200.ops.decoder``: each residual add in one pass with
 the norm after it, rotary positions of queries and keys in one launch, and the gated projections as one product (parameters and state
-dict stay the same; on the GPU the model is then float16 or bfloat16). A module that is more than what stands here (another one put in its place, a
-bias, hooks) is called, and the others around it stay fused.
+dict stay the same). A module that is more than what stands here (another one put in its place, a bias, hooks) is called, and so is what an
+operator does not take (the gated projections in float32 on the GPU or under autocast); the others around it stay fused.
 """
 import functools
 from dataclasses import dataclass
@@ -95,9 +95,9 @@ class Attention(nn.Module):
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.kv != self.h)
         return self.o(out.transpose(1, 2).reshape(b, s, self.h * self.hd))
 
-    def fused(self, x, freqs):
+    def fused(self, x, at):
         b, s, _ = x.shape
-        return self.o(attend(self.q(x).view(b, s, self.h, self.hd), self.k(x).view(b, s, self.kv, self.hd), self.v(x).view(b, s, self.kv, self.hd), freqs))
+        return self.o(attend(self.q(x).view(b, s, self.h, self.hd), self.k(x).view(b, s, self.kv, self.hd), self.v(x).view(b, s, self.kv, self.hd), at))
 
 
 # ---- the fused form. Every operator stands for modules that are then not called, so each use asks first whether calling them would do more.
@@ -123,33 +123,45 @@ class Positions:
         return rope_tables(*self._tables)
 
 
-def attend(q, k, v, freqs):
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def attend(q, k, v, at):
     """Causal attention of [batch, seq, heads, head dim], whose queries and keys are turned by their positions first: [batch, seq, heads * head dim]."""
-    q, k = ops.rotary(q, k, freqs)
+    if q.dtype in _TYPES:
+        q, k = ops.rotary(q, k, at.freqs)
+    else:
+        q, k = (apply_rope(t.transpose(1, 2), *at.tables).transpose(1, 2) for t in (q, k))
     out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=q.shape[2] != k.shape[2])
     return out.transpose(1, 2).flatten(2)
 
 
 def attention(module, n, at, kind):
-    return module.fused(n, at.freqs) if untouched(module, kind) else module(n, *at.tables)
+    return module.fused(n, at) if untouched(module, kind) else module(n, *at.tables)
 
 
 def gated(n, gate, up):
-    if untouched(gate, nn.Linear) and untouched(up, nn.Linear):
+    if (untouched(gate, nn.Linear) and untouched(up, nn.Linear) and n.dtype in _TYPES[:3 - n.is_cuda] and gate.weight.dtype == up.weight.dtype == n.dtype
+            and not torch.is_autocast_enabled(n.device.type)):
         return ops.gated_linear(n, gate.weight, up.weight)
     return F.silu(gate(n)) * up(n)
+
+
+def norms(norm, x):
+    """Whether the operators compute what `norm` does with x."""
+    return untouched(norm, RMSNorm) and x.dtype in _TYPES and norm.weight.dtype in (x.dtype, torch.float32)
 
 
 def norm_of(x, norm):
     if norm is None:
         return None
-    return ops.rms_norm(x, norm.weight, eps=norm.eps) if untouched(norm, RMSNorm) else norm(x)
+    return ops.rms_norm(x, norm.weight, eps=norm.eps) if norms(norm, x) else norm(x)
 
 
 def add_norm(x, branch, norm):
     """x + branch, and the norm of it; None where what comes next takes no norm."""
-    if norm is not None and untouched(norm, RMSNorm):
-        return ops.residual_norm(x, branch, norm.weight, eps=norm.eps)
+    if norm is not None and norms(norm, x) and torch.promote_types(x.dtype, branch.dtype) == x.dtype:
+        return ops.residual_norm(x, branch.to(x.dtype), norm.weight, eps=norm.eps)
     x = x + branch
     return x, norm_of(x, norm)
 

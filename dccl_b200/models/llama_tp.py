@@ -64,8 +64,8 @@ class ShardedAttention(nn.Module):
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.kv != self.h)
         return self._leave(out.transpose(1, 2).reshape(q.shape[0], q.shape[2], self.h * self.hd))
 
-    def fused(self, x, freqs):
-        return self._leave(attend(*self._project(x), freqs))
+    def fused(self, x, at):
+        return self._leave(attend(*self._project(x), at))
 
     def _leave(self, out):
         if self.sp:      # sum the partial products and keep this rank's part of the sequence (backward: all-gather)

@@ -839,6 +839,38 @@ def test_the_fused_decoder_split_over_ranks(dccl_lib, world):
         assert p.stdout.strip().splitlines()[-1].startswith("OK"), p.stdout
 
 
+def fused_against_plain(device, dtype, autocast, loss_bound, grad_bound, norm):
+    plain, fused, tokens = decoders(device, dtype)
+    losses = []
+    for m in (plain, fused):
+        with torch.autocast(device, torch.bfloat16, enabled=autocast):
+            losses.append(m.loss(tokens))
+        losses[-1].backward()
+    assert abs(losses[0] - losses[1]) <= loss_bound * abs(losses[0])
+    for (name, p), q in zip(plain.named_parameters(), fused.named_parameters()):
+        off, size = p.grad.double() - q[1].grad.double(), p.grad.double()
+        assert q[1].grad.dtype == p.grad.dtype and (off.norm() <= grad_bound * size.norm() if norm else off.abs().max() <= grad_bound * size.abs().max() + 1e-7), name
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype,autocast", [(torch.float32, False), (torch.float32, True), (torch.bfloat16, True), (torch.float64, False)], ids=str)
+def test_the_fused_decoder_takes_the_types_of_the_plain_one(device, dtype, autocast):
+    """fp32 as in test_the_fused_decoder_is_the_same_model, and of fp64 only what the norms and the turned heads round to fp32. Where bf16 comes in, about
+    thirty results on the way and as many back, each off by 2^-9 in the root mean square in both: twice 8 x 2^-9 of a gradient's norm."""
+    low = autocast or dtype is torch.bfloat16
+    fused_against_plain(device, dtype, autocast, 2.0 ** -7 if low else 1e-5, 0.032 if low else 3e-5, low)
+
+
+@pytest.mark.parametrize("norms,model", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)], ids=str)
+def test_norms_of_another_type_in_the_fused_decoder(norms, model):
+    plain, fused, tokens = decoders("cpu", model)
+    for m in (plain, fused):
+        for block in m.blocks:
+            block.n1.to(norms), block.n2.to(norms)
+    a, b = plain.loss(tokens), fused.loss(tokens)
+    assert abs(a - b) <= 2.0 ** -7 * abs(a)
+
+
 @gpu
 def test_the_fused_decoder_on_the_gpu():
     """bf16 on the GPU against the same operators on the CPU: about thirty bf16 results on the way to the loss and as many back, each off by
