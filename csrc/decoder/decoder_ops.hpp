@@ -53,7 +53,8 @@ long long dccl_gated_linear_workspace(int device, size_t tokens, size_t width, s
 
 /**
  * h = act(x Wg^T) .* (x Wu^T): x [tokens][width], Wg and Wu [ffn][width], h [tokens][ffn], all dense and of dtype float16 or bfloat16.
- * Where g and u are not null they receive the two products in fp32, in rows of pre_stride elements (a multiple of four).
+ * Where g and u are not null they receive the two products in fp32, in rows of pre_stride elements (a multiple of four). A product that does
+ * not end in time leaves NaN, and no later call on its device starts one.
  */
 int dccl_gated_linear(int device, int dtype, size_t tokens, size_t width, size_t ffn, const void* x, const void* w_gate, const void* w_up, int act, void* h,
                       float* g, float* u, size_t pre_stride, void* workspace, long long workspace_bytes, void* stream);

@@ -14,32 +14,20 @@
 #include "row_access.cuh"
 #include "../device/tcgen05.cuh"
 #include "../gpu/driver_api.hpp"
+#include "gated_tiles.hpp"
+#include <cstring>
 
 namespace dccl {
 
-enum Form {
-    GATED,          // C = act(x Wg^T) .* (x Wu^T): both operands contiguous along k; the columns of a tile are half of Wg and half of Wu
-    INPUT_GRAD,     // dx = dg Wg + du Wu: k runs through ffn twice; W is contiguous along the columns
-    WEIGHT_GRAD,    // dW = dg^T x, du^T x: k are the tokens, both operands contiguous along rows and columns of the result
-};
-
-constexpr int kTileM = 128, kTileK = 64;
 constexpr int kEpilogueWarps = 8, kGemmThreads = 32 * (kEpilogueWarps + 2);
 constexpr unsigned kLoader = kEpilogueWarps, kMultiplier = kEpilogueWarps + 1;
 constexpr int kStageRowsBytes = 128;                                // one row of a swizzled tile
 
-struct GemmArgs {
+struct GemmArgs : Tiling, Results {
     CUtensorMap a0, a1, b0, b1;
-    unsigned m, n;                  // rows and columns of the result
-    unsigned tiles_m, tiles_n, batch, splits, k_blocks;             // k_blocks: of one tile over all its k
     unsigned k_half;                // INPUT_GRAD: blocks of ffn, after which the second pair of operands follows
     unsigned descriptor;            // of one product
     int act;
-    void *c0, *c1;                  // results (c1: second of the batch)
-    float *g, *u;                   // GATED: the products, or null
-    size_t pre_stride;
-    float* partial;                 // [split][batch or gate, up][m][partial_stride] where splits > 1
-    size_t partial_stride;
     int* gave_up;                   // host memory: a wait that did not end
 };
 
@@ -117,22 +105,6 @@ template <typename T> __device__ __forceinline__ void store_as(const char* stage
         for (int r = 0; r < rows && r < 32; r++)
             to[(size_t)r * stride + lane] = Traits<T>::down(*reinterpret_cast<const float*>(stage + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
     }
-}
-
-/** Tile number -> place. Groups of 16 rows of tiles are walked column by column, so that the tiles of one moment share operands in L2. */
-struct Place { unsigned m, n, batch, split; };
-__device__ __forceinline__ Place place_of(unsigned tile, const GemmArgs& a) {
-    Place p;
-    p.split = tile % a.splits;
-    tile /= a.splits;
-    const unsigned per_batch = a.tiles_m * a.tiles_n;
-    p.batch = tile / per_batch;
-    tile %= per_batch;
-    const unsigned group = tile / (16 * a.tiles_n), first = group * 16, rows = a.tiles_m - first < 16 ? a.tiles_m - first : 16;
-    tile -= first * a.tiles_n;
-    p.m = first + tile % rows;
-    p.n = tile / rows;
-    return p;
 }
 
 template <int FORM, int N, bool PAIR> struct GemmShape {
@@ -320,6 +292,9 @@ template <typename T, int FORM, int N, bool PAIR> __device__ __forceinline__ voi
     __syncthreads();
     if (failed) {       // no wait is expected to run out: copies in flight still have to land, and products to end, before the memory is given back
         int late = 0;
+        mark_incomplete(FORM, a, a, Shape::kRows, Shape::kColumns, rank, first, step, threadIdx.x, kGemmThreads);
+        if (warp == kLoader && lane == 0 && rank != 0)      // its copies count on the leader's barriers: here only time tells that they have landed
+            for (const long long start = clock64(); clock64() - start < kLandClocks;) {}
         if (warp == kLoader && lane == 0 && rank == 0)
             for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
         if (warp == kMultiplier && lane == 0 && rank == 0) {
@@ -442,6 +417,10 @@ template <typename T, int N> __global__ void __launch_bounds__(kFewThreads, 2) k
         if (warp == 5 && lane == 0) {
             commit(drained);
             bar_wait(drained, 0, &late);
+        }
+        for (unsigned i = threadIdx.x; i < a.tokens * a.rows; i += kFewThreads) {
+            const unsigned t = i / a.rows, row = first + i % a.rows;
+            if (row < a.ffn) mark_incomplete(a.h, a.g, a.u, (size_t)t * a.ffn + row, t * a.pre_stride + row);
         }
         if (threadIdx.x == 0 && a.gave_up) *reinterpret_cast<volatile int*>(a.gave_up) = 1;
         __syncthreads();
@@ -579,18 +558,19 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) k_gate_gr
 
 /* ------------------------------------------------------------------------------------------------ host side */
 
-/** Set by a kernel whose wait ran out; looked at by the next call. Host memory that the device writes, for the life of the process. */
-static int* gave_up_flag() {
-    static int* flag = [] {
+/** Set by a kernel whose wait ran out, which leaves NaN in what it was to store; looked at by the next call on the device. Host memory that the device
+ *  writes, for the life of the process. */
+static int* gave_up_flag(int device) {
+    static int* const flags = [] {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         cudaThreadExchangeStreamCaptureMode(&mode);       // a first call may come while a stream is being captured
         void* p = nullptr;
-        if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { cudaGetLastError(); p = nullptr; }
+        if (cudaHostAlloc(&p, 64 * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { cudaGetLastError(); p = nullptr; }
         cudaThreadExchangeStreamCaptureMode(&mode);
-        if (p) *reinterpret_cast<int*>(p) = 0;
+        if (p) memset(p, 0, 64 * sizeof(int));
         return reinterpret_cast<int*>(p);
     }();
-    return flag;
+    return flags ? flags + device : nullptr;        // of the 64 devices that sm_count knows
 }
 
 /** The two dimensions of an operand by which one is contiguous, and the box of it. */
@@ -602,33 +582,6 @@ static cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, size_
     const CUresult r = d->TensorMapEncodeTiled(map, dtype == 6 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
                                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
-static size_t up_to(size_t v, size_t step) { return (v + step - 1) / step * step; }
-static unsigned blocks_of(size_t v, size_t block) { return (unsigned)((v + block - 1) / block); }
-
-/** Tiles of a product, 256 columns wide or 128, and the parts that its k is cut into. */
-struct GemmPlan { bool pair; int columns; unsigned tiles_m, tiles_n, batch, splits, k_blocks; size_t partial_bytes; };
-
-static GemmPlan plan_gemm(int sms, int form, size_t m, size_t n, size_t k) {
-    GemmPlan p;
-    p.pair = m > kTileM;
-    p.tiles_m = blocks_of(m, p.pair ? 2 * kTileM : kTileM);
-    p.batch = form == WEIGHT_GRAD ? 2 : 1;
-    p.k_blocks = blocks_of(k, kTileK) * (form == INPUT_GRAD ? 2 : 1);
-    const unsigned workers = p.pair ? sms / 2 : sms;
-    const auto tiles_of = [&](int columns) { return (size_t)p.tiles_m * blocks_of(n, form == GATED ? columns / 2 : columns) * p.batch; };
-    const auto splits_of = [&](int columns) {
-        const size_t tiles = tiles_of(columns), most = p.k_blocks / 4, s = workers / (tiles ? tiles : 1);
-        return s > most ? (most ? most : 1) : s ? s : 1;
-    };
-    // rounds of tiles, and what a round takes: a tile of half the width loads three quarters of the bytes, which is what these products wait for
-    const auto cost = [&](int columns) { return (columns == 128 ? 3 : 4) * 64 * ((tiles_of(columns) + workers - 1) / workers) / splits_of(columns); };
-    p.columns = cost(128) < cost(256) ? 128 : 256;
-    p.tiles_n = blocks_of(n, form == GATED ? p.columns / 2 : p.columns);
-    p.splits = (unsigned)splits_of(p.columns);
-    p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (form == INPUT_GRAD ? 1 : 2) * m * up_to(n, 4) * sizeof(float) : 0;
-    return p;
 }
 
 template <typename T, int FORM, int N, bool PAIR> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
@@ -647,7 +600,7 @@ template <typename T, int FORM, int N, bool PAIR> static cudaError_t run_gemm(in
     a.k_blocks = p.k_blocks;
     a.partial_stride = up_to(a.n, 4);
     a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == WEIGHT_GRAD, FORM != GATED, Shape::kRows, N);
-    a.gave_up = gave_up_flag();
+    a.gave_up = gave_up_flag(device);
     const size_t tiles = (size_t)p.tiles_m * p.tiles_n * p.batch * p.splits, workers = PAIR ? sm_count(device) / 2 : sm_count(device);
     cudaError_t e = launch_early_shared(kernel, (unsigned)(tiles < workers ? tiles : workers) * (PAIR ? 2 : 1), kGemmThreads, Shape::kShared, stream, a);
     if (e != cudaSuccess || p.splits == 1) return e;
@@ -659,20 +612,6 @@ template <typename T, int FORM, int N, bool PAIR> static cudaError_t run_gemm(in
 template <typename T, int FORM> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
     if (p.pair) return p.columns == 128 ? run_gemm<T, FORM, 128, true>(device, p, a, stream) : run_gemm<T, FORM, 256, true>(device, p, a, stream);
     return p.columns == 128 ? run_gemm<T, FORM, 128, false>(device, p, a, stream) : run_gemm<T, FORM, 256, false>(device, p, a, stream);
-}
-
-/** Whether k_gated_few takes a call: for wider layers than it has CTAs for, splits of k read the weights faster. */
-static bool few_tokens(int sms, size_t tokens, size_t width, size_t ffn) {
-    return tokens <= 128 && (width <= 4096 || 2 * blocks_of(ffn, 8) >= (size_t)sms);
-}
-
-/** Rows of each weight for one CTA of k_gated_few, two of which share an SM: as many CTAs as there is room for, in as few rounds as it takes,
- *  but not less than 32 rows while every SM has a CTA, since each CTA reads x as well (5632 rows: 32 take 13.7 us for one token and 16.9 for
- *  64, 24 take 14.3 and 19.9, and one CTA of 40 rows per SM 13.8 and 19.0). */
-static unsigned few_rows(int sms, size_t ffn) {
-    const size_t room = 2 * (size_t)sms, rounds = (ffn + 64 * room - 1) / (64 * room);
-    const unsigned rows = (unsigned)up_to((ffn + room * rounds - 1) / (room * rounds), 8);
-    return rows < 32 && ffn >= 32 * (size_t)sms ? 32 : rows;
 }
 
 /** Where the parts of a call's workspace lie. */
@@ -756,7 +695,7 @@ template <typename T> static cudaError_t gated_forward(int device, int dtype, co
         f.g = g;
         f.u = u;
         f.pre_stride = pre_stride;
-        f.gave_up = gave_up_flag();
+        f.gave_up = gave_up_flag(device);
         return columns == 16 ? run_few<T, 16>(device, f, stream) : columns == 32 ? run_few<T, 32>(device, f, stream) : columns == 64 ? run_few<T, 64>(device, f, stream)
                                                                                                                                     : run_few<T, 128>(device, f, stream);
     }
@@ -815,10 +754,10 @@ template <typename T> static cudaError_t gated_backward(int device, int dtype, c
     return e;
 }
 
-static bool gave_up(const char* who) {
-    const int* flag = gave_up_flag();
+static bool gave_up(const char* who, int device) {
+    const int* flag = gave_up_flag(device);
     if (!flag || !*reinterpret_cast<const volatile int*>(flag)) return false;
-    fprintf(stderr, "%s: an earlier product on this machine did not end in time; its results are incomplete\n", who);
+    fprintf(stderr, "%s: an earlier product of this process on device %d did not end in time; what it did not finish is NaN, and no other is started there\n", who, device);
     return true;
 }
 
@@ -841,7 +780,7 @@ extern "C" int dccl_gated_linear(int device, int dtype, size_t tokens, size_t wi
     if (!l.ok || !width || workspace_bytes < (long long)l.total || (dtype != 6 && dtype != 9) || act < 0 || act > DCCL_ACT_GELU_TANH || (!g != !u) || (g && pre_stride < ffn)
         || pre_stride % 4 || !aligned_to(16, {g, u, workspace}))
         return report(who, cudaErrorInvalidValue);
-    if (gave_up(who)) return -1;
+    if (gave_up(who, device)) return -1;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
     const auto run = dtype == 6 ? gated_forward<__half> : gated_forward<__nv_bfloat16>;
@@ -857,7 +796,7 @@ extern "C" int dccl_gated_linear_backward(int device, int dtype, size_t tokens, 
         || pre_stride < ffn || pre_stride % 4 || !aligned_to(16, {g, u, workspace, forward_workspace}) || (!dw_gate != !dw_up)
         || (l.padded && !forward_workspace))
         return report(who, cudaErrorInvalidValue);
-    if (gave_up(who)) return -1;
+    if (gave_up(who, device)) return -1;
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
     const auto run = dtype == 6 ? gated_backward<__half> : gated_backward<__nv_bfloat16>;

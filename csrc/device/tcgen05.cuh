@@ -27,6 +27,8 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 
 constexpr long long kWaitClocks = 1ll << 34;     // about nine seconds: what a wait inside one CTA never takes
 
+constexpr long long kLandClocks = 1ll << 24;     // about nine milliseconds: a thousand times what a copy takes
+
 /** Waits for the phase of this parity. False after nine seconds, or once another wait of the CTA gave up (`failed`, in shared memory). */
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
     if (bar_try(bar, parity)) return true;

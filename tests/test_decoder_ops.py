@@ -694,6 +694,31 @@ def test_gated_refusals_on_the_gpu():
         ops.gated_linear(torch.zeros(2, 8, device="cuda").half(), torch.zeros(6, 8).half(), torch.zeros(6, 8, device="cuda").half())
 
 
+@pytest.fixture(scope="module")
+def tiles_program(tmp_path_factory):
+    """tests/sim/gated_tiles.cpp: how products are cut, without a GPU."""
+    import os
+    import subprocess
+    exe = str(tmp_path_factory.mktemp("tiles") / "gated_tiles")
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", "-Werror", os.path.join(os.path.dirname(os.path.abspath(__file__)), "sim", "gated_tiles.cpp"), "-o", exe],
+                   check=True)
+    return exe
+
+
+def test_products_that_gave_up_leave_nan(tiles_program):
+    """A wait that runs out must not be made to happen on a GPU: the stores that follow one run here, for every CTA and thread."""
+    import subprocess
+    res = subprocess.run([tiles_program, "mark"], capture_output=True, text=True)
+    assert res.returncode == 0, res.stdout
+
+
+def test_kernels_that_give_up_mark_their_results():
+    import os
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc", "decoder", "gated_linear.cu")).read()
+    parts = text.split("if (failed) {")[1:]
+    assert len(parts) == 2 and all("mark_incomplete(" in p.split("*reinterpret_cast<volatile int*>(a.gave_up) = 1")[0] for p in parts)
+
+
 # ---------------------------------------------------------------------------------------------- together
 
 def decoders(device, dtype, **kw):
