@@ -4,7 +4,7 @@
  *
  * Two reads or writes of memory per element and a handful of operations: HBM bounds it. Angles are computed here and not read from
  * a table, so that no position lies outside of one: in 64 bits, since 32 hold no fraction of a turn at position 10^6, as
- * turns whose whole part is dropped before the sine and cosine in 32. A CTA takes consecutive tokens of one sequence and computes their
+ * turns whose whole part is dropped before the sine and cosine in 32, to which what the rounding of the rest took off is added. A CTA takes consecutive tokens of one sequence and computes their
  * angles, each once, into shared memory. A thread keeps its place within a token, its head and its elements, and walks along the
  * tokens with the loads of two or four of them in flight, the first under way while the angles are computed: what it takes to find an
  * element, as many instructions as to turn it, is paid once for all tokens.
@@ -142,9 +142,11 @@ __global__ void __launch_bounds__(kRotaryThreads, 2) k_rotary(const __grid_const
             const long long at = batch * a.pos_batch + (begin + of) * a.pos_seq;
             pos = a.wide_positions ? reinterpret_cast<const long long*>(a.positions)[at] : reinterpret_cast<const int*>(a.positions)[at];
         }
-        const double turns = (double)pos * (a.freqs[pair] * 0.15915494309189533577);      // 1 / (2 pi)
-        float sn, cs;
-        sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+        const double turns = (double)pos * (a.freqs[pair] * 0.15915494309189533577), part = turns - rint(turns);      // 1 / (2 pi)
+        const float near = (float)part, rest = (float)(part - near) * 6.2831853f;      // what rounding took off, in radians: under 2^-23, so its square is nothing
+        float s0, c0;
+        sincospif(2.0f * near, &s0, &c0);
+        const float sn = fmaf(c0, rest, s0), cs = fmaf(-s0, rest, c0);
         cosines[k] = cs * a.scale;
         sines[k] = (a.back ? -sn : sn) * a.scale;
     }

@@ -418,6 +418,21 @@ def test_rotary_positions_and_layouts(per_sequence, int32, front):
 
 
 @gpu
+def test_rotary_cosines_and_sines_are_exact_to_their_size():
+    """Pairs (1, 0) become (cos, sin) with no further rounding. Each is off by one step of sincospif, the correction's rounding and that of what it adds:
+    three steps of 2^-23 of the value itself, also next to zero (355 is 113 pi to 3e-5); and of the angle by what 64 bits lose."""
+    freqs = ops.rotary_frequencies(64, device="cuda")
+    pos = torch.cat((torch.tensor([0, 3, 22, 333, 355, 710, 103993, 104348, 312689, 833719]), torch.randint(0, 1 << 20, (2000,), generator=torch.Generator().manual_seed(4))))
+    x = torch.zeros(1, pos.numel(), 1, 64, device="cuda")
+    x[..., :32] = 1
+    got = ops.rotary(x, None, freqs, pos.cuda())[0, :, 0].double().cpu()
+    angle = pos.double().unsqueeze(-1) * freqs.cpu()
+    for name, v, want in (("cos", got[:, :32], angle.cos()), ("sin", got[:, 32:], angle.sin())):
+        off = (v - want).abs() - (3 * 2.0 ** -23 * want.abs() + angle * 2.0 ** -51)
+        assert off.max() <= 0, (name, off.max().item())
+
+
+@gpu
 def test_rotary_far_positions():
     rotary_run(2, 40, 4, 2, 64, 32, torch.float32, furthest=(1 << 31) - 1)
     q = torch.randn(1, 3, 2, 64, device="cuda")
