@@ -165,6 +165,35 @@ def test_norm_with_more_gates_than_ctas():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("width", [258, 2046, 2050, 6002, 8190, 8194, 16386])
+def test_norm_of_pairs(dtype, width):
+    """Widths of which accesses hold two 16-bit elements: several warps, and 8, 16 and 32 elements per thread."""
+    norm_run((11, width), dtype)
+    norm_run((2, 3, width), dtype, post=True, gate=(2, 1, width), scale=0.37, wide=True)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3000, 1451), (3000, 1450), (700, 6001), (700, 6002), (500, 8194), (500, 8193), (1400, 2048), (350, 8192)], ids=str)
+@pytest.mark.parametrize("form", ["sum", "all"])
+def test_norm_with_many_rows_for_a_cta(shape, form):
+    """More rows than CTAs can be resident (148 x 3 of up to 2048 elements, 148 of more), so that each CTA takes several, whatever its accesses."""
+    if form == "sum":
+        norm_run(shape, torch.bfloat16)
+    else:
+        norm_run(shape, torch.float16, post=True, gate=shape[-1:], scale=0.37)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,gates,width", [(torch.float16, 5200, 64), (torch.float16, 5200, 65), (torch.float16, 5200, 66), (torch.float32, 5200, 64), (torch.bfloat16, 1000, 2048),
+                                               (torch.bfloat16, 1000, 1999), (torch.bfloat16, 1000, 1998), (torch.bfloat16, 400, 4096), (torch.bfloat16, 400, 4001)], ids=str)
+def test_norm_with_more_units_than_ctas(dtype, gates, width):
+    """At most 148 x 23 CTAs of one warp, 148 x 3 of up to 2048 elements and 148 of more are resident, and every gate is a unit of its own: each CTA starts several.
+    5200 units are added by 32 threads a column, 163 each to a sum that grows from nothing and counts half, and their 32 sums: within the 128 of SUMS."""
+    norm_run((gates, 2, width), dtype, True, (gates, 1, width), 0.5)
+
+
+@gpu
 def test_norm_of_views():
     """Rows that start between two accesses, and tensors that are not dense: transposed, expanded."""
     g = torch.Generator(device="cuda").manual_seed(3)
@@ -627,6 +656,37 @@ SIZES = [(1, 64, 64), (1, 8, 8), (2, 1, 1), (3, 5, 7), (40, 256, 512), (128, 64,
 @pytest.mark.parametrize("sizes", SIZES, ids=str)
 def test_gated_at_its_sizes(dtype, sizes):
     gated_run(*sizes, dtype)
+
+
+# Reach with SIZES every kind of plan that the rule gives on 148 SMs: tiles of one CTA or a pair, 128 or 256 columns, whole or cut along k, and up to three
+# tiles for a CTA, with more blocks of k than it has stages and remainders in all dimensions.
+LARGE = [(461, 8, 200), (1, 8, 10992), (545, 520, 816), (9484, 544, 8), (1547, 1288, 824), (2411, 792, 1080), (3589, 3408, 522), (4336, 1128, 1956), (667, 6200, 682), (513, 272, 14291),
+         (17, 8200, 570)]
+
+
+@gpu
+@pytest.mark.parametrize("sizes", LARGE, ids=str)
+def test_gated_in_every_kind_of_plan(sizes):
+    gated_run(*sizes, torch.float16 if sizes[1] % 16 else torch.bfloat16)
+
+
+def test_sizes_reach_every_kind_of_plan(tiles_program):
+    import subprocess
+
+    def kind(form, m, n, k):
+        pair, columns, splits, rounds = (int(v) for v in subprocess.run([tiles_program, "plan", "148"] + [str(v) for v in (form, m, n, k)], capture_output=True, text=True, check=True).stdout.split())
+        return "gated dx dw".split()[form], "pair" if pair else "one", columns, "cut" if splits > 1 else min(rounds, 3)
+
+    found = set()
+    for tokens, width, ffn in SIZES + LARGE:
+        if tokens > 128 or (width > 4096 and ffn <= 73 * 8):         # few_tokens
+            found.add(kind(0, tokens, ffn, width))
+        found |= {kind(1, tokens, width, ffn), kind(2, ffn, width, tokens)}
+    wanted = {(form, "pair", columns, how) for form in ("gated", "dx", "dw") for columns in (128, 256) for how in ("cut", 1, 2, 3)}
+    wanted -= {("gated", "pair", 128, 3), ("dx", "pair", 128, 3)}             # the rule does not give these
+    wanted |= {("gated", "one", 128, "cut"), ("gated", "one", 256, "cut")}    # 128 tokens at most, and a layer too wide for k_gated_few
+    wanted |= {(form, "one", 128, how) for form in ("dx", "dw") for how in ("cut", 1)} | {("dx", "one", 256, "cut"), ("dw", "one", 256, "cut")}
+    assert wanted <= found, wanted - found
 
 
 @gpu
