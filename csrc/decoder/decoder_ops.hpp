@@ -7,6 +7,10 @@
 #include <cstddef>
 #include <cstdint>
 
+/** What the entry points take, and with them dccl_b200/ops/decoder.py: elements of a row, pairs of a head, elements of a token, and each dimension of
+ *  a gated layer below. */
+enum { DCCL_NORM_MAX_WIDTH = 32768, DCCL_ROTARY_MAX_PAIRS = 1024, DCCL_ROTARY_MAX_TOKEN = 1 << 24, DCCL_GATED_MAX_DIMENSION = 1 << 30 };
+
 /** Which of the vectors of a norm are fp32 and not of the activations' type. */
 enum { DCCL_NORM_WEIGHT_F32 = 1, DCCL_NORM_POST_F32 = 2, DCCL_NORM_GATE_F32 = 4 };
 

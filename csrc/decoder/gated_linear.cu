@@ -5,7 +5,7 @@
  *     du = dh .* act(g)            dWg = dg^T x,  dWu = du^T x
  *
  * 4 T F H operations forward and 8 T F H backward for T tokens: the tensor cores bound it, for few tokens the reading of the weights.
- * All products are one kernel in three forms. Operands keep the layout that they have in memory: whichever of their two
+ * All products are one kernel in three forms, except for those of few tokens forward (k_gated_few). Operands keep the layout that they have in memory: whichever of their two
  * dimensions is the contiguous one, a box of 64 of it fills the 128-byte rows of a swizzled tile, and the product is told the
  * tile's orientation. Sums stay in tensor memory in fp32 until the end of a tile.
  */
@@ -620,7 +620,7 @@ struct GatedLayout { size_t stride, x, gate, up, padded, dg, du, d_stride, parti
 static GatedLayout layout_of(int device, size_t tokens, size_t width, size_t ffn, bool aligned, bool backward) {
     GatedLayout l = {};
     const int sms = sm_count(device);
-    l.ok = sms > 0 && tokens < (1u << 30) && width < (1u << 30) && ffn < (1u << 30);
+    l.ok = sms > 0 && tokens < DCCL_GATED_MAX_DIMENSION && width < DCCL_GATED_MAX_DIMENSION && ffn < DCCL_GATED_MAX_DIMENSION;
     if (!l.ok) return l;
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t here = at; at += up_to(bytes, 256); return here; };

@@ -468,8 +468,6 @@ template <typename T, int SLICES> __global__ void __launch_bounds__(32 * SLICES)
     }
 }
 
-constexpr size_t kNormMaxWidth = 32768;
-
 /** Elements per thread and threads of a CTA that hold a row. */
 struct NormShape { int elements, threads; };
 static NormShape norm_shape(size_t width) {
@@ -576,7 +574,7 @@ extern "C" int dccl_residual_norm(int device, int dtype, size_t rows, size_t wid
                                   const void* gate, size_t rows_per_gate, int f32_vectors, double eps, double scale, void* y, void* n, void* rstd,
                                   void* rstd_post, void* stream) {
     if (!rows) return 0;
-    if (!width || width > kNormMaxWidth || rows > 0x7fffffffu || !x || !weight || !n || (branch && !y) || (gate && !rows_per_gate) || (post && !branch) || (gate && !branch))
+    if (!width || width > DCCL_NORM_MAX_WIDTH || rows > 0x7fffffffu || !x || !weight || !n || (branch && !y) || (gate && !rows_per_gate) || (post && !branch) || (gate && !branch))
         return report("dccl_residual_norm", cudaErrorInvalidValue);
     const NormArgs a = {x, branch, weight, post, gate, y, n, (float*)rstd, (float*)rstd_post, rows_per_gate, (unsigned)width, f32_vectors, (float)eps, (float)scale};
     const auto all = {x, branch, weight, post, gate, (const void*)y, (const void*)n};
@@ -599,7 +597,7 @@ extern "C" int dccl_residual_norm_backward(int device, int dtype, size_t rows, s
                                            void* workspace, size_t workspace_bytes, void* stream_v) {
     const char* who = "dccl_residual_norm_backward";
     const size_t gates = gate && rows_per_gate ? rows / rows_per_gate : 0;
-    if (!rows || rows > 0x7fffffffu || !width || width > kNormMaxWidth || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
+    if (!rows || rows > 0x7fffffffu || !width || width > DCCL_NORM_MAX_WIDTH || (gate && (!gates || gates * rows_per_gate != rows)) || (post && (!branch || !rstd_post)) || (gate && !branch) || (dn && !rstd)
         || !x || !weight || !dx || !workspace || (dbranch && !branch) || (!dbranch && branch && (post || gate || scale != 1.0)))
         return report(who, cudaErrorInvalidValue);
     const bool full = branch != nullptr;

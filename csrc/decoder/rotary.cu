@@ -191,8 +191,8 @@ extern "C" int dccl_rotary(int device, int dtype, size_t batch, size_t seq, int 
                            void* stream_v) {
     if (!batch || !seq || !head_dim || q->heads + k->heads == 0) return 0;
     const size_t limit = (1u << 31) - 1, tokens = batch * seq;
-    if (pairs < 1 || 2 * pairs > head_dim || pairs > 1024 || batch > limit || seq > limit || tokens > limit || q->heads < 0 || k->heads < 0
-        || (long long)(q->heads + k->heads) * head_dim > (1 << 24))
+    if (pairs < 1 || 2 * pairs > head_dim || pairs > DCCL_ROTARY_MAX_PAIRS || batch > limit || seq > limit || tokens > limit || q->heads < 0 || k->heads < 0
+        || (long long)(q->heads + k->heads) * head_dim > DCCL_ROTARY_MAX_TOKEN)
         return report("dccl_rotary", cudaErrorInvalidValue);
     const int size = dtype == 7 ? 4 : 2, rest = head_dim - 2 * pairs;
     int p = 16 / size;

@@ -44,8 +44,6 @@ struct Entries {
     decltype(&dccl_gated_linear_backward) gated_backward;
 } entry;
 
-constexpr int64_t kMaxWidth = 32768, kMaxPairs = 1024, kMaxToken = 1 << 24, kMaxDimension = 1 << 30;     // as dccl_b200/ops/decoder.py has them
-
 /** ncclDataType_t of the types that the kernels take, or -1. */
 int dtype_of(const Tensor& t) {
     const at::ScalarType s = t.scalar_type();
@@ -229,7 +227,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int dtype = dtype_of(x);
     if (dtype < 0 || x.dim() < 1) Py_RETURN_NOTIMPLEMENTED;
     const int64_t width = x.size(-1), gates = gates_of(x, gate);
-    if (width < 1 || width > kMaxWidth || gates < 0) Py_RETURN_NOTIMPLEMENTED;
+    if (width < 1 || width > DCCL_NORM_MAX_WIDTH || gates < 0) Py_RETURN_NOTIMPLEMENTED;
     const int64_t rows = x.numel() / width;
     if (rows > INT32_MAX || (branch.defined() && (branch.sizes() != x.sizes() || branch.scalar_type() != x.scalar_type() || branch.device() != x.device()))) Py_RETURN_NOTIMPLEMENTED;
     if (!branch.defined() && (post.defined() || gate.defined())) Py_RETURN_NOTIMPLEMENTED;
@@ -364,8 +362,8 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         heads += k.size(-2);
     }
     const Tensor& f = turn.freqs;
-    if (f.dim() != 1 || f.scalar_type() != at::kDouble || f.device() != q.device() || f.requires_grad() || f.size(0) < 1 || 2 * f.size(0) > dim || f.size(0) > kMaxPairs
-        || heads * dim > kMaxToken || seq > INT32_MAX)
+    if (f.dim() != 1 || f.scalar_type() != at::kDouble || f.device() != q.device() || f.requires_grad() || f.size(0) < 1 || 2 * f.size(0) > dim || f.size(0) > DCCL_ROTARY_MAX_PAIRS
+        || heads * dim > DCCL_ROTARY_MAX_TOKEN || seq > INT32_MAX)
         Py_RETURN_NOTIMPLEMENTED;
     const Tensor& p = turn.positions;
     if (p.defined()) {
@@ -454,7 +452,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         || wu.device() != x.device())
         Py_RETURN_NOTIMPLEMENTED;
     const int64_t tokens = x.numel() / width;
-    if (std::max({tokens, width, ffn}) >= kMaxDimension) Py_RETURN_NOTIMPLEMENTED;
+    if (std::max({tokens, width, ffn}) >= DCCL_GATED_MAX_DIMENSION) Py_RETURN_NOTIMPLEMENTED;
     if (observed(args, nargs)) Py_RETURN_NONE;
     check_forward_mode("gated_linear", {&x, &wg, &wu});
     Tensor h;

@@ -30,8 +30,8 @@ import torch
 from .._lib import lib
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
-_MAX_WIDTH, _MAX_PAIRS = 32768, 1024                 # kNormMaxWidth of csrc/decoder/residual_norm.cu, kRotaryPairs of rotary.cu
-
+# as csrc/decoder/decoder_ops.hpp has them
+_MAX_WIDTH, _MAX_PAIRS, _MAX_TOKEN, _MAX_DIMENSION = 32768, 1024, 1 << 24, 1 << 30
 
 _ENTRIES = ("dccl_residual_norm", "dccl_residual_norm_workspace", "dccl_residual_norm_backward", "dccl_rotary", "dccl_gated_linear_workspace", "dccl_gated_linear_pads",
             "dccl_gated_linear", "dccl_gated_linear_backward")
@@ -287,7 +287,7 @@ def rotary(q, k, freqs, positions=None, interleaved=False, scale=1.0):
         cos, sin = (angle.cos() * scale).float(), (angle.sin() * scale).float()
         q = _turn_on_cpu(q, cos, sin, interleaved)
         return q if k is None else (q, _turn_on_cpu(k, cos, sin, interleaved))
-    if (q.shape[-2] + (0 if k is None else k.shape[-2])) * dim > 1 << 24 or seq >= 1 << 31:
+    if (q.shape[-2] + (0 if k is None else k.shape[-2])) * dim > _MAX_TOKEN or seq >= 1 << 31:
         raise ValueError("rotary: a token has more than 2^24 elements, or a sequence 2^31 tokens")
     out = _ext().rotary(q, k, freqs, positions, interleaved, scale)
     if out is None:
@@ -379,6 +379,6 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
         return (_activate_on_cpu(v @ w_gate.float().t(), activation) * (v @ w_up.float().t())).to(x.dtype)
     if x.dtype is torch.float32:
         raise TypeError("gated_linear: float32 is taken on the CPU only; the tensor cores multiply float16 and bfloat16")
-    if max(x.numel() // width, width, ffn) >= 1 << 30:
+    if max(x.numel() // width, width, ffn) >= _MAX_DIMENSION:
         raise ValueError("gated_linear: a dimension of 2^30 or more")
     _refuse("gated_linear")

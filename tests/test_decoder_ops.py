@@ -51,6 +51,15 @@ def test_early_launched_kernels_promise_nothing_about_their_inputs():
     assert gemm.index("wait_for_stream()") < gemm.index("load(to_a")
 
 
+def test_limits_are_those_of_the_entry_points():
+    import os
+    import re
+    from dccl_b200.ops import decoder
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc", "decoder", "decoder_ops.hpp")).read()
+    limits = {k: eval(v) for k, v in re.findall(r"DCCL_(\w+_MAX_\w+) = ([0-9 <]+)", text)}
+    assert limits == {"NORM_MAX_WIDTH": decoder._MAX_WIDTH, "ROTARY_MAX_PAIRS": decoder._MAX_PAIRS, "ROTARY_MAX_TOKEN": decoder._MAX_TOKEN, "GATED_MAX_DIMENSION": decoder._MAX_DIMENSION}
+
+
 # ---------------------------------------------------------------------------------------------- norms
 
 def norm_case(shape, dtype, post, gate, wide, seed=0, device="cpu"):
