@@ -106,6 +106,9 @@ Tensor dense(const Tensor& t) {
     return v.is_contiguous() ? v : v.contiguous();
 }
 
+/** What a node saved, as the kernels read it: hooks may hand back a copy that lies otherwise in memory. */
+Tensor unpacked(const SavedVariable& v) { return dense(v.unpack()); }
+
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
 
@@ -186,7 +189,7 @@ struct NormBackward : public Node {
     bool has_branch = false, own_branch = false;      // own_branch: its gradient is not that of x
 
     variable_list apply(variable_list&& grads) override {
-        const Tensor x_ = x.unpack(), b = branch.unpack(), w = weight.unpack(), p = post.unpack(), g = gate.unpack(), ry = rstd.unpack(), rb = rstd_post.unpack();
+        const Tensor x_ = unpacked(x), b = unpacked(branch), w = unpacked(weight), p = unpacked(post), g = unpacked(gate), ry = unpacked(rstd), rb = unpacked(rstd_post);
         const Tensor dy = has_branch ? dense(grads[0]) : Tensor(), dn = dense(grads[has_branch ? 1 : 0]);
         variable_list out(5);
         if (!dy.defined() && !dn.defined()) return out;
@@ -325,7 +328,7 @@ struct RotaryBackward : public Node {
 
     variable_list apply(variable_list&& grads) override {
         Turn t = turn;
-        t.freqs = freqs.unpack();
+        t.freqs = unpacked(freqs);
         t.positions = positions.unpack();
         const Tensor dq = task_should_compute_output(0) ? dense_head(grads[0]) : Tensor(), dk = has_k && task_should_compute_output(1) ? dense_head(grads[1]) : Tensor();
         variable_list out(2);
@@ -401,6 +404,8 @@ bool gated_aligned(const Tensor& x, const Tensor& w_gate, const Tensor& w_up) {
     return ((uintptr_t)x.data_ptr() | (uintptr_t)w_gate.data_ptr() | (uintptr_t)w_up.data_ptr()) % 16 == 0;
 }
 
+Tensor on_16_bytes(const Tensor& t) { return t.defined() && (uintptr_t)t.data_ptr() % 16 ? t.clone() : t; }
+
 /** The workspace of a call; undefined where it needs none. */
 Tensor gated_work(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, bool backward) {
     const long long bytes = entry.gated_workspace(x.device().index(), x.numel() / x.size(-1), x.size(-1), w_gate.size(0), gated_aligned(x, w_gate, w_up), backward);
@@ -413,9 +418,11 @@ struct GatedBackward : public Node {
     int act = 0;
 
     variable_list apply(variable_list&& grads) override {
-        const Tensor x_ = x.unpack(), wg = w_gate.unpack(), wu = w_up.unpack(), g = gate.unpack(), u = up.unpack(), copies = padded.unpack(), dh = dense(grads[0]);
+        Tensor x_ = unpacked(x), wg = unpacked(w_gate), wu = unpacked(w_up);
+        const Tensor g = on_16_bytes(unpacked(gate)), u = on_16_bytes(unpacked(up)), copies = on_16_bytes(unpacked(padded)), dh = dense(grads[0]);
         variable_list out(3);
         if (!dh.defined()) return out;
+        if (!copies.defined()) x_ = on_16_bytes(x_), wg = on_16_bytes(wg), wu = on_16_bytes(wu);      // so the forward pass had them
         const bool weights = task_should_compute_output(1) || task_should_compute_output(2);
         const Tensor dx = task_should_compute_output(0) ? fresh_like(x_) : Tensor();
         const Tensor dg = weights ? fresh_like(wg) : Tensor(), du = weights ? fresh_like(wu) : Tensor();
