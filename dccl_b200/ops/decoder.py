@@ -280,9 +280,11 @@ def rotary(q, k, freqs, positions=None, interleaved=False, scale=1.0):
         raise TypeError("rotary: positions is None, an integer or a tensor of integers")
     elif not -2 ** 62 < positions < 2 ** 62:
         raise ValueError("rotary: position %d" % positions)
+    else:
+        positions = int(positions)
     scale, interleaved = float(scale), bool(interleaved)
     if not q.is_cuda:
-        at = positions if isinstance(positions, torch.Tensor) else torch.arange(positions, positions + seq)
+        at = positions if isinstance(positions, torch.Tensor) else torch.arange(positions, positions + seq, device=q.device)
         angle = (at.double().unsqueeze(-1) * freqs).unsqueeze(-2)
         cos, sin = (angle.cos() * scale).float(), (angle.sin() * scale).float()
         q = _turn_on_cpu(q, cos, sin, interleaved)

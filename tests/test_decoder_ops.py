@@ -1371,3 +1371,18 @@ def test_saved_tensors_may_come_back_from_elsewhere(how):
     # the norms' sums of a row of 64 fp32 terms have another order where a row starts elsewhere: a few steps of 2^-24 of terms of up to about ten
     for a, b in zip(plain, got):
         assert torch.equal(a, b) if a.dtype is torch.bfloat16 else torch.allclose(a, b, rtol=1e-4, atol=1e-4)
+
+
+def test_rotary_on_cpu_while_another_device_is_the_default():
+    q, freqs = torch.randn(1, 3, 2, 8), ops.rotary_frequencies(8)
+    want = ops.rotary(q, None, freqs, 5)
+    with torch.device("meta"):
+        assert torch.equal(ops.rotary(q, None, freqs, 5), want)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_rotary_takes_integers_of_other_classes(device):
+    import enum
+    first = enum.IntEnum("first", {"five": 5}).five
+    q, freqs = torch.randn(1, 3, 2, 8, device=device), ops.rotary_frequencies(8, device=device)
+    assert torch.equal(ops.rotary(q, None, freqs, first), ops.rotary(q, None, freqs, 5))
