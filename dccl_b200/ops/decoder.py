@@ -11,11 +11,13 @@
     gated_linear          act(x Wg^T) * (x Wu^T): the two projections of a gated feed-forward layer
     ====================  ==============================================================================
 
-All are differentiable. CUDA tensors run one kernel per call on the current stream of their device (csrc/decoder/residual_norm.cu,
-rotary.cu, gated_linear.cu) in float16, bfloat16 or float32 (gated_linear: not float32); sums and statistics are fp32 and every result is rounded once. CPU tensors take
-the same formulas in torch, so the same model code is tested without a GPU. Inputs may have any strides; what a kernel cannot
-read in place is copied first. A call allocates its outputs and its workspace from torch's allocator and nothing else, so it can be
-captured into a graph; a gradient has the same bits whenever its inputs do (no atomics).
+All are differentiable. CUDA tensors run kernels on the current stream of their device (csrc/decoder/residual_norm.cu, rotary.cu,
+gated_linear.cu) in float16, bfloat16 or float32 (gated_linear: not float32): one for a call, of gated_linear up to three (rows that do not start
+on 16 bytes are copied, and parts of a sum joined), and in the backward pass two at most for a norm, one for rotary and two to five for gated_linear. Sums and
+statistics are fp32 and every result is rounded once. CPU tensors take the same formulas in torch, so the same model code is tested without a
+GPU. Inputs may have any strides; what a kernel cannot read in place is copied first. A call allocates its outputs and its workspace from
+torch's allocator and nothing else, so it can be captured into a graph. There are no atomics: the order of a sum depends on sizes and, in a
+norm, on whether rows start on 16 bytes, so the same inputs in memory that lies alike give the same bits.
 
 Under a mode of torch's (other than the one behind ``torch.device``), a tracer, or with a subclass of Tensor, the same kernels run as operators
 of torch's dispatcher (``torch.ops.dccl``), which those see and record. Fake and transformed tensors are refused.
@@ -305,8 +307,8 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling=None, factor=1.0, orig
     ``"theta"``    theta grows so that the slowest pair is divided by the factor and the fastest is kept
     ``"turns"``    pairs that turn less than `slow` times in the original length are divided by the factor, those above `fast` (4) kept, and
                    between the two the frequency is mixed in proportion to the turns
-    ``"yarn"``     the same, mixed in proportion to the index of the pair between those that turn `fast` (32) and `slow` times; it goes
-                   with ``scale=0.1 * log(factor) + 1`` in ``rotary``"""
+    ``"yarn"``     the same, mixed in proportion to the index of the pair between those that turn `fast` (32) and `slow` times (Peng et al.,
+                   "YaRN: Efficient Context Window Extension of Large Language Models", 2023); it goes with ``scale=0.1 * log(factor) + 1`` in ``rotary``"""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_frequencies: rotary_dim is even, at least 2")
     if factor < 1 or theta <= 1:
@@ -357,8 +359,9 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     "gelu_tanh". Both products stay in fp32 up to the one rounding of the result.
 
     On the GPU x is float16 or bfloat16. The gradients of the two products are rounded to that type once, to be multiplied again: in float16
-    they overflow above 65504. For the backward pass the call keeps the two products in fp32 (8 bytes per element of the result):
-    from 16 bits their rounding would come on top of the one that their gradients need to be multiplied again."""
+    they overflow above 65504, and dx and the weights' gradients are 1.4 times as far off as their own rounding alone would put them. For the
+    backward pass the call keeps the two products in fp32 (8 bytes per element of the result): from 16 bits their rounding would come on top of
+    the one that their gradients need. A product that does not end in time (nine seconds) leaves NaN, and the next call on its device raises."""
     if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(activation, str):
         h = _ext().gated_linear(x, w_gate, w_up, _ACTIVATIONS.get(activation, -1))
         if h is None:
