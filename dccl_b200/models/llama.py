@@ -97,7 +97,8 @@ class Attention(nn.Module):
 
     def fused(self, x, at):
         b, s, _ = x.shape
-        return self.o(attend(self.q(x).view(b, s, self.h, self.hd), self.k(x).view(b, s, self.kv, self.hd), self.v(x).view(b, s, self.kv, self.hd), at))
+        return self.o(attend(self.q(x).view(b, s, self.h, self.hd), self.k(x).view(b, s, self.kv, self.hd), self.v(x).view(b, s, self.kv, self.hd), at,
+                             self.kv != self.h))
 
 
 # ---- the fused form. Every operator stands for modules that are then not called, so each use asks first whether calling them would do more.
@@ -126,13 +127,14 @@ class Positions:
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def attend(q, k, v, at):
-    """Causal attention of [batch, seq, heads, head dim], whose queries and keys are turned by their positions first: [batch, seq, heads * head dim]."""
+def attend(q, k, v, at, grouped):
+    """Causal attention of [batch, seq, heads, head dim], whose queries and keys are turned by their positions first: [batch, seq, heads * head dim].
+    grouped: k and v have fewer heads."""
     if q.dtype in _TYPES:
         q, k = ops.rotary(q, k, at.freqs)
     else:
         q, k = (apply_rope(t.transpose(1, 2), *at.tables).transpose(1, 2) for t in (q, k))
-    out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=q.shape[2] != k.shape[2])
+    out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=grouped)
     return out.transpose(1, 2).flatten(2)
 
 

@@ -65,7 +65,7 @@ class ShardedAttention(nn.Module):
         return self._leave(out.transpose(1, 2).reshape(q.shape[0], q.shape[2], self.h * self.hd))
 
     def fused(self, x, at):
-        return self._leave(attend(*self._project(x), at))
+        return self._leave(attend(*self._project(x), at, self.kv != self.h))
 
     def _leave(self, out):
         if self.sp:      # sum the partial products and keep this rank's part of the sequence (backward: all-gather)

@@ -1293,6 +1293,15 @@ def test_tracers_record_the_operators(tracer):
 
 
 @gpu
+def test_a_traced_decoder_reads_its_tokens():
+    _, fused, tokens = decoders("cuda", torch.bfloat16)
+    fused.requires_grad_(False)
+    traced = torch.jit.trace(fused, (tokens,))
+    other = tokens.flip(0, 1)
+    assert torch.equal(traced(other), fused(other)) and not torch.equal(fused(other), fused(tokens))
+
+
+@gpu
 def test_subclasses_of_tensor_see_the_operators():
     class Plain(torch.Tensor):
         pass
