@@ -26,6 +26,7 @@ The original has no such operators: its API ends at the collectives (reference i
 """
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -59,7 +60,7 @@ def _ext():
 _SCHEMAS = {"residual_norm": "Tensor x, Tensor? branch, Tensor weight, float eps, Tensor? post_weight, Tensor? gate, float scale",
             "rotary": "Tensor q, Tensor? k, Tensor freqs, Tensor? positions, int first, bool interleaved, float scale",
             "gated_linear": "Tensor x, Tensor w_gate, Tensor w_up, int activation"}
-_registered = {}
+_registered, _registering = {}, threading.Lock()
 
 
 def _run(name, args):
@@ -117,8 +118,9 @@ def _observed(name, *args):
     if name == "rotary":
         q, k, freqs, positions, interleaved, scale = args
         args = (q, k, freqs) + ((positions, 0) if isinstance(positions, torch.Tensor) else (None, positions)) + (interleaved, float(scale))
-    if name not in _registered:
-        _registered[name] = _register(name)
+    with _registering:
+        if name not in _registered:
+            _registered[name] = _register(name)
     out = _registered[name](*args)
     return out[0] if len(out) == 1 else tuple(out)
 

@@ -1302,6 +1302,31 @@ def test_a_traced_decoder_reads_its_tokens():
 
 
 @gpu
+def test_the_first_observed_calls_of_a_process_may_come_from_two_threads():
+    import os
+    import subprocess
+    import sys
+    code = """
+import threading, torch
+from dccl_b200 import ops
+from torch.utils.flop_counter import FlopCounterMode
+x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+want, got, start = ops.rms_norm(x, w), [], threading.Barrier(4)
+def call():
+    start.wait()
+    with FlopCounterMode(display=False):
+        got.append(ops.rms_norm(x, w))
+threads = [threading.Thread(target=call) for _ in range(4)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert len(got) == 4 and all(torch.equal(g, want) for g in got)
+print("OK")
+"""
+    res = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip().endswith("OK"), res.stdout + res.stderr[-2000:]
+
+
+@gpu
 def test_subclasses_of_tensor_see_the_operators():
     class Plain(torch.Tensor):
         pass
