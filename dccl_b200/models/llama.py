@@ -9,7 +9,7 @@ the "no library GEMM" rule of this project applies to the communication paths, n
 With ``LlamaConfig(fused=True)`` the same modules compute with the operators of ``dccl_b200.ops.decoder``: each residual add in one pass with
 the norm after it, rotary positions of queries and keys in one launch, and the gated projections as one product (parameters and state
 dict stay the same). A module that is more than what stands here (another one put in its place, a bias, hooks) is called, and so is what an
-operator does not take (the gated projections in float32 on the GPU or under autocast); the others around it stay fused.
+operator does not take (the gated projections in float32 on the GPU or under autocast, fake and transformed tensors); the others around it stay fused.
 """
 import functools
 from dataclasses import dataclass
@@ -127,10 +127,15 @@ class Positions:
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def taken(x):
+    """Whether x is a tensor that the operators take: of their types and devices, with values of its own."""
+    return x.dtype in _TYPES and x.device.type in ("cpu", "cuda") and type(x) in (torch.Tensor, nn.Parameter) and not torch._C._functorch.is_functorch_wrapped_tensor(x)
+
+
 def attend(q, k, v, at, grouped):
     """Causal attention of [batch, seq, heads, head dim], whose queries and keys are turned by their positions first: [batch, seq, heads * head dim].
     grouped: k and v have fewer heads."""
-    if q.dtype in _TYPES:
+    if taken(q):
         q, k = ops.rotary(q, k, at.freqs)
     else:
         q, k = (apply_rope(t.transpose(1, 2), *at.tables).transpose(1, 2) for t in (q, k))
@@ -143,7 +148,7 @@ def attention(module, n, at, kind):
 
 
 def gated(n, gate, up):
-    if (untouched(gate, nn.Linear) and untouched(up, nn.Linear) and n.dtype in _TYPES[:3 - n.is_cuda] and gate.weight.dtype == up.weight.dtype == n.dtype
+    if (untouched(gate, nn.Linear) and untouched(up, nn.Linear) and taken(n) and n.dtype in _TYPES[:3 - n.is_cuda] and gate.weight.dtype == up.weight.dtype == n.dtype
             and not torch.is_autocast_enabled(n.device.type)):
         return ops.gated_linear(n, gate.weight, up.weight)
     return F.silu(gate(n)) * up(n)
@@ -151,7 +156,7 @@ def gated(n, gate, up):
 
 def norms(norm, x):
     """Whether the operators compute what `norm` does with x."""
-    return untouched(norm, RMSNorm) and x.dtype in _TYPES and norm.weight.dtype in (x.dtype, torch.float32)
+    return untouched(norm, RMSNorm) and taken(x) and norm.weight.dtype in (x.dtype, torch.float32)
 
 
 def norm_of(x, norm):

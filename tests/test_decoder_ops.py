@@ -980,6 +980,49 @@ def test_norms_of_another_type_in_the_fused_decoder(norms, model):
     assert abs(a - b) <= 2.0 ** -7 * abs(a)
 
 
+@pytest.mark.parametrize("device", ["cpu", "meta", pytest.param("cuda", marks=gpu)])
+def test_the_fused_decoder_of_tensors_without_values(device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    plain, fused, tokens = decoders("cpu", torch.bfloat16)
+    if device == "meta":
+        logits = [m.to("meta")(tokens.to("meta")) for m in (plain, fused)]
+    else:
+        from dccl_b200.models.llama import LlamaDecoder
+        torch.set_default_dtype(torch.bfloat16)
+        try:
+            with FakeTensorMode(), torch.device(device):
+                logits = [LlamaDecoder(m.cfg)(torch.zeros(3, 33, dtype=torch.int64)) for m in (plain, fused)]
+        finally:
+            torch.set_default_dtype(torch.float32)
+    assert logits[0].shape == logits[1].shape and logits[1].device.type == device
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_the_fused_decoder_under_transforms(device):
+    """torch.func.grad, and functions of parameters: bounds of test_the_fused_decoder_is_the_same_model."""
+    plain, fused, tokens = decoders(device, torch.float32)
+    grads = []
+    for m in (plain, fused):
+        params = {k: v.detach() for k, v in m.named_parameters()}
+        grads.append(torch.func.grad(lambda p: torch.nn.functional.cross_entropy(torch.func.functional_call(m, p, (tokens[:, :-1],)).flatten(0, 1), tokens[:, 1:].flatten()))(params))
+    for k, g in grads[0].items():
+        assert (g - grads[1][k]).abs().max() <= 3e-5 * g.abs().max() + 1e-7, k
+
+
+@gpu
+def test_the_fused_decoder_compiled():
+    _, fused, tokens = decoders("cuda", torch.bfloat16)
+    want = fused.loss(tokens)
+    want.backward()
+    grads = {k: p.grad.clone() for k, p in fused.named_parameters()}
+    fused.zero_grad(set_to_none=True)
+    loss = torch.compile(fused.loss, backend="eager")(tokens)
+    loss.backward()
+    assert torch.equal(loss, want)
+    for k, p in fused.named_parameters():        # the gradient of attention may add in another order from call to call: two steps of bf16
+        assert (p.grad.double() - grads[k].double()).norm() <= 2.0 ** -6 * grads[k].double().norm(), k
+
+
 @gpu
 def test_the_fused_decoder_on_the_gpu():
     """bf16 on the GPU against the same operators on the CPU: about thirty bf16 results on the way to the loss and as many back, each off by
