@@ -12,10 +12,9 @@
 #include "decoder_ops.hpp"
 #include "../kernels/launch_early.cuh"
 #include "row_access.cuh"
-#include "../device/tcgen05.cuh"
-#include "../gpu/driver_api.hpp"
+#include "activation.cuh"
+#include "products.cuh"
 #include "gated_tiles.hpp"
-#include <cstring>
 
 namespace dccl {
 
@@ -30,82 +29,6 @@ struct GemmArgs : Tiling, Results {
     int act;
     int* gave_up;                   // host memory: a wait that did not end
 };
-
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
-
-constexpr float kTanhScale = 1.5957691216057308f, kTanhCubic = 0.044715f;      // 2 sqrt(2 / pi)
-
-/** 0.5 g (1 + tanh(z)) = g sigmoid(2 z). */
-template <int ACT> __device__ __forceinline__ float activate(float g) {
-    if constexpr (ACT == DCCL_ACT_SILU) return g * sigmoid(g);
-    else if constexpr (ACT == DCCL_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-    else return g * sigmoid(kTanhScale * fmaf(kTanhCubic * g * g, g, g));
-}
-
-/** The activation and its derivative. */
-template <int ACT> __device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
-    if constexpr (ACT == DCCL_ACT_SILU) {
-        const float s = sigmoid(g);
-        a = g * s;
-        da = s * fmaf(g, 1.0f - s, 1.0f);
-    } else if constexpr (ACT == DCCL_ACT_GELU) {
-        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-        a = g * cdf;
-        da = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), cdf);
-    } else {
-        const float s = sigmoid(kTanhScale * fmaf(kTanhCubic * g * g, g, g));
-        a = g * s;
-        da = fmaf(g * s * (1.0f - s), kTanhScale * fmaf(3.0f * kTanhCubic * g, g, 1.0f), s);
-    }
-}
-
-/** f with the activation as a constant: one choice for many elements. */
-template <typename F> __device__ __forceinline__ void with_activation(int act, F&& f) {
-    if (act == DCCL_ACT_SILU) f(std::integral_constant<int, DCCL_ACT_SILU>{});
-    else if (act == DCCL_ACT_GELU) f(std::integral_constant<int, DCCL_ACT_GELU>{});
-    else f(std::integral_constant<int, DCCL_ACT_GELU_TANH>{});
-}
-
-/** Rows of a tile's 32 columns pass through shared memory, so that a warp stores whole rows and not one line per lane. `stage`: 4 KB of
- *  this warp, 16-byte pieces of row r at piece ^ (r % 8). */
-__device__ __forceinline__ void stage_rows(char* stage, const float (&v)[32]) {
-    const int lane = threadIdx.x % 32;
-    __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 8; c++)
-        *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-    __syncwarp();
-}
-/** Stores the staged 32 x 32 values as fp32 at `to` (row 0, column 0), rows < rows and columns < columns. Rows start on 16 bytes. */
-__device__ __forceinline__ void store_fp32(const char* stage, float* to, size_t stride, int rows, int columns) {
-    const int lane = threadIdx.x % 32, c = lane % 8;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int r = i * 4 + lane / 8;
-        const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((c ^ (r & 7)) * 16));
-        if (r < rows && 4 * c < columns) *reinterpret_cast<float4*>(to + (size_t)r * stride + 4 * c) = v;      // up to three of the padding
-    }
-}
-/** The same as T, whose rows may start anywhere. */
-template <typename T> __device__ __forceinline__ void store_as(const char* stage, T* to, size_t stride, int rows, int columns, bool vec) {
-    const int lane = threadIdx.x % 32;
-    if (vec) {
-        const int c = lane % 4;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + lane / 4;
-            const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + (((2 * c) ^ (r & 7)) * 16));
-            const float4 w = *reinterpret_cast<const float4*>(stage + r * 128 + (((2 * c + 1) ^ (r & 7)) * 16));
-            Run<T, 8> o = {Traits<T>::down(v.x), Traits<T>::down(v.y), Traits<T>::down(v.z), Traits<T>::down(v.w),
-                           Traits<T>::down(w.x), Traits<T>::down(w.y), Traits<T>::down(w.z), Traits<T>::down(w.w)};
-            if (r < rows && 8 * c < columns) st_run<T, 8>(to + (size_t)r * stride + 8 * c, o);
-        }
-    } else if (lane < columns) {
-#pragma unroll 4
-        for (int r = 0; r < rows && r < 32; r++)
-            to[(size_t)r * stride + lane] = Traits<T>::down(*reinterpret_cast<const float*>(stage + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
-    }
-}
 
 template <int FORM, int N, bool PAIR> struct GemmShape {
     static constexpr int kRows = PAIR ? 2 * kTileM : kTileM, kHeldN = PAIR ? N / 2 : N;      // rows of a tile; columns whose operand one CTA holds
@@ -558,32 +481,6 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) k_gate_gr
 
 /* ------------------------------------------------------------------------------------------------ host side */
 
-/** Set by a kernel whose wait ran out, which leaves NaN in what it was to store; looked at by the next call on the device. Host memory that the device
- *  writes, for the life of the process. */
-static int* gave_up_flag(int device) {
-    static int* const flags = [] {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaThreadExchangeStreamCaptureMode(&mode);       // a first call may come while a stream is being captured
-        void* p = nullptr;
-        if (cudaHostAlloc(&p, 64 * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { cudaGetLastError(); p = nullptr; }
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        if (p) memset(p, 0, 64 * sizeof(int));
-        return reinterpret_cast<int*>(p);
-    }();
-    return flags ? flags + device : nullptr;        // of the 64 devices that sm_count knows
-}
-
-/** The two dimensions of an operand by which one is contiguous, and the box of it. */
-static cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, size_t inner, size_t outer, size_t stride, unsigned box_outer) {
-    const DriverApi* d = driver_api(nullptr);
-    if (!d || !d->TensorMapEncodeTiled) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {inner, outer}, strides[1] = {stride * 2};
-    const cuuint32_t box[2] = {64, box_outer}, steps[2] = {1, 1};
-    const CUresult r = d->TensorMapEncodeTiled(map, dtype == 6 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
-                                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
 template <typename T, int FORM, int N, bool PAIR> static cudaError_t run_gemm(int device, const GemmPlan& p, GemmArgs& a, cudaStream_t stream) {
     using Shape = GemmShape<FORM, N, PAIR>;
     void (*const kernel)(const GemmArgs) = PAIR ? k_gemm_pair<T, FORM, N> : k_gemm<T, FORM, N>;
@@ -752,13 +649,6 @@ template <typename T> static cudaError_t gated_backward(int device, int dtype, c
         e = run_gemm<T, WEIGHT_GRAD>(device, l.weight, a, stream);
     }
     return e;
-}
-
-static bool gave_up(const char* who, int device) {
-    const int* flag = gave_up_flag(device);
-    if (!flag || !*reinterpret_cast<const volatile int*>(flag)) return false;
-    fprintf(stderr, "%s: an earlier product of this process on device %d did not end in time; what it did not finish is NaN, and no other is started there\n", who, device);
-    return true;
 }
 
 } // namespace dccl

@@ -26,11 +26,11 @@ The original has no such operators: its API ends at the collectives (reference i
 """
 import ctypes
 import math
-import threading
 
 import torch
 
 from .._lib import lib
+from . import _registered
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 # as csrc/decoder/decoder_ops.hpp has them
@@ -60,7 +60,6 @@ def _ext():
 _SCHEMAS = {"residual_norm": "Tensor x, Tensor? branch, Tensor weight, float eps, Tensor? post_weight, Tensor? gate, float scale",
             "rotary": "Tensor q, Tensor? k, Tensor freqs, Tensor? positions, int first, bool interleaved, float scale",
             "gated_linear": "Tensor x, Tensor w_gate, Tensor w_up, int activation"}
-_registered, _registering = {}, threading.Lock()
 
 
 def _run(name, args):
@@ -74,55 +73,12 @@ def _run(name, args):
     return list(out) if isinstance(out, tuple) else [out]
 
 
-def _register(name):
-    """`name` as an operator of torch's dispatcher, dccl::name, and its gradient as another, so that modes see them and tracers record them. The
-    gradient runs the forward pass again: what that keeps is not among the results that a tracer could hand over."""
-    def forward(*args):
-        with torch._C.DisableTorchFunction(), torch.no_grad():
-            return _run(name, args)
-
-    def backward(grads, *rest):
-        *args, needed = rest
-        with torch._C.DisableTorchFunction(), torch.enable_grad():
-            args = [a.detach().contiguous().requires_grad_(n) if isinstance(a, torch.Tensor) else a for a, n in zip(args, needed)]
-            outs = [(o, g) for o, g in zip(_run(name, args), grads) if g is not None]
-            leaves = [a for a, n in zip(args, needed) if n]
-            found, seen = torch.autograd.grad([o for o, _ in outs], leaves, [g for _, g in outs], allow_unused=True), []
-            for leaf, g in zip(leaves, found):      # results of an operator are tensors of their own
-                seen.append(torch.zeros_like(leaf) if g is None else g.clone() if any(g is s for s in seen) else g)
-            return seen
-
-    run = torch.library.custom_op("dccl::" + name, forward, mutates_args=(), device_types="cuda", schema="(%s) -> Tensor[]" % _SCHEMAS[name])
-    run_back = torch.library.custom_op("dccl::%s_backward" % name, backward, mutates_args=(), device_types="cuda",
-                                       schema="(Tensor?[] grads, %s, bool[] needed) -> Tensor[]" % _SCHEMAS[name])
-
-    def setup(ctx, inputs, output):
-        ctx.set_materialize_grads(False)
-        ctx.others = [None if isinstance(a, torch.Tensor) else (a,) for a in inputs]
-        ctx.save_for_backward(*(a for a in inputs if isinstance(a, torch.Tensor)))
-
-    def gradients(ctx, grads):
-        needed = list(ctx.needs_input_grad)
-        if all(g is None for g in grads) or not any(needed):
-            return (None,) * len(needed)
-        tensors = iter(ctx.saved_tensors)
-        found = iter(run_back(list(grads), *(next(tensors) if o is None else o[0] for o in ctx.others), needed))
-        return tuple(next(found) if n else None for n in needed)
-
-    run.register_autograd(gradients, setup_context=setup)
-    return run
-
-
 def _observed(name, *args):
     """The call through torch's dispatcher, which tells whoever follows it."""
     if name == "rotary":
         q, k, freqs, positions, interleaved, scale = args
         args = (q, k, freqs) + ((positions, 0) if isinstance(positions, torch.Tensor) else (None, positions)) + (interleaved, float(scale))
-    with _registering:
-        if name not in _registered:
-            _registered[name] = _register(name)
-    out = _registered[name](*args)
-    return out[0] if len(out) == 1 else tuple(out)
+    return _registered.call(name, _SCHEMAS[name], _run, args)
 
 
 def _refuse(what):
