@@ -1,0 +1,5 @@
+#pragma once
+#include <torch/python.h>
+
+/** Adds the operators of dccl_b200/ops/gradients.py to the extension module; 0, or -1 with a Python error set. */
+int add_gradient_ops(PyObject* module);

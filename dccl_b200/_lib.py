@@ -116,6 +116,20 @@ def _declare(lib):
         "dccl_gated_linear": (i, [i, i, sz, sz, sz, vp, vp, vp, i, vp, vp, vp, sz, vp, c.c_longlong, vp]),
         "dccl_gated_linear_pads": (i, [sz, i]),
         "dccl_gated_linear_backward": (i, [i, i, sz, sz, sz, vp, vp, vp, sz, vp, vp, vp, vp, i, vp, vp, vp, vp, c.c_longlong, vp]),
+        "dccl_route": (i, [i, i, sz, i] + [vp] * 6),
+        "dccl_route_backward": (i, [i, i, sz, i] + [vp] * 6),
+        "dccl_expert_plan": (i, [i, sz, i, vp, i, vp, vp, vp, vp]),
+        "dccl_dispatch": (i, [i, i, sz, i, sz] + [vp] * 5),
+        "dccl_combine": (i, [i, i, sz, i, sz, vp, vp, vp, i, vp, vp]),
+        "dccl_combine_backward": (i, [i, i, sz, i, sz] + [vp] * 5 + [i, vp, vp, vp]),
+        "dccl_expert_linear_workspace": (c.c_longlong, [i, sz, i, sz, sz, i, i]),
+        "dccl_expert_linear_pads": (i, [sz, i]),
+        "dccl_expert_linear": (i, [i, i, sz, i, sz, sz, vp, vp, vp, i, vp, vp, sz, vp, c.c_longlong, vp]),
+        "dccl_expert_linear_backward": (i, [i, i, sz, i, sz, sz, vp, vp, sz, vp, vp, vp, vp, i, vp, vp, vp, c.c_longlong, vp]),
+        "dccl_grad_parts": (sz, [i, sz, vp]),
+        "dccl_grad_squares": (i, [i, sz, vp, vp, vp]),
+        "dccl_grad_total": (i, [i, vp, sz, vp, vp, vp]),
+        "dccl_grad_clip": (i, [i, sz, vp, vp, sz, c.c_double, vp, vp]),
         "dccl_emu_early_producer": (i, [vp, vp, sz, c.c_uint, vp, vp]),
         "dccl_emu_early_observer": (i, [vp, vp]),
         "dccl_debug_bounds_build": (i, []),

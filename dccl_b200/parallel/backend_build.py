@@ -1,4 +1,4 @@
-"""Builds the PyTorch extension (csrc/torch: the process-group backend and the host side of the AdamW update and of the decoder operators) in-tree, next to
+"""Builds the PyTorch extension (csrc/torch: the process-group backend and the host side of the AdamW update and of the operators of models) in-tree, next to
 libdccl.so, and loads it.
 
 The extension only uses the library's public C++ API and libtorch; it is compiled with the system
@@ -20,9 +20,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _PKG = os.path.dirname(_HERE)
 _ROOT = os.path.dirname(_PKG)
 SRC_DIR = os.path.join(_ROOT, "csrc", "torch")
-SRCS = [os.path.join(SRC_DIR, name) for name in ("pg_dccl.cpp", "adamw_step.cpp", "decoder_ops.cpp")]
-HEADERS = [os.path.join(SRC_DIR, name) for name in ("adamw_step.hpp", "decoder_ops.hpp")]
-HEADERS += [os.path.join(_ROOT, "csrc", "kernels", "adamw.hpp"), os.path.join(_ROOT, "csrc", "decoder", "decoder_ops.hpp")] + [os.path.join(_ROOT, "include", "dccl", "dccl.hpp")]
+SRCS = [os.path.join(SRC_DIR, name) for name in ("pg_dccl.cpp", "adamw_step.cpp", "decoder_ops.cpp", "expert_ops.cpp", "gradient_ops.cpp")]
+HEADERS = [os.path.join(SRC_DIR, name) for name in ("adamw_step.hpp", "decoder_ops.hpp", "expert_ops.hpp", "gradient_ops.hpp", "tensor_args.hpp")]
+HEADERS += [os.path.join(_ROOT, "csrc", *name) for name in (("kernels", "adamw.hpp"), ("decoder", "decoder_ops.hpp"), ("experts", "expert_ops.hpp"), ("gradients", "grad_norm.hpp"))]
+HEADERS += [os.path.join(_ROOT, "include", "dccl", "dccl.hpp")]
 OUT = os.path.join(_PKG, "lib", "_dccl_torch-%s-torch%s.so" % (sys.implementation.cache_tag, torch.__version__))
 
 

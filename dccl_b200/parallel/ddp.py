@@ -19,6 +19,7 @@ Two ways in:
 import torch
 
 from ..comm import Communicator
+from ..ops.gradients import clip_grad_norm
 
 
 class GradientAllReducer:
@@ -103,6 +104,11 @@ class GradientAllReducer:
                 b["event"] = None
             b["pending"] = len(b["params"])
             b["launched"] = False
+
+    def clip(self, max_norm):
+        """Call after ``finish``: cuts all gradients back to the norm `max_norm`, in their buckets, and returns the norm before (a float32 tensor on their device). Every
+        rank has the same reduced gradients, so nothing is exchanged."""
+        return clip_grad_norm([b["buffer"] for b in self.buckets], max_norm)
 
     def zero_grad(self):
         """Zero all gradients with one fill per bucket (instead of one per parameter)."""

@@ -9,6 +9,15 @@ with the counts swapped.
     moe = ExpertParallelMLP(d_model, d_hidden, num_experts, comm)
     y = moe(x)                         # x, y: [tokens on this rank, d_model]
 
+With ``fused=True`` the layer computes with the operators of ``dccl_b200.ops.experts``: any number of experts for a token, chosen and weighted as ``ops.route``
+takes it, tokens put in the experts' order and added up by kernels, and one product for all experts of a rank instead of two for each segment::
+
+    moe = ExpertParallelMLP(d_model, d_hidden, num_experts, comm, dtype=torch.bfloat16, device="cuda", fused=True, top_k=8,
+                            routing=dict(scores="sigmoid", renormalize=True, scale=2.5))
+
+Its experts' weights are one parameter each for all experts of the rank (``w_in`` [experts, h, d], ``w_out`` [experts, d, h]); a state dict of either form loads
+into the other. One rank alone never reads anything back to the host, and can be captured into a graph.
+
 The router is replicated; its gradient on a rank covers that rank's tokens only and is summed with the other
 replicated parameters (``tensor_parallel.sync_replicated_grads``) when the ranks hold different tokens.
 """
@@ -16,6 +25,7 @@ import math
 
 import torch
 
+from ..ops import experts as ops
 from ..ops import functional as F
 
 
@@ -33,18 +43,28 @@ def router_weight(d_model, num_experts, seed, dtype=torch.float32, device="cpu")
 
 
 class ExpertParallelMLP(torch.nn.Module):
-    def __init__(self, d_model, d_hidden, num_experts, comm, seed=0, dtype=torch.float32, device="cpu"):
+    def __init__(self, d_model, d_hidden, num_experts, comm, seed=0, dtype=torch.float32, device="cpu", fused=False, top_k=1, routing=None):
+        """routing: keyword arguments of ``ops.route``; without it the weights are the softmax's, as they are without `fused`."""
         super().__init__()
         if num_experts % comm.world:
             raise ValueError("num_experts must split evenly over the ranks")
+        if not fused and (top_k != 1 or routing is not None):
+            raise ValueError("top_k and routing need fused=True")
         self.comm, self.num_experts, self.per = comm, num_experts, num_experts // comm.world
+        self.fused, self.top_k, self.routing = fused, top_k, dict(renormalize=False) if routing is None else dict(routing)
         self.router = torch.nn.Parameter(router_weight(d_model, num_experts, seed, dtype, device))
         first = comm.rank * self.per
         ws = [expert_weights(d_model, d_hidden, first + j, seed, dtype, device) for j in range(self.per)]
-        self.w_in = torch.nn.ParameterList([torch.nn.Parameter(w[0]) for w in ws])
-        self.w_out = torch.nn.ParameterList([torch.nn.Parameter(w[1]) for w in ws])
+        if fused:
+            self.w_in, self.w_out = (torch.nn.Parameter(torch.stack(w)) for w in zip(*ws))
+        else:
+            self.w_in = torch.nn.ParameterList([torch.nn.Parameter(w[0]) for w in ws])
+            self.w_out = torch.nn.ParameterList([torch.nn.Parameter(w[1]) for w in ws])
+        self.register_load_state_dict_pre_hook(_take_either_form)
 
     def forward(self, x):
+        if self.fused:
+            return self._forward_fused(x)
         comm, n, per, E = self.comm, self.comm.world, self.per, self.num_experts
         probs = torch.softmax(torch.nn.functional.linear(x, self.router), dim=-1)
         gate, top = probs.max(dim=-1)
@@ -68,3 +88,39 @@ class ExpertParallelMLP(torch.nn.Module):
         back = F.all_to_all(done, recv_counts, send_counts, comm)           # combine: the way they came
         y = torch.zeros_like(x)
         return y.index_add(0, order, back * gate[order].unsqueeze(-1))
+
+    def _forward_fused(self, x):
+        comm, n, per = self.comm, self.comm.world, self.per
+        weights, experts = ops.route(torch.nn.functional.linear(x, self.router), self.top_k, **self.routing)
+        plan = ops.expert_plan(experts, self.num_experts)
+        rows = ops.dispatch(x, plan)                            # in the order of the experts, hence of their ranks
+        if n == 1:
+            return ops.combine(self._experts(rows, plan), plan, weights)
+        incoming = torch.empty_like(plan.counts)
+        comm.all_to_all(plan.counts, incoming)                  # row p: what rank p sends to my experts
+        send_counts, recv_counts = (c.view(n, per).sum(1).tolist() for c in (plan.counts, incoming))
+        used = sum(send_counts)
+        got = F.all_to_all(rows[:used], send_counts, recv_counts, comm)         # dispatch: grouped by source, then by expert
+        of = torch.arange(per, device=x.device).repeat(n).repeat_interleave(incoming, output_size=sum(recv_counts))
+        mine = ops.expert_plan(of.unsqueeze(-1), per)
+        done = ops.combine(self._experts(ops.dispatch(got, mine), mine), mine)
+        back = F.all_to_all(done, recv_counts, send_counts, comm)               # combine: the way they came
+        return ops.combine(torch.nn.functional.pad(back, (0, 0, 0, rows.shape[0] - used)), plan, weights)
+
+    def _experts(self, rows, plan):
+        """Both products of every expert of this rank, for rows in their order."""
+        if rows.is_cuda and rows.dtype is torch.float32:        # which the tensor cores do not multiply
+            done = [torch.nn.functional.linear(torch.nn.functional.gelu(torch.nn.functional.linear(r, self.w_in[j])), self.w_out[j])
+                    for j, r in enumerate(rows[:int(plan.starts[-1])].split(plan.counts.tolist()))]
+            return torch.nn.functional.pad(torch.cat(done), (0, 0, 0, rows.shape[0] - sum(d.shape[0] for d in done)))
+        return ops.expert_linear(ops.expert_linear(rows, self.w_in, plan, activation="gelu"), self.w_out, plan)
+
+
+def _take_either_form(module, state, prefix, *_):
+    """Experts' weights in a list or in one tensor, as the module has them."""
+    for name in ("w_in", "w_out"):
+        one, each = prefix + name, ["%s%s.%d" % (prefix, name, j) for j in range(module.per)]
+        if module.fused and each[0] in state and all(k in state for k in each):
+            state[one] = torch.stack([state.pop(k) for k in each])
+        elif not module.fused and one in state:
+            state.update(zip(each, state.pop(one)))

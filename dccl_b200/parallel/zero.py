@@ -9,6 +9,7 @@ drop to 1/world per rank.
 
     params -> one flat buffer per dtype (padded to world x 16 bytes), ``p.data`` and ``p.grad`` are views
     step:    reduce_scatter(avg) flat_grad -> grad slice (fp32 copy when the parameters are 16-bit)
+             with max_norm: the slices cut back by the norm of all ranks' slices (dccl_b200.ops.gradients)
              inner optimizer on the master slice (fp32); AdamW runs as one kernel together with the casts on either side
              all_gather the updated slice (cast back) into the flat parameter buffer
 
@@ -29,6 +30,7 @@ from torch.utils._device import DeviceContext
 
 from .._lib import lib
 from ..comm import DcclError, current_stream_handle, dtype_of
+from ..ops.gradients import clip_grad_norm
 from . import backend_build
 
 _FUSED_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -131,14 +133,21 @@ def _a_mode_is_active():
 
 
 class ShardedOptimizer:
-    """optimizer_cls(params, **kwargs) is built over ONE tensor per dtype: this rank's fp32 master slice."""
+    """optimizer_cls(params, **kwargs) is built over ONE tensor per dtype: this rank's fp32 master slice. With `max_norm` a step first cuts the averaged
+    gradients back to that norm, over all parameters and ranks, and leaves the norm before in ``grad_norm`` (a float32 tensor on their device, which the host need not read)."""
 
-    def __init__(self, params, comm, optimizer_cls=torch.optim.AdamW, symmetric=True, **kwargs):
+    def __init__(self, params, comm, optimizer_cls=torch.optim.AdamW, symmetric=True, *, max_norm=None, **kwargs):
         self.comm = comm
+        self.max_norm, self.grad_norm = max_norm, None
         self._sym = []
         params = [p for p in params if p.requires_grad]
         if not params:
             raise ValueError("no trainable parameters")
+        if max_norm is not None:
+            if not float(max_norm) >= 0:
+                raise ValueError("max_norm is %r" % (max_norm,))
+            if len({p.device for p in params}) > 1:
+                raise ValueError("max_norm takes parameters of one device")
         n, r = comm.world, comm.rank
         self.groups = []
         by_dtype = {}
@@ -183,6 +192,8 @@ class ShardedOptimizer:
         if n > 1:
             for g in self.groups:
                 comm.reduce_scatter(g["grad"], g["grad_slice"], op="avg")
+        if self.max_norm is not None:
+            self.grad_norm = clip_grad_norm([g["grad_slice"] if n > 1 else g["grad"] for g in self.groups], self.max_norm, comm=comm if n > 1 else None)
         updates = self._adamw_updates()
         if updates is not None:
             self._adamw_range(updates)
