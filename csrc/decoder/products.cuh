@@ -40,9 +40,8 @@ template <typename T> __device__ __forceinline__ void store_as(const char* stage
             const int r = i * 8 + lane / 4;
             const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + (((2 * c) ^ (r & 7)) * 16));
             const float4 w = *reinterpret_cast<const float4*>(stage + r * 128 + (((2 * c + 1) ^ (r & 7)) * 16));
-            Run<T, 8> o = {Traits<T>::down(v.x), Traits<T>::down(v.y), Traits<T>::down(v.z), Traits<T>::down(v.w),
-                           Traits<T>::down(w.x), Traits<T>::down(w.y), Traits<T>::down(w.z), Traits<T>::down(w.w)};
-            if (r < rows && 8 * c < columns) st_run<T, 8>(to + (size_t)r * stride + 8 * c, o);
+            const float f[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
+            if (r < rows && 8 * c < columns) st_run<T, 8>(to + (size_t)r * stride + 8 * c, round_run<T, 8>(f));
         }
     } else if (lane < columns) {
 #pragma unroll 4
@@ -72,8 +71,15 @@ inline cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, int r
     if (!d || !d->TensorMapEncodeTiled) return cudaErrorNotSupported;
     const cuuint64_t dims[3] = {size[0], size[1], size[2]}, strides[2] = {stride[0] * 2, stride[1] * 2};
     const cuuint32_t box[3] = {64, box_outer, 1}, steps[3] = {1, 1, 1};
-    const CUresult r = d->TensorMapEncodeTiled(map, dtype == 6 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, steps,
-                                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto encode = [&] {
+        return d->TensorMapEncodeTiled(map, dtype == 6 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, steps,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {      // the thread's first call of CUDA: the runtime has its device, but no context current yet
+        int device = 0;
+        if (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = encode();
+    }
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 inline cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, size_t inner, size_t outer, size_t stride, unsigned box_outer) {

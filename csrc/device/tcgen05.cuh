@@ -102,6 +102,18 @@ __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"((int)add)
                  : "memory");
 }
+/** The same with the descriptors by their low halves, which hold the addresses (16 bytes each), and one high half: their sums take one instruction. */
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t desc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(desc), "r"((int)add)
+                 : "memory");
+}
+/** One lane of a whole warp, the same for the same warp: the compiler knows that what it is alone to do is uniform, which it does not of `lane == 0`. */
+__device__ __forceinline__ bool elect_one() {
+    uint32_t mine;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(mine));
+    return mine != 0;
+}
 /** One arrival on the barrier when this thread's products so far are done. */
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");

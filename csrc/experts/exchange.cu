@@ -17,6 +17,7 @@ namespace dccl {
 /* ---- the order of the experts ---- */
 
 constexpr int kPlanCtas = 8;            // a cluster of the portable size
+constexpr int kPlanKept = 8;            // places of a lane that stay in registers
 
 struct PlanArgs {
     const void* chosen;
@@ -43,9 +44,19 @@ __device__ __forceinline__ unsigned of_other_cta(const unsigned* mine, unsigned 
     return v;
 }
 
+/** Lanes with the same number as this one, of `bits` bits that decide: as many ballots, a third of the time of a match of 32-bit numbers. */
+__device__ __forceinline__ unsigned lanes_alike(unsigned e, int bits) {
+    unsigned alike = 0xffffffffu;
+    for (int b = 0; b < bits; b++) {
+        const unsigned set = __ballot_sync(0xffffffffu, e >> b & 1);
+        alike &= e >> b & 1 ? set : ~set;
+    }
+    return alike;
+}
+
 /**
- * One launch of one CTA, or of a cluster of eight that exchange their counts through shared memory. Every warp has a run of consecutive places; the ranks of
- * equal experts among 32 places come from a match, and one lane of each kind counts on. Two walks over the places: how many there are, and where they go.
+ * One launch of one CTA, or of a cluster of eight that exchange their counts through shared memory. Every warp has a run of consecutive places, and counts of its
+ * own. Two walks over the places: how many there are of each expert, and where they go; among 32 places one lane of each kind counts on.
  */
 template <bool MANY> __device__ __forceinline__ void plan(const PlanArgs& a) {
     extern __shared__ unsigned counted[];           // [warps][experts], then [experts] of the CTA, then [32]
@@ -55,22 +66,28 @@ template <bool MANY> __device__ __forceinline__ void plan(const PlanArgs& a) {
     unsigned* const sums = total + E;
     unsigned rank = 0;
     if constexpr (MANY) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    const unsigned ctas = MANY ? kPlanCtas : 1, runs = ctas * warps, per = (((a.places + runs - 1) / runs) + 31) / 32 * 32;
+    constexpr unsigned ctas = MANY ? kPlanCtas : 1;
+    const unsigned runs = ctas * warps, per = (((a.places + runs - 1) / runs) + 31) / 32 * 32;
     // in 64 bits: the last warps' runs may start behind everything
     const unsigned long long begin = (unsigned long long)(rank * warps + warp) * per;
     const unsigned from = begin < a.places ? (unsigned)begin : a.places, to = a.places - from < per ? a.places : from + per;
     for (unsigned i = threadIdx.x; i < warps * E; i += blockDim.x) counted[i] = 0;
     __syncthreads();
     wait_for_stream();
-    for (unsigned base = from; base < to; base += 32) {
-        const unsigned e = base + lane < to ? plan_expert(a, base + lane) : 0xffffffffu;
-        const unsigned alike = __match_any_sync(0xffffffffu, e);
-        if (e < E && lane == (unsigned)__ffs(alike) - 1) mine[e] += __popc(alike);
-        __syncwarp();
+    unsigned kept[kPlanKept];                       // the first of the run, for the second walk
+#pragma unroll
+    for (int k = 0; k < kPlanKept; k++) kept[k] = from + 32 * k + lane < to ? plan_expert(a, from + 32 * k + lane) : 0xffffffffu;
+#pragma unroll
+    for (int k = 0; k < kPlanKept; k++)
+        if (kept[k] < E) atomicAdd(mine + kept[k], 1);
+    for (unsigned i = from + 32 * kPlanKept + lane; i < to; i += 32) {
+        const unsigned e = plan_expert(a, i);
+        if (e < E) atomicAdd(mine + e, 1);
     }
     __syncthreads();
     for (unsigned e = threadIdx.x; e < E; e += blockDim.x) {
         unsigned sum = 0;
+#pragma unroll 8
         for (unsigned w = 0; w < warps; w++) {
             const unsigned n = counted[w * E + e];
             counted[w * E + e] = sum;
@@ -79,46 +96,62 @@ template <bool MANY> __device__ __forceinline__ void plan(const PlanArgs& a) {
         total[e] = sum;
     }
     plan_cluster_sync(MANY);
-    // starts of the experts: threads take runs of consecutive ones
-    const unsigned each = (E + blockDim.x - 1) / blockDim.x, first = min(threadIdx.x * each, E), last = min(first + each, E);
-    unsigned own = 0;
-    for (unsigned e = first; e < last; e++)
-        for (unsigned c = 0; c < ctas; c++) own += MANY ? of_other_cta(total + e, c) : total[e];
-    unsigned before = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= (unsigned)o) before += v;
-    }
-    if (lane == 31) sums[warp] = before;
-    __syncthreads();
-    unsigned start = before - own;
-    for (unsigned w = 0; w < warp; w++) start += sums[w];
-    for (unsigned e = first; e < last; e++) {
+    // every thread of a round has one expert: what the CTAs before have of it, and all
+    unsigned start = 0;                             // of the round's first expert
+    for (unsigned round = 0; round < E; round += blockDim.x) {
+        const unsigned e = round + threadIdx.x;
         unsigned n = 0, here = 0;
-        for (unsigned c = 0; c < ctas; c++) {
-            const unsigned v = MANY ? of_other_cta(total + e, c) : total[e];
-            here += c < rank ? v : 0;
-            n += v;
+        if (e < E) {
+            unsigned v[ctas];
+#pragma unroll
+            for (unsigned c = 0; c < ctas; c++) v[c] = MANY ? of_other_cta(total + e, c) : total[e];
+#pragma unroll
+            for (unsigned c = 0; c < ctas; c++) {
+                here += c < rank ? v[c] : 0;
+                n += v[c];
+            }
         }
-        if (rank == 0) {
-            a.starts[e] = (int)start;
-            a.counts[e] = (int)n;
-            if (e == E - 1) a.starts[E] = (int)(start + n);
+        unsigned upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (unsigned)o) upto += v;
         }
-        for (unsigned w = 0; w < warps; w++) counted[w * E + e] += start + here;
-        start += n;
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        unsigned before = start, all = 0;
+        for (unsigned w = 0; w < warps; w++) {
+            before += w < warp ? sums[w] : 0;
+            all += sums[w];
+        }
+        before += upto - n;
+        if (e < E) {
+            if (rank == 0) {
+                a.starts[e] = (int)before;
+                a.counts[e] = (int)n;
+                if (e == E - 1) a.starts[E] = (int)(before + n);
+            }
+#pragma unroll 8
+            for (unsigned w = 0; w < warps; w++) counted[w * E + e] += before + here;
+        }
+        start += all;
+        __syncthreads();
     }
     plan_cluster_sync(MANY);        // nobody's totals go before the others have read them, either
-    for (unsigned base = from; base < to; base += 32) {
-        const unsigned i = base + lane, e = i < to ? plan_expert(a, i) : 0xffffffffu;
-        const unsigned alike = __match_any_sync(0xffffffffu, e);
+    const int bits = 32 - __clz(E);                 // a number of no expert is E
+    const auto place = [&](unsigned i, unsigned e) {
+        e = e < E ? e : E;
+        const unsigned alike = lanes_alike(e, bits);
         const unsigned at = e < E ? mine[e] : 0;
         __syncwarp();
         if (e < E && lane == (unsigned)__ffs(alike) - 1) mine[e] = at + __popc(alike);
         if (i < to) a.rows[i] = e < E ? (int)(at + __popc(alike & ((1u << lane) - 1))) : -1;
         __syncwarp();
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kPlanKept; k++)
+        if (from + 32 * k < to) place(from + 32 * k + lane, kept[k]);
+    for (unsigned base = from + 32 * kPlanKept; base < to; base += 32) place(base + lane, base + lane < to ? plan_expert(a, base + lane) : E);
 }
 __global__ void __launch_bounds__(1024) k_plan(const __grid_constant__ PlanArgs a) { plan<false>(a); }
 __global__ void __launch_bounds__(1024) __cluster_dims__(kPlanCtas, 1, 1) k_plan_cluster(const __grid_constant__ PlanArgs a) { plan<true>(a); }
@@ -129,107 +162,175 @@ struct RowsArgs {
     const void *x, *in, *weights;       // of a token, and of rows in the experts' order
     void *out, *out2;
     const int *rows, *used;
-    unsigned tokens, k;
+    unsigned tokens, k, across;
     size_t width;
     bool weights32;
 };
 
-constexpr int kRowThreads = 128;
+/**
+ * A token belongs to `across` threads (whole warps), which take U runs of N elements each at a time, so far apart that a warp's accesses are of neighbours. A CTA has as
+ * many tokens as fit. Lane j of every warp has the token's j-th row and weight, and hands them round: loads of them between those of the rows, under conditions of their
+ * own, kept the latter from being in flight together (combine of 16384 x 2048 bf16 by 4: 84 us, and 58 without).
+ */
+constexpr int kRowThreads = 128, kHeld = 2;
+constexpr unsigned kNoRow = 0xffffffffu;
 
-/** Where the row of a place is, or -1: a number that is none of a row is not followed. */
-__device__ __forceinline__ int row_of(const RowsArgs& a, size_t place) {
-    const int row = a.rows[place];
-    return (unsigned)row < a.tokens * a.k ? row : -1;
-}
-
-template <typename T> __device__ __forceinline__ float weight_of(const RowsArgs& a, size_t place) {
-    return !a.weights ? 1.0f : a.weights32 ? reinterpret_cast<const float*>(a.weights)[place] : Traits<T>::up(reinterpret_cast<const T*>(a.weights)[place]);
+struct Token { size_t index; unsigned thread, row; float weight; bool there; };
+template <typename T> __device__ __forceinline__ Token token_of(const RowsArgs& a) {
+    Token t;
+    t.index = (size_t)blockIdx.x * (kRowThreads / a.across) + threadIdx.x / a.across;
+    t.thread = threadIdx.x % a.across;
+    t.there = t.index < a.tokens && threadIdx.x / a.across < kRowThreads / a.across;
+    t.row = kNoRow;
+    t.weight = 1.0f;
+    const unsigned lane = threadIdx.x % 32;
+    if (t.there && lane < a.k) {
+        const size_t place = t.index * a.k + lane;
+        t.row = (unsigned)a.rows[place];
+        if (t.row >= a.tokens * a.k) t.row = kNoRow;        // a number that is none of a row is not followed
+        if (a.weights) t.weight = a.weights32 ? reinterpret_cast<const float*>(a.weights)[place] : Traits<T>::up(reinterpret_cast<const T*>(a.weights)[place]);
+        if (t.row == kNoRow) t.weight = 0.0f;
+    }
+    return t;
 }
 
 /** Zeros in those of the rows that stand at this token's places in `to` which nobody uses. */
-template <typename T, int N> __device__ __forceinline__ void clear_unused(const RowsArgs& a, T* to, size_t token) {
+template <typename T, int N> __device__ __forceinline__ void clear_unused(const RowsArgs& a, T* to, const Token& t) {
     const unsigned used = (unsigned)*a.used;
-    if ((token + 1) * a.k <= used) return;
+    if ((t.index + 1) * a.k <= used) return;
     for (unsigned j = 0; j < a.k; j++) {
-        const size_t row = token * a.k + j;
+        const size_t row = t.index * a.k + j;
         if (row < used) continue;
-        for (size_t i = threadIdx.x * N; i < a.width; i += kRowThreads * N) st_run<T, N>(to + row * a.width + i, Run<T, N>{});
+        for (unsigned i = t.thread * N; i < a.width; i += a.across * N) st_run<T, N>(to + row * a.width + i, Run<T, N>{});
     }
 }
 
 /** Rows are bytes here: T is an unsigned integer of the elements' size. */
-template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) k_dispatch(const __grid_constant__ RowsArgs a) {
+template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThreads) k_dispatch(const __grid_constant__ RowsArgs a) {
     wait_for_stream();
-    const size_t token = blockIdx.x;
-    const T* from = reinterpret_cast<const T*>(a.x) + token * a.width;
-    T* out = reinterpret_cast<T*>(a.out);
-    for (size_t i = threadIdx.x * N; i < a.width; i += kRowThreads * N) {
-        const Run<T, N> v = ld_run<T, N>(from + i);
-        for (unsigned j = 0; j < a.k; j++) {
-            const int row = row_of(a, token * a.k + j);
-            if (row >= 0) st_run<T, N>(out + (size_t)row * a.width + i, v);
-        }
-    }
-    clear_unused<T, N>(a, out, token);
-}
-
-template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) k_combine(const __grid_constant__ RowsArgs a) {
-    wait_for_stream();
-    const size_t token = blockIdx.x;
-    const T* in = reinterpret_cast<const T*>(a.in);
-    for (size_t i = threadIdx.x * N; i < a.width; i += kRowThreads * N) {
-        float sum[N] = {};
-        for (unsigned j = 0; j < a.k; j++) {
-            const int row = row_of(a, token * a.k + j);
-            if (row < 0) continue;
-            const float w = weight_of<T>(a, token * a.k + j);
-            const Run<T, N> v = ld_run<T, N>(in + (size_t)row * a.width + i);
+    const Token t = token_of<T>(a);
+    if (!t.there) return;
+    const T* from = reinterpret_cast<const T*>(a.x) + t.index * a.width;
+    T* const out = reinterpret_cast<T*>(a.out);
+    const unsigned step = a.across * N;
+    for (unsigned first = (t.thread & ~31u) * N; first < a.width; first += U * step) {       // of the warp, which goes on as one
+        const unsigned i = first + (t.thread & 31) * N;
+        Run<T, N> v[U];
 #pragma unroll
-            for (int e = 0; e < N; e++) sum[e] = fmaf(w, Traits<T>::up(v.e[e]), sum[e]);
+        for (int u = 0; u < U; u++)
+            if (i + u * step < a.width) v[u] = ld_run<T, N>(from + i + u * step);
+        for (unsigned j = 0; j < a.k; j++) {
+            const unsigned row = __shfl_sync(0xffffffffu, t.row, j);
+            if (row == kNoRow) continue;
+            T* const to = out + (size_t)row * a.width + i;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (i + u * step < a.width) st_run<T, N>(to + u * step, v[u]);
         }
-        st_run<T, N>(reinterpret_cast<T*>(a.out) + token * a.width + i, round_run<T, N>(sum));
+    }
+    clear_unused<T, N>(a, out, t);
+}
+
+/** kHeld of a token's rows from the j0-th on, zeros where there is none. */
+template <typename T, int N, int U> __device__ __forceinline__ void hold_rows(const RowsArgs& a, const Token& t, unsigned j0, unsigned i, unsigned step, Run<T, N> (&v)[kHeld][U]) {
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) {
+        const unsigned row = __shfl_sync(0xffffffffu, t.row, j0 + j);
+        const T* const from = reinterpret_cast<const T*>(a.in) + (size_t)row * a.width + i;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            v[j][u] = Run<T, N>{};
+            if (row != kNoRow && i + u * step < a.width) v[j][u] = ld_run<T, N>(from + u * step);
+        }
     }
 }
 
-template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) k_combine_grad(const __grid_constant__ RowsArgs a) {
+template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThreads, 10) k_combine(const __grid_constant__ RowsArgs a) {
+    wait_for_stream();
+    const Token t = token_of<T>(a);
+    if (!t.there) return;
+    const unsigned step = a.across * N;
+    for (unsigned first = (t.thread & ~31u) * N; first < a.width; first += U * step) {
+        const unsigned i = first + (t.thread & 31) * N;
+        float sum[U][N] = {};
+        for (unsigned j0 = 0; j0 < a.k; j0 += kHeld) {          // at most 32, and lanes behind the last have none
+            Run<T, N> v[kHeld][U];
+            hold_rows<T, N, U>(a, t, j0, i, step, v);
+#pragma unroll
+            for (int j = 0; j < kHeld; j++) {
+                const float w = __shfl_sync(0xffffffffu, t.weight, j0 + j);
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) sum[u][e] = fmaf(w, Traits<T>::up(v[j][u].e[e]), sum[u][e]);
+            }
+        }
+        T* const to = reinterpret_cast<T*>(a.out) + t.index * a.width + i;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i + u * step < a.width) st_run<T, N>(to + u * step, round_run<T, N>(sum[u]));
+    }
+}
+
+template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThreads, 10) k_combine_grad(const __grid_constant__ RowsArgs a) {
     wait_for_stream();
     __shared__ float dots[kRowThreads / 32][DCCL_EXPERTS_MAX_CHOSEN];
-    const size_t token = blockIdx.x;
-    const T* dy = reinterpret_cast<const T*>(a.x) + token * a.width;
-    const T* in = reinterpret_cast<const T*>(a.in);
-    T* din = reinterpret_cast<T*>(a.out);
-    for (unsigned j = 0; j < a.k; j++) {
-        const size_t place = token * a.k + j;
-        const int row = row_of(a, place);
-        float dot = 0.0f;
-        if (row >= 0) {
-            const float w = weight_of<T>(a, place);
-            for (size_t i = threadIdx.x * N; i < a.width; i += kRowThreads * N) {
-                const Run<T, N> g = ld_run<T, N>(dy + i);
-                float to[N];
-                if (a.out2) {
-                    const Run<T, N> v = ld_run<T, N>(in + (size_t)row * a.width + i);
+    const Token t = token_of<T>(a);
+    T* const din = reinterpret_cast<T*>(a.out);
+    const unsigned step = a.across * N;
+    if (t.there) {
+        const T* dy = reinterpret_cast<const T*>(a.x) + t.index * a.width;
+        for (unsigned j0 = 0; j0 < a.k; j0 += kHeld) {
+            float dot[kHeld] = {};
+            for (unsigned first = (t.thread & ~31u) * N; first < a.width; first += U * step) {
+                const unsigned i = first + (t.thread & 31) * N;
+                Run<T, N> g[U], v[kHeld][U];
 #pragma unroll
-                    for (int e = 0; e < N; e++) dot = fmaf(Traits<T>::up(g.e[e]), Traits<T>::up(v.e[e]), dot);
+                for (int u = 0; u < U; u++) {
+                    g[u] = Run<T, N>{};
+                    if (i + u * step < a.width) g[u] = ld_run<T, N>(dy + i + u * step);
                 }
-                if (din) {
+                if (a.out2) hold_rows<T, N, U>(a, t, j0, i, step, v);
 #pragma unroll
-                    for (int e = 0; e < N; e++) to[e] = w * Traits<T>::up(g.e[e]);
-                    st_run<T, N>(din + (size_t)row * a.width + i, round_run<T, N>(to));
+                for (int j = 0; j < kHeld; j++) {
+                    if (a.out2) {
+#pragma unroll
+                        for (int u = 0; u < U; u++)
+#pragma unroll
+                            for (int e = 0; e < N; e++) dot[j] = fmaf(Traits<T>::up(g[u].e[e]), Traits<T>::up(v[j][u].e[e]), dot[j]);
+                    }
+                    const unsigned row = __shfl_sync(0xffffffffu, t.row, j0 + j);
+                    const float w = __shfl_sync(0xffffffffu, t.weight, j0 + j);
+                    if (!din || row == kNoRow) continue;
+                    T* const to = din + (size_t)row * a.width + i;
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        float f[N];
+#pragma unroll
+                        for (int e = 0; e < N; e++) f[e] = w * Traits<T>::up(g[u].e[e]);
+                        if (i + u * step < a.width) st_run<T, N>(to + u * step, round_run<T, N>(f));
+                    }
+                }
+            }
+            if (a.out2) {
+#pragma unroll
+                for (int j = 0; j < kHeld; j++) {
+                    float d = dot[j];
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+                    if (threadIdx.x % 32 == 0 && j0 + j < a.k) dots[threadIdx.x / 32][j0 + j] = d;
                 }
             }
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (threadIdx.x % 32 == 0) dots[threadIdx.x / 32][j] = dot;
+        if (din) clear_unused<T, N>(a, din, t);
     }
-    if (din) clear_unused<T, N>(a, din, token);
     if (!a.out2) return;
     __syncthreads();
-    if (threadIdx.x < a.k) {
+    if (t.there && t.thread < a.k) {            // the first warp of the token, whose lane j has place j
         float dot = 0.0f;
-        for (int w = 0; w < kRowThreads / 32; w++) dot += dots[w][threadIdx.x];
-        const size_t place = token * a.k + threadIdx.x;
+        for (unsigned w = 0; w < a.across / 32; w++) dot += dots[threadIdx.x / 32 + w][t.thread];
+        const size_t place = t.index * a.k + t.thread;
+        if (t.row == kNoRow) dot = 0.0f;        // of a gradient that is not finite
         if (a.weights32) reinterpret_cast<float*>(a.out2)[place] = dot;
         else reinterpret_cast<T*>(a.out2)[place] = Traits<T>::down(dot);
     }
@@ -245,6 +346,14 @@ static bool rows_fit(size_t tokens, int k, size_t width) {
 template <typename T> static int run_of(size_t width, std::initializer_list<const void*> ps) {
     const int most = 16 / sizeof(T), few = 4 / sizeof(T);
     return width % most == 0 && aligned_to(16, ps) ? most : width % few == 0 && aligned_to(4, ps) ? few : 1;
+}
+
+/** Threads of a token: as many as one round of accesses needs, up to a CTA of them. */
+static cudaError_t run_rows(void (*kernel)(const RowsArgs), int n, int u, RowsArgs& a, cudaStream_t stream) {
+    const size_t warps = (a.width + 32 * n * u - 1) / (32 * n * u);
+    a.across = warps >= kRowThreads / 32 ? kRowThreads : (unsigned)warps * 32;
+    const unsigned tokens = kRowThreads / a.across;
+    return launch_early_shared(kernel, (a.tokens + tokens - 1) / tokens, kRowThreads, 0, stream, a);
 }
 
 } // namespace dccl
@@ -286,29 +395,28 @@ extern "C" int dccl_dispatch(int device, int dtype, size_t tokens, int k, size_t
     a.tokens = (unsigned)tokens;
     a.k = (unsigned)k;
     a.width = width;
-    const auto go = [&](auto kernel) { return launch_early(kernel, a.tokens, kRowThreads, (cudaStream_t)stream, a); };
-    if (dtype == 7) {
-        const int n = run_of<uint32_t>(width, {x, out});
-        return report(who, n == 4 ? go(k_dispatch<uint32_t, 4>) : go(k_dispatch<uint32_t, 1>));
-    }
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == 7) return report(who, run_of<uint32_t>(width, {x, out}) == 4 ? run_rows(k_dispatch<uint32_t, 4, 1>, 4, 1, a, s) : run_rows(k_dispatch<uint32_t, 1, 4>, 1, 4, a, s));
     const int n = run_of<uint16_t>(width, {x, out});
-    return report(who, n == 8 ? go(k_dispatch<uint16_t, 8>) : n == 2 ? go(k_dispatch<uint16_t, 2>) : go(k_dispatch<uint16_t, 1>));
+    return report(who, n == 8 ? run_rows(k_dispatch<uint16_t, 8, 1>, 8, 1, a, s) : n == 2 ? run_rows(k_dispatch<uint16_t, 2, 2>, 2, 2, a, s) : run_rows(k_dispatch<uint16_t, 1, 4>, 1, 4, a, s));
 }
 
-template <typename T> static cudaError_t run_combine(const RowsArgs& a, cudaStream_t stream) {
-    const auto go = [&](auto kernel) { return launch_early(kernel, a.tokens, kRowThreads, stream, a); };
+template <typename T> static cudaError_t run_combine(RowsArgs& a, cudaStream_t stream) {
+    constexpr int most = 16 / sizeof(T), few = 4 / sizeof(T);
     const int n = run_of<T>(a.width, {a.in, a.out});
-    if (n == 16 / (int)sizeof(T)) return go(k_combine<T, 16 / sizeof(T)>);
-    if (sizeof(T) == 2 && n == 2) return go(k_combine<T, 2>);
-    return go(k_combine<T, 1>);
+    if (n == most) return run_rows(k_combine<T, most, 1>, most, 1, a, stream);
+    if constexpr (few > 1)
+        if (n == few) return run_rows(k_combine<T, few, 2>, few, 2, a, stream);
+    return run_rows(k_combine<T, 1, 4>, 1, 4, a, stream);
 }
 
-template <typename T> static cudaError_t run_combine_grad(const RowsArgs& a, cudaStream_t stream) {
-    const auto go = [&](auto kernel) { return launch_early(kernel, a.tokens, kRowThreads, stream, a); };
+template <typename T> static cudaError_t run_combine_grad(RowsArgs& a, cudaStream_t stream) {
+    constexpr int most = 16 / sizeof(T), few = 4 / sizeof(T);
     const int n = run_of<T>(a.width, {a.x, a.in, a.out});
-    if (n == 16 / (int)sizeof(T)) return go(k_combine_grad<T, 16 / sizeof(T)>);
-    if (sizeof(T) == 2 && n == 2) return go(k_combine_grad<T, 2>);
-    return go(k_combine_grad<T, 1>);
+    if (n == most) return run_rows(k_combine_grad<T, most, 1>, most, 1, a, stream);
+    if constexpr (few > 1)
+        if (n == few) return run_rows(k_combine_grad<T, few, 2>, few, 2, a, stream);
+    return run_rows(k_combine_grad<T, 1, 4>, 1, 4, a, stream);
 }
 
 extern "C" int dccl_combine(int device, int dtype, size_t tokens, int k, size_t width, const void* in, const int* rows, const void* weights, int weights32, void* y, void* stream) {

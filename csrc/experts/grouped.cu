@@ -20,54 +20,99 @@ constexpr int kGroupedWarps = 8, kGroupedThreads = 32 * (kGroupedWarps + 2);    
 constexpr unsigned kGroupedLoader = kGroupedWarps, kGroupedMultiplier = kGroupedWarps + 1;
 constexpr int kNoActivation = -1;
 
-struct GroupedArgs : Grouped {
+/**
+ * The normal distribution's cdf(z) and e^(-z^2 / 2), which its density needs as well. erfc(x) = t (c1 + ... + c7 t^6) e^(-x^2) with t = 1 / (1 + p x), the form of
+ * Abramowitz and Stegun, "Handbook of Mathematical Functions", 7.1.26, with one more term pair and coefficients fitted on [0, 8] for an error that stays small against
+ * erfc itself: 2e-8 near 0, 3e-6 of erfc at 4; in fp32 the cdf is off by 1.5e-7 at most. With erff the epilogue of a tile took longer than its
+ * products, and k_act_grad, bound by its arithmetic, 177 us for 16384 x 5632 bf16 instead of 124.
+ */
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    constexpr float root = 0.70710678118654752f;
+    e = __expf(-0.5f * z * z);
+    const float t = __fdividef(1.0f, fmaf(0.36f * root, fabsf(z), 1.0f));
+    float c = fmaf(t, -0.1658067272f, 0.5732104218f);
+    c = fmaf(t, c, -0.3708126889f);
+    c = fmaf(t, c, 0.4417887144f);
+    c = fmaf(t, c, 0.1015090368f);
+    c = fmaf(t, c, 0.2180343121f);
+    c = fmaf(t, c, 0.2020769013f);
+    const float tail = 0.5f * t * c * e;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+template <int ACT> __device__ __forceinline__ float value_of(float z) {
+    if constexpr (ACT == DCCL_ACT_GELU) {
+        float e;
+        return z * normal_cdf(z, e);
+    } else {
+        return activate<ACT>(z);
+    }
+}
+template <int ACT> __device__ __forceinline__ float slope_of(float z) {
+    if constexpr (ACT == DCCL_ACT_GELU) {
+        float e;
+        const float cdf = normal_cdf(z, e);
+        return fmaf(z * 0.3989422804014327f, e, cdf);
+    } else {
+        float value, slope;
+        activate_grad<ACT>(z, value, slope);
+        return slope;
+    }
+}
+
+struct GroupedArgs : Grouped, GroupedResults {
     CUtensorMap a, b;
     const int* starts;
     unsigned descriptor;            // of one product
     int act;
-    void* c;
-    float* z;
-    size_t z_stride;
     int* gave_up;
 };
 
-template <int N> struct GroupedShape {
-    static constexpr int kBytesA = kTileM * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kBytes;
-    static constexpr int kShared = kStages * kBytes + kGroupedWarps * 4096 + 1024;      // 1024: the tiles' alignment
-    static_assert(kShared + 2 * 1024 <= 227 * 1024, "with the list of tiles and the barriers");
+/** Tiles of M x N. A product reads 128 rows of the first operand from shared memory: behind M of them lies something else, and nobody reads what becomes of it. */
+template <int M, int N> struct GroupedShape {
+    static constexpr int kCtas = M < kTileM ? 2 : 1;        // of an SM: for small tiles, what one thread takes to give products out is what bounds a CTA
+    static constexpr int kBytesA = M * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kCtas / kBytes;
+    static constexpr int kStagings = M < kTileM ? 2 : kGroupedWarps;                    // warps that have rows to store
+    static constexpr int kShared = kStages * kBytes + kStagings * 4096 + 1024;          // 1024: the tiles' alignment
+    static_assert(kCtas * (kShared + 2 * 1024) <= 227 * 1024, "with the list of tiles and the barriers");
+    static_assert(kTileM * kTileK * 2 - kBytes <= kStagings * 4096, "what the last stage's product reads");
 };
 
-/** The list of tiles, by one warp: first[i], the rows of tiles before expert i * stride, and all of them. */
-__device__ __forceinline__ void list_tiles(const Grouped& a, const int* starts, unsigned* first) {
+/** The list of tiles, by one warp: first[i], the rows of tiles before expert i * stride, and all of them. own: the starts, where every expert is listed. */
+__device__ __forceinline__ void list_tiles(const Grouped& a, const int* starts, unsigned* first, int* own) {
     const unsigned lane = threadIdx.x % 32, entries = listed_of(a);
     unsigned before = 0;
     for (unsigned base = 0; base < entries; base += 32) {
         const unsigned i = base + lane;
         unsigned n = 0;
-        for (unsigned e = i * a.stride; e < (i + 1) * a.stride && e <= a.experts; e++) n += tall_of(starts, e, a.experts, a.rows);
-        const unsigned own = n;
+        for (unsigned e = i * a.stride; e < (i + 1) * a.stride && e <= a.experts; e++) n += tall_of(starts, e, a);
+        if (a.stride == 1 && i < entries) own[i] = starts[i];
+        const unsigned mine = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const unsigned v = __shfl_up_sync(0xffffffffu, n, o);
             if (lane >= (unsigned)o) n += v;
         }
-        if (i < entries) first[i] = before + n - own;
+        if (i < entries) first[i] = before + n - mine;
         before += __shfl_sync(0xffffffffu, n, 31);
     }
     if (lane == 0) first[entries] = before;
 }
 
 /**
- * One CTA per SM walks over tiles of 128 rows and N columns; one warp loads, one multiplies, eight store: a warp reaches the quarter of the tile's rows that its
+ * One CTA per SM walks over tiles of M rows and N columns; one warp loads, one multiplies, eight store: a warp reaches the quarter of the tile's rows that its
  * number gives, so two share one and take half of the columns each. The sums of two tiles fit into tensor memory, so that one is stored while the next is
  * multiplied.
+ *
+ * What an SM can load bounds it (58 bytes a clock: 48 KB of a tile of 128 x 256 take 1.6 times as long as its products would): the loader must never pause, and finds its
+ * place in a tile from shared memory and without divisions.
  */
-template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupedThreads, 1) k_grouped(const __grid_constant__ GroupedArgs a) {
-    using Shape = GroupedShape<N>;
+template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(kGroupedThreads, GroupedShape<M, N>::kCtas) k_grouped(const __grid_constant__ GroupedArgs a) {
+    using Shape = GroupedShape<M, N>;
     constexpr int kStages = Shape::kStages;
     extern __shared__ char shared[];
     __shared__ uint64_t bars[2 * kStages + 5];
-    __shared__ unsigned first[FORM == EXPERTS_WEIGHT ? 1 : kListed + 1];
+    __shared__ unsigned first[kListed + 1];
+    __shared__ int own[kListed + 1];
     __shared__ uint32_t tmem_base;
     __shared__ int failed;
     char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
@@ -87,44 +132,51 @@ template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupe
         prefetch_map(&a.b);
     }
     wait_for_stream();
-    if (FORM != EXPERTS_WEIGHT && warp == 1) list_tiles(a, a.starts, first);
+    if (warp == 1) list_tiles(a, a.starts, first, own);
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
+    const int* const starts = a.stride == 1 ? own : a.starts;
     const uint32_t sums = tmem_base;
-    const unsigned long long total = grouped_tiles(FORM, a, first);
+    const unsigned total = grouped_tiles(FORM, a, first);
     unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
     if (warp == kGroupedLoader && lane == 0) {
-        for (unsigned long long tile = blockIdx.x; tile < total; tile += gridDim.x) {
-            const GroupedPlace p = grouped_place(FORM, tile, N, a, first, a.starts);
+        unsigned s = 0, parity = 1;
+        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
             const unsigned blocks = (p.k_count + kTileK - 1) / kTileK;
-            unsigned kb = 0;
+            // of few rows all CTAs read the same lines: each begins somewhere else in k, or those lines' part of L2 is what they wait for (16 rows of 2048 x 5632: 60 us)
+            unsigned kb = 0, ahead = M < kTileM && blocks ? blockIdx.x * 5 % blocks : 0;
             for (; kb < blocks; kb++, filled++) {
-                const unsigned s = filled % kStages;
-                if (!bar_wait(empty + 8 * s, (filled / kStages & 1) ^ 1, &failed)) break;
+                if (!bar_wait(empty + 8 * s, parity, &failed)) break;
                 const uint32_t to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA, bar = full + 8 * s;
+                const int k = p.k_from + (M < kTileM ? ahead : kb) * kTileK;
+                if (M < kTileM && ++ahead == blocks) ahead = 0;
                 bar_expect(bar, Shape::kBytes);
                 if constexpr (FORM == EXPERTS_FORWARD) {
-                    load_box(to_a, &a.a, kb * kTileK, p.row, bar);
-                    load_box(to_b, &a.b, kb * kTileK, p.column, p.expert, bar);
+                    load_box(to_a, &a.a, k, p.row, bar);
+                    load_box(to_b, &a.b, k, p.column, p.expert, bar);
                 } else if constexpr (FORM == EXPERTS_INPUT) {
-                    load_box(to_a, &a.a, kb * kTileK, p.row, bar);
+                    load_box(to_a, &a.a, k, p.row, bar);
 #pragma unroll
-                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, kb * kTileK, p.expert, bar);
+                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, p.expert, bar);
                 } else {
-                    const int row = p.k_from + kb * kTileK;
 #pragma unroll
-                    for (int i = 0; i < kTileM / 64; i++) load_box(to_a + i * 64 * 128, &a.a, p.row + 64 * i, row, bar);
+                    for (int i = 0; i < M / 64; i++) load_box(to_a + i * 64 * 128, &a.a, p.row + 64 * i, k, bar);
 #pragma unroll
-                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, row, bar);
+                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, bar);
                 }
+                if (++s == kStages) { s = 0; parity ^= 1; }
             }
             if (kb < blocks) break;
         }
     } else if (warp == kGroupedMultiplier) {
-        unsigned done = 0;
-        for (unsigned long long tile = blockIdx.x; tile < total; tile += gridDim.x) {
-            const GroupedPlace p = grouped_place(FORM, tile, N, a, first, a.starts);
+        unsigned done = 0, s = 0, parity = 0;
+        const uint64_t of_a = tile_descriptor(shared_addr(tiles), FORM == EXPERTS_WEIGHT ? 64 * 128 : 16);
+        const uint64_t of_b = tile_descriptor(shared_addr(tiles) + Shape::kBytesA, FORM == EXPERTS_FORWARD ? 16 : 64 * 128);
+        const uint32_t first_a = (uint32_t)of_a, high_a = (uint32_t)(of_a >> 32), first_b = (uint32_t)of_b, high_b = (uint32_t)(of_b >> 32);
+        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
             const unsigned blocks = (p.k_count + kTileK - 1) / kTileK;
             if (!blocks) continue;
             const unsigned buffer = done & 1;
@@ -133,8 +185,7 @@ template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupe
             const uint32_t d = sums + buffer * N;
             unsigned kb = 0;
             for (; kb < blocks; kb++, filled++) {
-                const unsigned s = filled % kStages;
-                if (!bar_wait_warp(full + 8 * s, filled / kStages & 1, &failed)) break;
+                if (!bar_wait_warp(full + 8 * s, parity, &failed)) break;
                 tc_after_sync();
                 char* const at = tiles + s * Shape::kBytes;
                 unsigned steps = kTileK / 16;
@@ -143,39 +194,38 @@ template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupe
                     if (left < (unsigned)kTileK) {      // rows of the next expert, and whatever they are: as many as the last product of 16 would add
                         steps = (left + 15) / 16;
                         const unsigned pieces = (steps * 16 - left) * 8;
-                        for (unsigned i = lane; i < pieces * (kTileM + N) / 64; i += 32)
+                        for (unsigned i = lane; i < pieces * (M + N) / 64; i += 32)
                             *reinterpret_cast<uint4*>(at + i / pieces * 64 * 128 + left * 128 + i % pieces * 16) = uint4{};
                         shared_writes_before_products();
                         __syncwarp();
                     }
                 }
-                const uint32_t at_a = shared_addr(at), at_b = at_a + Shape::kBytesA;
-                if (lane == 0) {
+                if (elect_one()) {
+                    const uint32_t da = first_a + s * (Shape::kBytes >> 4), db = first_b + s * (Shape::kBytes >> 4);
 #pragma unroll
                     for (unsigned k = 0; k < kTileK / 16; k++) {
                         if (FORM == EXPERTS_WEIGHT && k >= steps) break;
                         // 16 k: 32 bytes further along K-major rows, or 16 rows of 128 bytes further
-                        const uint64_t da = FORM == EXPERTS_WEIGHT ? tile_descriptor(at_a + k * 2048, 64 * 128) : tile_descriptor(at_a + k * 32, 16);
-                        const uint64_t db = FORM == EXPERTS_FORWARD ? tile_descriptor(at_b + k * 32, 16) : tile_descriptor(at_b + k * 2048, 64 * 128);
-                        product(d, da, db, a.descriptor, kb || k);
+                        product(d, da + k * (FORM == EXPERTS_WEIGHT ? 128 : 2), high_a, db + k * (FORM == EXPERTS_FORWARD ? 2 : 128), high_b, a.descriptor, kb || k);
                     }
                     commit(empty + 8 * s);
                 }
                 __syncwarp();
+                if (++s == kStages) { s = 0; parity ^= 1; }
             }
             if (kb < blocks) break;
-            if (lane == 0) commit(sums_full + 8 * buffer);
+            if (elect_one()) commit(sums_full + 8 * buffer);
             done++;
         }
     } else if (warp < kGroupedWarps) {
-        char* const stage = staging + warp * 4096;
+        char* const stage = staging + (M < kTileM ? warp / 4 : warp) * 4096;
         unsigned done = 0;
         const bool vec = a.n % 8 == 0 && aligned16(a.c);
         const unsigned quarter = warp % 4, half = warp / 4;
-        for (unsigned long long tile = blockIdx.x; tile < total; tile += gridDim.x) {
-            const GroupedPlace p = grouped_place(FORM, tile, N, a, first, a.starts);
+        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
             const int rows = quarter * 32 < p.rows ? (int)(p.rows - quarter * 32 < 32 ? p.rows - quarter * 32 : 32) : 0;
-            T* const to = reinterpret_cast<T*>(a.c) + (rows ? grouped_row(FORM, p, quarter * 32, a) : 0);
+            const size_t row = grouped_row(FORM, p, quarter * 32, a);
             const bool summed = p.k_count != 0;         // otherwise nothing was: rows of nobody, an expert without rows
             const unsigned buffer = done & 1;
             if (summed) {
@@ -196,20 +246,25 @@ template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupe
 #pragma unroll
                     for (int e = 0; e < 32; e++) v[e] = __uint_as_float(r[e]);
                 }
+                if (a.splits.d > 1) {
+                    stage_rows(stage, v);
+                    store_fp32(stage, a.partial + (p.split * grouped_rows(FORM, a) + row) * a.partial_stride + column, a.partial_stride, rows, columns);
+                    continue;
+                }
                 if constexpr (FORM == EXPERTS_FORWARD) {
                     if (summed && a.act != kNoActivation) {
                         if (a.z) {
                             stage_rows(stage, v);
-                            store_fp32(stage, a.z + (p.row + quarter * 32) * a.z_stride + column, a.z_stride, rows, columns);
+                            store_fp32(stage, a.z + row * a.z_stride + column, a.z_stride, rows, columns);
                         }
                         with_activation(a.act, [&](auto act) {
 #pragma unroll
-                            for (int e = 0; e < 32; e++) v[e] = activate<decltype(act)::value>(v[e]);
+                            for (int e = 0; e < 32; e++) v[e] = value_of<decltype(act)::value>(v[e]);
                         });
                     }
                 }
                 stage_rows(stage, v);
-                store_as<T>(stage, to + column, a.n, rows, columns, vec);
+                store_as<T>(stage, reinterpret_cast<T*>(a.c) + row * a.n + column, a.n, rows, columns, vec);
             }
             if (!summed) continue;
             done++;
@@ -221,10 +276,10 @@ template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupe
     __syncthreads();
     if (failed) {       // no wait is expected to run out: copies in flight still have to land, and products to end, before the memory is given back
         int late = 0;
-        grouped_mark(FORM, a, N, first, a.starts, reinterpret_cast<uint16_t*>(a.c), a.z, a.z_stride, blockIdx.x, gridDim.x, threadIdx.x, kGroupedThreads);
+        grouped_mark(FORM, a, a, first, starts, blockIdx.x, gridDim.x, threadIdx.x, kGroupedThreads);
         if (warp == kGroupedLoader && lane == 0)
             for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
-        if (warp == kGroupedMultiplier && lane == 0) {
+        if (warp == kGroupedMultiplier && elect_one()) {        // the lane whose products they are
             commit(drained);
             bar_wait(drained, 0, &late);
         }
@@ -235,37 +290,91 @@ template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupe
     if (warp == kGroupedMultiplier) tmem_free(sums, 2 * N);
 }
 
-struct PadRowsArgs { const void* from[2]; void* to[2]; size_t rows[2]; unsigned width, stride; };
+struct JoinPartsArgs { const float* partial; size_t rows, stride; unsigned n, splits, runs; int act; void* c; float* z; size_t z_stride; bool vec; };
 
-/** Rows that do not start on 16 bytes, copied to some that do, for the tiled loads: eight elements per thread. Nobody reads what is behind a row. */
-__global__ void __launch_bounds__(256) k_pad_rows(const __grid_constant__ PadRowsArgs a) {
+/** Adds the parts that splits of k left, in the order of k, and finishes: four columns per thread. */
+template <typename T> __global__ void __launch_bounds__(256) k_join_parts(const __grid_constant__ JoinPartsArgs a) {
     wait_for_stream();
-    const unsigned runs = a.stride / 8;
-    size_t index = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int w = index >= a.rows[0] * runs;
-    if (w) index -= a.rows[0] * runs;
-    if (index >= a.rows[w] * runs) return;
-    const size_t row = index / runs;
-    const unsigned column = (unsigned)(index % runs) * 8;
-    const uint16_t* from = reinterpret_cast<const uint16_t*>(a.from[w]) + row * a.width + column;
-    Run<uint16_t, 8> r = {};
+    const size_t index = (size_t)blockIdx.x * 256 + threadIdx.x, row = index / a.runs;
+    if (row >= a.rows) return;
+    const unsigned column = (unsigned)(index - row * a.runs) * 4;
+    const float* from = a.partial + row * a.stride + column;
+    Run<float, 4> v = {};
+#pragma unroll 4
+    for (unsigned s = 0; s < a.splits; s++) {
+        const Run<float, 4> p = ld_run<float, 4>(from + s * a.rows * a.stride);
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-        if (column + e < a.width) r.e[e] = from[e];
-    st_run<uint16_t, 8>(reinterpret_cast<uint16_t*>(a.to[w]) + row * a.stride + column, r);
+        for (int e = 0; e < 4; e++) v.e[e] += p.e[e];
+    }
+    if (a.act != kNoActivation) {
+        if (a.z) st_run<float, 4>(a.z + row * a.z_stride + column, v);      // rows of these end on four elements as well
+        with_activation(a.act, [&](auto act) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v.e[e] = value_of<decltype(act)::value>(v.e[e]);
+        });
+    }
+    T* to = reinterpret_cast<T*>(a.c) + row * a.n + column;
+    if (a.vec) st_run<T, 4>(to, round_run<T, 4>(v.e));
+    else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (column + e < a.n) to[e] = Traits<T>::down(v.e[e]);
 }
 
-struct ActGradArgs { const void* dh; const float* z; void* dz; const int* starts; size_t z_stride, stride; unsigned rows, experts, n; int act; };
+constexpr int kRowCta = 256;
+
+struct PadRowsArgs { const uint16_t* from[2]; uint16_t* to[2]; size_t rows[2]; unsigned width, runs, across; };
+
+/**
+ * Rows that do not start on 16 bytes, copied to some that do, for the tiled loads; zeros behind a row. A thread writes eight elements at a time and reads the two
+ * aligned pieces of 16 bytes that hold them, where those lie inside of the operand; the second is the neighbour's first, and comes from L1.
+ */
+__global__ void __launch_bounds__(kRowCta) k_pad_rows(const __grid_constant__ PadRowsArgs a) {
+    wait_for_stream();
+    size_t row = (size_t)blockIdx.x * (kRowCta / a.across) + threadIdx.x / a.across;
+    if (threadIdx.x / a.across >= kRowCta / a.across) return;
+    const int w = row >= a.rows[0];
+    if (w) row -= a.rows[0];
+    if (row >= a.rows[w]) return;
+    const uint16_t *begin = a.from[w], *from = begin + row * a.width, *end = begin + a.rows[w] * a.width;
+    const unsigned off = reinterpret_cast<uintptr_t>(from) % 16 / 2;        // elements behind a boundary
+    for (unsigned i = threadIdx.x % a.across; i < a.runs; i += a.across) {
+        const uint16_t* at = from + 8 * i;
+        Run<uint16_t, 8> r = {};
+        if (at - off >= begin && at - off + 16 <= end && 8 * i + 8 <= a.width) {
+            uint32_t v[8];
+            *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(at - off);
+            *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(at - off + 8);
+            // first by whole words, then by half of one
+#pragma unroll
+            for (int by = 4; by >= 1; by /= 2)
+                if (off / 2 & by) {
+#pragma unroll
+                    for (int q = 0; q + by < 8; q++) v[q] = v[q + by];
+                }
+            uint32_t* const o = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+            for (int q = 0; q < 4; q++) o[q] = off & 1 ? __funnelshift_r(v[q], v[q + 1], 16) : v[q];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (8 * i + e < a.width) r.e[e] = at[e];
+        }
+        st_run<uint16_t, 8>(a.to[w] + (row * a.runs + i) * 8, r);
+    }
+}
+
+struct ActGradArgs { const void* dh; const float* z; void* dz; const int* starts; size_t z_stride, stride; unsigned rows, experts, n, from, threads; Divisor runs; int act; };
 
 /** dz from dh and the saved products, eight elements per thread; rows of nobody, whose products nobody wrote, are left out. Only the rows of dh may start
- *  anywhere (VEC: they do not). */
-template <typename T, bool VEC> __global__ void __launch_bounds__(256) k_act_grad(const __grid_constant__ ActGradArgs a) {
+ *  anywhere (VEC: they do not). HBM bounds it: 8 bytes per element. */
+template <typename T, bool VEC> __global__ void __launch_bounds__(kRowCta) k_act_grad(const __grid_constant__ ActGradArgs a) {
     wait_for_stream();
-    const unsigned runs = (a.n + 7) / 8;
-    const size_t index = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const size_t row = index / runs;
-    if (row >= a.rows || row >= row_within(a.starts[a.experts], a.rows)) return;
-    const unsigned column = (unsigned)(index % runs) * 8;
+    const unsigned index = blockIdx.x * kRowCta + threadIdx.x;
+    if (index >= a.threads) return;
+    const unsigned line = a.runs.quotient(index), column = (index - line * a.runs.d) * 8;
+    const size_t row = (size_t)a.from + line;
+    if (row >= row_within(a.starts[a.experts], a.rows)) return;
     float z[8] = {}, d[8];
 #pragma unroll
     for (int q = 0; q < 2; q++) {
@@ -285,11 +394,7 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) k_act_gra
     }
     with_activation(a.act, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            float value, slope;
-            activate_grad<decltype(act)::value>(z[e], value, slope);
-            d[e] *= slope;
-        }
+        for (int e = 0; e < 8; e++) d[e] *= slope_of<decltype(act)::value>(z[e]);
     });
     st_run<T, 8>(reinterpret_cast<T*>(a.dz) + row * a.stride + column, round_run<T, 8>(d));
 }
@@ -297,11 +402,14 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) k_act_gra
 /* ------------------------------------------------------------------------------------------------ host side */
 
 /** Where the parts of a call's workspace lie. */
-struct GroupedLayout { size_t stride, x, w, padded, dz, d_stride, total; bool ok; };
+struct GroupedLayout { size_t stride, x, w, padded, dz, d_stride, partial, total; GroupedPlan forward, input, weight; bool ok; };
+
+static size_t parts_of(const GroupedPlan& p, size_t rows, size_t n) { return p.splits > 1 ? p.splits * rows * up_to(n, 4) * sizeof(float) : 0; }
 
 static GroupedLayout grouped_layout(int device, size_t rows, int experts, size_t width, size_t out, bool aligned, bool backward) {
     GroupedLayout l = {};
-    l.ok = sm_count(device) > 0 && rows <= DCCL_EXPERTS_MAX_PLACES && experts >= 1 && experts <= DCCL_EXPERTS_MAX && width >= 1 && width <= DCCL_EXPERTS_MAX_WIDTH && out >= 1
+    const int sms = sm_count(device);
+    l.ok = sms > 0 && rows <= DCCL_EXPERTS_MAX_PLACES && experts >= 1 && experts <= DCCL_EXPERTS_MAX && width >= 1 && width <= DCCL_EXPERTS_MAX_WIDTH && out >= 1
            && out <= DCCL_EXPERTS_MAX_WIDTH;
     if (!l.ok) return l;
     size_t at = 0;
@@ -315,46 +423,80 @@ static GroupedLayout grouped_layout(int device, size_t rows, int experts, size_t
         if (backward) at = 0;
     }
     l.d_stride = up_to(out, 8);
-    if (backward) l.dz = take(rows * l.d_stride * 2);
+    l.forward = plan_grouped(EXPERTS_FORWARD, sms, rows, experts, 0, out, width);
+    l.input = plan_grouped(EXPERTS_INPUT, sms, rows, experts, 0, width, out);
+    l.weight = plan_grouped(EXPERTS_WEIGHT, sms, rows, experts, out, width, 0);
+    if (backward) {
+        l.dz = take(rows * l.d_stride * 2);
+        const size_t input = parts_of(l.input, rows, width), weight = parts_of(l.weight, experts * out, width);
+        l.partial = take(input > weight ? input : weight);
+    } else {
+        l.partial = take(parts_of(l.forward, rows, out));
+    }
     l.total = at;
     return l;
 }
 
-template <typename T, int FORM, int N> static cudaError_t run_grouped(int device, GroupedArgs& a, size_t most_tiles, cudaStream_t stream) {
+template <typename T, int FORM, int M, int N> static cudaError_t run_grouped(int device, GroupedArgs& a, cudaStream_t stream) {
     static std::atomic<bool> ready[64];
     if (!ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k_grouped<T, FORM, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, GroupedShape<N>::kShared);
+        const cudaError_t e = cudaFuncSetAttribute(k_grouped<T, FORM, M, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, GroupedShape<M, N>::kShared);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_relaxed);
     }
     a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == EXPERTS_WEIGHT, FORM != EXPERTS_FORWARD, kTileM, N);
-    a.gave_up = gave_up_flag(device);
-    const size_t workers = sm_count(device);
-    return launch_early_shared(k_grouped<T, FORM, N>, (unsigned)(most_tiles < workers ? most_tiles : workers), kGroupedThreads, GroupedShape<N>::kShared, stream, a);
+    const unsigned workers = (unsigned)sm_count(device) * GroupedShape<M, N>::kCtas;
+    return launch_early_shared(k_grouped<T, FORM, M, N>, a.most < workers ? a.most : workers, kGroupedThreads, GroupedShape<M, N>::kShared, stream, a);
 }
 
-/** Tiles of 128 columns where those of 256 would leave SMs without one, with the rows spread evenly. */
-static int grouped_columns(int device, int form, const GroupedArgs& a) {
-    const size_t rows_of_tiles = form == EXPERTS_WEIGHT ? (size_t)a.experts * blocks_of(a.m, kTileM)
-                                 : a.experts < a.rows   ? a.experts * (size_t)blocks_of(blocks_of(a.rows, a.experts), kTileM)
-                                                        : a.rows;
-    return rows_of_tiles * blocks_of(a.n, 256) < (size_t)sm_count(device) ? 128 : 256;
-}
-
-template <typename T, int FORM> static cudaError_t run_grouped(int device, GroupedArgs& a, cudaStream_t stream) {
-    const int columns = grouped_columns(device, FORM, a);
-    a.tiles_m = FORM == EXPERTS_WEIGHT ? blocks_of(a.m, kTileM) : 0;
-    a.tiles_n = blocks_of(a.n, columns);
+template <typename T, int FORM> static cudaError_t run_grouped(int device, const GroupedPlan& p, GroupedArgs& a, cudaStream_t stream) {
+    a.tile_rows = p.tile_rows;
+    a.tile_columns = p.tile_columns;
+    a.tiles_m = FORM == EXPERTS_WEIGHT ? blocks_of(a.m, p.tile_rows) : 0;
+    a.tiles_n = By(blocks_of(a.n, p.tile_columns));
+    a.group = By(16 * a.tiles_n.d);
+    a.expert = By(FORM == EXPERTS_WEIGHT ? a.tiles_m * a.tiles_n.d : 1);
+    a.splits = By(p.splits);
     // every expert may have a row of tiles that is not full, and the rows of nobody another
-    const size_t most = (FORM == EXPERTS_WEIGHT ? (size_t)a.experts * a.tiles_m : blocks_of(a.rows, kTileM) + (size_t)a.experts + 1) * a.tiles_n;
-    return columns == 128 ? run_grouped<T, FORM, 128>(device, a, most, stream) : run_grouped<T, FORM, 256>(device, a, most, stream);
+    const unsigned long long most = (FORM == EXPERTS_WEIGHT ? (unsigned long long)a.experts * a.tiles_m : blocks_of(a.rows, p.tile_rows) + a.experts + 1ull) * a.tiles_n.d * p.splits;
+    if (most > 1u << 30 || 16ull * a.tiles_n.d * (a.tiles_m ? a.tiles_m : 1) > 1u << 30) return cudaErrorInvalidValue;      // places are counted in 31 bits
+    a.most = (unsigned)most;
+    a.partial_stride = up_to(a.n, 4);
+    a.gave_up = gave_up_flag(device);
+    cudaError_t e;
+    if constexpr (FORM == EXPERTS_FORWARD) {
+        e = p.tile_rows == 32        ? run_grouped<T, FORM, 32, 64>(device, a, stream)
+            : p.tile_columns == 128 ? run_grouped<T, FORM, 128, 128>(device, a, stream)
+                                    : run_grouped<T, FORM, 128, 256>(device, a, stream);
+    } else {
+        e = p.tile_columns == 128 ? run_grouped<T, FORM, 128, 128>(device, a, stream) : run_grouped<T, FORM, 128, 256>(device, a, stream);
+    }
+    if (e != cudaSuccess || p.splits == 1) return e;
+    const JoinPartsArgs j = {a.partial, grouped_rows(FORM, a), a.partial_stride, a.n, p.splits, (unsigned)(a.partial_stride / 4), a.act, a.c, a.z, a.z_stride,
+                             a.n % 4 == 0 && aligned_to(8, {a.c})};
+    return launch_early(k_join_parts<T>, (unsigned)((j.rows * j.runs + 255) / 256), 256, stream, j);
 }
 
 static cudaError_t pad_rows(const void*& x, const void*& w, size_t rows, size_t w_rows, size_t width, size_t stride, void* to_x, void* to_w, cudaStream_t stream) {
-    const PadRowsArgs a = {{x, w}, {to_x, to_w}, {rows, w_rows}, (unsigned)width, (unsigned)stride};
+    PadRowsArgs a = {{(const uint16_t*)x, (const uint16_t*)w}, {(uint16_t*)to_x, (uint16_t*)to_w}, {rows, w_rows}, (unsigned)width, (unsigned)(stride / 8), kRowCta};
+    if (a.runs < kRowCta) a.across = (a.runs + 31) / 32 * 32;
     x = to_x;
     w = to_w;
-    return launch_early(k_pad_rows, (unsigned)(((rows + w_rows) * (stride / 8) + 255) / 256), 256, stream, a);
+    const size_t per = kRowCta / a.across;
+    return launch_early(k_pad_rows, (unsigned)((rows + w_rows + per - 1) / per), kRowCta, stream, a);
+}
+
+/** In launches of less than 2^31 threads. */
+template <typename T> static cudaError_t run_act_grad(ActGradArgs a, bool vec, cudaStream_t stream) {
+    a.runs = Divisor((a.n + 7) / 8);
+    const unsigned most = ((1u << 31) - 1) / a.runs.d;
+    cudaError_t e = cudaSuccess;
+    for (size_t from = 0; from < a.rows && e == cudaSuccess; from += most) {
+        a.from = (unsigned)from;
+        a.threads = (unsigned)(a.rows - from < most ? a.rows - from : most) * a.runs.d;
+        e = launch_early(vec ? k_act_grad<T, true> : k_act_grad<T, false>, (a.threads + kRowCta - 1) / kRowCta, kRowCta, stream, a);
+    }
+    return e;
 }
 
 struct GroupedCall {
@@ -365,12 +507,13 @@ struct GroupedCall {
     cudaStream_t stream;
 };
 
-static GroupedArgs grouped_args(const GroupedCall& k) {
+static GroupedArgs grouped_args(const GroupedCall& k, const GroupedLayout& l) {
     GroupedArgs a = {};
+    a.partial = (float*)(k.workspace + l.partial);
     a.rows = (unsigned)k.rows;
     a.experts = (unsigned)k.experts;
     a.starts = k.starts;
-    a.act = k.act;
+    a.act = kNoActivation;
     a.stride = (a.experts + kListed) / kListed;       // experts and rows of nobody in at most kListed entries
     return a;
 }
@@ -378,15 +521,16 @@ static GroupedArgs grouped_args(const GroupedCall& k) {
 template <typename T> static cudaError_t grouped_forward(const GroupedCall& k, const GroupedLayout& l, const void* x, const void* w, void* h, float* z, size_t z_stride) {
     cudaError_t e = cudaSuccess;
     if (l.padded) e = pad_rows(x, w, k.rows, (size_t)k.experts * k.out, k.width, l.stride, k.workspace + l.x, k.workspace + l.w, k.stream);
-    GroupedArgs a = grouped_args(k);
+    GroupedArgs a = grouped_args(k, l);
     a.n = (unsigned)k.out;
     a.k_blocks = blocks_of(k.width, kTileK);
+    a.act = k.act;
     a.c = h;
     a.z = z;
     a.z_stride = z_stride;
-    if (e == cudaSuccess) e = make_map(&a.a, k.dtype, x, k.width, k.rows, l.stride, kTileM);
-    if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts}, {l.stride, l.stride * k.out}, grouped_columns(k.device, EXPERTS_FORWARD, a));
-    return e == cudaSuccess ? run_grouped<T, EXPERTS_FORWARD>(k.device, a, k.stream) : e;
+    if (e == cudaSuccess) e = make_map(&a.a, k.dtype, x, k.width, k.rows, l.stride, l.forward.tile_rows);
+    if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts}, {l.stride, l.stride * k.out}, l.forward.tile_columns);
+    return e == cudaSuccess ? run_grouped<T, EXPERTS_FORWARD>(k.device, l.forward, a, k.stream) : e;
 }
 
 template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, const GroupedLayout& l, const void* dh, const float* z, size_t z_stride, const void* x, const void* w,
@@ -395,8 +539,18 @@ template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, 
     const void* dz = dh;
     const bool vec = k.out % 8 == 0 && aligned_to(16, {dh});
     if (k.act != kNoActivation) {
-        const ActGradArgs d = {dh, z, k.workspace + l.dz, k.starts, z_stride, l.d_stride, (unsigned)k.rows, (unsigned)k.experts, (unsigned)k.out, k.act};
-        e = launch_early(vec ? k_act_grad<T, true> : k_act_grad<T, false>, (unsigned)((k.rows * ((k.out + 7) / 8) + 255) / 256), 256, k.stream, d);
+        ActGradArgs d = {};
+        d.dh = dh;
+        d.z = z;
+        d.dz = k.workspace + l.dz;
+        d.starts = k.starts;
+        d.z_stride = z_stride;
+        d.stride = l.d_stride;
+        d.rows = (unsigned)k.rows;
+        d.experts = (unsigned)k.experts;
+        d.n = (unsigned)k.out;
+        d.act = k.act;
+        e = run_act_grad<T>(d, vec, k.stream);
         dz = d.dz;
     } else if (!vec) {
         const void* none = nullptr;
@@ -408,22 +562,22 @@ template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, 
     }
     const size_t d_stride = dz == dh ? k.out : l.d_stride;
     if (e == cudaSuccess && dx) {
-        GroupedArgs a = grouped_args(k);
+        GroupedArgs a = grouped_args(k, l);
         a.n = (unsigned)k.width;
         a.k_blocks = blocks_of(k.out, kTileK);
         a.c = dx;
         e = make_map(&a.a, k.dtype, dz, k.out, k.rows, d_stride, kTileM);
         if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts}, {l.stride, l.stride * k.out}, kTileK);
-        if (e == cudaSuccess) e = run_grouped<T, EXPERTS_INPUT>(k.device, a, k.stream);
+        if (e == cudaSuccess) e = run_grouped<T, EXPERTS_INPUT>(k.device, l.input, a, k.stream);
     }
     if (e == cudaSuccess && dw) {
-        GroupedArgs a = grouped_args(k);
+        GroupedArgs a = grouped_args(k, l);
         a.m = (unsigned)k.out;
         a.n = (unsigned)k.width;
         a.c = dw;
         e = make_map(&a.a, k.dtype, dz, k.out, k.rows, d_stride, kTileK);
         if (e == cudaSuccess) e = make_map(&a.b, k.dtype, x, k.width, k.rows, l.stride, kTileK);
-        if (e == cudaSuccess) e = run_grouped<T, EXPERTS_WEIGHT>(k.device, a, k.stream);
+        if (e == cudaSuccess) e = run_grouped<T, EXPERTS_WEIGHT>(k.device, l.weight, a, k.stream);
     }
     return e;
 }

@@ -13,15 +13,32 @@ enum GroupedForm {
     EXPERTS_WEIGHT,         // dW = dz^T x: the rows of a tile are some of `out`, its columns some of `width`, and k are the expert's rows
 };
 
+/** Division of n < 2^31 by a number that the host knows, as Divisor of row_access.cuh does it. */
+struct By {
+    unsigned d, m, s;
+    By() = default;
+    explicit By(unsigned divisor) : d(divisor), s(0) {
+        while (s < 31 && (1u << s) < d) s++;
+        m = (unsigned)((((uint64_t)1 << (32 + s)) + d - 1) / d - ((uint64_t)1 << 32));
+    }
+    DCCL_BOTH unsigned quotient(unsigned n) const { return ((unsigned)((uint64_t)n * m >> 32) + n) >> s; }
+};
+
 struct Grouped {
     unsigned rows, experts;                 // of all
     unsigned m, n;                          // EXPERTS_WEIGHT: rows of one expert's result; columns of the result
-    unsigned tiles_m, tiles_n, k_blocks;    // EXPERTS_WEIGHT: rows of tiles; columns of tiles; otherwise: blocks of k
+    unsigned tile_rows, tile_columns;
+    unsigned tiles_m, k_blocks;             // EXPERTS_WEIGHT: rows of tiles; otherwise: blocks of k
     unsigned stride;                        // otherwise: experts of one entry of the list of tiles
+    unsigned most;                          // tiles, whatever the starts are
+    By tiles_n, group, expert, splits;      // columns of tiles; tiles of 16 rows of them; EXPERTS_WEIGHT: of an expert; parts that the k of a tile is cut into
 };
 
+/** What a product leaves where: c of 16 bits, and in fp32 the products before their activation (EXPERTS_FORWARD), or the parts of a sum that is cut, [split][row][partial_stride]. */
+struct GroupedResults { void* c; float* z; size_t z_stride; float* partial; size_t partial_stride; };
+
 /** The list has room for this many entries and the end: shared memory beside the tiles has no more. */
-constexpr unsigned kListed = 256;
+constexpr unsigned kListed = 120;
 
 /** Rows of an expert, whatever the numbers are: inside of [0, rows), and none where the next starts before. The last is of nobody, and goes to the end. */
 struct Span { unsigned from, count; };
@@ -31,82 +48,125 @@ DCCL_BOTH Span span_of(const int* starts, unsigned e, unsigned experts, unsigned
     return {from, to > from ? to - from : 0};
 }
 
-DCCL_BOTH unsigned tall_of(const int* starts, unsigned e, unsigned experts, unsigned rows) { return (span_of(starts, e, experts, rows).count + kTileM - 1) / kTileM; }
+DCCL_BOTH unsigned tall_of(const int* starts, unsigned e, const Grouped& a) { return (span_of(starts, e, a.experts, a.rows).count + a.tile_rows - 1) / a.tile_rows; }
 
 /** Entries of the list: the experts and the rows of nobody, `stride` each. */
 DCCL_BOTH unsigned listed_of(const Grouped& a) { return (a.experts + a.stride) / a.stride; }
 
-/** One tile: rows [row, row + rows) of the result (EXPERTS_WEIGHT: of the expert's), columns from `column`, and the k that it adds up. */
-struct GroupedPlace { unsigned expert, row, rows, column, k_from, k_count; };
+/** One tile, or a part of it: rows [row, row + rows) of the result (EXPERTS_WEIGHT: of the expert's), columns from `column`, and the k that it adds up. */
+struct GroupedPlace { unsigned expert, row, rows, column, k_from, k_count, split; };
 
 /**
- * Tile number -> place, of tiles of kTileM x `columns`. first[i]: rows of tiles before expert i * stride, and all of them (the rows of nobody are the last
- * "expert"). Groups of 16 rows of tiles are walked column by column, so that the tiles of one moment share operands in L2.
+ * Tile number -> place. first[i]: rows of tiles before expert i * stride, and all of them (the rows of nobody are the last "expert"). Groups of 16 rows of tiles
+ * are walked column by column, so that the tiles of one moment share operands in L2.
  */
-DCCL_BOTH GroupedPlace grouped_place(int form, unsigned long long tile, unsigned columns, const Grouped& a, const unsigned* first, const int* starts) {
+DCCL_BOTH GroupedPlace grouped_place(int form, unsigned tile, const Grouped& a, const unsigned* first, const int* starts) {
     GroupedPlace p;
-    unsigned tiles_m, within;
+    unsigned tiles_m, within, part = a.splits.quotient(tile);
+    p.split = tile - part * a.splits.d;
     if (form == EXPERTS_WEIGHT) {
-        const unsigned per = a.tiles_m * a.tiles_n;
-        p.expert = (unsigned)(tile / per);
-        within = (unsigned)(tile % per);
+        p.expert = a.expert.quotient(part);
+        within = part - p.expert * a.expert.d;
         tiles_m = a.tiles_m;
     } else {
         unsigned low = 0, high = listed_of(a);
         while (high - low > 1) {
             const unsigned mid = (low + high) / 2;
-            if ((unsigned long long)first[mid] * a.tiles_n <= tile) low = mid;
+            if ((unsigned long long)first[mid] * a.tiles_n.d <= part) low = mid;
             else high = mid;
         }
-        unsigned long long at = (unsigned long long)first[low] * a.tiles_n;
+        unsigned long long at = (unsigned long long)first[low] * a.tiles_n.d;
         p.expert = low * a.stride;
-        tiles_m = tall_of(starts, p.expert, a.experts, a.rows);
-        while (p.expert < a.experts && tile - at >= (unsigned long long)tiles_m * a.tiles_n) {
-            at += (unsigned long long)tiles_m * a.tiles_n;
-            tiles_m = tall_of(starts, ++p.expert, a.experts, a.rows);
+        tiles_m = tall_of(starts, p.expert, a);
+        while (p.expert < a.experts && part - at >= (unsigned long long)tiles_m * a.tiles_n.d) {
+            at += (unsigned long long)tiles_m * a.tiles_n.d;
+            tiles_m = tall_of(starts, ++p.expert, a);
         }
-        within = (unsigned)(tile - at);
+        within = (unsigned)(part - at);
     }
-    const unsigned group = within / (16 * a.tiles_n), top = group * 16, tall = tiles_m - top < 16 ? tiles_m - top : 16;
-    within -= top * a.tiles_n;
-    const unsigned m = top + within % tall;
-    p.column = within / tall * columns;
+    const unsigned group = a.group.quotient(within), top = group * 16, tall = tiles_m - top < 16 ? tiles_m - top : 16;
+    within -= group * a.group.d;
+    const unsigned n = tall == 16 ? within / 16 : within / tall, m = top + within - n * tall;
+    p.column = n * a.tile_columns;
     const Span s = span_of(starts, p.expert, a.experts, a.rows);
+    unsigned count, blocks;
     if (form == EXPERTS_WEIGHT) {
-        p.row = m * kTileM;
-        p.rows = a.m - p.row < (unsigned)kTileM ? a.m - p.row : kTileM;
+        p.row = m * a.tile_rows;
+        p.rows = a.m - p.row < a.tile_rows ? a.m - p.row : a.tile_rows;
         p.k_from = s.from;
-        p.k_count = s.count;
+        count = s.count;
     } else {
-        p.row = s.from + m * kTileM;
+        p.row = s.from + m * a.tile_rows;
         // (starts that are not in order may give more tiles than can be counted)
-        p.rows = m * kTileM >= s.count ? 0 : s.count - m * kTileM < (unsigned)kTileM ? s.count - m * kTileM : kTileM;
+        p.rows = m * a.tile_rows >= s.count ? 0 : s.count - m * a.tile_rows < a.tile_rows ? s.count - m * a.tile_rows : a.tile_rows;
         p.k_from = 0;
-        p.k_count = p.expert < a.experts ? a.k_blocks * kTileK : 0;
+        count = p.expert < a.experts ? a.k_blocks * kTileK : 0;
     }
+    blocks = (count + kTileK - 1) / kTileK;
+    if (a.splits.d > 1) {           // whole blocks for each part, in order
+        const unsigned from = (unsigned)((uint64_t)blocks * p.split / a.splits.d) * kTileK, to = (unsigned)((uint64_t)blocks * (p.split + 1) / a.splits.d) * kTileK;
+        p.k_from += from;
+        count = (to < count ? to : count) - from;
+    }
+    p.k_count = count;
     return p;
 }
 
-/** Tiles of a whole product. */
-DCCL_BOTH unsigned long long grouped_tiles(int form, const Grouped& a, const unsigned* first) {
-    return form == EXPERTS_WEIGHT ? (unsigned long long)a.experts * a.tiles_m * a.tiles_n : (unsigned long long)first[listed_of(a)] * a.tiles_n;
+/** Tiles of a whole product, parts of tiles counted each. */
+DCCL_BOTH unsigned grouped_tiles(int form, const Grouped& a, const unsigned* first) {
+    if (form == EXPERTS_WEIGHT) return a.most;
+    const unsigned long long tiles = (unsigned long long)first[listed_of(a)] * a.tiles_n.d * a.splits.d;
+    return tiles < a.most ? (unsigned)tiles : a.most;
 }
 
-/** First element of a row of the result. */
-DCCL_BOTH size_t grouped_row(int form, const GroupedPlace& p, unsigned row, const Grouped& a) { return ((size_t)(form == EXPERTS_WEIGHT ? p.expert : 0) * a.m + p.row + row) * a.n; }
+/** Number of a row of the result. */
+DCCL_BOTH size_t grouped_row(int form, const GroupedPlace& p, unsigned row, const Grouped& a) { return (size_t)(form == EXPERTS_WEIGHT ? p.expert : 0) * a.m + p.row + row; }
+/** Rows of the result. */
+DCCL_BOTH size_t grouped_rows(int form, const Grouped& a) { return form == EXPERTS_WEIGHT ? (size_t)a.experts * a.m : a.rows; }
 
-/** NaN in all that one CTA stores (first tile, step), by each of its threads. */
-DCCL_BOTH void grouped_mark(int form, const Grouped& a, unsigned columns, const unsigned* first, const int* starts, uint16_t* c, float* z, size_t z_stride, unsigned long long tile,
-                            unsigned long long step, unsigned thread, unsigned threads) {
-    for (const unsigned long long tiles = grouped_tiles(form, a, first); tile < tiles; tile += step) {
-        const GroupedPlace p = grouped_place(form, tile, columns, a, first, starts);
-        for (unsigned i = thread; i < p.rows * columns; i += threads) {
-            const unsigned row = i / columns, column = p.column + i % columns;
+/** NaN in all that one CTA stores (first tile, step), by each of its threads. What joins the parts hands the NaN of one on. */
+DCCL_BOTH void grouped_mark(int form, const Grouped& a, const GroupedResults& to, const unsigned* first, const int* starts, unsigned tile, unsigned step, unsigned thread, unsigned threads) {
+    for (const unsigned tiles = grouped_tiles(form, a, first); tile < tiles; tile += step) {
+        const GroupedPlace p = grouped_place(form, tile, a, first, starts);
+        for (unsigned i = thread; i < p.rows * a.tile_columns; i += threads) {
+            const unsigned row = i / a.tile_columns, column = p.column + i % a.tile_columns;
             if (column >= a.n) continue;
-            c[grouped_row(form, p, row, a) + column] = kNoResult16;
-            if (z && p.expert < a.experts) z[(p.row + row) * z_stride + column] = __builtin_nanf("");
+            const size_t at = grouped_row(form, p, row, a);
+            if (a.splits.d > 1) {
+                to.partial[(p.split * grouped_rows(form, a) + at) * to.partial_stride + column] = __builtin_nanf("");
+            } else {
+                reinterpret_cast<uint16_t*>(to.c)[at * a.n + column] = kNoResult16;
+                if (to.z && p.expert < a.experts) to.z[at * to.z_stride + column] = __builtin_nanf("");
+            }
         }
     }
+}
+
+/** Rows and columns of tiles, and the parts of k. */
+struct GroupedPlan { unsigned tile_rows, tile_columns, splits; };
+
+/**
+ * As if the experts had equal shares of the rows, which the host does not know. What a plan takes, in nanoseconds, is what one CTA takes for its tiles: a block of k is
+ * bound by what an SM can load, 117 GB/s (32 KB of a tile of 128 x 128 in 280 ns, 48 KB of one of 128 x 256 in 420), and a tile takes about one microsecond more;
+ * parts are stored in fp32, and added up by another launch.
+ * Up to 32 rows of an expert, forward: tiles of 32 x 64. Then reading the weights is all there is to do, and the tile's own rows should not be most of what it loads.
+ */
+inline GroupedPlan plan_grouped(int form, int sms, size_t rows, size_t experts, size_t m, size_t n, size_t k) {
+    const size_t busy = experts < rows ? experts : rows, each = busy ? (rows + busy - 1) / busy : 0;
+    if (form == EXPERTS_FORWARD && each <= 32) return {32, 64, 1};
+    const size_t high = form == EXPERTS_WEIGHT ? experts * blocks_of(m, kTileM) : busy * blocks_of(each, kTileM), blocks = blocks_of(form == EXPERTS_WEIGHT ? each : k, kTileK);
+    const size_t results = form == EXPERTS_WEIGHT ? experts * m : rows;
+    GroupedPlan best = {kTileM, 256, 1};
+    double least = 0;
+    for (unsigned columns = 256; columns >= 128; columns /= 2)
+        for (unsigned splits = 1; splits <= 16 && (splits == 1 || splits * 4 <= blocks); splits++) {
+            const size_t tiles = high * blocks_of(n, columns) * splits, rounds = (tiles + sms - 1) / sms;
+            if (splits > 1 && rounds > 4) break;
+            double cost = (double)rounds * ((double)((blocks + splits - 1) / splits) * (columns == 256 ? 420 : 280) + 1000);
+            if (splits > 1) cost += 3000 + (double)results * n * 8 * splits / 5000;
+            if (!least || cost < least) { least = cost; best = {kTileM, columns, splits}; }
+        }
+    return best;
 }
 
 } // namespace dccl

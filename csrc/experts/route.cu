@@ -6,9 +6,9 @@
  *     g = scale * dw;  renormalised: dz_j = r_j (g_j - sum g_i r_i) * (1, or 1 - s_j) with r the weights without scale, else
  *     softmax: dz_e = s_e (g_e - sum of the chosen s_i g_i),  sigmoid: dz_j = g_j s_j (1 - s_j)
  *
- * One warp per token, its logits in registers. Which expert is chosen must not hang on the rounding of an exponential. Without a bias both
- * scores grow with the logit, and logits are compared. With one, scores are compared in fp32; where two that matter lie closer
- * than fp32 can tell (about one token in two thousand of random fp32 logits), the warp does its token again in 64 bits.
+ * One warp per token, its logits in registers. Which expert is chosen must not hang on the rounding of an exponential: without a bias both
+ * scores grow with the logit, and logits are compared. With one scores are, in fp32; where two that matter lie closer
+ * than fp32 can tell (about one token in a thousand of random fp32 logits), the warp does its token again in 64 bits.
  */
 #include "expert_ops.hpp"
 #include "../kernels/launch_early.cuh"
@@ -29,118 +29,226 @@ struct RouteArgs {
     unsigned tokens, experts;
     DcclRouting how;
     Divisor group;              // by the experts of a group
+    unsigned ctas;              // at most
+    bool vec;                   // rows of the gradient start on 16 bytes
 };
 
 /** fp32 as a number whose order is that of the values. No NaN comes here. */
 __device__ __forceinline__ unsigned ordered(float v) {
     const unsigned b = __float_as_uint(v + 0.0f);       // of the two zeros the positive one
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float from_ordered(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ float from_ordered(unsigned k) { return __uint_as_float(k ^ (~(unsigned)((int)k >> 31) | 0x80000000u)); }
+constexpr unsigned kNothing = 0x007fffffu;             // ordered(-infinity)
 
-/** The largest value of the warp, and the lowest of the numbers that come with it; minus infinity and some number where all are. */
-__device__ __forceinline__ void best_of_warp(float& v, int& at) {
-    const unsigned key = ordered(v), top = __reduce_max_sync(kAll, key);
-    at = (int)__reduce_min_sync(kAll, key == top ? (unsigned)at : 0x7fffffffu);
-    v = from_ordered(top);
-}
-__device__ __forceinline__ void best_of_warp(double& v, int& at) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const double w = __shfl_xor_sync(kAll, v, o);
-        const int b = __shfl_xor_sync(kAll, at, o);
-        if (w > v || (w == v && b < at)) { v = w; at = b; }
-    }
-}
+__device__ __forceinline__ float largest_of_warp(float v) { return from_ordered(__reduce_max_sync(kAll, ordered(v))); }
 template <typename S> __device__ __forceinline__ S warp_sum(S v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
     return v;
 }
 
-template <typename S> __device__ __forceinline__ S nothing() { return -(S)INFINITY; }
-
 template <typename T> __device__ __forceinline__ float logit(const RouteArgs& a, size_t token, int e) {
     return Traits<T>::up(reinterpret_cast<const T*>(a.logits)[token * a.experts + e]);
 }
 
+/** The logits of the experts lane + 32 i; minus infinity behind the last. */
+template <typename T, int PER> __device__ __forceinline__ void load_logits(const RouteArgs& a, size_t token, float (&z)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int e = threadIdx.x % 32 + 32 * i;
+        z[i] = e < (int)a.experts ? logit<T>(a, token, e) : -INFINITY;
+    }
+}
+
+/** The two best of a set, and of another one that has none of its elements, or of one more element. */
+__device__ __forceinline__ void join_best(float& first, float& second, float f, float s) {
+    second = fmaxf(fminf(first, f), fmaxf(second, s));
+    first = fmaxf(first, f);
+}
+__device__ __forceinline__ void join_best(float& first, float& second, float c) {
+    second = fmaxf(second, fminf(first, c));
+    first = fmaxf(first, c);
+}
+
 /**
- * The choice by scores c[i] of the experts lane + 32 i (minus infinity: none): lane j < k gets the j-th expert, or -1. False where two that decide lie
- * within `unsure` (below zero: nobody asks) of each other, two groups within twice that, and are not the same numbers.
+ * The two best over the warp of each register: lane l gets those of register l / (32 / PER). With every step half of the registers go to the lanes that will keep
+ * them, and the others come.
  */
-template <typename T, typename S, int PER> __device__ __forceinline__ bool choose(const RouteArgs& a, size_t token, S (&c)[PER], S unsure, int& mine) {
+template <int PER> __device__ __forceinline__ void best_of_registers(float (&first)[PER], float (&second)[PER]) {
+    int o = 16;
+#pragma unroll
+    for (int n = PER / 2; n >= 1; n /= 2, o /= 2) {
+        const bool up = threadIdx.x & o;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const float f = __shfl_xor_sync(kAll, up ? first[i] : first[i + n], o), s = __shfl_xor_sync(kAll, up ? second[i] : second[i + n], o);
+            first[i] = up ? first[i + n] : first[i];
+            second[i] = up ? second[i + n] : second[i];
+            join_best(first[i], second[i], f, s);
+        }
+    }
+    for (; o; o /= 2) join_best(first[0], second[0], __shfl_xor_sync(kAll, first[0], o), __shfl_xor_sync(kAll, second[0], o));
+}
+
+/** A sorted list of a lane's keys, the largest first: Batcher's odd-even merge sort. */
+template <int PER> __device__ __forceinline__ void sort_keys(unsigned (&key)[PER]) {
+#pragma unroll
+    for (int p = 1; p < PER; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < PER; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; i++)
+                    if (i + j + k < PER && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const unsigned x = key[i + j], y = key[i + j + k];
+                        key[i + j] = max(x, y);
+                        key[i + j + k] = min(x, y);
+                    }
+}
+
+/**
+ * The choice by scores c[i] of the experts lane + 32 i (minus infinity: none): lane j < k gets the j-th expert, or -1. False where two that decide lie so close
+ * that their order is not known: within `unsure`, or within `part` of their sizes, and are not the same numbers; two groups within twice that.
+ *
+ * The lowest bits of a score's key give way to the number of its register, lower ones first, so that a key says all: of equal ones the lowest i, and of those the
+ * first lane, is the lowest expert. What those bits told is in `part`.
+ */
+template <typename T, int PER> __device__ __forceinline__ bool choose(const RouteArgs& a, size_t token, float (&c)[PER], float unsure, int& mine) {
     const int lane = threadIdx.x % 32;
+    unsigned beyond = kNothing;         // of k = 32
+    int beyond_lane = 0;
+    constexpr float part = (PER + 2) * (1.0f / (1 << 23));
     bool sure = true;
     if (a.how.groups > 1) {
-        S of_group = nothing<S>();
-        const int size = (int)a.group.d;
-        for (int g = 0; g < a.how.groups; g++) {
-            S first = nothing<S>(), second = nothing<S>();
+        constexpr int spread = 32 / PER;
+        const int size = (int)a.group.d, whole = size % 32 ? 0 : size / 32;       // registers of a group, where it has whole ones
+        float first[PER], second[PER];          // where it has, of the group that ends with this register; otherwise in the first
+        if (whole) {
+            float f = -INFINITY, t = -INFINITY;
+            int left = whole;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                const int e = lane + 32 * i;
-                const S v = e >= g * size && e < (g + 1) * size ? c[i] : nothing<S>();
-                second = v > first ? first : v > second ? v : second;
-                first = v > first ? v : first;
+                join_best(f, t, c[i]);
+                const bool ends = --left == 0;
+                first[i] = ends ? f : -INFINITY;
+                second[i] = ends ? t : -INFINITY;
+                if (ends) {
+                    f = t = -INFINITY;
+                    left = whole;
+                }
             }
+            best_of_registers(first, second);
+        } else {
+            float f = -INFINITY, t = -INFINITY;
+            for (int g = 0; g < a.how.groups; g++) {
+                float one = -INFINITY, two = -INFINITY;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const S f = __shfl_xor_sync(kAll, first, o), s = __shfl_xor_sync(kAll, second, o);
-                const S low = f > first ? first : f;
-                first = f > first ? f : first;
-                second = s > second ? s : second;
-                second = low > second ? low : second;
+                for (int i = 0; i < PER; i++) {
+                    const int e = lane + 32 * i - g * size;
+                    join_best(one, two, e >= 0 && e < size ? c[i] : -INFINITY);
+                }
+                const unsigned key = ordered(one), top = __reduce_max_sync(kAll, key);
+                const int winner = __ffs(__ballot_sync(kAll, key == top)) - 1;
+                const unsigned next = __reduce_max_sync(kAll, lane == winner ? ordered(two) : key);
+                if (lane == g) { f = from_ordered(top); t = from_ordered(next); }
             }
-            if (lane == g) of_group = a.how.top2 && second > nothing<S>() ? first + second : first;
+            first[0] = f;
+            second[0] = t;
         }
-        unsigned kept = 0;
-        S last = 0;
+        const bool two = a.how.top2 && second[0] > -INFINITY;
+        unsigned kept = 0, key = ordered(two ? first[0] + second[0] : first[0]);
+        const float sizes = first[0] > -INFINITY ? fabsf(first[0]) + (two ? fabsf(second[0]) : 0.0f) : 0.0f;
+        const float largest = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(sizes)));
+        if (whole && lane % spread) key = kNothing;         // one lane speaks for a register
+        float last = 0.0f;
         for (int j = 0; j <= a.how.top_groups && j < a.how.groups; j++) {
-            S v = kept >> lane & 1 ? nothing<S>() : of_group;
-            int at = lane;
-            best_of_warp(v, at);
-            if (!(v > nothing<S>())) break;
+            const unsigned top = __reduce_max_sync(kAll, key);
+            if (top <= kNothing) break;
             if (j == a.how.top_groups) {        // the first that does not stay
-                sure = last - v > 2 * unsure;
+                sure = last - from_ordered(top) > 2 * (unsure + part * largest);
                 break;
             }
+            const int at = __ffs(__ballot_sync(kAll, key == top)) - 1;
             kept |= 1u << at;
-            last = v;
+            if (lane == at) key = kNothing;
+            last = from_ordered(top);
         }
+        if (whole) {
+            int end = whole - 1;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int e = lane + 32 * i;
-            if (e < (int)a.experts && !(kept >> a.group.quotient(e) & 1)) c[i] = nothing<S>();
+            for (int i = 0; i < PER; i++) {
+                if (!(kept >> (end * spread & 31) & 1)) c[i] = -INFINITY;
+                if (i == end) end += whole;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (lane + 32 * i < (int)a.experts && !(kept >> a.group.quotient(lane + 32 * i) & 1)) c[i] = -INFINITY;
         }
     }
-    mine = -1;
-    S last = 0;
-    int last_at = -1;
-    for (int j = 0; j <= a.how.k; j++) {
-        if (j == a.how.k && unsure < 0) break;          // nobody asks for the first that is not chosen
-        S v = c[0];
-        int at = lane;
+    unsigned key[PER];
 #pragma unroll
-        for (int i = 1; i < PER; i++)
-            if (c[i] > v) { v = c[i]; at = lane + 32 * i; }
-        best_of_warp(v, at);
-        if (!(v > nothing<S>())) break;
-        if (unsure >= 0 && j > 0 && !(last - v > unsure)
-            && !(logit<T>(a, token, last_at) == logit<T>(a, token, at) && (!a.bias || a.bias[last_at] == a.bias[at])))
+    for (int i = 0; i < PER; i++) key[i] = (ordered(c[i]) & ~(unsigned)(PER - 1)) | (PER - 1 - i);
+    if constexpr (PER <= 8) sort_keys(key);
+    unsigned mine_key = kNothing;
+    int mine_lane = 0;
+    for (int j = 0; j <= a.how.k; j++) {            // one more to see how far the first is that is not chosen
+        unsigned best = key[0];
+        if constexpr (PER > 8) {
+#pragma unroll
+            for (int i = 1; i < PER; i++) best = max(best, key[i]);
+        }
+        const unsigned top = __reduce_max_sync(kAll, best);
+        if (top <= kNothing) break;
+        const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
+        if constexpr (PER > 8) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (lane == winner && key[i] == top) key[i] = 0;
+        } else if (lane == winner) {
+#pragma unroll
+            for (int i = 0; i + 1 < PER; i++) key[i] = key[i + 1];
+            key[PER - 1] = 0;
+        }
+        if (lane == j) { mine_key = top; mine_lane = winner; }
+        if (j == a.how.k) { beyond = top; beyond_lane = winner; }
+    }
+    // lane j against lane j + 1; the last of 32 against what came after it
+    const bool there = mine_key > kNothing;
+    mine = there ? mine_lane + 32 * (PER - 1 - (int)(mine_key & (PER - 1))) : -1;
+    unsigned next_key = __shfl_down_sync(kAll, mine_key, 1);
+    int next = __shfl_down_sync(kAll, mine, 1);
+    if (lane == 31) {
+        next_key = beyond;
+        next = beyond_lane + 32 * (PER - 1 - (int)(beyond & (PER - 1)));
+    }
+    if (there && lane < a.how.k && next_key > kNothing) {
+        const float v = from_ordered(mine_key), w = from_ordered(next_key);
+        if (!(v - w > unsure + part * fmaxf(fabsf(v), fabsf(w)))
+            && !(logit<T>(a, token, mine) == logit<T>(a, token, next) && (!a.bias || a.bias[mine] == a.bias[next])))
             sure = false;
-        if (j == a.how.k) break;
-        if (lane == j) mine = at;
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (lane + 32 * i == at) c[i] = nothing<S>();
-        last = v;
-        last_at = at;
     }
+    sure = __all_sync(kAll, sure);
+    if (lane >= a.how.k) mine = -1;
     return sure;
 }
 
-/** The choice in 64 bits. */
-template <typename T, int PER> __device__ __noinline__ int choose_exactly(const RouteArgs& a, size_t token) {
+/** The same for 64 bits, in two halves: the largest value of the warp, and the first lane that has it. */
+__device__ __forceinline__ unsigned long long ordered(double v) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double largest_of_warp(double v, int& lane) {
+    const unsigned long long key = ordered(v);
+    const unsigned high = (unsigned)(key >> 32), top = __reduce_max_sync(kAll, high), low = __reduce_max_sync(kAll, high == top ? (unsigned)key : 0u);
+    lane = __ffs(__ballot_sync(kAll, high == top && (unsigned)key == low)) - 1;
+    return __shfl_sync(kAll, v, lane);
+}
+
+/** The choice in 64 bits. plain: by the logits. */
+template <typename T, int PER> __device__ __noinline__ int choose_exactly(const RouteArgs& a, size_t token, bool plain) {
     const int lane = threadIdx.x % 32;
     double c[PER], top = -INFINITY;
 #pragma unroll
@@ -150,9 +258,9 @@ template <typename T, int PER> __device__ __noinline__ int choose_exactly(const 
         top = c[i] > top ? c[i] : top;
     }
     double sum = 1;
-    if (!a.how.sigmoid) {
-        int at = 0;
-        best_of_warp(top, at);
+    if (!plain && !a.how.sigmoid) {
+        int at;
+        top = largest_of_warp(top, at);
         double part = 0;
 #pragma unroll
         for (int i = 0; i < PER; i++) part += c[i] > -INFINITY ? exp(c[i] - top) : 0.0;
@@ -160,25 +268,64 @@ template <typename T, int PER> __device__ __noinline__ int choose_exactly(const 
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        const int e = lane + 32 * i;
         if (!(c[i] > -INFINITY)) { c[i] = -INFINITY; continue; }
-        c[i] = (a.how.sigmoid ? 1.0 / (1.0 + exp(-c[i])) : exp(c[i] - top) / sum) + (a.bias ? (double)a.bias[e] : 0.0);
+        if (!plain) c[i] = (a.how.sigmoid ? 1.0 / (1.0 + exp(-c[i])) : exp(c[i] - top) / sum) + (a.bias ? (double)a.bias[lane + 32 * i] : 0.0);
         if (!(c[i] > -INFINITY)) c[i] = -INFINITY;          // NaN as well
     }
-    int mine;
-    choose<T, double, PER>(a, token, c, -1.0, mine);
+    if (a.how.groups > 1) {
+        const int size = (int)a.group.d;
+        double of_group = -INFINITY;
+        for (int g = 0; g < a.how.groups; g++) {
+            double first = -INFINITY, second = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int e = lane + 32 * i - g * size;
+                const double v = e >= 0 && e < size ? c[i] : -INFINITY;
+                second = v > first ? first : v > second ? v : second;
+                first = v > first ? v : first;
+            }
+            int at;
+            const double f = largest_of_warp(first, at);
+            if (a.how.top2) second = largest_of_warp(lane == at ? second : first, at);
+            first = f;
+            if (lane == g) of_group = a.how.top2 && second > -INFINITY ? first + second : first;
+        }
+        unsigned kept = 0;
+        for (int j = 0; j < a.how.top_groups; j++) {
+            int at;
+            if (!(largest_of_warp(kept >> lane & 1 ? -INFINITY : of_group, at) > -INFINITY)) break;
+            kept |= 1u << at;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (lane + 32 * i < (int)a.experts && !(kept >> a.group.quotient(lane + 32 * i) & 1)) c[i] = -INFINITY;
+    }
+    int mine = -1;
+    for (int j = 0; j < a.how.k; j++) {
+        double v = c[0];
+        int of = 0, at;
+#pragma unroll
+        for (int i = 1; i < PER; i++)
+            if (c[i] > v) { v = c[i]; of = i; }
+        // equal ones in two lanes: the lower register, then the lower lane
+        const double top = largest_of_warp(v, at);
+        if (!(top > -INFINITY)) break;
+        const int low = (int)__reduce_min_sync(kAll, v == top ? (unsigned)(32 * of + lane) : ~0u);
+        if (lane == j) mine = low;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (lane + 32 * i == low) c[i] = -INFINITY;
+    }
     return mine;
 }
 
 /**
- * How close two scores of at most `largest`, with biases up to `bias`, may lie for their order not to be known, in units of 2^-23. A sigmoid is off by two
- * (exponential one, sum and quotient half each). A softmax by its own exponential, difference and quotient likewise, and by the sum that all of the row
- * share: one of its terms, and half for each of the PER + 5 additions. Twice that for two, and half of the result's size for the sum with the bias.
- * Two groups lie within twice all this: two scores each, and the rounding of their sum.
+ * What two scores of at most `largest` before their biases may be off against each other, in units of 2^-23. __expf is off by 2 + 1.173 |x| of e^x. A sigmoid,
+ * s (1 - s) (2 + 1.173 |x|) < 0.8 from it, 0.5 from the sum and 2 from __fdividef; a softmax 2 from it (largest at x = 0), 0.2 from the difference, and 1.5 from
+ * the quotient and the product. Twice that for two. All of a softmax share their sum: 2.2 of its terms and half for each of the PER + 5 additions. (The rounding of the
+ * sum with the bias is in choose's `part`.)
  */
-template <int PER> __device__ __forceinline__ float unsure_within(bool sigmoid, float largest, float bias) {
-    return ((sigmoid ? 8 : PER + 16) * largest + 2 * (largest + bias)) * (1.0f / (1 << 23));
-}
+template <int PER> __device__ __forceinline__ float unsure_within(bool sigmoid, float largest) { return (sigmoid ? 8 : PER + 16) * largest * (1.0f / (1 << 23)); }
 
 /** sigmoid(z) and a common factor of all that makes up for z far below zero: 1 / (e^-c + e^(-z - c)), c = max(0, -largest z). */
 __device__ __forceinline__ float sigmoid_beside(float z, float largest) {
@@ -188,85 +335,97 @@ __device__ __forceinline__ float sigmoid_beside(float z, float largest) {
 
 /** Lane j's share r_j of the chosen, from its logit z (none: -infinity); 0 where there is none. */
 __device__ __forceinline__ float share_of(const DcclRouting& how, bool there, float z) {
-    int at = 0;
-    float top = there ? z : -INFINITY;
-    best_of_warp(top, at);
+    const float top = largest_of_warp(there ? z : -INFINITY);
     const float s = !there ? 0.0f : how.sigmoid ? sigmoid_beside(z, top) : expf(z - top);
     const float sum = warp_sum(s);
     return there ? s / sum : 0.0f;
 }
 
 /**
- * Bytes are few (16384 tokens of 256 fp32 logits: 17 MB, 2.6 us); the choice is what takes time: k + 1 rounds of a comparison per register and two reductions
- * of the warp.
+ * Bytes are few (16384 tokens of 256 fp32 logits: 17 MB, 2.6 us); the instructions of the choice take the time. Groups of whole registers are judged all at once,
+ * and each of the k + 1 rounds is one reduction of the lists' heads. A warp loads its next token before it chooses for this one.
  */
-template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarps) k_route(const __grid_constant__ RouteArgs a) {
+template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarps, PER <= 8 ? 6 : 1) k_route(const __grid_constant__ RouteArgs a) {
     wait_for_stream();
     const int lane = threadIdx.x % 32;
-    const size_t token = (size_t)blockIdx.x * kRouteWarps + threadIdx.x / 32;
-    if (token >= a.tokens) return;
-    float z[PER], c[PER], top = -INFINITY;
-    bool poisoned = false;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane + 32 * i;
-        z[i] = e < (int)a.experts ? logit<T>(a, token, e) : -INFINITY;
-        poisoned |= z[i] != z[i];
-        top = z[i] > top ? z[i] : top;
-    }
-    poisoned = __any_sync(kAll, poisoned);
     // whether the order of the scores is that of the logits
     const bool plain = !a.bias && (a.how.groups == 1 || !a.how.top2);
-    float sum = 1.0f, bias = 0.0f;
-    if (!a.how.sigmoid && (!plain || !a.how.renormalize)) {
-        int at = 0;
-        best_of_warp(top, at);
-        float part = 0.0f;
+    float bias[PER], ahead[PER];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            c[i] = z[i] > -INFINITY ? expf(z[i] - top) : 0.0f;
-            part += c[i];
-        }
-        sum = warp_sum(part);
-    }
+    for (int i = 0; i < PER; i++) bias[i] = a.bias && lane + 32 * i < (int)a.experts ? a.bias[lane + 32 * i] : 0.0f;
+    const unsigned step = gridDim.x * kRouteWarps;
+    unsigned token = blockIdx.x * kRouteWarps + threadIdx.x / 32;
+    if (token < a.tokens) load_logits<T, PER>(a, token, ahead);
+    for (; token < a.tokens; token += step) {
+        float c[PER], top = -INFINITY, sum = 1.0f;
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane + 32 * i;
-        float s = z[i];
-        if (!plain && z[i] > -INFINITY) {
-            const float b = a.bias ? a.bias[e] : 0.0f;
-            s = (a.how.sigmoid ? 1.0f / (1.0f + expf(-z[i])) : c[i] / sum) + b;
-            if (fabsf(b) < INFINITY) bias = fmaxf(bias, fabsf(b));
+        for (int i = 0; i < PER; i++) c[i] = ahead[i];
+        if (token + step < a.tokens) load_logits<T, PER>(a, token + step, ahead);
+        bool poisoned = false;
+        if (!a.how.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                poisoned |= c[i] != c[i];
+                top = fmaxf(top, c[i]);
+            }
+            poisoned = __any_sync(kAll, poisoned);
+            if (!plain || !a.how.renormalize) top = largest_of_warp(top);
         }
-        c[i] = s > -INFINITY ? s : -INFINITY;           // NaN is not chosen
-    }
-    if (a.bias) bias = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(bias)));
-    int mine;
-    // of a softmax the largest score is 1 / sum
-    const float unsure = plain ? -1.0f : unsure_within<PER>(a.how.sigmoid, a.how.sigmoid ? 1.0f : 1.0f / sum, bias);
-    if (!choose<T, float, PER>(a, token, c, unsure, mine) && !plain) mine = choose_exactly<T, PER>(a, token);
-    const bool there = mine >= 0;
-    const float zm = there ? logit<T>(a, token, mine) : -INFINITY;
-    float w;
-    if (a.how.renormalize) w = share_of(a.how, there, zm);
-    else w = !there ? 0.0f : a.how.sigmoid ? 1.0f / (1.0f + expf(-zm)) : expf(zm - top) / sum;
-    if (poisoned && there && !a.how.sigmoid) w = NAN;
-    if (lane < a.how.k) {
-        a.weights[token * a.how.k + lane] = a.how.scale * w;
-        a.chosen[token * a.how.k + lane] = mine;
+        if (!a.how.renormalize && !a.how.sigmoid) {         // the weights will take this sum
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; i++) part += c[i] == -INFINITY ? 0.0f : expf(c[i] - top);
+            sum = warp_sum(part);
+        }
+        float unsure = 1e-37f;          // of logits: below the normal numbers, steps are not parts of a size
+        if (!plain) {
+            if (a.how.sigmoid) {
+#pragma unroll
+                for (int i = 0; i < PER; i++) c[i] = c[i] == -INFINITY ? c[i] : __fdividef(1.0f, 1.0f + __expf(-c[i])) + bias[i];
+                unsure = 1.0f;
+            } else {
+                float part = 0.0f;
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const float e = __expf(c[i] - top);
+                    part += c[i] == -INFINITY ? 0.0f : e;
+                    c[i] = c[i] == -INFINITY ? c[i] : e;
+                }
+                unsure = __fdividef(1.0f, warp_sum(part));          // of a softmax the largest score
+#pragma unroll
+                for (int i = 0; i < PER; i++) c[i] = fmaf(c[i], unsure, bias[i]);
+            }
+            unsure = unsure_within<PER>(a.how.sigmoid, unsure);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) c[i] = fmaxf(c[i], -INFINITY);          // NaN is not chosen
+        int mine;
+        if (!choose<T, PER>(a, token, c, unsure, mine)) mine = choose_exactly<T, PER>(a, token, plain);
+        const bool there = mine >= 0;
+        const float zm = there ? logit<T>(a, token, mine) : -INFINITY;
+        float w;
+        if (a.how.renormalize) w = share_of(a.how, there, zm);
+        else w = !there ? 0.0f : a.how.sigmoid ? 1.0f / (1.0f + expf(-zm)) : expf(zm - top) / sum;
+        if (poisoned && there) w = NAN;
+        if (lane < a.how.k) {
+            a.weights[(size_t)token * a.how.k + lane] = a.how.scale * w;
+            a.chosen[(size_t)token * a.how.k + lane] = mine;
+        }
     }
 }
 
+/** The row goes through shared memory: what every expert gets first, then what the chosen get. */
 template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarps) k_route_grad(const __grid_constant__ RouteArgs a) {
     wait_for_stream();
+    __shared__ alignas(16) float rows[kRouteWarps][32 * PER];
     const int lane = threadIdx.x % 32, k = a.how.k;
     const size_t token = (size_t)blockIdx.x * kRouteWarps + threadIdx.x / 32;
     if (token >= a.tokens) return;
+    float* const row = rows[threadIdx.x / 32];
     const int mine = lane < k ? a.chosen[token * k + lane] : -1;
     const bool there = mine >= 0 && mine < (int)a.experts;
     const float zm = there ? logit<T>(a, token, mine) : -INFINITY;
     const float g = there ? a.how.scale * a.dweights[token * k + lane] : 0.0f;
-    T* to = reinterpret_cast<T*>(a.dlogits) + token * a.experts;
     float d[PER] = {}, dm = 0.0f;
     if (a.how.renormalize) {
         const float r = share_of(a.how, there, zm);
@@ -277,14 +436,10 @@ template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarp
         dm = g * s * (1.0f / (1.0f + expf(zm)));
     } else {
         float top = -INFINITY, part = 0.0f;
+        load_logits<T, PER>(a, token, d);
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int e = lane + 32 * i;
-            d[i] = e < (int)a.experts ? logit<T>(a, token, e) : -INFINITY;
-            top = d[i] > top ? d[i] : top;
-        }
-        int at = 0;
-        best_of_warp(top, at);
+        for (int i = 0; i < PER; i++) top = fmaxf(top, d[i]);
+        top = largest_of_warp(top);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             d[i] = d[i] == -INFINITY ? 0.0f : expf(d[i] - top);
@@ -295,27 +450,43 @@ template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarp
         for (int i = 0; i < PER; i++) d[i] = d[i] == 0.0f ? 0.0f : -(d[i] / sum) * common;
         dm = s * (g - common);
     }
-    for (int j = 0; j < k; j++) {
-        const int e = __shfl_sync(kAll, there ? mine : -1, j);
-        const float v = __shfl_sync(kAll, dm, j);
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (lane + 32 * i == e) d[i] = v;
+    for (int i = 0; i < PER; i++) row[lane + 32 * i] = d[i];
+    __syncwarp();
+    if (there) row[mine] = dm;
+    __syncwarp();
+    T* to = reinterpret_cast<T*>(a.dlogits) + token * a.experts;
+    constexpr int M = 16 / sizeof(T);
+    if (a.vec) {
+        for (int e = lane * M; e < (int)a.experts; e += 32 * M) {
+            float f[M];
+#pragma unroll
+            for (int q = 0; q < M; q += 4) {
+                const Run<float, 4> r = ld_run<float, 4>(row + e + q);
+#pragma unroll
+                for (int p = 0; p < 4; p++) f[q + p] = r.e[p];
+            }
+            st_run<T, M>(to + e, round_run<T, M>(f));
+        }
+    } else {
+        for (int e = lane; e < (int)a.experts; e += 32) to[e] = Traits<T>::down(row[e]);
     }
-#pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (lane + 32 * i < (int)a.experts) to[lane + 32 * i] = Traits<T>::down(d[i]);
 }
 
-template <typename T> static cudaError_t run_route(const RouteArgs& a, bool backward, cudaStream_t stream) {
-    const unsigned grid = (a.tokens + kRouteWarps - 1) / kRouteWarps, per = (a.experts + 31) / 32;
-    const auto go = [&](auto kernel) { return launch_early(kernel, grid, 32 * kRouteWarps, stream, a); };
-    if (per <= 1) return go(backward ? k_route_grad<T, 1> : k_route<T, 1>);
-    if (per <= 2) return go(backward ? k_route_grad<T, 2> : k_route<T, 2>);
-    if (per <= 4) return go(backward ? k_route_grad<T, 4> : k_route<T, 4>);
-    if (per <= 8) return go(backward ? k_route_grad<T, 8> : k_route<T, 8>);
-    if (per <= 16) return go(backward ? k_route_grad<T, 16> : k_route<T, 16>);
-    return go(backward ? k_route_grad<T, 32> : k_route<T, 32>);
+template <typename T, int PER> static cudaError_t run_route(const RouteArgs& a, bool backward, cudaStream_t stream) {
+    const unsigned ctas = (a.tokens + kRouteWarps - 1) / kRouteWarps;
+    if (backward) return launch_early(k_route_grad<T, PER>, ctas, 32 * kRouteWarps, stream, a);
+    return launch_early(k_route<T, PER>, ctas < a.ctas ? ctas : a.ctas, 32 * kRouteWarps, stream, a);
+}
+template <typename T> static cudaError_t run_route(RouteArgs a, bool backward, cudaStream_t stream) {
+    a.vec = a.experts % (16 / sizeof(T)) == 0 && aligned_to(16, {a.dlogits});
+    const unsigned per = (a.experts + 31) / 32;
+    if (per <= 1) return run_route<T, 1>(a, backward, stream);
+    if (per <= 2) return run_route<T, 2>(a, backward, stream);
+    if (per <= 4) return run_route<T, 4>(a, backward, stream);
+    if (per <= 8) return run_route<T, 8>(a, backward, stream);
+    if (per <= 16) return run_route<T, 16>(a, backward, stream);
+    return run_route<T, 32>(a, backward, stream);
 }
 
 static int route(const char* who, int device, int dtype, size_t tokens, int experts, RouteArgs a, const DcclRouting* how, bool backward, void* stream) {
@@ -329,6 +500,7 @@ static int route(const char* who, int device, int dtype, size_t tokens, int expe
     a.tokens = (unsigned)tokens;
     a.experts = (unsigned)experts;
     a.how = *how;
+    a.ctas = 8 * (unsigned)sm_count(device);
     a.group = Divisor((unsigned)(experts / how->groups));
     const cudaStream_t s = (cudaStream_t)stream;
     return report(who, dtype == 6 ? run_route<__half>(a, backward, s) : dtype == 7 ? run_route<float>(a, backward, s) : run_route<__nv_bfloat16>(a, backward, s));

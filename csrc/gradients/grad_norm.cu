@@ -14,7 +14,7 @@ namespace dccl {
 
 constexpr int kClipThreads = 256, kClipUnroll = 4;
 constexpr size_t kMaxPiece = 64 * 1024, kMinPiece = 4 * 1024;
-constexpr int kManyTensors = 512, kFewTensors = 24;
+constexpr int kManyTensors = 512, kSomeTensors = 120, kFewTensors = 24;
 
 enum { TYPE_HALF = 0, TYPE_BF16 = 1, TYPE_FLOAT = 2, TYPE_TO_FLOAT = 4 };      // of a tensor; TO_FLOAT: what is written is fp32
 
@@ -265,7 +265,7 @@ extern "C" int dccl_grad_squares(int device, size_t tensors, const DcclGradient*
         const size_t n = tensors - i < kManyTensors ? tensors - i : kManyTensors;
         ClipPlan p;
         if (!plan_clip(device, n, t + i, p)) return report(who, cudaErrorInvalidValue);
-        const cudaError_t e = n <= kFewTensors ? run_squares<kFewTensors>(n, t + i, p, parts, (cudaStream_t)stream) : run_squares<kManyTensors>(n, t + i, p, parts, (cudaStream_t)stream);
+        const cudaError_t e = (n <= kFewTensors ? run_squares<kFewTensors> : n <= kSomeTensors ? run_squares<kSomeTensors> : run_squares<kManyTensors>)(n, t + i, p, parts, (cudaStream_t)stream);
         if (e != cudaSuccess) return report(who, e);
         parts += p.ctas;
     }
@@ -292,7 +292,7 @@ extern "C" int dccl_grad_clip(int device, size_t tensors, const DcclGradient* t,
         for (size_t j = 0; j < n; j++)
             if (!t[i + j].out) return report(who, cudaErrorInvalidValue);
         const ClipArgs a = {parts, count, limit, norm};
-        const cudaError_t e = n <= kFewTensors ? run_clip<kFewTensors>(n, t + i, p, a, (cudaStream_t)stream) : run_clip<kManyTensors>(n, t + i, p, a, (cudaStream_t)stream);
+        const cudaError_t e = (n <= kFewTensors ? run_clip<kFewTensors> : n <= kSomeTensors ? run_clip<kSomeTensors> : run_clip<kManyTensors>)(n, t + i, p, a, (cudaStream_t)stream);
         if (e != cudaSuccess) return report(who, e);
     }
     return 0;

@@ -46,7 +46,7 @@ def test_early_launched_kernels_promise_nothing_about_their_inputs():
                 kernel = signature[:signature.rindex("(")].split("k_")[-1].split("(")[0]
                 assert "wait_for_stream()" in body.split("\n}", 1)[0] or "plan<" in body.split("\n", 1)[0], kernel
                 found.add(kernel)
-    assert found >= {"route", "route_grad", "plan", "plan_cluster", "dispatch", "combine", "combine_grad", "grouped", "pad_rows", "act_grad", "grad_squares", "grad_total", "grad_clip"}
+    assert found >= {"route", "route_grad", "plan", "plan_cluster", "dispatch", "combine", "combine_grad", "grouped", "join_parts", "pad_rows", "act_grad", "grad_squares", "grad_total", "grad_clip"}
     plan = open(os.path.join(ROOT, "csrc", "experts", "exchange.cu")).read().split("void plan(")[1]
     assert plan.index("wait_for_stream()") < plan.index("plan_expert(a")
 
@@ -59,11 +59,17 @@ def test_limits_are_those_of_the_entry_points():
     assert limits == {"": experts._MAX_EXPERTS, "_CHOSEN": experts._MAX_CHOSEN, "_GROUPS": experts._MAX_GROUPS, "_WIDTH": experts._MAX_WIDTH, "_PLACES": experts._MAX_PLACES}
 
 
-def test_tiles_cover_every_expert(tmp_path):
-    """tests/sim/grouped_tiles.cpp: which tiles a product has, and what one that gave up leaves, without a GPU."""
-    exe = str(tmp_path / "grouped_tiles")
+@pytest.fixture(scope="module")
+def tiles_program(tmp_path_factory):
+    """tests/sim/grouped_tiles.cpp: how products are cut, without a GPU."""
+    exe = str(tmp_path_factory.mktemp("tiles") / "grouped_tiles")
     subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", "-Werror", os.path.join(ROOT, "tests", "sim", "grouped_tiles.cpp"), "-o", exe], check=True)
-    res = subprocess.run([exe], capture_output=True, text=True)
+    return exe
+
+
+def test_tiles_cover_every_expert(tiles_program):
+    """Which tiles a product has, and what one that gave up leaves."""
+    res = subprocess.run([tiles_program], capture_output=True, text=True)
     assert res.returncode == 0 and res.stdout == "OK\n", res.stdout
 
 
@@ -599,9 +605,33 @@ def test_expert_linear_activations(act):
     linear_run([70, 10, 0, 133], 131, 203, torch.float16, act)
 
 
-# Rows of tiles enough for columns of 256, in all three products, and more tiles than CTAs.
+# Sums that are cut into parts, in each of the products: few tiles with a long k.
+CUT = [([128], 2048, 128), ([100, 28], 2001, 100), ([128], 136, 2048), ([70, 0, 50], 99, 2050), ([3000], 128, 136), ([1500, 1, 1400], 130, 121), ([2500], 200, 72)]
+
+
 @gpu
-@pytest.mark.parametrize("counts,width,out", [([2000, 1300, 0, 1011], 776, 1544), ([700] * 8, 520, 1032), ([3000], 1288, 808), ([9, 5000], 72, 1800)], ids=str)
+@pytest.mark.parametrize("sizes", CUT, ids=str)
+def test_expert_linear_of_parts(sizes):
+    linear_run(*sizes, torch.bfloat16 if sizes[1] % 2 else torch.float16, ACTS[len(sizes[0]) % 4], behind=len(sizes[0]) % 2 * 40)
+
+
+def test_sizes_reach_every_kind_of_plan(tiles_program):
+    seen = set()
+    for counts, width, out in COUNTS + CUT + MANY:
+        rows = str(sum(counts) + len(counts) % 3 * 70)
+        for form, m, n, k in ((0, 0, out, width), (1, 0, width, out), (2, out, width, 0)):
+            tall, columns, splits = subprocess.run([tiles_program, "plan", "148", str(form), rows, str(len(counts)), str(m), str(n), str(k)], capture_output=True, text=True,
+                                                   check=True).stdout.split()
+            seen.add((form, tall, columns, int(splits) > 1))
+    assert seen >= {(0, "32", "64", False)} | {(f, "128", c, cut) for f in range(3) for c, cut in (("128", False), ("128", True), ("256", False))}, sorted(seen)
+
+
+# Rows of tiles enough for columns of 256, in all three products, and more tiles than CTAs.
+MANY = [([2000, 1300, 0, 1011], 776, 1544), ([700] * 8, 520, 1032), ([3000], 1288, 808), ([9, 5000], 72, 1800)]
+
+
+@gpu
+@pytest.mark.parametrize("counts,width,out", MANY, ids=str)
 def test_expert_linear_of_many_tiles(counts, width, out):
     linear_run(counts, width, out, torch.bfloat16, "silu", behind=130)
 
@@ -809,6 +839,34 @@ print("OK")
 @gpu
 def test_the_first_call_of_a_process_can_be_captured():
     res = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip().endswith("OK"), res.stdout + res.stderr[-2000:]
+
+
+THREADS = """
+import threading, torch
+from dccl_b200 import ops
+x, w, starts = torch.randn(40, 64, device="cuda").bfloat16(), torch.randn(2, 72, 64, device="cuda").bfloat16(), torch.tensor([0, 15, 40], dtype=torch.int32, device="cuda")
+w.requires_grad_(True)
+y, room = ops.expert_linear(x, w, starts), [torch.empty(1 << 20, device="cuda") for _ in range(4)]
+del room
+torch.cuda.synchronize()
+g, = torch.autograd.grad(y, w, torch.ones_like(y))          # the autograd engine's thread
+got = []
+def call():
+    got.append(ops.expert_linear(x, w, starts))
+    got.append(ops.gated_linear(x, w[0], w[1]))
+thread = threading.Thread(target=call)
+thread.start()
+thread.join()
+assert torch.equal(got[0], y) and torch.equal(got[1], ops.gated_linear(x, w[0], w[1])) and bool((g != 0).any())
+print("OK")
+"""
+
+
+@gpu
+def test_the_first_call_of_a_thread():
+    """Threads that have not called CUDA before: the one that runs backward passes, and one of the user's."""
+    res = subprocess.run([sys.executable, "-c", THREADS], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and res.stdout.strip().endswith("OK"), res.stdout + res.stderr[-2000:]
 
 
