@@ -65,12 +65,12 @@ inline int* gave_up_flag(int device) {
     return flags ? flags + device : nullptr;        // of the 64 devices that sm_count knows
 }
 
-/** An operand by its dimensions, the contiguous one first, the strides of the others in elements, and the box of it (one of the last of three). */
-inline cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, int rank, const size_t (&size)[3], const size_t (&stride)[2], unsigned box_outer) {
+/** An operand by its dimensions, the contiguous one first, the strides of the others in elements, and the box of it. */
+inline cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, int rank, const size_t (&size)[4], const size_t (&stride)[3], const unsigned (&box_of)[4]) {
     const DriverApi* d = driver_api(nullptr);
     if (!d || !d->TensorMapEncodeTiled) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {size[0], size[1], size[2]}, strides[2] = {stride[0] * 2, stride[1] * 2};
-    const cuuint32_t box[3] = {64, box_outer, 1}, steps[3] = {1, 1, 1};
+    const cuuint64_t dims[4] = {size[0], size[1], size[2], size[3]}, strides[3] = {stride[0] * 2, stride[1] * 2, stride[2] * 2};
+    const cuuint32_t box[4] = {box_of[0], box_of[1], box_of[2], box_of[3]}, steps[4] = {1, 1, 1, 1};
     const auto encode = [&] {
         return d->TensorMapEncodeTiled(map, dtype == 6 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, steps,
                                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -83,7 +83,7 @@ inline cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, int r
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 inline cudaError_t make_map(CUtensorMap* map, int dtype, const void* base, size_t inner, size_t outer, size_t stride, unsigned box_outer) {
-    return make_map(map, dtype, base, 2, {inner, outer, 1}, {stride, 0}, box_outer);
+    return make_map(map, dtype, base, 2, {inner, outer, 1, 1}, {stride, 0, 0}, {64, box_outer, 1, 1});
 }
 
 inline bool gave_up(const char* who, int device) {

@@ -57,6 +57,12 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, in
                  "r"(bar)
                  : "memory");
 }
+/** And of four. */
+__device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
 /** What this thread wrote to shared memory is seen by products that are issued after it. */
 __device__ __forceinline__ void shared_writes_before_products() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }

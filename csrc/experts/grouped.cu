@@ -64,6 +64,7 @@ struct GroupedArgs : Grouped, GroupedResults {
     const int* starts;
     unsigned descriptor;            // of one product
     int act;
+    bool whole_a, whole_b;          // one box holds all blocks of 64 columns of an operand
     int* gave_up;
 };
 
@@ -158,13 +159,19 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
                     load_box(to_b, &a.b, k, p.column, p.expert, bar);
                 } else if constexpr (FORM == EXPERTS_INPUT) {
                     load_box(to_a, &a.a, k, p.row, bar);
+                    if (a.whole_b) load_box(to_b, &a.b, 0, k, p.column / 64, p.expert, bar);
+                    else
 #pragma unroll
-                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, p.expert, bar);
+                        for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, p.expert, bar);
                 } else {
+                    if (a.whole_a) load_box(to_a, &a.a, 0, k, p.row / 64, bar);
+                    else
 #pragma unroll
-                    for (int i = 0; i < M / 64; i++) load_box(to_a + i * 64 * 128, &a.a, p.row + 64 * i, k, bar);
+                        for (int i = 0; i < M / 64; i++) load_box(to_a + i * 64 * 128, &a.a, p.row + 64 * i, k, bar);
+                    if (a.whole_b) load_box(to_b, &a.b, 0, k, p.column / 64, bar);
+                    else
 #pragma unroll
-                    for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, bar);
+                        for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, bar);
                 }
                 if (++s == kStages) { s = 0; parity ^= 1; }
             }
@@ -414,15 +421,16 @@ static GroupedLayout grouped_layout(int device, size_t rows, int experts, size_t
     if (!l.ok) return l;
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t here = at; at += up_to(bytes, 256); return here; };
+    // rows of whole lines: the tiled loads take twice as long for pieces of 128 bytes that lie in two
     const bool pad = !aligned || width % 8;
-    l.stride = pad ? up_to(width, 8) : width;
+    l.stride = pad ? up_to(width, 64) : width;
     if (pad) {      // at the same places in both directions: the backward pass finds them in what the forward pass left
         l.x = take(rows * l.stride * 2);
         l.w = take((size_t)experts * out * l.stride * 2);
         l.padded = at;
         if (backward) at = 0;
     }
-    l.d_stride = up_to(out, 8);
+    l.d_stride = up_to(out, 64);
     l.forward = plan_grouped(EXPERTS_FORWARD, sms, rows, experts, 0, out, width);
     l.input = plan_grouped(EXPERTS_INPUT, sms, rows, experts, 0, width, out);
     l.weight = plan_grouped(EXPERTS_WEIGHT, sms, rows, experts, out, width, 0);
@@ -477,6 +485,18 @@ template <typename T, int FORM> static cudaError_t run_grouped(int device, const
     return launch_early(k_join_parts<T>, (unsigned)((j.rows * j.runs + 255) / 256), 256, stream, j);
 }
 
+/**
+ * The map of an operand whose rows are summed over, [matrices][rows][columns], of which a tile takes `blocks` blocks of 64 columns. Where rows are whole blocks apart, the
+ * blocks are a dimension of their own and one box holds them all: a load takes the loader some 60 clocks to give out, and six a block were as long as its products.
+ */
+static cudaError_t map_of_blocks(CUtensorMap* map, bool& whole, int dtype, const void* base, size_t matrices, size_t rows, size_t columns, size_t stride, unsigned blocks) {
+    whole = stride % 64 == 0;
+    if (whole && matrices) return make_map(map, dtype, base, 4, {64, rows, stride / 64, matrices}, {stride, 64, stride * rows}, {64, kTileK, blocks, 1});
+    if (whole) return make_map(map, dtype, base, 3, {64, rows, stride / 64, 1}, {stride, 64, 0}, {64, kTileK, blocks, 1});
+    if (matrices) return make_map(map, dtype, base, 3, {columns, rows, matrices, 1}, {stride, stride * rows, 0}, {64, kTileK, 1, 1});
+    return make_map(map, dtype, base, columns, rows, stride, kTileK);
+}
+
 static cudaError_t pad_rows(const void*& x, const void*& w, size_t rows, size_t w_rows, size_t width, size_t stride, void* to_x, void* to_w, cudaStream_t stream) {
     PadRowsArgs a = {{(const uint16_t*)x, (const uint16_t*)w}, {(uint16_t*)to_x, (uint16_t*)to_w}, {rows, w_rows}, (unsigned)width, (unsigned)(stride / 8), kRowCta};
     if (a.runs < kRowCta) a.across = (a.runs + 31) / 32 * 32;
@@ -529,7 +549,7 @@ template <typename T> static cudaError_t grouped_forward(const GroupedCall& k, c
     a.z = z;
     a.z_stride = z_stride;
     if (e == cudaSuccess) e = make_map(&a.a, k.dtype, x, k.width, k.rows, l.stride, l.forward.tile_rows);
-    if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts}, {l.stride, l.stride * k.out}, l.forward.tile_columns);
+    if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts, 1}, {l.stride, l.stride * k.out, 0}, {64, l.forward.tile_columns, 1, 1});
     return e == cudaSuccess ? run_grouped<T, EXPERTS_FORWARD>(k.device, l.forward, a, k.stream) : e;
 }
 
@@ -567,7 +587,7 @@ template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, 
         a.k_blocks = blocks_of(k.out, kTileK);
         a.c = dx;
         e = make_map(&a.a, k.dtype, dz, k.out, k.rows, d_stride, kTileM);
-        if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts}, {l.stride, l.stride * k.out}, kTileK);
+        if (e == cudaSuccess) e = map_of_blocks(&a.b, a.whole_b, k.dtype, w, k.experts, k.out, k.width, l.stride, l.input.tile_columns / 64);
         if (e == cudaSuccess) e = run_grouped<T, EXPERTS_INPUT>(k.device, l.input, a, k.stream);
     }
     if (e == cudaSuccess && dw) {
@@ -575,8 +595,8 @@ template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, 
         a.m = (unsigned)k.out;
         a.n = (unsigned)k.width;
         a.c = dw;
-        e = make_map(&a.a, k.dtype, dz, k.out, k.rows, d_stride, kTileK);
-        if (e == cudaSuccess) e = make_map(&a.b, k.dtype, x, k.width, k.rows, l.stride, kTileK);
+        e = map_of_blocks(&a.a, a.whole_a, k.dtype, dz, 0, k.rows, k.out, d_stride, kTileM / 64);
+        if (e == cudaSuccess) e = map_of_blocks(&a.b, a.whole_b, k.dtype, x, 0, k.rows, k.width, l.stride, l.weight.tile_columns / 64);
         if (e == cudaSuccess) e = run_grouped<T, EXPERTS_WEIGHT>(k.device, l.weight, a, k.stream);
     }
     return e;
