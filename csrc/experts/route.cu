@@ -29,7 +29,7 @@ struct RouteArgs {
     unsigned tokens, experts;
     DcclRouting how;
     Divisor group;              // by the experts of a group
-    unsigned ctas;              // at most
+    unsigned ends;              // registers with which a group of whole registers ends
     bool vec;                   // rows of the gradient start on 16 bytes
 };
 
@@ -127,16 +127,14 @@ template <typename T, int PER> __device__ __forceinline__ bool choose(const Rout
         float first[PER], second[PER];          // where it has, of the group that ends with this register; otherwise in the first
         if (whole) {
             float f = -INFINITY, t = -INFINITY;
-            int left = whole;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
                 join_best(f, t, c[i]);
-                const bool ends = --left == 0;
-                first[i] = ends ? f : -INFINITY;
-                second[i] = ends ? t : -INFINITY;
-                if (ends) {
+                first[i] = second[i] = -INFINITY;
+                if (a.ends >> i & 1) {
+                    first[i] = f;
+                    second[i] = t;
                     f = t = -INFINITY;
-                    left = whole;
                 }
             }
             best_of_registers(first, second);
@@ -176,11 +174,11 @@ template <typename T, int PER> __device__ __forceinline__ bool choose(const Rout
             last = from_ordered(top);
         }
         if (whole) {
-            int end = whole - 1;
+            bool stays = false;
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                if (!(kept >> (end * spread & 31) & 1)) c[i] = -INFINITY;
-                if (i == end) end += whole;
+            for (int i = PER - 1; i >= 0; i--) {
+                if (a.ends >> i & 1) stays = kept >> (i * spread) & 1;
+                if (!stays) c[i] = -INFINITY;
             }
         } else {
 #pragma unroll
@@ -343,74 +341,71 @@ __device__ __forceinline__ float share_of(const DcclRouting& how, bool there, fl
 
 /**
  * Bytes are few (16384 tokens of 256 fp32 logits: 17 MB, 2.6 us); the instructions of the choice take the time. Groups of whole registers are judged all at once,
- * and each of the k + 1 rounds is one reduction of the lists' heads. A warp loads its next token before it chooses for this one.
+ * and each of the k + 1 rounds is one reduction of the lists' heads.
  */
-template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarps, PER <= 8 ? 6 : 1) k_route(const __grid_constant__ RouteArgs a) {
+template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarps, PER <= 8 ? 8 : 1) k_route(const __grid_constant__ RouteArgs a) {
     wait_for_stream();
     const int lane = threadIdx.x % 32;
     // whether the order of the scores is that of the logits
     const bool plain = !a.bias && (a.how.groups == 1 || !a.how.top2);
-    float bias[PER], ahead[PER];
+    const size_t token = (size_t)blockIdx.x * kRouteWarps + threadIdx.x / 32;
+    if (token >= a.tokens) return;
+    float c[PER], top = -INFINITY, sum = 1.0f;
+    load_logits<T, PER>(a, token, c);
+    bool poisoned = false;
+    if (!a.how.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) bias[i] = a.bias && lane + 32 * i < (int)a.experts ? a.bias[lane + 32 * i] : 0.0f;
-    const unsigned step = gridDim.x * kRouteWarps;
-    unsigned token = blockIdx.x * kRouteWarps + threadIdx.x / 32;
-    if (token < a.tokens) load_logits<T, PER>(a, token, ahead);
-    for (; token < a.tokens; token += step) {
-        float c[PER], top = -INFINITY, sum = 1.0f;
-#pragma unroll
-        for (int i = 0; i < PER; i++) c[i] = ahead[i];
-        if (token + step < a.tokens) load_logits<T, PER>(a, token + step, ahead);
-        bool poisoned = false;
-        if (!a.how.sigmoid) {
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                poisoned |= c[i] != c[i];
-                top = fmaxf(top, c[i]);
-            }
-            poisoned = __any_sync(kAll, poisoned);
-            if (!plain || !a.how.renormalize) top = largest_of_warp(top);
+        for (int i = 0; i < PER; i++) {
+            poisoned |= c[i] != c[i];
+            top = fmaxf(top, c[i]);
         }
-        if (!a.how.renormalize && !a.how.sigmoid) {         // the weights will take this sum
+        poisoned = __any_sync(kAll, poisoned);
+        if (!plain || !a.how.renormalize) top = largest_of_warp(top);
+    }
+    if (!a.how.renormalize && !a.how.sigmoid) {         // the weights will take this sum
+        float part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) part += c[i] == -INFINITY ? 0.0f : expf(c[i] - top);
+        sum = warp_sum(part);
+    }
+    float unsure = 1e-37f;          // of logits: below the normal numbers, steps are not parts of a size
+    if (!plain) {
+        if (a.how.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) c[i] = c[i] == -INFINITY ? c[i] : __fdividef(1.0f, 1.0f + __expf(-c[i]));
+            unsure = 1.0f;
+        } else {
             float part = 0.0f;
 #pragma unroll
-            for (int i = 0; i < PER; i++) part += c[i] == -INFINITY ? 0.0f : expf(c[i] - top);
-            sum = warp_sum(part);
-        }
-        float unsure = 1e-37f;          // of logits: below the normal numbers, steps are not parts of a size
-        if (!plain) {
-            if (a.how.sigmoid) {
-#pragma unroll
-                for (int i = 0; i < PER; i++) c[i] = c[i] == -INFINITY ? c[i] : __fdividef(1.0f, 1.0f + __expf(-c[i])) + bias[i];
-                unsure = 1.0f;
-            } else {
-                float part = 0.0f;
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const float e = __expf(c[i] - top);
-                    part += c[i] == -INFINITY ? 0.0f : e;
-                    c[i] = c[i] == -INFINITY ? c[i] : e;
-                }
-                unsure = __fdividef(1.0f, warp_sum(part));          // of a softmax the largest score
-#pragma unroll
-                for (int i = 0; i < PER; i++) c[i] = fmaf(c[i], unsure, bias[i]);
+            for (int i = 0; i < PER; i++) {
+                const float e = __expf(c[i] - top);
+                part += c[i] == -INFINITY ? 0.0f : e;
+                c[i] = c[i] == -INFINITY ? c[i] : e;
             }
-            unsure = unsure_within<PER>(a.how.sigmoid, unsure);
-        }
+            unsure = __fdividef(1.0f, warp_sum(part));          // of a softmax the largest score
 #pragma unroll
-        for (int i = 0; i < PER; i++) c[i] = fmaxf(c[i], -INFINITY);          // NaN is not chosen
-        int mine;
-        if (!choose<T, PER>(a, token, c, unsure, mine)) mine = choose_exactly<T, PER>(a, token, plain);
-        const bool there = mine >= 0;
-        const float zm = there ? logit<T>(a, token, mine) : -INFINITY;
-        float w;
-        if (a.how.renormalize) w = share_of(a.how, there, zm);
-        else w = !there ? 0.0f : a.how.sigmoid ? 1.0f / (1.0f + expf(-zm)) : expf(zm - top) / sum;
-        if (poisoned && there) w = NAN;
-        if (lane < a.how.k) {
-            a.weights[(size_t)token * a.how.k + lane] = a.how.scale * w;
-            a.chosen[(size_t)token * a.how.k + lane] = mine;
+            for (int i = 0; i < PER; i++) c[i] *= unsure;
         }
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (lane + 32 * i < (int)a.experts) c[i] += a.bias[lane + 32 * i];
+        }
+        unsure = unsure_within<PER>(a.how.sigmoid, unsure);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) c[i] = fmaxf(c[i], -INFINITY);          // NaN is not chosen
+    int mine;
+    if (!choose<T, PER>(a, token, c, unsure, mine)) mine = choose_exactly<T, PER>(a, token, plain);
+    const bool there = mine >= 0;
+    const float zm = there ? logit<T>(a, token, mine) : -INFINITY;
+    float w;
+    if (a.how.renormalize) w = share_of(a.how, there, zm);
+    else w = !there ? 0.0f : a.how.sigmoid ? 1.0f / (1.0f + expf(-zm)) : expf(zm - top) / sum;
+    if (poisoned && there) w = NAN;
+    if (lane < a.how.k) {
+        a.weights[token * a.how.k + lane] = a.how.scale * w;
+        a.chosen[token * a.how.k + lane] = mine;
     }
 }
 
@@ -475,8 +470,7 @@ template <typename T, int PER> __global__ void __launch_bounds__(32 * kRouteWarp
 
 template <typename T, int PER> static cudaError_t run_route(const RouteArgs& a, bool backward, cudaStream_t stream) {
     const unsigned ctas = (a.tokens + kRouteWarps - 1) / kRouteWarps;
-    if (backward) return launch_early(k_route_grad<T, PER>, ctas, 32 * kRouteWarps, stream, a);
-    return launch_early(k_route<T, PER>, ctas < a.ctas ? ctas : a.ctas, 32 * kRouteWarps, stream, a);
+    return launch_early(backward ? k_route_grad<T, PER> : k_route<T, PER>, ctas, 32 * kRouteWarps, stream, a);
 }
 template <typename T> static cudaError_t run_route(RouteArgs a, bool backward, cudaStream_t stream) {
     a.vec = a.experts % (16 / sizeof(T)) == 0 && aligned_to(16, {a.dlogits});
@@ -500,7 +494,7 @@ static int route(const char* who, int device, int dtype, size_t tokens, int expe
     a.tokens = (unsigned)tokens;
     a.experts = (unsigned)experts;
     a.how = *how;
-    a.ctas = 8 * (unsigned)sm_count(device);
+    for (unsigned i = 0, whole = experts / how->groups / 32; i < 32 && experts / how->groups % 32 == 0; i++) a.ends |= (unsigned)((i + 1) % whole == 0) << i;
     a.group = Divisor((unsigned)(experts / how->groups));
     const cudaStream_t s = (cudaStream_t)stream;
     return report(who, dtype == 6 ? run_route<__half>(a, backward, s) : dtype == 7 ? run_route<float>(a, backward, s) : run_route<__nv_bfloat16>(a, backward, s));
