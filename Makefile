@@ -114,7 +114,7 @@ $(LIB): $(HOST_OBJS) $(CU_OBJS)
 
 dccl_b200/lib/libdccl.so: $(LIB)
 	@mkdir -p dccl_b200/lib
-	cp $(LIB) $@
+	cp $(LIB) $@.part && mv $@.part $@
 
 $(BUILD)/dccl_cli: tools/dccl_cli.cpp tools/tool_common.hpp $(LIB)
 	$(CXX) $(CXXFLAGS) $(TOOL_DEFS) $< -o $@ -L$(BUILD) -ldccl -Wl,-rpath,'$$ORIGIN' $(CUDA_LIBS) $(LDFLAGS)
