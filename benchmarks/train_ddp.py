@@ -27,6 +27,7 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 from dccl_b200.models.llama import LlamaConfig, LlamaDecoder  # noqa: E402
+from dccl_b200.ops import clip_grad_norm  # noqa: E402
 
 
 def main():
@@ -39,6 +40,7 @@ def main():
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--bucket-mb", type=int, default=25)
     ap.add_argument("--fused", action="store_true", help="the decoder computes with the fused operators of dccl_b200.ops.decoder")
+    ap.add_argument("--clip", type=float, default=None, help="cut the gradients back to this norm before the optimizer's step (dccl_b200.ops.clip_grad_norm)")
     ap.add_argument("--plain-buckets", action="store_true",
                     help="dccl_ddp: leave DDP's gradient buckets in ordinary memory (default: they come from a memory pool of symmetric memory)")
     args = ap.parse_args()
@@ -100,6 +102,11 @@ def main():
             loss.backward()
         if reducer is not None:
             reducer.finish()
+        if args.clip is not None:
+            if reducer is not None:
+                reducer.clip(args.clip)
+            else:
+                clip_grad_norm([p.grad for p in model.parameters()], args.clip)
         opt.step()
         if reducer is not None:
             reducer.zero_grad()
@@ -157,7 +164,7 @@ def main():
             "data": "synthetic", "backend": args.backend, "gpu_launches": int(launches),
             "e2e": {"h2d_bytes_per_step": host_tokens.numel() * 8, "d2h_bytes_per_step": 4, "included": True},
             "config": {"model": "llama-1.1b" if args.model == "1b" else "llama-tiny", "params": cfg.num_params(), "global_batch": world * args.batch,
-                       "seq_len": seq, "parallelism": "dp%d" % world, "bucket_mb": args.bucket_mb, "fused_operators": bool(args.fused), "optimizer": "AdamW fused, bf16 params"},
+                       "seq_len": seq, "parallelism": "dp%d" % world, "bucket_mb": args.bucket_mb, "fused_operators": bool(args.fused), "clip": args.clip, "optimizer": "AdamW fused, bf16 params"},
             "final_loss": round(losses[-1], 4)}))
     if reducer is not None:
         reducer.close()

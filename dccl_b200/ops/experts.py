@@ -149,7 +149,9 @@ def route(logits, k, scores="softmax", bias=None, groups=1, top_groups=1, group_
 
     Of equal scores the expert with the lower number is chosen, and of equal groups likewise. Which experts are chosen is decided as if the scores were exact to 64
     bits. An expert whose logit is minus infinity or NaN is not chosen, nor one whose bias makes its score minus infinity. Where fewer than k are left, the number is -1 and
-    the weight 0: a token of padding is one whose logits are all minus infinity. A NaN among the logits makes a softmax, and all weights of its token, NaN."""
+    the weight 0: a token of padding is one whose logits are all minus infinity. A NaN among the logits (or plus infinity) makes a softmax NaN, and with it all weights of its
+    token; where scores are compared and not logits (with a bias, or ``"top2"``), such a token has no experts. The experts are kept for the backward pass and must not be
+    overwritten before it."""
     top2, sigmoid = group_score == "top2", scores == "sigmoid"
     if isinstance(logits, torch.Tensor) and logits.is_cuda and scores in ("softmax", "sigmoid") and group_score in ("max", "top2"):
         out = _kernel("route", logits, k, sigmoid, bias, groups, top_groups, top2, bool(renormalize), scale)
@@ -223,7 +225,7 @@ def expert_plan(experts, num_experts):
     flat = experts.reshape(-1).long()
     there = (flat >= 0) & (flat < num_experts)
     order = torch.where(there, flat, num_experts).argsort(stable=True)
-    rows = torch.empty_like(flat).scatter_(0, order, torch.arange(flat.numel()))
+    rows = torch.empty_like(flat).scatter_(0, order, torch.arange(flat.numel(), device=flat.device))
     counts = torch.bincount(flat[there], minlength=num_experts)
     starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
     return ExpertPlan(torch.where(there, rows, -1).int().view(experts.shape), counts.int(), starts.int())
@@ -338,5 +340,5 @@ def expert_linear(rows, weight, plan, activation=None):
         if end > start or e == 0:       # a product of no rows ties the result to its inputs
             end = max(start, end)
             v = rows[start:end].float() @ weight[e].float().t()
-            out = out.index_copy(0, torch.arange(start, end), (v if activation is None else _activate_on_cpu(v, activation)).to(rows.dtype))
+            out = out.index_copy(0, torch.arange(start, end, device=rows.device), (v if activation is None else _activate_on_cpu(v, activation)).to(rows.dtype))
     return out

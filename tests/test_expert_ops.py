@@ -244,6 +244,29 @@ def test_route_with_nan(device):
 
 
 @pytest.mark.parametrize("device", EACH)
+def test_route_with_infinities(device):
+    z = logits_of(2, 20, device=device)
+    z[1, 11] = math.inf
+    weights, experts = ops.route(z, 3, "sigmoid")
+    assert experts[1, 0] == 11 and bool(weights.isfinite().all()) and bool(((weights.sum(-1) - 1).abs() < 1e-6).all())
+    weights, experts = ops.route(z, 3, "sigmoid", bias_of(20, device), renormalize=False)
+    assert 11 in experts[1].tolist() and bool(weights.isfinite().all())
+    weights, experts = ops.route(z, 3)
+    assert experts[1, 0] == 11 and bool(weights[1].isnan().all()) and bool(weights[0].isfinite().all())
+    bias = torch.zeros(20, device=device)
+    bias[3], bias[5], bias[6] = math.inf, math.inf, math.nan
+    _, experts = ops.route(z[:1], 18, "sigmoid", bias)
+    assert experts[0, :2].tolist() == [3, 5] and 6 not in experts[0].tolist()
+
+
+@pytest.mark.parametrize("device", EACH)
+def test_route_zeros_of_either_sign_are_equal(device):
+    z = torch.zeros(1, 12, device=device)
+    z[0, ::2] = -0.0
+    assert ops.route(z, 4)[1].tolist() == [[0, 1, 2, 3]] and ops.route(z, 4, bias=z[0] * 1.0)[1].tolist() == [[0, 1, 2, 3]]
+
+
+@pytest.mark.parametrize("device", EACH)
 def test_route_scores_that_underflow(device):
     """Shares of the chosen exist where the scores themselves are zero in fp32."""
     z = torch.tensor([[-120.0, -121.0, -500.0, -130.0], [90.0, 89.0, -90.0, 88.0], [-3.0e38, -3.1e38, -3.2e38, -3.3e38]], device=device)
@@ -775,6 +798,72 @@ def test_a_layer_of_all_operators(device):
     # five roundings in a row, or 2^-18 for the whole chain in fp32, of the largest value
     for a, b in zip([y] + list(grads), [want] + list(want_grads)):
         assert (a.double() - b).abs().max() <= (5 * half_step(dtype) + 2.0 ** -18) * b.abs().max()
+
+
+def test_a_layer_on_cpu_while_another_device_is_the_default():
+    case = [t.requires_grad_(True) for t in layer_case(9, 12, 8, 4, torch.float32, "cpu")]
+    want = layer(*case, 2)
+    grads = torch.autograd.grad(want.sum(), case)
+    with torch.device("meta"):
+        got = layer(*case, 2)
+        again = torch.autograd.grad(got.sum(), case)
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(again, grads))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements of rows, results and saved products: the last rows are what they are alone."""
+    tokens, width = 300_001, 1024
+    experts = torch.full((tokens, 8), 1, dtype=torch.int32, device="cuda")
+    experts[-3:] = torch.tensor([2, 1, 0, 2, 2, 1, 0, 0], dtype=torch.int32, device="cuda")
+    plan = ops.expert_plan(experts, 3)
+    x = torch.zeros(tokens, width, device="cuda", dtype=torch.bfloat16)
+    x[-3:] = torch.randn(3, width, device="cuda").bfloat16()
+    rows = ops.dispatch(x, plan)
+    assert rows.numel() > 2 ** 31 and torch.equal(rows[-9:], x[-3:].repeat_interleave(3, 0)[:9])
+    w = torch.rand(tokens, 8, device="cuda")
+    y = ops.combine(rows, plan, w)
+    want = (x[-3:].double() * w[-3:].double().sum(-1, keepdim=True))
+    check("y", y[-3:], want, half_step(torch.bfloat16) * want.abs() + 9 * 2.0 ** -24 * want.abs())
+    rows.requires_grad_(True)
+    dy = torch.zeros_like(y)
+    dy[-1] = 1.0
+    drows, = torch.autograd.grad(ops.combine(rows, plan, w), rows, dy)
+    got = drows[plan.rows[-1].long()]
+    assert bool((got == w[-1].bfloat16().unsqueeze(-1)).all()) and drows[-9:].count_nonzero() == 3 * width       # of the last token's three rows of expert 2
+    del rows, drows, dy, y, x, plan, experts
+    n, out = 530_000, 4104
+    x = torch.zeros(n, 64, device="cuda", dtype=torch.bfloat16)
+    x[-200:] = torch.randn(200, 64, device="cuda").bfloat16()
+    weight = torch.randn(2, out, 64, device="cuda").bfloat16() / 8
+    starts = torch.tensor([0, n - 130, n - 5], dtype=torch.int32, device="cuda")
+    few = torch.tensor([0, 70, 195], dtype=torch.int32, device="cuda")
+    mine, alone = x.clone().requires_grad_(True), x[-200:].clone().requires_grad_(True)
+    h, g = ops.expert_linear(mine, weight, starts, activation="silu"), ops.expert_linear(alone, weight, few, activation="silu")
+    assert h.numel() > 2 ** 31
+    # k is not cut in either, and one block of it: the same sums
+    assert torch.equal(h[-200:], g)
+    dh = torch.zeros_like(h)
+    dh[-200:] = torch.randn(200, out, device="cuda").bfloat16()
+    big, = torch.autograd.grad(h, mine, dh)
+    small, = torch.autograd.grad(g, alone, dh[-200:])
+    size = torch.zeros(200, 64, dtype=torch.float64, device="cuda")
+    for i, j, e in ((0, 70, 0), (70, 195, 1)):
+        size[i:j] = dh[-200:][i:j].double().abs() @ weight[e].double().abs() * 1.13
+    check("dx", big[-200:], small.double(), 2 * half_step(torch.bfloat16) * small.double().abs() + out * 2.0 ** -23 * size)
+    assert big[:-200].count_nonzero() == 0
+
+
+@gpu
+def test_compiled_functions_stay_right():
+    """The compiler leaves the operators out of its graphs and calls them between."""
+    case = [t.requires_grad_(True) for t in layer_case(33, 64, 72, 8, torch.bfloat16, "cuda")]
+    want = layer(*case, 2)
+    grads = torch.autograd.grad(want.sum(), case)
+    compiled = torch.compile(layer, backend="eager")
+    for _ in range(2):
+        got = compiled(*case, 2)
+        assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got.sum(), case), grads))
 
 
 @gpu

@@ -256,6 +256,71 @@ def test_clipping_on_a_device_that_is_not_the_current_one():
     assert torch.cuda.current_device() == 0
 
 
+@gpu
+def test_offsets_beyond_32_bits():
+    t = torch.zeros(2 ** 32 + 1001, device="cuda", dtype=torch.bfloat16)
+    t[-3:] = torch.tensor([3.0, 4.0, 12.0], device="cuda")
+    out = torch.empty_like(t)
+    assert ops.clip_grad_norm([t], 6.5, out=[out]).item() == 13.0
+    assert out[-3:].tolist() == [1.5, 2.0, 6.0] and out.count_nonzero() == 3
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_steps_that_clip_on_the_gpu(dccl_lib, dtype):
+    """The sharded optimizer (the general step and the one-kernel one after it) and the reducer, on one rank, against clipping by torch."""
+    from dccl_b200 import Communicator
+    from dccl_b200.parallel.ddp import GradientAllReducer
+    from dccl_b200.parallel.zero import ShardedOptimizer
+    comm = Communicator(rank=0, world=1, device=0)
+    try:
+        def make():
+            torch.manual_seed(3)
+            return torch.nn.Sequential(torch.nn.Linear(33, 65), torch.nn.GELU(), torch.nn.Linear(65, 7)).cuda().to(dtype)
+        x = torch.randn(40, 33, device="cuda").to(dtype)
+        plain, sharded, reduced = make(), make(), make()
+        masters = [torch.nn.Parameter(p.detach().float()) for p in plain.parameters()]
+        opt, mine = torch.optim.AdamW(masters, lr=1e-2), ShardedOptimizer(sharded.parameters(), comm, lr=1e-2, max_norm=0.25)
+        reducer = GradientAllReducer(reduced, comm)
+        for step in range(4):
+            for model in (plain, sharded, reduced):
+                model.zero_grad(set_to_none=False) if model is plain else (mine.zero_grad() if model is sharded else reducer.zero_grad())
+                (model(x).float() - step).pow(2).sum().backward()
+            reducer.finish()
+            want = torch.nn.utils.clip_grad_norm_(plain.parameters(), 0.25)
+            if step == 0:               # later the models differ
+                assert abs(reducer.clip(0.25) - want) <= 2.0 ** -6 * want
+                assert all(torch.allclose(a.grad, b.grad, rtol=2.0 ** -6, atol=1e-6) for a, b in zip(plain.parameters(), reduced.parameters()))
+            for m, p in zip(masters, plain.parameters()):
+                m.grad = p.grad.float()
+            opt.step()
+            mine.step()
+            with torch.no_grad():
+                for m, p in zip(masters, plain.parameters()):
+                    p.copy_(m)
+            # clipped gradients rounded once to their type in both
+            assert mine.grad_norm.dtype is torch.float32 and abs(mine.grad_norm - want) <= 2.0 ** -5 * want
+            # a step moves a parameter by lr at most, and by how much hangs on its gradient's rounding
+            for a, b in zip(plain.parameters(), sharded.parameters()):
+                assert (a.float() - b.float()).abs().max() <= (step + 1) * 2e-2 * (0.25 if dtype is torch.bfloat16 else 0.05) + torch.finfo(dtype).eps
+        reducer.close()
+        mine.close()
+    finally:
+        comm.finalize()
+
+
+def test_limits_of_the_sharded_optimizer(dccl_lib):
+    from dccl_b200 import Communicator
+    from dccl_b200.parallel.zero import ShardedOptimizer
+    comm = Communicator(rank=0, world=1)
+    try:
+        for bad in (-1.0, math.nan):
+            with pytest.raises(ValueError):
+                ShardedOptimizer([torch.nn.Parameter(torch.ones(3))], comm, max_norm=bad)
+    finally:
+        comm.finalize()
+
+
 @pytest.mark.parametrize("world", [1, 3])
 def test_norms_over_ranks(dccl_lib, world):
     """Gradients of which every rank has its own: grad_norm and clip_grad_norm with a communicator, the sharded optimizer's max_norm and the reducer's clip, against all of
