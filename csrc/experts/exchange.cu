@@ -169,10 +169,10 @@ struct RowsArgs {
 
 /**
  * A token belongs to `across` threads (whole warps), which take U runs of N elements each at a time, so far apart that a warp's accesses are of neighbours. A CTA has as
- * many tokens as fit. Lane j of every warp has the token's j-th row and weight, and hands them round: loads of them between those of the rows, under conditions of their
+ * many tokens as fit; H of a token's rows are read at once. Lane j of every warp has the token's j-th row and weight, and hands them round: loads of them between those of the rows, under conditions of their
  * own, kept the latter from being in flight together (combine of 16384 x 2048 bf16 by 4: 84 us, and 58 without).
  */
-constexpr int kRowThreads = 128, kHeld = 2;
+constexpr int kRowThreads = 128;
 constexpr unsigned kNoRow = 0xffffffffu;
 
 struct Token { size_t index; unsigned thread, row; float weight; bool there; };
@@ -231,10 +231,10 @@ template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThread
     clear_unused<T, N>(a, out, t);
 }
 
-/** kHeld of a token's rows from the j0-th on, zeros where there is none. */
-template <typename T, int N, int U> __device__ __forceinline__ void hold_rows(const RowsArgs& a, const Token& t, unsigned j0, unsigned i, unsigned step, Run<T, N> (&v)[kHeld][U]) {
+/** H of a token's rows from the j0-th on, zeros where there is none. */
+template <typename T, int N, int U, int H> __device__ __forceinline__ void hold_rows(const RowsArgs& a, const Token& t, unsigned j0, unsigned i, unsigned step, Run<T, N> (&v)[H][U]) {
 #pragma unroll
-    for (int j = 0; j < kHeld; j++) {
+    for (int j = 0; j < H; j++) {
         const unsigned row = __shfl_sync(0xffffffffu, t.row, j0 + j);
         const T* const from = reinterpret_cast<const T*>(a.in) + (size_t)row * a.width + i;
 #pragma unroll
@@ -245,7 +245,7 @@ template <typename T, int N, int U> __device__ __forceinline__ void hold_rows(co
     }
 }
 
-template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThreads, 9) k_combine(const __grid_constant__ RowsArgs a) {
+template <typename T, int N, int U, int H> __global__ void __launch_bounds__(kRowThreads, 9) k_combine(const __grid_constant__ RowsArgs a) {
     wait_for_stream();
     const Token t = token_of<T>(a);
     if (!t.there) return;
@@ -253,11 +253,11 @@ template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThread
     for (unsigned first = (t.thread & ~31u) * N; first < a.width; first += U * step) {
         const unsigned i = first + (t.thread & 31) * N;
         float sum[U][N] = {};
-        for (unsigned j0 = 0; j0 < a.k; j0 += kHeld) {          // at most 32, and lanes behind the last have none
-            Run<T, N> v[kHeld][U];
-            hold_rows<T, N, U>(a, t, j0, i, step, v);
+        for (unsigned j0 = 0; j0 < a.k; j0 += H) {          // at most 32, and lanes behind the last have none
+            Run<T, N> v[H][U];
+            hold_rows<T, N, U, H>(a, t, j0, i, step, v);
 #pragma unroll
-            for (int j = 0; j < kHeld; j++) {
+            for (int j = 0; j < H; j++) {
                 const float w = __shfl_sync(0xffffffffu, t.weight, j0 + j);
 #pragma unroll
                 for (int u = 0; u < U; u++)
@@ -272,7 +272,7 @@ template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThread
     }
 }
 
-template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThreads, 9) k_combine_grad(const __grid_constant__ RowsArgs a) {
+template <typename T, int N, int U, int H> __global__ void __launch_bounds__(kRowThreads, 9) k_combine_grad(const __grid_constant__ RowsArgs a) {
     wait_for_stream();
     __shared__ float dots[kRowThreads / 32][DCCL_EXPERTS_MAX_CHOSEN];
     const Token t = token_of<T>(a);
@@ -280,19 +280,19 @@ template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThread
     const unsigned step = a.across * N;
     if (t.there) {
         const T* dy = reinterpret_cast<const T*>(a.x) + t.index * a.width;
-        for (unsigned j0 = 0; j0 < a.k; j0 += kHeld) {
-            float dot[kHeld] = {};
+        for (unsigned j0 = 0; j0 < a.k; j0 += H) {
+            float dot[H] = {};
             for (unsigned first = (t.thread & ~31u) * N; first < a.width; first += U * step) {
                 const unsigned i = first + (t.thread & 31) * N;
-                Run<T, N> g[U], v[kHeld][U];
+                Run<T, N> g[U], v[H][U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     g[u] = Run<T, N>{};
                     if (i + u * step < a.width) g[u] = ld_run<T, N>(dy + i + u * step);
                 }
-                if (a.out2) hold_rows<T, N, U>(a, t, j0, i, step, v);
+                if (a.out2) hold_rows<T, N, U, H>(a, t, j0, i, step, v);
 #pragma unroll
-                for (int j = 0; j < kHeld; j++) {
+                for (int j = 0; j < H; j++) {
                     if (a.out2) {
 #pragma unroll
                         for (int u = 0; u < U; u++)
@@ -314,7 +314,7 @@ template <typename T, int N, int U> __global__ void __launch_bounds__(kRowThread
             }
             if (a.out2) {
 #pragma unroll
-                for (int j = 0; j < kHeld; j++) {
+                for (int j = 0; j < H; j++) {
                     float d = dot[j];
 #pragma unroll
                     for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
@@ -404,19 +404,23 @@ extern "C" int dccl_dispatch(int device, int dtype, size_t tokens, int k, size_t
 template <typename T> static cudaError_t run_combine(RowsArgs& a, cudaStream_t stream) {
     constexpr int most = 16 / sizeof(T), few = 4 / sizeof(T);
     const int n = run_of<T>(a.width, {a.in, a.out});
-    if (n == most) return run_rows(k_combine<T, most, 1>, most, 1, a, stream);
+    // of one row two runs of a thread, of several a run each of two: 38 us by the latter for 16384 x 2048 bf16 by one, 32 by the former
+    if (n == most && a.k == 1) return run_rows(k_combine<T, most, 2, 1>, most, 2, a, stream);
+    if (n == most) return run_rows(k_combine<T, most, 1, 2>, most, 1, a, stream);
     if constexpr (few > 1)
-        if (n == few) return run_rows(k_combine<T, few, 2>, few, 2, a, stream);
-    return run_rows(k_combine<T, 1, 4>, 1, 4, a, stream);
+        if (n == few) return run_rows(k_combine<T, few, 2, 2>, few, 2, a, stream);
+    return run_rows(k_combine<T, 1, 4, 2>, 1, 4, a, stream);
 }
 
 template <typename T> static cudaError_t run_combine_grad(RowsArgs& a, cudaStream_t stream) {
     constexpr int most = 16 / sizeof(T), few = 4 / sizeof(T);
     const int n = run_of<T>(a.width, {a.x, a.in, a.out});
-    if (n == most) return run_rows(k_combine_grad<T, most, 1>, most, 1, a, stream);
+    // of one row two runs of a thread, of several a run each of two: 62 us by the latter for 16384 x 2048 bf16 by one, 51 by the former
+    if (n == most && a.k == 1) return run_rows(k_combine_grad<T, most, 2, 1>, most, 2, a, stream);
+    if (n == most) return run_rows(k_combine_grad<T, most, 1, 2>, most, 1, a, stream);
     if constexpr (few > 1)
-        if (n == few) return run_rows(k_combine_grad<T, few, 2>, few, 2, a, stream);
-    return run_rows(k_combine_grad<T, 1, 4>, 1, 4, a, stream);
+        if (n == few) return run_rows(k_combine_grad<T, few, 2, 2>, few, 2, a, stream);
+    return run_rows(k_combine_grad<T, 1, 4, 2>, 1, 4, a, stream);
 }
 
 extern "C" int dccl_combine(int device, int dtype, size_t tokens, int k, size_t width, const void* in, const int* rows, const void* weights, int weights32, void* y, void* stream) {
