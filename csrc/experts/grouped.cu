@@ -104,8 +104,12 @@ __device__ __forceinline__ void list_tiles(const Grouped& a, const int* starts, 
  * number gives, so two share one and take half of the columns each. The sums of two tiles fit into tensor memory, so that one is stored while the next is
  * multiplied.
  *
- * What an SM can load bounds it (58 bytes a clock: 48 KB of a tile of 128 x 256 take 1.6 times as long as its products would): the loader must never pause, and finds its
- * place in a tile from shared memory and without divisions.
+ * What an SM can load bounds it while its clock is high: the 48 KB of a block of 64 in k for 128 x 256 take 450 ns (57 bytes a clock), and their products 270; for 128 x 128, 32 KB
+ * and 275 ns. So the loader must never pause: it finds its place in a tile from shared memory and without divisions, and as a load takes it some 60 clocks to give out, one box holds all
+ * blocks of an operand where rows allow. Large products run into the power cap before: 16384 rows of 8 experts, 2048 x 5632, bf16: h 288 us (with GELU and z 340), dx 273 to 285,
+ * dW 286 (333 with a box per block of 64 columns), 1.3 PFLOP/s where the library's largest product gets 1.4 under that cap. Tiles of 128 x 128 serve where the larger would leave SMs
+ * without work; tiles of 32 x 64, two CTAs of an SM, where experts have few rows and reading the weights takes the time (16 rows of those experts: 41 us, 4.4 TB/s); there, what one
+ * thread takes to give products out counts: 60 us with descriptors made anew for each, 44 with their low words counted up.
  */
 template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(kGroupedThreads, GroupedShape<M, N>::kCtas) k_grouped(const __grid_constant__ GroupedArgs a) {
     using Shape = GroupedShape<M, N>;
@@ -146,13 +150,11 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
         for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
             const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
             const unsigned blocks = (p.k_count + kTileK - 1) / kTileK;
-            // of few rows all CTAs read the same lines: each begins somewhere else in k, or those lines' part of L2 is what they wait for (16 rows of 2048 x 5632: 60 us)
-            unsigned kb = 0, ahead = M < kTileM && blocks ? blockIdx.x * 5 % blocks : 0;
+            unsigned kb = 0;
             for (; kb < blocks; kb++, filled++) {
                 if (!bar_wait(empty + 8 * s, parity, &failed)) break;
                 const uint32_t to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA, bar = full + 8 * s;
-                const int k = p.k_from + (M < kTileM ? ahead : kb) * kTileK;
-                if (M < kTileM && ++ahead == blocks) ahead = 0;
+                const int k = p.k_from + kb * kTileK;
                 bar_expect(bar, Shape::kBytes);
                 if constexpr (FORM == EXPERTS_FORWARD) {
                     load_box(to_a, &a.a, k, p.row, bar);
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(kRowCta) k_pad_rows(const __grid_constant__ Pa
 struct ActGradArgs { const void* dh; const float* z; void* dz; const int* starts; size_t z_stride, stride; unsigned rows, experts, n, from, threads; Divisor runs; int act; };
 
 /** dz from dh and the saved products, eight elements per thread; rows of nobody, whose products nobody wrote, are left out. Only the rows of dh may start
- *  anywhere (VEC: they do not). HBM bounds it: 8 bytes per element. */
+ *  anywhere (VEC: they do not). HBM bounds it: 8 bytes per element, 16384 x 5632 in 125 us (5.9 TB/s). */
 template <typename T, bool VEC> __global__ void __launch_bounds__(kRowCta) k_act_grad(const __grid_constant__ ActGradArgs a) {
     wait_for_stream();
     const unsigned index = blockIdx.x * kRowCta + threadIdx.x;

@@ -146,9 +146,9 @@ DCCL_BOTH void grouped_mark(int form, const Grouped& a, const GroupedResults& to
 struct GroupedPlan { unsigned tile_rows, tile_columns, splits; };
 
 /**
- * As if the experts had equal shares of the rows, which the host does not know. What a plan takes, in nanoseconds, is what one CTA takes for its tiles: a block of k is
- * bound by what an SM can load, 117 GB/s (32 KB of a tile of 128 x 128 in 280 ns, 48 KB of one of 128 x 256 in 420), and a tile takes about one microsecond more;
- * parts are stored in fp32, and added up by another launch.
+ * As if the experts had equal shares of the rows, which the host does not know. What a plan takes, in nanoseconds, is what one CTA takes for its tiles: a block of k takes
+ * 280 for a tile of 128 x 128 and 420 for one of 128 x 256 (275 and 450 measured, with every SM at work), and a tile about one microsecond more; parts are stored in fp32, and added up by
+ * another launch.
  * Up to 32 rows of an expert, forward: tiles of 32 x 64. Then reading the weights is all there is to do, and the tile's own rows should not be most of what it loads.
  */
 inline GroupedPlan plan_grouped(int form, int sms, size_t rows, size_t experts, size_t m, size_t n, size_t k) {

@@ -56,19 +56,23 @@ std::vector<DcclGradient> table(const std::vector<Tensor>& in, const std::vector
     return t;
 }
 
-/** Whether what is written overlaps anything but, as a whole, the tensor that it comes from. */
+/** Whether what is written overlaps anything but, as a whole and of the same type, the tensor that it comes from. What is only read may be read twice. */
 bool overlaps(const std::vector<DcclGradient>& t, bool apart) {
     const auto bytes = [](size_t n, int dtype) { return n * (dtype == 7 ? 4 : 2); };
-    struct Range { uintptr_t from, to; };
+    struct Range { uintptr_t from, to; bool written; };
     std::vector<Range> r;
     r.reserve(t.size() * (apart ? 2 : 1));
     for (const DcclGradient& g : t) {
-        r.push_back({(uintptr_t)g.out, (uintptr_t)g.out + bytes(g.elements, g.out_dtype)});
-        if (apart && g.in != g.out) r.push_back({(uintptr_t)g.in, (uintptr_t)g.in + bytes(g.elements, g.dtype)});
+        r.push_back({(uintptr_t)g.out, (uintptr_t)g.out + bytes(g.elements, g.out_dtype), true});
+        if (apart && (g.in != g.out || g.dtype != g.out_dtype)) r.push_back({(uintptr_t)g.in, (uintptr_t)g.in + bytes(g.elements, g.dtype), false});
     }
     std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
-    for (size_t i = 1; i < r.size(); i++)
-        if (r[i].from < r[i - 1].to) return true;
+    uintptr_t written = 0, any = 0;         // the ends of those before
+    for (const Range& g : r) {
+        if (g.from < (g.written ? any : written)) return true;
+        any = std::max(any, g.to);
+        if (g.written) written = std::max(written, g.to);
+    }
     return false;
 }
 

@@ -19,8 +19,9 @@ One layer is::
 
 Nothing of it is read by the host: how many rows an expert has stays on the device, every size is known before (a row for each of a token's experts, whether
 it has one or not), and the layer can be captured into a graph. All but expert_plan are differentiable. CUDA tensors run kernels on the current
-stream of their device (csrc/experts/route.cu, exchange.cu, grouped.cu) in float16, bfloat16 or float32 (expert_linear: not float32): one for a call, of
-expert_linear up to two (rows that do not start on 16 bytes are copied), and in the backward pass one each, of expert_linear up to three. Sums are fp32 and every
+stream of their device (csrc/experts/route.cu, exchange.cu, grouped.cu) in float16, bfloat16 or float32 (expert_linear: not float32): one for a call and
+one for its backward pass. expert_linear has up to three (rows that do not start on 16 bytes are copied, and a product of few tiles is cut along what it sums over and
+joined), and in the backward pass one for the activation's gradient and one or two for each of the others. Sums are fp32 and every
 result is rounded once. CPU tensors take the same formulas in torch. Inputs may have any strides; what a kernel cannot read in place is copied first. A call
 allocates its outputs and its workspace from torch's allocator and nothing else. There are no atomics: the same inputs give the same bits.
 

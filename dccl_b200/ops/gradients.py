@@ -94,7 +94,8 @@ def clip_grad_norm(tensors, max_norm, out=None, comm=None):
     ``torch.nn.utils.clip_grad_norm_`` does; where nothing has to change nothing is written in place.
 
     What is written must not share memory with any other of the tensors."""
-    if type(tensors) is list and comm is None and tensors and isinstance(tensors[0], torch.Tensor) and tensors[0].is_cuda and isinstance(max_norm, (int, float)):
+    if (type(tensors) is list and comm is None and tensors and isinstance(tensors[0], torch.Tensor) and tensors[0].is_cuda and isinstance(max_norm, (int, float))
+            and (out is None or type(out) is list)):
         norm = _ext().clip_grad_norm(tensors, out, max_norm, None)
         if isinstance(norm, torch.Tensor):
             return norm

@@ -16,7 +16,8 @@ takes it, tokens put in the experts' order and added up by kernels, and one prod
                             routing=dict(scores="sigmoid", renormalize=True, scale=2.5))
 
 Its experts' weights are one parameter each for all experts of the rank (``w_in`` [experts, h, d], ``w_out`` [experts, d, h]); a state dict of either form loads
-into the other. One rank alone never reads anything back to the host, and can be captured into a graph.
+into the other. One rank alone never reads anything back to the host, and can be captured into a graph. (In float32 on the GPU, without autocast, the experts' products are
+the plain layer's, and how many rows each has is read.)
 
 The router is replicated; its gradient on a rank covers that rank's tokens only and is summed with the other
 replicated parameters (``tensor_parallel.sync_replicated_grads``) when the ranks hold different tokens.
@@ -95,7 +96,7 @@ class ExpertParallelMLP(torch.nn.Module):
         plan = ops.expert_plan(experts, self.num_experts)
         rows = ops.dispatch(x, plan)                            # in the order of the experts, hence of their ranks
         if n == 1:
-            return ops.combine(self._experts(rows, plan), plan, weights)
+            return ops.combine(self._experts(rows, plan).to(x.dtype), plan, weights)
         incoming = torch.empty_like(plan.counts)
         comm.all_to_all(plan.counts, incoming)                  # row p: what rank p sends to my experts
         send_counts, recv_counts = (c.view(n, per).sum(1).tolist() for c in (plan.counts, incoming))
@@ -104,16 +105,19 @@ class ExpertParallelMLP(torch.nn.Module):
         of = torch.arange(per, device=x.device).repeat(n).repeat_interleave(incoming, output_size=sum(recv_counts))
         mine = ops.expert_plan(of.unsqueeze(-1), per)
         done = ops.combine(self._experts(ops.dispatch(got, mine), mine), mine)
-        back = F.all_to_all(done, recv_counts, send_counts, comm)               # combine: the way they came
+        back = F.all_to_all(done, recv_counts, send_counts, comm).to(x.dtype)   # combine: the way they came
         return ops.combine(torch.nn.functional.pad(back, (0, 0, 0, rows.shape[0] - used)), plan, weights)
 
     def _experts(self, rows, plan):
-        """Both products of every expert of this rank, for rows in their order."""
+        """Both products of every expert of this rank, for rows in their order; under autocast in its type, as a linear layer's."""
+        w_in, w_out = self.w_in, self.w_out
+        if torch.is_autocast_enabled(rows.device.type):
+            rows, w_in, w_out = (t.to(torch.get_autocast_dtype(rows.device.type)) for t in (rows, w_in, w_out))
         if rows.is_cuda and rows.dtype is torch.float32:        # which the tensor cores do not multiply
-            done = [torch.nn.functional.linear(torch.nn.functional.gelu(torch.nn.functional.linear(r, self.w_in[j])), self.w_out[j])
+            done = [torch.nn.functional.linear(torch.nn.functional.gelu(torch.nn.functional.linear(r, w_in[j])), w_out[j])
                     for j, r in enumerate(rows[:int(plan.starts[-1])].split(plan.counts.tolist()))]
             return torch.nn.functional.pad(torch.cat(done), (0, 0, 0, rows.shape[0] - sum(d.shape[0] for d in done)))
-        return ops.expert_linear(ops.expert_linear(rows, self.w_in, plan, activation="gelu"), self.w_out, plan)
+        return ops.expert_linear(ops.expert_linear(rows, w_in, plan, activation="gelu"), w_out, plan)
 
 
 def _take_either_form(module, state, prefix, *_):

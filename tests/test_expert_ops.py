@@ -1190,3 +1190,31 @@ def test_the_fused_layer_on_the_gpu(dccl_lib, dtype):
                 assert torch.equal(out, fused(still))
     finally:
         comm.finalize()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_the_fused_layer_under_autocast(dccl_lib, dtype):
+    """fp32 parameters, multiplied in 16 bits: what comes out has the types of the plain layer. Both round the tokens, the weights, h and the experts' results; the plain one
+    what the activation takes as well, and the gradients of all of those: as in the test above."""
+    from dccl_b200 import Communicator
+    from dccl_b200.parallel.expert_parallel import ExpertParallelMLP
+    comm = Communicator(rank=0, world=1, device=0)
+    try:
+        plain = ExpertParallelMLP(64, 72, 8, comm, device="cuda")
+        fused = ExpertParallelMLP(64, 72, 8, comm, device="cuda", fused=True)
+        fused.load_state_dict(plain.state_dict())
+        x = torch.randn(50, 64, generator=torch.Generator().manual_seed(3)).cuda()
+        a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+        with torch.autocast("cuda", dtype=dtype):
+            ya, yb = plain(a), fused(b)
+        assert yb.dtype is ya.dtype
+        dy = torch.randn_like(ya)
+        ya.backward(dy)
+        yb.backward(dy)
+        pairs = [(ya, yb), (a.grad, b.grad), (plain.router.grad, fused.router.grad)]
+        pairs += [(p[j].grad, f.grad[j]) for p, f in ((plain.w_in, fused.w_in), (plain.w_out, fused.w_out)) for j in range(8) if p[j].grad is not None]
+        for p, f in pairs:
+            assert p.dtype is f.dtype and (p.double() - f.double()).abs().max() <= 16 * half_step(dtype) * p.double().abs().max()
+    finally:
+        comm.finalize()

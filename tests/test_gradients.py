@@ -187,6 +187,42 @@ def test_refusals(device):
         assert abs(t.norm().item() - 1) < 1e-5
 
 
+@pytest.mark.parametrize("device", EACH)
+def test_gradients_that_are_read_twice(device):
+    """What is only read may be in the list more than once, and in part; what is written may not be what another one reads."""
+    t = gradients([1000, 70], [torch.bfloat16], device)
+    clip_check([t[0], t[0], t[0][:100], t[1], t[1]], 0.5, [torch.empty_like(v) for v in (t[0], t[0], t[0][:100], t[1], t[1])])
+    if device == "cuda":
+        for to in ([t[0], torch.empty_like(t[0])], [torch.empty_like(t[0]), t[0]]):
+            with pytest.raises(ValueError):
+                ops.clip_grad_norm([t[0], t[0]], 0.5, out=to)
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm([t[0], t[0][:900], t[0][10:20]], 0.5, out=[torch.empty_like(t[0]), torch.empty_like(t[0][:900]), t[0][950:960]])
+
+
+@gpu
+def test_gradients_are_not_widened_in_place():
+    """An element of fp32 lies where two of bf16 are read."""
+    wide = torch.ones(1000, device="cuda")
+    narrow = wide.view(torch.bfloat16)[:1000]
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm([narrow], 0.5, out=[wide])
+    assert bool((wide == 1).all())
+
+
+@pytest.mark.parametrize("device", EACH)
+def test_any_sequence_takes_what_is_clipped(device):
+    t = gradients([100, 1], [torch.float32], device)
+    want, factor = reference(t, 0.5)
+    for tensors, out in ((t, lambda o: iter(o)), (t, tuple), (tuple(t), list), (iter(t), tuple)):
+        to = [torch.zeros_like(v) for v in t]
+        assert abs(ops.clip_grad_norm(tensors, 0.5, out=out(to)).item() - want) <= NORM * want
+        assert all(bool(((o.double() - v.double() * factor).abs() <= v.double().abs() * (2.0 ** -24 + 2 * NORM)).all()) for o, v in zip(to, t))
+    one, to = t[:1], torch.zeros_like(t[0])
+    ops.clip_grad_norm(one, 0.5, out=to)
+    assert abs(to.norm().item() - 0.5) < 1e-5
+
+
 class SeesDispatch(torch.utils._python_dispatch.TorchDispatchMode):
     def __init__(self):
         super().__init__()
