@@ -151,6 +151,16 @@ __device__ __forceinline__ void pair_load_box(uint32_t to, const CUtensorMap* ma
                  "r"(cluster_bar)
                  : "memory");
 }
+__device__ __forceinline__ void pair_load_box(uint32_t to, const CUtensorMap* map, int x, int y, int z, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(cluster_bar)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_load_box(uint32_t to, const CUtensorMap* map, int x, int y, int z, int w, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x),
+                 "r"(y), "r"(z), "r"(w), "r"(cluster_bar)
+                 : "memory");
+}
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t to_shared, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to_shared), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -158,6 +168,12 @@ __device__ __forceinline__ void pair_tmem_alloc(uint32_t to_shared, uint32_t col
 __device__ __forceinline__ void pair_tmem_free(uint32_t addr, uint32_t columns) { asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns)); }
 __device__ __forceinline__ void pair_product(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"((int)add)
+                 : "memory");
+}
+/** And by halves. */
+__device__ __forceinline__ void pair_product(uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t desc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(desc), "r"((int)add)
                  : "memory");
 }
 /** One arrival on the barrier at this offset in both CTAs when the leader's products so far are done. */

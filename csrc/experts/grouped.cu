@@ -68,10 +68,15 @@ struct GroupedArgs : Grouped, GroupedResults {
     int* gave_up;
 };
 
-/** Tiles of M x N. A product reads 128 rows of the first operand from shared memory: behind M of them lies something else, and nobody reads what becomes of it. */
+/**
+ * Tiles of M x N. A product reads 128 rows of the first operand from shared memory: behind M of them lies something else, and nobody reads what becomes of it. Tiles of more
+ * are those of a pair of CTAs, each of which holds 128 of the rows and half of what makes the columns.
+ */
 template <int M, int N> struct GroupedShape {
+    static constexpr bool kPair = M > kTileM;
+    static constexpr int kHeldM = kPair ? kTileM : M, kHeldN = kPair ? N / 2 : N;
     static constexpr int kCtas = M < kTileM ? 2 : 1;        // of an SM: for small tiles, what one thread takes to give products out is what bounds a CTA
-    static constexpr int kBytesA = M * kTileK * 2, kBytesB = N * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kCtas / kBytes;
+    static constexpr int kBytesA = kHeldM * kTileK * 2, kBytesB = kHeldN * kTileK * 2, kBytes = kBytesA + kBytesB, kStages = 192 * 1024 / kCtas / kBytes;
     static constexpr int kStagings = M < kTileM ? 2 : kGroupedWarps;                    // warps that have rows to store
     static constexpr int kShared = kStages * kBytes + kStagings * 4096 + 1024;          // 1024: the tiles' alignment
     static_assert(kCtas * (kShared + 2 * 1024) <= 227 * 1024, "with the list of tiles and the barriers");
@@ -100,35 +105,55 @@ __device__ __forceinline__ void list_tiles(const Grouped& a, const int* starts, 
 }
 
 /**
+ * Zeros in the rows of a block of k behind `left` of them, for both operands, which stand in LINES / 64 blocks of 64 rows of 128 bytes: rows of the next expert, and whatever
+ * they are; as many as the last product of 16 would add. By one warp.
+ */
+template <int LINES> __device__ __forceinline__ void clear_rows(char* at, unsigned left, unsigned lane) {
+    const unsigned pieces = ((left + 15) / 16 * 16 - left) * 8;
+    for (unsigned i = lane; i < pieces * LINES / 64; i += 32) *reinterpret_cast<uint4*>(at + i / pieces * 64 * 128 + left * 128 + i % pieces * 16) = uint4{};
+    shared_writes_before_products();
+    __syncwarp();
+}
+
+/**
  * One CTA per SM walks over tiles of M rows and N columns; one warp loads, one multiplies, eight store: a warp reaches the quarter of the tile's rows that its
  * number gives, so two share one and take half of the columns each. The sums of two tiles fit into tensor memory, so that one is stored while the next is
  * multiplied.
  *
- * What an SM can load bounds it while its clock is high: the 48 KB of a block of 64 in k for 128 x 256 take 450 ns (57 bytes a clock), and their products 270; for 128 x 128, 32 KB
- * and 275 ns. So the loader must never pause: it finds its place in a tile from shared memory and without divisions, and as a load takes it some 60 clocks to give out, one box holds all
- * blocks of an operand where rows allow. Large products run into the power cap before: 16384 rows of 8 experts, 2048 x 5632, bf16: h 288 us (with GELU and z 340), dx 273 to 285,
- * dW 286 (333 with a box per block of 64 columns), 1.3 PFLOP/s where the library's largest product gets 1.4 under that cap. Tiles of 128 x 128 serve where the larger would leave SMs
- * without work; tiles of 32 x 64, two CTAs of an SM, where experts have few rows and reading the weights takes the time (16 rows of those experts: 41 us, 4.4 TB/s); there, what one
- * thread takes to give products out counts: 60 us with descriptors made anew for each, 44 with their low words counted up.
+ * What an SM can load bounds a single CTA: the 48 KB of a block of 64 in k for 128 x 256 take 450 ns (57 bytes a clock), their products 270; for 128 x 128, 32 KB and 275 ns. As a
+ * pair, two CTAs share tiles of 256 x 256 and load 32 KB each. The leader's barriers count the bytes of both, and the leader multiplies; only where rows behind the last are
+ * cleared, each does that to its own, and the other one tells the leader (by an arrival for every block it took 900 ns a block). 16384 rows of 8 experts, 2048 x 5632,
+ * bf16, pairs (and single CTAs): h 249 us (288), dx 247 (273), dW 278 (289), 1.36 to 1.53 PFLOP/s, where power bounds them as it does the library's products.
+ * The loader must never pause: it finds its place in a tile from shared memory and without divisions, and as a load takes it some 60 clocks to give out, one box holds all
+ * blocks of an operand where rows allow (dW of single CTAs 333 us with a box per block of 64 columns, 286 with one).
+ * Tiles of 128 x 128 and 128 x 256 serve where the larger would leave SMs without work; tiles of 32 x 64, two CTAs of an SM, where experts have few rows and reading the weights
+ * takes the time (16 rows of those experts: 41 us, 4.4 TB/s); there, what one thread takes to give products out counts: 60 us with descriptors made anew for each, 44 with
+ * their low words counted up.
  */
-template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(kGroupedThreads, GroupedShape<M, N>::kCtas) k_grouped(const __grid_constant__ GroupedArgs a) {
+template <typename T, int FORM, int M, int N> __device__ __forceinline__ void grouped(const GroupedArgs& a) {
     using Shape = GroupedShape<M, N>;
     constexpr int kStages = Shape::kStages;
+    constexpr bool PAIR = Shape::kPair;
     extern __shared__ char shared[];
-    __shared__ uint64_t bars[2 * kStages + 5];
+    __shared__ uint64_t bars[(PAIR ? 3 : 2) * kStages + 5];
     __shared__ unsigned first[kListed + 1];
     __shared__ int own[kListed + 1];
     __shared__ uint32_t tmem_base;
     __shared__ int failed;
     char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
     char* const staging = tiles + kStages * Shape::kBytes;
-    const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16, drained = sums_empty + 16;
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (warp == kGroupedMultiplier) tmem_alloc(shared_addr(&tmem_base), 2 * N);
+    const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16, drained = sums_empty + 16, landed = drained + 8;
+    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = PAIR ? cluster_rank() : 0;
+    const unsigned worker = PAIR ? blockIdx.x / 2 : blockIdx.x, workers = PAIR ? gridDim.x / 2 : gridDim.x;
+    if (warp == kGroupedMultiplier) {
+        if constexpr (PAIR) pair_tmem_alloc(shared_addr(&tmem_base), 2 * N);
+        else tmem_alloc(shared_addr(&tmem_base), 2 * N);
+    }
     if (threadIdx.x == 0) {
         failed = 0;
         for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
-        for (int i = 0; i < 2; i++) { bar_init(sums_full + 8 * i, 1); bar_init(sums_empty + 8 * i, kGroupedWarps); }
+        for (int i = 0; PAIR && i < kStages; i++) bar_init(landed + 8 * i, 1);
+        for (int i = 0; i < 2; i++) { bar_init(sums_full + 8 * i, 1); bar_init(sums_empty + 8 * i, (PAIR ? 2 : 1) * kGroupedWarps); }
         bar_init(drained, 1);
         bar_init_fence();
     }
@@ -140,6 +165,7 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
     if (warp == 1) list_tiles(a, a.starts, first, own);
     tc_before_sync();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();
     tc_after_sync();
     const int* const starts = a.stride == 1 ? own : a.starts;
     const uint32_t sums = tmem_base;
@@ -147,44 +173,66 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
     unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
     if (warp == kGroupedLoader && lane == 0) {
         unsigned s = 0, parity = 1;
-        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+        const auto load = [](auto... box) {
+            if constexpr (PAIR) pair_load_box(box...);
+            else load_box(box...);
+        };
+        for (unsigned tile = worker; tile < total; tile += workers) {
             const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
+            const unsigned row = p.row + rank * Shape::kHeldM, column = p.column + rank * Shape::kHeldN;
             const unsigned blocks = (p.k_count + kTileK - 1) / kTileK;
             unsigned kb = 0;
             for (; kb < blocks; kb++, filled++) {
                 if (!bar_wait(empty + 8 * s, parity, &failed)) break;
-                const uint32_t to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA, bar = full + 8 * s;
+                const bool tail = PAIR && FORM == EXPERTS_WEIGHT && kb + 1 == blocks && p.k_count % kTileK;          // where each CTA clears rows first
+                const uint32_t to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA, bar = tail ? in_cta(landed + 8 * s, rank) : PAIR ? in_cta(full + 8 * s, 0) : full + 8 * s;
                 const int k = p.k_from + kb * kTileK;
-                bar_expect(bar, Shape::kBytes);
+                if (tail) bar_expect(landed + 8 * s, Shape::kBytes);
+                else if (rank == 0) bar_expect(full + 8 * s, (PAIR ? 2 : 1) * Shape::kBytes);         // the leader counts both CTAs' bytes
                 if constexpr (FORM == EXPERTS_FORWARD) {
-                    load_box(to_a, &a.a, k, p.row, bar);
-                    load_box(to_b, &a.b, k, p.column, p.expert, bar);
+                    load(to_a, &a.a, k, row, bar);
+                    load(to_b, &a.b, k, column, p.expert, bar);
                 } else if constexpr (FORM == EXPERTS_INPUT) {
-                    load_box(to_a, &a.a, k, p.row, bar);
-                    if (a.whole_b) load_box(to_b, &a.b, 0, k, p.column / 64, p.expert, bar);
+                    load(to_a, &a.a, k, row, bar);
+                    if (a.whole_b) load(to_b, &a.b, 0, k, column / 64, p.expert, bar);
                     else
 #pragma unroll
-                        for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, p.expert, bar);
+                        for (int i = 0; i < Shape::kHeldN / 64; i++) load(to_b + i * 64 * 128, &a.b, column + 64 * i, k, p.expert, bar);
                 } else {
-                    if (a.whole_a) load_box(to_a, &a.a, 0, k, p.row / 64, bar);
+                    if (a.whole_a) load(to_a, &a.a, 0, k, row / 64, bar);
                     else
 #pragma unroll
-                        for (int i = 0; i < M / 64; i++) load_box(to_a + i * 64 * 128, &a.a, p.row + 64 * i, k, bar);
-                    if (a.whole_b) load_box(to_b, &a.b, 0, k, p.column / 64, bar);
+                        for (int i = 0; i < Shape::kHeldM / 64; i++) load(to_a + i * 64 * 128, &a.a, row + 64 * i, k, bar);
+                    if (a.whole_b) load(to_b, &a.b, 0, k, column / 64, bar);
                     else
 #pragma unroll
-                        for (int i = 0; i < N / 64; i++) load_box(to_b + i * 64 * 128, &a.b, p.column + 64 * i, k, bar);
+                        for (int i = 0; i < Shape::kHeldN / 64; i++) load(to_b + i * 64 * 128, &a.b, column + 64 * i, k, bar);
                 }
                 if (++s == kStages) { s = 0; parity ^= 1; }
             }
             if (kb < blocks) break;
         }
+    } else if (warp == kGroupedMultiplier && rank != 0) {       // the leader multiplies
+        if constexpr (FORM == EXPERTS_WEIGHT) {
+            unsigned used = 0, parities = 0;
+            for (unsigned tile = worker; tile < total; tile += workers) {
+                const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
+                used += (p.k_count + kTileK - 1) / kTileK;
+                const unsigned left = p.k_count % kTileK;
+                if (!left) continue;
+                const unsigned s = (used - 1) % kStages;
+                if (!bar_wait_warp(landed + 8 * s, parities >> s & 1, &failed)) break;
+                parities ^= 1u << s;
+                clear_rows<Shape::kHeldM + Shape::kHeldN>(tiles + s * Shape::kBytes, left, lane);
+                if (elect_one()) bar_arrive_remote(in_cta(full + 8 * s, 0));
+            }
+        }
     } else if (warp == kGroupedMultiplier) {
-        unsigned done = 0, s = 0, parity = 0;
+        unsigned done = 0, s = 0, parity = 0, parities = 0;
         const uint64_t of_a = tile_descriptor(shared_addr(tiles), FORM == EXPERTS_WEIGHT ? 64 * 128 : 16);
         const uint64_t of_b = tile_descriptor(shared_addr(tiles) + Shape::kBytesA, FORM == EXPERTS_FORWARD ? 16 : 64 * 128);
         const uint32_t first_a = (uint32_t)of_a, high_a = (uint32_t)(of_a >> 32), first_b = (uint32_t)of_b, high_b = (uint32_t)(of_b >> 32);
-        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+        for (unsigned tile = worker; tile < total; tile += workers) {
             const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
             const unsigned blocks = (p.k_count + kTileK - 1) / kTileK;
             if (!blocks) continue;
@@ -202,11 +250,11 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
                     const unsigned left = p.k_count - kb * kTileK;
                     if (left < (unsigned)kTileK) {      // rows of the next expert, and whatever they are: as many as the last product of 16 would add
                         steps = (left + 15) / 16;
-                        const unsigned pieces = (steps * 16 - left) * 8;
-                        for (unsigned i = lane; i < pieces * (M + N) / 64; i += 32)
-                            *reinterpret_cast<uint4*>(at + i / pieces * 64 * 128 + left * 128 + i % pieces * 16) = uint4{};
-                        shared_writes_before_products();
-                        __syncwarp();
+                        if constexpr (PAIR) {
+                            if (!bar_wait_warp(landed + 8 * s, parities >> s & 1, &failed)) break;
+                            parities ^= 1u << s;
+                        }
+                        clear_rows<Shape::kHeldM + Shape::kHeldN>(at, left, lane);
                     }
                 }
                 if (elect_one()) {
@@ -215,26 +263,32 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
                     for (unsigned k = 0; k < kTileK / 16; k++) {
                         if (FORM == EXPERTS_WEIGHT && k >= steps) break;
                         // 16 k: 32 bytes further along K-major rows, or 16 rows of 128 bytes further
-                        product(d, da + k * (FORM == EXPERTS_WEIGHT ? 128 : 2), high_a, db + k * (FORM == EXPERTS_FORWARD ? 2 : 128), high_b, a.descriptor, kb || k);
+                        const uint32_t at_a = da + k * (FORM == EXPERTS_WEIGHT ? 128 : 2), at_b = db + k * (FORM == EXPERTS_FORWARD ? 2 : 128);
+                        if constexpr (PAIR) pair_product(d, at_a, high_a, at_b, high_b, a.descriptor, kb || k);
+                        else product(d, at_a, high_a, at_b, high_b, a.descriptor, kb || k);
                     }
-                    commit(empty + 8 * s);
+                    if constexpr (PAIR) pair_commit(empty + 8 * s);
+                    else commit(empty + 8 * s);
                 }
                 __syncwarp();
                 if (++s == kStages) { s = 0; parity ^= 1; }
             }
             if (kb < blocks) break;
-            if (elect_one()) commit(sums_full + 8 * buffer);
+            if (elect_one()) {
+                if constexpr (PAIR) pair_commit(sums_full + 8 * buffer);
+                else commit(sums_full + 8 * buffer);
+            }
             done++;
         }
     } else if (warp < kGroupedWarps) {
         char* const stage = staging + (M < kTileM ? warp / 4 : warp) * 4096;
         unsigned done = 0;
         const bool vec = a.n % 8 == 0 && aligned16(a.c);
-        const unsigned quarter = warp % 4, half = warp / 4;
-        for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+        const unsigned quarter = warp % 4, half = warp / 4, above = rank * kTileM + quarter * 32;
+        for (unsigned tile = worker; tile < total; tile += workers) {
             const GroupedPlace p = grouped_place(FORM, tile, a, first, starts);
-            const int rows = quarter * 32 < p.rows ? (int)(p.rows - quarter * 32 < 32 ? p.rows - quarter * 32 : 32) : 0;
-            const size_t row = grouped_row(FORM, p, quarter * 32, a);
+            const int rows = above < p.rows ? (int)(p.rows - above < 32 ? p.rows - above : 32) : 0;
+            const size_t row = grouped_row(FORM, p, above, a);
             const bool summed = p.k_count != 0;         // otherwise nothing was: rows of nobody, an expert without rows
             const unsigned buffer = done & 1;
             if (summed) {
@@ -279,24 +333,40 @@ template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(
             done++;
             tc_before_sync();
             __syncwarp();
-            if (lane == 0) bar_arrive(sums_empty + 8 * buffer);
+            if (lane == 0) {
+                if constexpr (PAIR) bar_arrive_remote(in_cta(sums_empty + 8 * buffer, 0));
+                else bar_arrive(sums_empty + 8 * buffer);
+            }
         }
     }
     __syncthreads();
     if (failed) {       // no wait is expected to run out: copies in flight still have to land, and products to end, before the memory is given back
         int late = 0;
-        grouped_mark(FORM, a, a, first, starts, blockIdx.x, gridDim.x, threadIdx.x, kGroupedThreads);
-        if (warp == kGroupedLoader && lane == 0)
+        grouped_mark(FORM, a, a, first, starts, worker, workers, threadIdx.x, kGroupedThreads);
+        if (warp == kGroupedLoader && lane == 0 && rank != 0)       // its copies count on the leader's barriers: here only time tells that they have landed
+            for (const long long start = clock64(); clock64() - start < kLandClocks;) {}
+        if (warp == kGroupedLoader && lane == 0 && rank == 0)
             for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
-        if (warp == kGroupedMultiplier && elect_one()) {        // the lane whose products they are
-            commit(drained);
+        if (rank == 0 && warp == kGroupedMultiplier && elect_one()) {        // the lane whose products they are
+            if constexpr (PAIR) pair_commit(drained);
+            else commit(drained);
             bar_wait(drained, 0, &late);
         }
         if (threadIdx.x == 0 && a.gave_up) *reinterpret_cast<volatile int*>(a.gave_up) = 1;
         __syncthreads();
     }
+    if constexpr (PAIR) cluster_sync();      // neither CTA's memory goes before the other is done with it
     tc_after_sync();
-    if (warp == kGroupedMultiplier) tmem_free(sums, 2 * N);
+    if (warp == kGroupedMultiplier) {
+        if constexpr (PAIR) pair_tmem_free(sums, 2 * N);
+        else tmem_free(sums, 2 * N);
+    }
+}
+template <typename T, int FORM, int M, int N> __global__ void __launch_bounds__(kGroupedThreads, GroupedShape<M, N>::kCtas) k_grouped(const __grid_constant__ GroupedArgs a) {
+    grouped<T, FORM, M, N>(a);
+}
+template <typename T, int FORM, int N> __global__ void __launch_bounds__(kGroupedThreads, 1) __cluster_dims__(2, 1, 1) k_grouped_pair(const __grid_constant__ GroupedArgs a) {
+    grouped<T, FORM, 2 * kTileM, N>(a);
 }
 
 struct JoinPartsArgs { const float* partial; size_t rows, stride; unsigned n, splits, runs; int act; void* c; float* z; size_t z_stride; bool vec; };
@@ -447,16 +517,23 @@ static GroupedLayout grouped_layout(int device, size_t rows, int experts, size_t
     return l;
 }
 
+template <typename T, int FORM, int M, int N> static auto grouped_kernel() {
+    if constexpr (GroupedShape<M, N>::kPair) return k_grouped_pair<T, FORM, N>;
+    else return k_grouped<T, FORM, M, N>;
+}
+
 template <typename T, int FORM, int M, int N> static cudaError_t run_grouped(int device, GroupedArgs& a, cudaStream_t stream) {
+    using Shape = GroupedShape<M, N>;
+    const auto kernel = grouped_kernel<T, FORM, M, N>();
     static std::atomic<bool> ready[64];
     if (!ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k_grouped<T, FORM, M, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, GroupedShape<M, N>::kShared);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_relaxed);
     }
-    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == EXPERTS_WEIGHT, FORM != EXPERTS_FORWARD, kTileM, N);
-    const unsigned workers = (unsigned)sm_count(device) * GroupedShape<M, N>::kCtas;
-    return launch_early_shared(k_grouped<T, FORM, M, N>, a.most < workers ? a.most : workers, kGroupedThreads, GroupedShape<M, N>::kShared, stream, a);
+    a.descriptor = product_descriptor(std::is_same<T, __nv_bfloat16>::value, FORM == EXPERTS_WEIGHT, FORM != EXPERTS_FORWARD, Shape::kPair ? M : kTileM, N);
+    const unsigned workers = Shape::kPair ? (unsigned)sm_count(device) / 2 : (unsigned)sm_count(device) * Shape::kCtas;
+    return launch_early_shared(kernel, (a.most < workers ? a.most : workers) * (Shape::kPair ? 2 : 1), kGroupedThreads, Shape::kShared, stream, a);
 }
 
 template <typename T, int FORM> static cudaError_t run_grouped(int device, const GroupedPlan& p, GroupedArgs& a, cudaStream_t stream) {
@@ -474,13 +551,13 @@ template <typename T, int FORM> static cudaError_t run_grouped(int device, const
     a.partial_stride = up_to(a.n, 4);
     a.gave_up = gave_up_flag(device);
     cudaError_t e;
-    if constexpr (FORM == EXPERTS_FORWARD) {
-        e = p.tile_rows == 32        ? run_grouped<T, FORM, 32, 64>(device, a, stream)
-            : p.tile_columns == 128 ? run_grouped<T, FORM, 128, 128>(device, a, stream)
-                                    : run_grouped<T, FORM, 128, 256>(device, a, stream);
-    } else {
-        e = p.tile_columns == 128 ? run_grouped<T, FORM, 128, 128>(device, a, stream) : run_grouped<T, FORM, 128, 256>(device, a, stream);
-    }
+    const auto large = [&] {
+        return p.tile_rows > kTileM       ? run_grouped<T, FORM, 2 * kTileM, 256>(device, a, stream)
+               : p.tile_columns == 128 ? run_grouped<T, FORM, 128, 128>(device, a, stream)
+                                       : run_grouped<T, FORM, 128, 256>(device, a, stream);
+    };
+    if constexpr (FORM == EXPERTS_FORWARD) e = p.tile_rows == 32 ? run_grouped<T, FORM, 32, 64>(device, a, stream) : large();
+    else e = large();
     if (e != cudaSuccess || p.splits == 1) return e;
     const JoinPartsArgs j = {a.partial, grouped_rows(FORM, a), a.partial_stride, a.n, p.splits, (unsigned)(a.partial_stride / 4), a.act, a.c, a.z, a.z_stride,
                              a.n % 4 == 0 && aligned_to(8, {a.c})};
@@ -550,8 +627,8 @@ template <typename T> static cudaError_t grouped_forward(const GroupedCall& k, c
     a.c = h;
     a.z = z;
     a.z_stride = z_stride;
-    if (e == cudaSuccess) e = make_map(&a.a, k.dtype, x, k.width, k.rows, l.stride, l.forward.tile_rows);
-    if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts, 1}, {l.stride, l.stride * k.out, 0}, {64, l.forward.tile_columns, 1, 1});
+    if (e == cudaSuccess) e = make_map(&a.a, k.dtype, x, k.width, k.rows, l.stride, l.forward.held_rows());
+    if (e == cudaSuccess) e = make_map(&a.b, k.dtype, w, 3, {k.width, k.out, (size_t)k.experts, 1}, {l.stride, l.stride * k.out, 0}, {64, l.forward.held_columns(), 1, 1});
     return e == cudaSuccess ? run_grouped<T, EXPERTS_FORWARD>(k.device, l.forward, a, k.stream) : e;
 }
 
@@ -589,7 +666,7 @@ template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, 
         a.k_blocks = blocks_of(k.out, kTileK);
         a.c = dx;
         e = make_map(&a.a, k.dtype, dz, k.out, k.rows, d_stride, kTileM);
-        if (e == cudaSuccess) e = map_of_blocks(&a.b, a.whole_b, k.dtype, w, k.experts, k.out, k.width, l.stride, l.input.tile_columns / 64);
+        if (e == cudaSuccess) e = map_of_blocks(&a.b, a.whole_b, k.dtype, w, k.experts, k.out, k.width, l.stride, l.input.held_columns() / 64);
         if (e == cudaSuccess) e = run_grouped<T, EXPERTS_INPUT>(k.device, l.input, a, k.stream);
     }
     if (e == cudaSuccess && dw) {
@@ -598,7 +675,7 @@ template <typename T> static cudaError_t grouped_backward(const GroupedCall& k, 
         a.n = (unsigned)k.width;
         a.c = dw;
         e = map_of_blocks(&a.a, a.whole_a, k.dtype, dz, 0, k.rows, k.out, d_stride, kTileM / 64);
-        if (e == cudaSuccess) e = map_of_blocks(&a.b, a.whole_b, k.dtype, x, 0, k.rows, k.width, l.stride, l.weight.tile_columns / 64);
+        if (e == cudaSuccess) e = map_of_blocks(&a.b, a.whole_b, k.dtype, x, 0, k.rows, k.width, l.stride, l.weight.held_columns() / 64);
         if (e == cudaSuccess) e = run_grouped<T, EXPERTS_WEIGHT>(k.device, l.weight, a, k.stream);
     }
     return e;

@@ -142,30 +142,40 @@ DCCL_BOTH void grouped_mark(int form, const Grouped& a, const GroupedResults& to
     }
 }
 
-/** Rows and columns of tiles, and the parts of k. */
-struct GroupedPlan { unsigned tile_rows, tile_columns, splits; };
+/** Rows and columns of tiles, and the parts of k. More rows than a CTA's are those of two, which hold half of what makes the columns each. */
+struct GroupedPlan {
+    unsigned tile_rows, tile_columns, splits;
+    unsigned held_rows() const { return tile_rows < kTileM ? tile_rows : kTileM; }
+    unsigned held_columns() const { return tile_rows > kTileM ? tile_columns / 2 : tile_columns; }
+};
 
 /**
- * As if the experts had equal shares of the rows, which the host does not know. What a plan takes, in nanoseconds, is what one CTA takes for its tiles: a block of k takes
- * 280 for a tile of 128 x 128 and 420 for one of 128 x 256 (275 and 450 measured, with every SM at work), and a tile about one microsecond more; parts are stored in fp32, and added up by
- * another launch.
+ * As if the experts had equal shares of the rows, which the host does not know, or, where that makes more tiles, shares about equal that fill half of their last one. What a
+ * plan takes, in nanoseconds, is what one CTA takes for its tiles, or two that share some of 256 x 256: a block of k takes 360 for one of these, 420 for one of 128 x 256 and
+ * 280 for 128 x 128 (with every SM at work 396 under the power cap, 450 and 275 measured), and a tile about one microsecond more; parts are stored in fp32, and added up by
+ * another launch. 16384 rows of 8 experts, 2048 x 5632, by pairs and by single CTAs:
+ * h 249 us and 288, dx 247 and 273, dW 278 and 289; 5 experts of 140 rows, where pairs have half of their rows to spare, 20.1 and 19.8.
  * Up to 32 rows of an expert, forward: tiles of 32 x 64. Then reading the weights is all there is to do, and the tile's own rows should not be most of what it loads.
  */
 inline GroupedPlan plan_grouped(int form, int sms, size_t rows, size_t experts, size_t m, size_t n, size_t k) {
     const size_t busy = experts < rows ? experts : rows, each = busy ? (rows + busy - 1) / busy : 0;
     if (form == EXPERTS_FORWARD && each <= 32) return {32, 64, 1};
-    const size_t high = form == EXPERTS_WEIGHT ? experts * blocks_of(m, kTileM) : busy * blocks_of(each, kTileM), blocks = blocks_of(form == EXPERTS_WEIGHT ? each : k, kTileK);
+    const size_t blocks = blocks_of(form == EXPERTS_WEIGHT ? each : k, kTileK);
     const size_t results = form == EXPERTS_WEIGHT ? experts * m : rows;
     GroupedPlan best = {kTileM, 256, 1};
     double least = 0;
-    for (unsigned columns = 256; columns >= 128; columns /= 2)
-        for (unsigned splits = 1; splits <= 16 && (splits == 1 || splits * 4 <= blocks); splits++) {
-            const size_t tiles = high * blocks_of(n, columns) * splits, rounds = (tiles + sms - 1) / sms;
+    const struct { unsigned rows, columns, block, tile; } shapes[] = {{2 * kTileM, 256, 360, 1500}, {kTileM, 256, 420, 1000}, {kTileM, 128, 280, 1000}};
+    for (const auto& s : shapes) {
+        const size_t shares = (rows + busy * s.rows / 2) / s.rows, workers = s.rows > kTileM ? sms / 2 : sms;
+        const size_t equal = busy * blocks_of(each, s.rows), high = form == EXPERTS_WEIGHT ? experts * blocks_of(m, s.rows) : busy < 2 || equal > shares ? equal : shares;
+        for (unsigned splits = 1; workers && splits <= 16 && (splits == 1 || splits * 4 <= blocks); splits++) {
+            const size_t tiles = high * blocks_of(n, s.columns) * splits, rounds = (tiles + workers - 1) / workers;
             if (splits > 1 && rounds > 4) break;
-            double cost = (double)rounds * ((double)((blocks + splits - 1) / splits) * (columns == 256 ? 420 : 280) + 1000);
+            double cost = (double)rounds * ((double)((blocks + splits - 1) / splits) * s.block + s.tile);
             if (splits > 1) cost += 3000 + (double)results * n * 8 * splits / 5000;
-            if (!least || cost < least) { least = cost; best = {kTileM, columns, splits}; }
+            if (!least || cost < least) { least = cost; best = {s.rows, s.columns, splits}; }
         }
+    }
     return best;
 }
 

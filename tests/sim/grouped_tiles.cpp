@@ -104,14 +104,14 @@ int main(int argc, char** argv) {
         for (unsigned e = 0; e <= experts; e++) starts[e] = e == 0 ? 0 : e == experts ? (int)used : (int)(used ? rand() % (used + 1) : 0);
         for (unsigned i = 1; i < experts; i++)      // in order
             for (unsigned j = i; j > 1 && starts[j] < starts[j - 1]; j--) { const int v = starts[j]; starts[j] = starts[j - 1]; starts[j - 1] = v; }
-        const unsigned m = 1 + rand() % 300, n = 1 + rand() % 40, columns = 16, splits = round % 4 ? 1 : 1 + rand() % 4, tall = round % 7 == 3 ? 32 : 128;
+        const unsigned m = 1 + rand() % 300, n = 1 + rand() % 40, columns = 16, splits = round % 4 ? 1 : 1 + rand() % 4, tall = round % 7 == 3 ? 32 : round % 5 == 2 ? 256 : 128, high = tall < 128 ? 128 : tall;
         wrong |= check(EXPERTS_FORWARD, rows, experts, 0, n, tall, columns, splits, starts, true);
-        wrong |= check(EXPERTS_INPUT, rows, experts, 0, n, 128, columns, splits, starts, true);
-        wrong |= check(EXPERTS_WEIGHT, rows, experts < 9 ? experts : 8, m, n, 128, columns, splits, starts, true);
+        wrong |= check(EXPERTS_INPUT, rows, experts, 0, n, high, columns, splits, starts, true);
+        wrong |= check(EXPERTS_WEIGHT, rows, experts < 9 ? experts : 8, m, n, high, columns, splits, starts, true);
         for (int& s : starts) s = rand() % 5 ? s : (rand() % 2 ? -rand() : rand());       // numbers of nothing
         if (experts < 20) {
             wrong |= check(EXPERTS_FORWARD, rows, experts, 0, n, tall, columns, splits, starts, false);
-            wrong |= check(EXPERTS_WEIGHT, rows, experts < 9 ? experts : 8, m, n, 128, columns, splits, starts, false);
+            wrong |= check(EXPERTS_WEIGHT, rows, experts < 9 ? experts : 8, m, n, high, columns, splits, starts, false);
         }
     }
     if (!wrong) printf("OK\n");
