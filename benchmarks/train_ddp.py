@@ -10,7 +10,8 @@ Shape of the benchmark configuration: 22 layers, hidden 2048, 32 heads, 4 KV hea
 vocabulary 32000 (1.1 B parameters), random init, synthetic tokens uniform over the vocabulary,
 sequence 2048, micro-batch 8 per GPU. Every step copies its tokens from pinned host memory, runs
 forward, backward (with the gradient all-reduce overlapped), the optimizer step, and reads the loss
-back to the host. Reports tokens/s over all GPUs (CUDA-event time, max over ranks) and the exposed
+back to the host. With --clip the gradients are cut back to a norm before the optimizer's step.
+Reports tokens/s over all GPUs (CUDA-event time, max over ranks) and the exposed
 communication time = step time minus the time of the same step with the all-reduce switched off.
 
 --backend dccl      GradientAllReducer: symmetric-memory buckets, zero-copy switch reduction

@@ -152,10 +152,10 @@ struct GroupedPlan {
 /**
  * As if the experts had equal shares of the rows, which the host does not know, or, where that makes more tiles, shares about equal that fill half of their last one. What a
  * plan takes, in nanoseconds, is what one CTA takes for its tiles, or two that share some of 256 x 256: a block of k takes 390 for one of these, 450 for one of 128 x 256 and
- * 280 for 128 x 128 (with every SM at work 396, 450 and 275 measured), a tile about one microsecond more, and the start of pairs four; parts are stored in fp32,
- * and added up by another launch (products that need it are small for pairs). 16384 rows of 8 experts, 2048 x 5632, by pairs and by single CTAs:
- * h 249 us and 288, dx 247 and 273, dW 278 and 289; 5 experts of some 140 rows, 1001 x 2731 fp16, which have half of a pair's rows, 24
- * and 20.
+ * 280 for 128 x 128 (with every SM at work 396, 450 and 275 measured), a tile about one microsecond more, but what its results take to be stored at least (4.2 and 3.7
+ * measured at four blocks), and the start of pairs four more; parts are stored in fp32, and added up by another launch (products that need it are small for pairs).
+ * 16384 rows of 8 experts, 2048 x 5632, by pairs and by single CTAs: h 249 us and 288, dx 247 and 273, dW 278 and 289; of 64 experts, 2048 x 768, h with GELU 71 and 78,
+ * dW 93 and 77; 5 experts of some 140 rows, 1001 x 2731 fp16, which have half of a pair's rows, h 24 and 20.
  * Up to 32 rows of an expert, forward: tiles of 32 x 64. Then reading the weights is all there is to do, and the tile's own rows should not be most of what it loads.
  */
 inline GroupedPlan plan_grouped(int form, int sms, size_t rows, size_t experts, size_t m, size_t n, size_t k) {
@@ -165,14 +165,15 @@ inline GroupedPlan plan_grouped(int form, int sms, size_t rows, size_t experts, 
     const size_t results = form == EXPERTS_WEIGHT ? experts * m : rows;
     GroupedPlan best = {kTileM, 256, 1};
     double least = 0;
-    const struct { unsigned rows, columns, block, once; } shapes[] = {{2 * kTileM, 256, 390, 4000}, {kTileM, 256, 450, 0}, {kTileM, 128, 280, 0}};
+    const struct { unsigned rows, columns, block, least, once; } shapes[] = {{2 * kTileM, 256, 390, 4200, 4000}, {kTileM, 256, 450, 3700, 0}, {kTileM, 128, 280, 1900, 0}};
     for (const auto& s : shapes) {
         const size_t shares = (rows + busy * s.rows / 2) / s.rows, workers = s.rows > kTileM ? sms / 2 : sms;
         const size_t equal = busy * blocks_of(each, s.rows), high = form == EXPERTS_WEIGHT ? experts * blocks_of(m, s.rows) : busy < 2 || equal > shares ? equal : shares;
         for (unsigned splits = 1; workers && splits <= 16 && (splits == 1 || (s.rows == kTileM && splits * 4 <= blocks)); splits++) {
             const size_t tiles = high * blocks_of(n, s.columns) * splits, rounds = (tiles + workers - 1) / workers;
             if (splits > 1 && rounds > 4) break;
-            double cost = (double)rounds * ((double)((blocks + splits - 1) / splits) * s.block + 1000) + s.once;
+            const size_t tile = (blocks + splits - 1) / splits * s.block + 1000;
+            double cost = (double)rounds * (tile < s.least ? s.least : tile) + s.once;
             if (splits > 1) cost += 3000 + (double)results * n * 8 * splits / 5000;
             if (!least || cost < least) { least = cost; best = {s.rows, s.columns, splits}; }
         }
