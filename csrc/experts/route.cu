@@ -340,7 +340,7 @@ __device__ __forceinline__ float share_of(const DcclRouting& how, bool there, fl
 }
 
 /**
- * Bytes are few (16384 tokens of 256 fp32 logits: 17 MB, 2.6 us); the instructions of the choice take the time. Groups of whole registers are judged all at once,
+ * Bytes are few (16384 tokens of 256 fp32 logits: 17 MB, 2.6 us); the instructions of the choice take the time. Groups of whole registers get their scores all at once,
  * and each of the k + 1 rounds is one reduction of the lists' heads. 16384 tokens of 256 fp32 logits, sigmoid with a bias, the best 4 of 8 groups by their two best, 8 experts: 30.6 us, and
  * 6.8 for the gradient; with a warp that had its next token's logits in flight, and so fewer warps of an SM, 34. 16 tokens take 2.6 us, of which the launch is most.
  */

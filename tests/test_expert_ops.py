@@ -44,11 +44,14 @@ def test_early_launched_kernels_promise_nothing_about_their_inputs():
             for part in text.split("__global__")[1:]:
                 signature, body = part.split("{", 1)
                 kernel = signature[:signature.rindex("(")].split("k_")[-1].split("(")[0]
-                assert "wait_for_stream()" in body.split("\n}", 1)[0] or "plan<" in body.split("\n", 1)[0], kernel
+                body = body.split("\n}", 1)[0]
+                assert "wait_for_stream()" in body or "plan<" in body.split("\n", 1)[0] or body.strip().startswith("grouped<"), kernel
                 found.add(kernel)
-    assert found >= {"route", "route_grad", "plan", "plan_cluster", "dispatch", "combine", "combine_grad", "grouped", "join_parts", "pad_rows", "act_grad", "grad_squares", "grad_total", "grad_clip"}
+    assert found >= {"route", "route_grad", "plan", "plan_cluster", "dispatch", "combine", "combine_grad", "grouped", "grouped_pair", "join_parts", "pad_rows", "act_grad", "grad_squares", "grad_total", "grad_clip"}
     plan = open(os.path.join(ROOT, "csrc", "experts", "exchange.cu")).read().split("void plan(")[1]
     assert plan.index("wait_for_stream()") < plan.index("plan_expert(a")
+    grouped = open(os.path.join(ROOT, "csrc", "experts", "grouped.cu")).read().split("void grouped(")[1].split("\n}", 1)[0]
+    assert grouped.index("wait_for_stream()") < grouped.index("list_tiles(") < grouped.index("grouped_place(") < grouped.index(" load(")
 
 
 def test_limits_are_those_of_the_entry_points():
@@ -660,6 +663,46 @@ MANY = [([2000, 1300, 0, 1011], 776, 1544), ([700] * 8, 520, 1032), ([3000], 128
 @pytest.mark.parametrize("counts,width,out", MANY, ids=str)
 def test_expert_linear_of_many_tiles(counts, width, out):
     linear_run(counts, width, out, torch.bfloat16, "silu", behind=130)
+
+
+@gpu
+@pytest.mark.parametrize("counts,width,out", [([130, 1, 269], 4350, 3327), ([131, 269, 0], 3328, 4352), ([4330], 512, 4864)], ids=str)
+def test_pairs_in_graphs_and_on_two_streams(counts, width, out):
+    """Products of pairs of CTAs (forward, for the rows' gradient, for the weights'), captured and replayed on new values, and two at once: the bits of calls alone."""
+    n, experts = sum(counts), len(counts)
+    starts = torch.tensor([sum(counts[:e]) for e in range(experts + 1)], dtype=torch.int32, device="cuda")
+
+    def inputs(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        return [torch.randn(*size, generator=g, device="cuda").mul(scale).bfloat16() for size, scale in (((n, width), 1.0), ((experts, out, width), width ** -0.5), ((n, out), 1.0))]
+
+    def step(x, w, dh):
+        x, w = (t.detach().requires_grad_(True) for t in (x, w))
+        h = ops.expert_linear(x, w, starts, activation="gelu")
+        return (h.detach(), *torch.autograd.grad(h, (x, w), dh))
+
+    states = [inputs(seed) for seed in range(3)]
+    want = [step(*s) for s in states]
+    torch.cuda.synchronize()
+    still, stream = [t.clone() for t in states[0]], torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        got = step(*still)
+    for s, wanted in zip(states, want):
+        for t, v in zip(still, s):
+            t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, wanted))
+    streams, both = [stream, torch.cuda.Stream()], [None, None]
+    for _ in range(3):
+        for i, side in enumerate(streams):
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                both[i] = step(*states[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(2) for a, b in zip(both[i], want[i]))
 
 
 @gpu
