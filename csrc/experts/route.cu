@@ -110,7 +110,8 @@ template <int PER> __device__ __forceinline__ void sort_keys(unsigned (&key)[PER
 
 /**
  * The choice by scores c[i] of the experts lane + 32 i (minus infinity: none): lane j < k gets the j-th expert, or -1. False where two that decide lie so close
- * that their order is not known: within `unsure`, or within `part` of their sizes, and are not the same numbers; two groups within twice that.
+ * that their order is not known: within `unsure`, or within `part` of their sizes, and are not the same numbers; two groups within twice that. Those that decide are each of
+ * the chosen and the one behind it, and, where the last one and the first that is not chosen are the same numbers, the last one and all that are left.
  *
  * The lowest bits of a score's key give way to the number of its register, lower ones first, so that a key says all: of equal ones the lowest i, and of those the
  * first lane, is the lowest expert. What those bits told is in `part`.
@@ -186,6 +187,7 @@ template <typename T, int PER> __device__ __forceinline__ bool choose(const Rout
                 if (lane + 32 * i < (int)a.experts && !(kept >> a.group.quotient(lane + 32 * i) & 1)) c[i] = -INFINITY;
         }
     }
+    const auto expert_of = [](unsigned key, int lane) { return lane + 32 * (PER - 1 - (int)(key & (PER - 1))); };
     unsigned key[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) key[i] = (ordered(c[i]) & ~(unsigned)(PER - 1)) | (PER - 1 - i);
@@ -215,18 +217,27 @@ template <typename T, int PER> __device__ __forceinline__ bool choose(const Rout
     }
     // lane j against lane j + 1; the last of 32 against what came after it
     const bool there = mine_key > kNothing;
-    mine = there ? mine_lane + 32 * (PER - 1 - (int)(mine_key & (PER - 1))) : -1;
+    mine = there ? expert_of(mine_key, mine_lane) : -1;
     unsigned next_key = __shfl_down_sync(kAll, mine_key, 1);
     int next = __shfl_down_sync(kAll, mine, 1);
     if (lane == 31) {
         next_key = beyond;
-        next = beyond_lane + 32 * (PER - 1 - (int)(beyond & (PER - 1)));
+        next = expert_of(beyond, beyond_lane);
     }
-    if (there && lane < a.how.k && next_key > kNothing) {
-        const float v = from_ordered(mine_key), w = from_ordered(next_key);
-        if (!(v - w > unsure + part * fmaxf(fabsf(v), fabsf(w)))
-            && !(logit<T>(a, token, mine) == logit<T>(a, token, next) && (!a.bias || a.bias[mine] == a.bias[next])))
-            sure = false;
+    const auto apart = [&](float v, float w) { return v - w > unsure + part * fmaxf(fabsf(v), fabsf(w)); };
+    const auto same = [&](int e, int f) { return logit<T>(a, token, e) == logit<T>(a, token, f) && (!a.bias || a.bias[e] == a.bias[f]); };
+    bool tied = false;
+    if (there && lane < a.how.k && next_key > kNothing && !apart(from_ordered(mine_key), from_ordered(next_key))) {
+        tied = same(mine, next);
+        sure &= tied;
+    }
+    // a tie of the last one is not settled by the first that is not chosen: any of the rest may be above both, where fp32 cannot tell it from them
+    if (__shfl_sync(kAll, tied, a.how.k - 1)) {
+        const float v = from_ordered(__shfl_sync(kAll, mine_key, a.how.k - 1));
+        const int e = __shfl_sync(kAll, mine, a.how.k - 1);
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (key[i] > kNothing && !apart(v, from_ordered(key[i])) && !same(e, expert_of(key[i], lane))) sure = false;
     }
     sure = __all_sync(kAll, sure);
     if (lane >= a.how.k) mine = -1;

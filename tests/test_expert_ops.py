@@ -204,6 +204,64 @@ def test_route_decides_beyond_fp32():
             assert torch.equal(experts.cpu().long(), want), (scores, kw)
 
 
+def choice_check(z, k, scores, bias, **kw):
+    _, experts = ops.route(z, k, scores, bias, **kw)
+    _, want = route_reference(z.cpu(), k, scores, None if bias is None else bias.cpu(), kw.get("groups", 1), kw.get("top_groups", 1), kw.get("group_score", "max"), True, 1.0)
+    wrong = (experts.cpu().long() != want).any(-1).nonzero().squeeze(-1)
+    assert not len(wrong), (len(wrong), wrong[0].item(), experts[wrong[0]].tolist(), want[wrong[0]].tolist())
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("experts", [33, 40, 64, 96, 128, 200, 256, 512, 1000, 1024])
+def test_route_at_a_border_of_equal_scores(device, experts):
+    """The last chosen and the first that is not are the same numbers, and one further back is a step above or below them, or so close that fp32 cannot tell."""
+    def case(low, high, above=()):
+        """Pairs of `low` and one of `high` at many places, the largest distance apart among them; before them experts that are above both."""
+        rows = []
+        for a, b, c in ((0, 1, 32), (0, 32, experts - 1), (1, experts - 2, experts - 1), (31, 32, 2), (experts - 3, experts - 1, 0), (5, 30, 32), (0, 2, 3)):
+            if len({a, b, c}) < 3:
+                continue
+            row = torch.zeros(experts)
+            row[[a, b]], row[c] = low, high
+            for v in above:
+                row[[e for e in range(7, experts) if row[e] == 0][0]] = v
+            rows.append(row)
+        return torch.stack(rows).to(device)
+
+    step = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0)).item()
+    same = torch.full((experts,), 0.25, device=device)
+    for above in ((), (2.0,), (2.0, 3.0, 2.0)):
+        for more in (0, 1):
+            k = len(above) + 1 + more
+            for low, high in ((1.0, step), (step, 1.0), (-1.0, -step), (1.0, 1.0)):
+                choice_check(case(low, high, above), k, "softmax", None)
+                choice_check(case(low, high, above), k, "sigmoid", None)
+            for low, high in ((20.0, 30.0), (30.0, 20.0), (18.0, 18.125), (25.0, 25.0)):
+                for bias in (torch.zeros(experts, device=device), same):
+                    choice_check(case(low, high, [v + 29 for v in above]), k, "sigmoid", bias)
+            for low, high in ((-40.0, -30.0), (-30.0, -30.5), (-20.0, -20.0)):          # beside a softmax's first, which has all but nothing left
+                z = case(low, high) - 50.0 * (case(low, high) == 0)
+                z[:, 6] = 1.0
+                choice_check(z, 1 + k, "softmax", torch.zeros(experts, device=device))
+    if experts % 8 == 0:
+        for kw in ({"groups": 4, "top_groups": 2}, {"groups": 8, "top_groups": 8}, {"groups": 4, "top_groups": 3, "group_score": "top2"}):
+            for low, high in ((20.0, 30.0), (30.0, 20.0), (20.0, 20.0)):
+                choice_check(case(low, high), 1, "sigmoid", torch.zeros(experts, device=device), **kw)
+                choice_check(case(low, high), 2, "sigmoid", None, **kw)
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("experts,k", [(64, 1), (64, 6), (96, 2), (128, 1), (256, 8), (512, 3), (1024, 32)])
+def test_route_of_scores_that_saturate(device, experts, k):
+    """bf16 logits of a wide spread, many of them equal, and many sigmoids within a step of 1."""
+    z = logits_of(700, experts, torch.bfloat16, device, std=8.0).clamp(-30, 30)
+    for bias in (torch.zeros(experts, device=device), torch.full((experts,), 0.5, device=device), (torch.arange(experts, device=device) % 3).float() / 4):
+        choice_check(z, k, "sigmoid", bias)
+        choice_check(z, k, "softmax", bias)
+    choice_check(z, k, "sigmoid", None)
+    choice_check(z, k, "sigmoid", torch.zeros(experts, device=device), groups=8, top_groups=max(2, -(-8 * k // experts)), group_score="top2")
+
+
 @pytest.mark.parametrize("device", EACH)
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
