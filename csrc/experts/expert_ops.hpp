@@ -49,7 +49,7 @@ long long dccl_expert_linear_workspace(int device, size_t rows, int experts, siz
 int dccl_expert_linear_pads(size_t width, int aligned);
 
 /**
- * h[r] = act(x[r] W[e]^T) for the rows r from starts[e] to starts[e + 1], and zeros in the rows from starts[experts] on: x [rows][width], W [experts][out][width],
+ * h[r] = act(x[r] W[e]^T) for the rows r from starts[e] to starts[e + 1], and zeros in the rows before starts[0] and from starts[experts] on: x [rows][width], W [experts][out][width],
  * h [rows][out], all dense and of dtype float16 or bfloat16; act: DCCL_ACT_* or -1 for none. Where z is not null it receives the products in fp32, in rows of
  * z_stride elements (a multiple of four). A product that does not end in time leaves NaN, and no later call on its device starts one.
  */

@@ -544,8 +544,8 @@ template <typename T, int FORM> static cudaError_t run_grouped(int device, const
     a.group = By(16 * a.tiles_n.d);
     a.expert = By(FORM == EXPERTS_WEIGHT ? a.tiles_m * a.tiles_n.d : 1);
     a.splits = By(p.splits);
-    // every expert may have a row of tiles that is not full, and the rows of nobody another
-    const unsigned long long most = (FORM == EXPERTS_WEIGHT ? (unsigned long long)a.experts * a.tiles_m : blocks_of(a.rows, p.tile_rows) + a.experts + 1ull) * a.tiles_n.d * p.splits;
+    // every expert may have a row of tiles that is not full, and the rows of nobody one at each end
+    const unsigned long long most = (FORM == EXPERTS_WEIGHT ? (unsigned long long)a.experts * a.tiles_m : blocks_of(a.rows, p.tile_rows) + a.experts + 2ull) * a.tiles_n.d * p.splits;
     if (most > 1u << 30 || 16ull * a.tiles_n.d * (a.tiles_m ? a.tiles_m : 1) > 1u << 30) return cudaErrorInvalidValue;      // places are counted in 31 bits
     a.most = (unsigned)most;
     a.partial_stride = up_to(a.n, 4);

@@ -40,7 +40,8 @@ struct GroupedResults { void* c; float* z; size_t z_stride; float* partial; size
 /** The list has room for this many entries and the end: shared memory beside the tiles has no more. */
 constexpr unsigned kListed = 120;
 
-/** Rows of an expert, whatever the numbers are: inside of [0, rows), and none where the next starts before. The last is of nobody, and goes to the end. */
+/** Rows of an expert, whatever the numbers are: inside of [0, rows), and none where the next starts before. The last is of nobody, and goes to the end. (The rows before the
+ *  first start are nobody's either; their tiles come behind those of the last.) */
 struct Span { unsigned from, count; };
 DCCL_BOTH unsigned row_within(int v, unsigned rows) { return v < 0 ? 0 : (unsigned)v < rows ? (unsigned)v : rows; }
 DCCL_BOTH Span span_of(const int* starts, unsigned e, unsigned experts, unsigned rows) {
@@ -48,7 +49,11 @@ DCCL_BOTH Span span_of(const int* starts, unsigned e, unsigned experts, unsigned
     return {from, to > from ? to - from : 0};
 }
 
-DCCL_BOTH unsigned tall_of(const int* starts, unsigned e, const Grouped& a) { return (span_of(starts, e, a.experts, a.rows).count + a.tile_rows - 1) / a.tile_rows; }
+/** Rows of tiles. */
+DCCL_BOTH unsigned tall_of(unsigned rows, const Grouped& a) { return (rows + a.tile_rows - 1) / a.tile_rows; }
+DCCL_BOTH unsigned tall_of(const int* starts, unsigned e, const Grouped& a) {
+    return tall_of(span_of(starts, e, a.experts, a.rows).count, a) + (e == a.experts ? tall_of(row_within(starts[0], a.rows), a) : 0);
+}
 
 /** Entries of the list: the experts and the rows of nobody, `stride` each. */
 DCCL_BOTH unsigned listed_of(const Grouped& a) { return (a.experts + a.stride) / a.stride; }
@@ -86,9 +91,14 @@ DCCL_BOTH GroupedPlace grouped_place(int form, unsigned tile, const Grouped& a, 
     }
     const unsigned group = a.group.quotient(within), top = group * 16, tall = tiles_m - top < 16 ? tiles_m - top : 16;
     within -= group * a.group.d;
-    const unsigned n = tall == 16 ? within / 16 : within / tall, m = top + within - n * tall;
+    const unsigned n = tall == 16 ? within / 16 : within / tall;
+    unsigned m = top + within - n * tall;
     p.column = n * a.tile_columns;
-    const Span s = span_of(starts, p.expert, a.experts, a.rows);
+    Span s = span_of(starts, p.expert, a.experts, a.rows);
+    if (form != EXPERTS_WEIGHT && p.expert == a.experts && m >= tall_of(s.count, a)) {
+        m -= tall_of(s.count, a);
+        s = {0, row_within(starts[0], a.rows)};
+    }
     unsigned count, blocks;
     if (form == EXPERTS_WEIGHT) {
         p.row = m * a.tile_rows;

@@ -302,8 +302,9 @@ def combine(rows, plan, weights=None):
 def expert_linear(rows, weight, plan, activation=None):
     """``act(x @ weight[e].T)`` for the rows x of every expert e: [n, out] of rows [n, width] in the order of the experts and weight [experts, out, width] of one type.
     `plan` is an ``ExpertPlan``, or the int32 tensor [experts + 1] that says where the experts' rows start; `activation` is None, "silu", "gelu" or
-    "gelu_tanh". Products stay in fp32 up to the one rounding of the result. Rows that nobody has, behind the last expert's, are not read; their results and
-    gradients are zeros. Starts are taken as if they lay within [0, n], and an expert whose end lies before its start has no rows.
+    "gelu_tanh". Products stay in fp32 up to the one rounding of the result. Rows that nobody has, before the first expert's and behind the last one's, are not
+    read; their results and gradients are zeros: ``expert_linear(rows, weight[2:5], plan.starts[2:6])`` multiplies the rows of three experts. Starts are taken as if they lay
+    within [0, n], and an expert whose end lies before its start has no rows.
 
     On the GPU rows and weights are float16 or bfloat16. With an activation the gradient of the product is rounded to that type once, to be multiplied
     again, and the call keeps the product in fp32 for it (4 bytes per element of the result), as ``gated_linear`` does. A product that does not end in time (nine

@@ -76,6 +76,14 @@ def test_tiles_cover_every_expert(tiles_program):
     assert res.returncode == 0 and res.stdout == "OK\n", res.stdout
 
 
+def test_every_row_is_stored_once(tmp_path):
+    """tests/sim/expert_rows.cpp: rows before the first start, and behind the last, as well as those of the experts."""
+    exe = str(tmp_path / "expert_rows")
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", "-Werror", os.path.join(ROOT, "tests", "sim", "expert_rows.cpp"), "-o", exe], check=True)
+    res = subprocess.run([exe], capture_output=True, text=True)
+    assert res.returncode == 0 and res.stdout == "OK\n", res.stdout
+
+
 def test_kernels_that_give_up_mark_their_results():
     text = open(os.path.join(ROOT, "csrc", "experts", "grouped.cu")).read()
     parts = text.split("if (failed) {")[1:]
@@ -795,6 +803,56 @@ def test_expert_linear_of_starts_that_are_none():
     assert torch.equal(h, want)
     h = ops.expert_linear(x, w, torch.tensor([0, 50, 20, 120], dtype=torch.int32, device="cuda"))
     assert torch.equal(h[:20], ops.expert_linear(x, w, torch.tensor([0, 50, 50, 50], dtype=torch.int32, device="cuda"))[:20])
+
+
+def soil(*like):
+    """NaN in the memory that the next tensors of these sizes will get."""
+    held = [torch.full_like(t, math.nan) for t in like for _ in range(4)]
+    if any(t.is_cuda for t in like):
+        torch.cuda.synchronize()
+    del held
+
+
+# Rows before the first start, experts and their rows, width, out: of every kind of tile, of sums in parts, and of more experts than the list of tiles holds one by one.
+SOME = [(3, [5, 0, 17], 64, 72), (40, [1], 8, 8), (1, [129, 127, 1], 72, 136), (300, [63, 64, 65], 333, 191), (513, [700] * 3, 520, 1032), (200, [131, 269, 0], 3328, 4352), (128, [128], 2048, 128),
+        (77, [70, 0, 50], 99, 2050), (900, [1500], 130, 121), (9, [2] * 300, 40, 24), (130, [100] * 140, 136, 250), (50, [0, 0], 24, 40), (7, [0] * 200, 16, 8)]
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("before,counts,width,out", SOME, ids=lambda v: str(v) if isinstance(v, int) else "%dof%d" % (sum(v), len(v)))
+def test_expert_linear_of_some_of_the_experts(device, before, counts, width, out):
+    """The weights of some experts and where their rows start: rows before the first start are nobody's, as those behind the last end are."""
+    if device == "cpu" and width * out > 1 << 18:
+        pytest.skip("sizes of the kernels")
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16 if before % 2 else torch.float16
+    x, w, dh, starts = linear_case([before] + counts, width, out, dtype, device, behind=len(counts) % 3 * 35)
+    w, starts = w[1:].contiguous().requires_grad_(True), starts[1:]
+    x.requires_grad_(True)
+    for act in ("gelu", None):
+        soil(dh)
+        with torch.no_grad():
+            h = ops.expert_linear(x, w, starts, activation=act)
+        soil(dh, x, w)
+        h2 = ops.expert_linear(x, w, starts, activation=act)
+        assert torch.equal(h, h2)
+        soil(dh, x, w)
+        grads = torch.autograd.grad(h2, (x, w), dh)
+        linear_check(x, w, dh, starts, act, h, grads)
+        assert bool((h[:before] == 0).all()) and bool((grads[0][:before] == 0).all())
+
+
+@pytest.mark.parametrize("device", EACH)
+def test_expert_linear_by_a_part_of_a_plan(device):
+    """Slices of weights and of a plan's starts: the rows that the whole product has there, and zeros."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    plan = ops.expert_plan(chosen_case(90, 2, 8, device=device), 8)
+    x, w, dh, _ = linear_case([180] + [0] * 7, 64, 72, dtype, device)
+    whole, starts = ops.expert_linear(x, w, plan, activation="silu"), plan.starts.tolist()
+    for i, j in ((0, 8), (2, 5), (7, 8), (1, 2)):
+        soil(dh)
+        part = ops.expert_linear(x, w[i:j], plan.starts[i:j + 1], activation="silu")
+        assert torch.equal(part[starts[i]:starts[j]], whole[starts[i]:starts[j]])
+        assert bool((part[:starts[i]] == 0).all()) and bool((part[starts[j]:] == 0).all())
 
 
 @gpu
