@@ -51,7 +51,7 @@ int dccl_expert_linear_pads(size_t width, int aligned);
 /**
  * h[r] = act(x[r] W[e]^T) for the rows r from starts[e] to starts[e + 1], and zeros in the rows before starts[0] and from starts[experts] on: x [rows][width], W [experts][out][width],
  * h [rows][out], all dense and of dtype float16 or bfloat16; act: DCCL_ACT_* or -1 for none. Where z is not null it receives the products in fp32, in rows of
- * z_stride elements (a multiple of four). A product that does not end in time leaves NaN, and no later call on its device starts one.
+ * z_stride elements (a multiple of four). Starts are taken inside of [0, rows], and none before those ahead of it. A product that does not end in time leaves NaN, and no later call on its device starts one.
  */
 int dccl_expert_linear(int device, int dtype, size_t rows, int experts, size_t width, size_t out, const void* x, const void* w, const int* starts, int act, void* h, float* z,
                        size_t z_stride, void* workspace, long long workspace_bytes, void* stream);

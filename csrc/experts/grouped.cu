@@ -62,6 +62,7 @@ template <int ACT> __device__ __forceinline__ float slope_of(float z) {
 struct GroupedArgs : Grouped, GroupedResults {
     CUtensorMap a, b;
     const int* starts;
+    int* ordered;                   // room for the starts in order, where the list has not one entry for each
     unsigned descriptor;            // of one product
     int act;
     bool whole_a, whole_b;          // one box holds all blocks of 64 columns of an operand
@@ -83,14 +84,21 @@ template <int M, int N> struct GroupedShape {
     static_assert(kTileM * kTileK * 2 - kBytes <= kStagings * 4096, "what the last stage's product reads");
 };
 
-/** The list of tiles, by one warp: first[i], the rows of tiles before expert i * stride, and all of them. own: the starts, where every expert is listed. */
-__device__ __forceinline__ void list_tiles(const Grouped& a, const int* starts, unsigned* first, int* own) {
+/**
+ * The list of tiles, by one warp: first[i], the rows of tiles before expert i * stride, and all of them. own: the starts, where every expert is listed. False where a start lies before
+ * those ahead of it.
+ */
+__device__ __forceinline__ bool list_tiles(const Grouped& a, const int* starts, unsigned* first, int* own) {
     const unsigned lane = threadIdx.x % 32, entries = listed_of(a);
     unsigned before = 0;
+    bool back = false;
     for (unsigned base = 0; base < entries; base += 32) {
         const unsigned i = base + lane;
         unsigned n = 0;
-        for (unsigned e = i * a.stride; e < (i + 1) * a.stride && e <= a.experts; e++) n += tall_of(starts, e, a);
+        for (unsigned e = i * a.stride; e < (i + 1) * a.stride && e <= a.experts; e++) {
+            n += tall_of(starts, e, a);
+            back |= goes_back(starts, e, a);
+        }
         if (a.stride == 1 && i < entries) own[i] = starts[i];
         const unsigned mine = n;
 #pragma unroll
@@ -102,6 +110,24 @@ __device__ __forceinline__ void list_tiles(const Grouped& a, const int* starts, 
         before += __shfl_sync(0xffffffffu, n, 31);
     }
     if (lane == 0) first[entries] = before;
+    return !__any_sync(0xffffffffu, back);
+}
+
+/** The starts in order, each as far as those ahead of it. By one warp; several CTAs may write the same numbers to the same place. */
+__device__ __noinline__ void order_starts(const Grouped& a, const int* starts, volatile int* ordered) {
+    const unsigned lane = threadIdx.x % 32;
+    unsigned reached = 0;
+    for (unsigned base = 0; base <= a.experts; base += 32) {
+        unsigned reach = base + lane <= a.experts ? max(reached, row_within(starts[base + lane], a.rows)) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, reach, o);
+            if (lane >= (unsigned)o) reach = max(reach, v);
+        }
+        if (base + lane <= a.experts) ordered[base + lane] = (int)reach;
+        reached = __reduce_max_sync(0xffffffffu, reach);
+    }
+    __syncwarp();
 }
 
 /**
@@ -139,7 +165,7 @@ template <typename T, int FORM, int M, int N> __device__ __forceinline__ void gr
     __shared__ unsigned first[kListed + 1];
     __shared__ int own[kListed + 1];
     __shared__ uint32_t tmem_base;
-    __shared__ int failed;
+    __shared__ int failed, in_order;
     char* const tiles = shared + (1024 - shared_addr(shared) % 1024) % 1024;
     char* const staging = tiles + kStages * Shape::kBytes;
     const uint32_t full = shared_addr(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16, drained = sums_empty + 16, landed = drained + 8;
@@ -162,12 +188,19 @@ template <typename T, int FORM, int M, int N> __device__ __forceinline__ void gr
         prefetch_map(&a.b);
     }
     wait_for_stream();
-    if (warp == 1) list_tiles(a, a.starts, first, own);
+    if (warp == 1) {
+        const bool sound = list_tiles(a, a.starts, first, own);
+        in_order = sound;
+        if (!sound) {
+            order_starts(a, a.starts, a.stride == 1 ? own : a.ordered);
+            list_tiles(a, a.stride == 1 ? own : a.ordered, first, own);
+        }
+    }
     tc_before_sync();
     __syncthreads();
     if constexpr (PAIR) cluster_sync();
     tc_after_sync();
-    const int* const starts = a.stride == 1 ? own : a.starts;
+    const int* const starts = a.stride == 1 ? own : in_order ? a.starts : a.ordered;
     const uint32_t sums = tmem_base;
     const unsigned total = grouped_tiles(FORM, a, first);
     unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
@@ -445,15 +478,25 @@ __global__ void __launch_bounds__(kRowCta) k_pad_rows(const __grid_constant__ Pa
 
 struct ActGradArgs { const void* dh; const float* z; void* dz; const int* starts; size_t z_stride, stride; unsigned rows, experts, n, from, threads; Divisor runs; int act; };
 
-/** dz from dh and the saved products, eight elements per thread; rows of nobody, whose products nobody wrote, are left out. Only the rows of dh may start
+/** dz from dh and the saved products, eight elements per thread; rows behind the last expert's, whose products nobody wrote, are left out. Only the rows of dh may start
  *  anywhere (VEC: they do not). HBM bounds it: 8 bytes per element, 16384 x 5632 in 125 us (5.9 TB/s). */
 template <typename T, bool VEC> __global__ void __launch_bounds__(kRowCta) k_act_grad(const __grid_constant__ ActGradArgs a) {
     wait_for_stream();
-    const unsigned index = blockIdx.x * kRowCta + threadIdx.x;
+    __shared__ unsigned reach[kRowCta / 32];
+    const unsigned index = blockIdx.x * kRowCta + threadIdx.x, last = min(blockIdx.x * kRowCta + kRowCta, a.threads) - 1;
+    unsigned used = row_within(a.starts[a.experts], a.rows);
+    if ((size_t)a.from + a.runs.quotient(last) >= used) {       // some of the CTA: a start ahead of the last may lie further
+        unsigned most = 0;
+        for (unsigned e = threadIdx.x; e < a.experts; e += kRowCta) most = max(most, row_within(a.starts[e], a.rows));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (threadIdx.x % 32 == 0) reach[threadIdx.x / 32] = most;
+        __syncthreads();
+        for (unsigned w = 0; w < kRowCta / 32; w++) used = max(used, reach[w]);
+    }
     if (index >= a.threads) return;
     const unsigned line = a.runs.quotient(index), column = (index - line * a.runs.d) * 8;
     const size_t row = (size_t)a.from + line;
-    if (row >= row_within(a.starts[a.experts], a.rows)) return;
+    if (row >= used) return;
     float z[8] = {}, d[8];
 #pragma unroll
     for (int q = 0; q < 2; q++) {
@@ -481,7 +524,7 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(kRowCta) k_act
 /* ------------------------------------------------------------------------------------------------ host side */
 
 /** Where the parts of a call's workspace lie. */
-struct GroupedLayout { size_t stride, x, w, padded, dz, d_stride, partial, total; GroupedPlan forward, input, weight; bool ok; };
+struct GroupedLayout { size_t stride, x, w, padded, dz, d_stride, partial, ordered, total; GroupedPlan forward, input, weight; bool ok; };
 
 static size_t parts_of(const GroupedPlan& p, size_t rows, size_t n) { return p.splits > 1 ? p.splits * rows * up_to(n, 4) * sizeof(float) : 0; }
 
@@ -513,6 +556,7 @@ static GroupedLayout grouped_layout(int device, size_t rows, int experts, size_t
     } else {
         l.partial = take(parts_of(l.forward, rows, out));
     }
+    if (listed_by(experts) > 1) l.ordered = take((experts + 1) * sizeof(int));
     l.total = at;
     return l;
 }
@@ -613,7 +657,8 @@ static GroupedArgs grouped_args(const GroupedCall& k, const GroupedLayout& l) {
     a.experts = (unsigned)k.experts;
     a.starts = k.starts;
     a.act = kNoActivation;
-    a.stride = (a.experts + kListed) / kListed;       // experts and rows of nobody in at most kListed entries
+    a.stride = listed_by(a.experts);
+    if (a.stride > 1) a.ordered = (int*)(k.workspace + l.ordered);
     return a;
 }
 

@@ -40,8 +40,8 @@ struct GroupedResults { void* c; float* z; size_t z_stride; float* partial; size
 /** The list has room for this many entries and the end: shared memory beside the tiles has no more. */
 constexpr unsigned kListed = 120;
 
-/** Rows of an expert, whatever the numbers are: inside of [0, rows), and none where the next starts before. The last is of nobody, and goes to the end. (The rows before the
- *  first start are nobody's either; their tiles come behind those of the last.) */
+/** Rows of an expert by starts in order, whatever the numbers are: inside of [0, rows). The last is of nobody, and goes to the end. (The rows before the first start are
+ *  nobody's either; their tiles come behind those of the last.) */
 struct Span { unsigned from, count; };
 DCCL_BOTH unsigned row_within(int v, unsigned rows) { return v < 0 ? 0 : (unsigned)v < rows ? (unsigned)v : rows; }
 DCCL_BOTH Span span_of(const int* starts, unsigned e, unsigned experts, unsigned rows) {
@@ -49,12 +49,17 @@ DCCL_BOTH Span span_of(const int* starts, unsigned e, unsigned experts, unsigned
     return {from, to > from ? to - from : 0};
 }
 
+/** Whether the start behind this one lies before it. Such starts are put in order first, each as far as those ahead of it: so no row is of two experts. */
+DCCL_BOTH bool goes_back(const int* starts, unsigned e, const Grouped& a) { return e < a.experts && row_within(starts[e + 1], a.rows) < row_within(starts[e], a.rows); }
+
 /** Rows of tiles. */
 DCCL_BOTH unsigned tall_of(unsigned rows, const Grouped& a) { return (rows + a.tile_rows - 1) / a.tile_rows; }
 DCCL_BOTH unsigned tall_of(const int* starts, unsigned e, const Grouped& a) {
     return tall_of(span_of(starts, e, a.experts, a.rows).count, a) + (e == a.experts ? tall_of(row_within(starts[0], a.rows), a) : 0);
 }
 
+/** Experts of one entry, so that they and the rows of nobody have at most kListed. */
+inline unsigned listed_by(unsigned experts) { return (experts + kListed) / kListed; }
 /** Entries of the list: the experts and the rows of nobody, `stride` each. */
 DCCL_BOTH unsigned listed_of(const Grouped& a) { return (a.experts + a.stride) / a.stride; }
 
@@ -107,7 +112,6 @@ DCCL_BOTH GroupedPlace grouped_place(int form, unsigned tile, const Grouped& a, 
         count = s.count;
     } else {
         p.row = s.from + m * a.tile_rows;
-        // (starts that are not in order may give more tiles than can be counted)
         p.rows = m * a.tile_rows >= s.count ? 0 : s.count - m * a.tile_rows < a.tile_rows ? s.count - m * a.tile_rows : a.tile_rows;
         p.k_from = 0;
         count = p.expert < a.experts ? a.k_blocks * kTileK : 0;

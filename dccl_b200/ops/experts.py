@@ -31,6 +31,7 @@ Fake and transformed tensors are refused.
 The original has no such operators: its API ends at the collectives (reference include/dccl/dccl.hpp:143-420).
 """
 import ctypes
+import itertools
 import math
 import operator
 
@@ -304,7 +305,7 @@ def expert_linear(rows, weight, plan, activation=None):
     `plan` is an ``ExpertPlan``, or the int32 tensor [experts + 1] that says where the experts' rows start; `activation` is None, "silu", "gelu" or
     "gelu_tanh". Products stay in fp32 up to the one rounding of the result. Rows that nobody has, before the first expert's and behind the last one's, are not
     read; their results and gradients are zeros: ``expert_linear(rows, weight[2:5], plan.starts[2:6])`` multiplies the rows of three experts. Starts are taken as if they lay
-    within [0, n], and an expert whose end lies before its start has no rows.
+    within [0, n] and none before those ahead of it: no row is of two experts, and one whose end lies before its start has none.
 
     On the GPU rows and weights are float16 or bfloat16. With an activation the gradient of the product is rounded to that type once, to be multiplied
     again, and the call keeps the product in fp32 for it (4 bytes per element of the result), as ``gated_linear`` does. A product that does not end in time (nine
@@ -337,10 +338,9 @@ def expert_linear(rows, weight, plan, activation=None):
         out = _kernel("expert_linear", rows, weight, starts, act)
         return out if out is not NotImplemented else _refuse("expert_linear")
     n = rows.shape[0]
-    out, at = rows.new_zeros(n, out_width), [min(max(s, 0), n) for s in starts.tolist()]
+    out, at = rows.new_zeros(n, out_width), list(itertools.accumulate((min(max(s, 0), n) for s in starts.tolist()), max))
     for e, (start, end) in enumerate(zip(at, at[1:])):
         if end > start or e == 0:       # a product of no rows ties the result to its inputs
-            end = max(start, end)
             v = rows[start:end].float() @ weight[e].float().t()
             out = out.index_copy(0, torch.arange(start, end, device=rows.device), (v if activation is None else _activate_on_cpu(v, activation)).to(rows.dtype))
     return out

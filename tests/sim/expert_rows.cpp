@@ -1,4 +1,4 @@
-// Host run of csrc/experts/grouped_tiles.hpp: for many tables of where experts' rows start, also such as leave rows before the first, every row of the results is stored
+// Host run of csrc/experts/grouped_tiles.hpp: for many tables of where experts' rows start, also such as leave rows before the first, go back or are no rows at all, every row of the results is stored
 // exactly once for each part of k, those of an expert by products with its weights and those of nobody as zeros, and every expert's rows are summed over once.
 #include "../../csrc/experts/grouped_tiles.hpp"
 #include <cstdio>
@@ -7,20 +7,27 @@
 
 using namespace dccl;
 
-struct Table { std::vector<unsigned> first; };
+struct Table { std::vector<unsigned> first; std::vector<int> starts; };
 
-/** What list_tiles leaves in shared memory. */
+/** What list_tiles and order_starts leave. */
 static Table list(const Grouped& a, const std::vector<int>& starts) {
-    Table t;
+    Table t = {{}, starts};
+    bool back = false;
+    for (unsigned e = 0; e <= a.experts; e++) back |= goes_back(starts.data(), e, a);
+    unsigned reached = 0;
+    for (unsigned e = 0; e <= a.experts && back; e++) {
+        const unsigned start = row_within(starts[e], a.rows);
+        reached = start > reached ? start : reached;
+        t.starts[e] = (int)reached;
+    }
     unsigned before = 0;
     for (unsigned i = 0; i < listed_of(a); i++) {
         t.first.push_back(before);
-        for (unsigned e = i * a.stride; e < (i + 1) * a.stride && e <= a.experts; e++) before += tall_of(starts.data(), e, a);
+        for (unsigned e = i * a.stride; e < (i + 1) * a.stride && e <= a.experts; e++) before += tall_of(t.starts.data(), e, a);
     }
     t.first.push_back(before);
     return t;
 }
-static GroupedPlace place(int form, unsigned tile, const Grouped& a, const Table& t, const std::vector<int>& starts) { return grouped_place(form, tile, a, t.first.data(), starts.data()); }
 
 static int fail(const char* what, const Grouped& a, int form) {
     printf("%s: %u rows, %u experts, form %d, tiles of %u\n", what, a.rows, a.experts, form, a.tile_rows);
@@ -41,7 +48,7 @@ static int check(int form, unsigned rows, unsigned experts, unsigned m, unsigned
     a.expert = By(form == EXPERTS_WEIGHT ? a.tiles_m * a.tiles_n.d : 1);
     a.splits = By(splits);
     a.k_blocks = 5;
-    a.stride = (experts + kListed) / kListed;
+    a.stride = listed_by(experts);
     a.most = (form == EXPERTS_WEIGHT ? experts * a.tiles_m : blocks_of(rows, tall) + experts + 2) * a.tiles_n.d * splits;
     const Table t = list(a, starts);
     // whose each row is, from the table's meaning alone
@@ -54,7 +61,7 @@ static int check(int form, unsigned rows, unsigned experts, unsigned m, unsigned
     if (form != EXPERTS_WEIGHT && (unsigned long long)t.first.back() * a.tiles_n.d * splits > a.most) return fail("more tiles than a launch has", a, form);
     std::vector<unsigned> stored(form == EXPERTS_WEIGHT ? (size_t)experts * m * n : (size_t)rows * n, 0), summed(rows, 0);
     for (unsigned i = 0; i < grouped_tiles(form, a, t.first.data()); i++) {
-        const GroupedPlace p = place(form, i, a, t, starts);
+        const GroupedPlace p = grouped_place(form, i, a, t.first.data(), t.starts.data());
         if (p.expert > experts || !p.rows || p.rows > tall || p.column >= n || p.split >= splits) return fail("place", a, form);
         for (unsigned r = 0; r < p.rows; r++) {
             if (form != EXPERTS_WEIGHT && (p.row + r >= rows || owner[p.row + r] != p.expert)) return fail("a row of another", a, form);
@@ -89,6 +96,11 @@ int main() {
             for (unsigned j = i; j > 0 && starts[j] < starts[j - 1]; j--) { const int v = starts[j]; starts[j] = starts[j - 1]; starts[j - 1] = v; }
         if (round % 3 == 1) starts[experts] = rows;
         if (round % 8 == 1) starts[0] = 0;
+        wrong |= check(EXPERTS_FORWARD, rows, experts, 0, n, tall, splits, starts);
+        wrong |= check(EXPERTS_INPUT, rows, experts, 0, n, high, splits, starts);
+        wrong |= check(EXPERTS_WEIGHT, rows, experts, m, n, high, splits, starts);
+        for (int& s : starts) s = rand() % 5 ? s : rand() % 3 ? rand() % (int)(rows + 1) : rand() % 2 ? -rand() : rand();        // some that go back, and numbers of nothing
+        if (round % 2) starts[experts] = rand() % (rows + 1);
         wrong |= check(EXPERTS_FORWARD, rows, experts, 0, n, tall, splits, starts);
         wrong |= check(EXPERTS_INPUT, rows, experts, 0, n, high, splits, starts);
         wrong |= check(EXPERTS_WEIGHT, rows, experts, m, n, high, splits, starts);

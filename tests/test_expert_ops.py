@@ -855,6 +855,46 @@ def test_expert_linear_by_a_part_of_a_plan(device):
         assert bool((part[:starts[i]] == 0).all()) and bool((part[starts[j]:] == 0).all())
 
 
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("starts", [[0, 50, 20, 120], [40, 90, 10, 30], [-5, 70, 130, 60], [120, 0, 0, 0], [2 ** 31 - 1, -2 ** 31, 5, 90], [0, 119, 118, 117]], ids=str)
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_expert_linear_of_starts_that_go_back(device, starts, act):
+    """A start that lies before one ahead of it counts as that one: no row is of two experts, and every row is stored."""
+    x, w, dh, _ = linear_case([40, 40, 40], 64, 72, torch.float32 if device == "cpu" else torch.bfloat16, device)
+    go_back_check(x, w, dh, starts, act)
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("experts,tokens,width,out", [(11, 700, 72, 136), (119, 900, 24, 40), (120, 900, 24, 40), (300, 1500, 40, 24), (1024, 3000, 16, 8), (4, 6000, 520, 1032)])
+def test_expert_linear_of_many_starts_that_go_back(device, experts, tokens, width, out):
+    if device == "cpu" and tokens > 900:
+        pytest.skip("sizes of the kernels")
+    g = torch.Generator().manual_seed(experts)
+    x, w, dh, _ = linear_case([tokens] + [0] * (experts - 1), width, out, torch.float32 if device == "cpu" else torch.float16, device)
+    for table in range(2):
+        starts = torch.randint(0, tokens + 1, (experts + 1,), generator=g).sort().values
+        some = torch.rand(experts + 1, generator=g) < 0.1
+        starts = torch.where(some, torch.randint(-tokens, starts[-1].item() if table else tokens + 1, (experts + 1,), generator=g), starts)
+        go_back_check(x, w, dh, starts.tolist(), "silu")
+
+
+def go_back_check(x, w, dh, starts, act):
+    table, want, reached = torch.tensor(starts, dtype=torch.int32, device=x.device), [], 0
+    for s in starts:
+        reached = max(reached, min(max(s, 0), x.shape[0]))
+        want.append(reached)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w)]
+    runs = []
+    for _ in range(2):
+        soil(dh, x, w)
+        h = ops.expert_linear(*leaves, table, activation=act)
+        soil(dh, x, w)
+        runs.append((h.detach(), *torch.autograd.grad(h, leaves, dh)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    linear_check(x, w, dh, torch.tensor(want), act, runs[0][0], runs[0][1:])
+    assert bool((runs[0][0][:want[0]] == 0).all()) and bool((runs[0][1][:want[0]] == 0).all())
+
+
 @gpu
 def test_expert_linear_of_views():
     x, w, dh, starts = linear_case([20, 0, 13], 128, 96, torch.bfloat16, "cuda")
