@@ -203,7 +203,7 @@ template <typename T, int FORM, int M, int N> __device__ __forceinline__ void gr
     const int* const starts = a.stride == 1 ? own : in_order ? a.starts : a.ordered;
     const uint32_t sums = tmem_base;
     const unsigned total = grouped_tiles(FORM, a, first);
-    unsigned filled = 0;            // stages that the producer filled, or that the multiplier used
+    InFlight loads;                 // of the loader
     if (warp == kGroupedLoader && lane == 0) {
         unsigned s = 0, parity = 1;
         const auto load = [](auto... box) {
@@ -215,11 +215,12 @@ template <typename T, int FORM, int M, int N> __device__ __forceinline__ void gr
             const unsigned row = p.row + rank * Shape::kHeldM, column = p.column + rank * Shape::kHeldN;
             const unsigned blocks = (p.k_count + kTileK - 1) / kTileK;
             unsigned kb = 0;
-            for (; kb < blocks; kb++, filled++) {
+            for (; kb < blocks; kb++) {
                 if (!bar_wait(empty + 8 * s, parity, &failed)) break;
                 const bool tail = PAIR && FORM == EXPERTS_WEIGHT && kb + 1 == blocks && p.k_count % kTileK;          // where each CTA clears rows first
                 const uint32_t to_a = shared_addr(tiles) + s * Shape::kBytes, to_b = to_a + Shape::kBytesA, bar = tail ? in_cta(landed + 8 * s, rank) : PAIR ? in_cta(full + 8 * s, 0) : full + 8 * s;
                 const int k = p.k_from + kb * kTileK;
+                loads.load(s, tail);
                 if (tail) bar_expect(landed + 8 * s, Shape::kBytes);
                 else if (rank == 0) bar_expect(full + 8 * s, (PAIR ? 2 : 1) * Shape::kBytes);         // the leader counts both CTAs' bytes
                 if constexpr (FORM == EXPERTS_FORWARD) {
@@ -274,7 +275,7 @@ template <typename T, int FORM, int M, int N> __device__ __forceinline__ void gr
             tc_after_sync();
             const uint32_t d = sums + buffer * N;
             unsigned kb = 0;
-            for (; kb < blocks; kb++, filled++) {
+            for (; kb < blocks; kb++) {
                 if (!bar_wait_warp(full + 8 * s, parity, &failed)) break;
                 tc_after_sync();
                 char* const at = tiles + s * Shape::kBytes;
@@ -379,7 +380,8 @@ template <typename T, int FORM, int M, int N> __device__ __forceinline__ void gr
         if (warp == kGroupedLoader && lane == 0 && rank != 0)       // its copies count on the leader's barriers: here only time tells that they have landed
             for (const long long start = clock64(); clock64() - start < kLandClocks;) {}
         if (warp == kGroupedLoader && lane == 0 && rank == 0)
-            for (unsigned i = filled > kStages ? filled - kStages : 0; i < filled; i++) bar_wait(full + 8 * (i % kStages), i / kStages & 1, &late);
+            for (unsigned i = loads.oldest(kStages); i < loads.filled; i++)
+                bar_wait((loads.on_landed(i, kStages) ? landed : full) + 8 * (i % kStages), loads.parity(i, kStages), &late);
         if (rank == 0 && warp == kGroupedMultiplier && elect_one()) {        // the lane whose products they are
             if constexpr (PAIR) pair_commit(drained);
             else commit(drained);

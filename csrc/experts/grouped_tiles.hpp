@@ -156,6 +156,23 @@ DCCL_BOTH void grouped_mark(int form, const Grouped& a, const GroupedResults& to
     }
 }
 
+/**
+ * What the loading thread of a CTA has under way, by the stages that its blocks go round: which barrier counts a stage's bytes, and the parity of their phase there. A block whose
+ * rows are cleared before it is used (`tail`, of a pair of CTAs) lands on a barrier of its own, `landed`, and the other one, `full`, is completed by the other CTA's arrival alone.
+ */
+struct InFlight {
+    unsigned filled = 0, tails = 0, turns = 0;      // blocks so far; stages whose last one was a tail, and that have had an odd number of them
+    DCCL_BOTH void load(unsigned stage, bool tail) {
+        filled++;
+        tails = tail ? tails | 1u << stage : tails & ~(1u << stage);
+        turns ^= (unsigned)tail << stage;
+    }
+    /** The blocks that may not have landed: the last ones, one of each stage. */
+    DCCL_BOTH unsigned oldest(unsigned stages) const { return filled > stages ? filled - stages : 0; }
+    DCCL_BOTH bool on_landed(unsigned block, unsigned stages) const { return tails >> block % stages & 1; }
+    DCCL_BOTH unsigned parity(unsigned block, unsigned stages) const { return on_landed(block, stages) ? ~(turns >> block % stages) & 1 : block / stages & 1; }
+};
+
 /** Rows and columns of tiles, and the parts of k. More rows than a CTA's are those of two, which hold half of what makes the columns each. */
 struct GroupedPlan {
     unsigned tile_rows, tile_columns, splits;

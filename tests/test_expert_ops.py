@@ -84,6 +84,14 @@ def test_every_row_is_stored_once(tmp_path):
     assert res.returncode == 0 and res.stdout == "OK\n", res.stdout
 
 
+def test_kernels_that_give_up_wait_for_their_copies(tmp_path):
+    """tests/sim/loads_in_flight.cpp: the barriers and parities of what is under way."""
+    exe = str(tmp_path / "loads_in_flight")
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", "-Werror", os.path.join(ROOT, "tests", "sim", "loads_in_flight.cpp"), "-o", exe], check=True)
+    res = subprocess.run([exe], capture_output=True, text=True)
+    assert res.returncode == 0 and res.stdout == "OK\n", res.stdout
+
+
 def test_kernels_that_give_up_mark_their_results():
     text = open(os.path.join(ROOT, "csrc", "experts", "grouped.cu")).read()
     parts = text.split("if (failed) {")[1:]
