@@ -64,15 +64,29 @@ template <typename T> __device__ __forceinline__ size_t before_boundary(const T*
     return head < n ? head : n;
 }
 
-/** Squares of one access are added in fp32, and those sums in 64 bits. */
+/** Squares of this thread's accesses in 64 bits. A function of its own: it is seldom called, and its registers are not the other's. */
+template <typename T> __device__ __noinline__ double squares_exactly(const T* body, size_t runs) {
+    constexpr int N = 16 / sizeof(T);
+    double sum = 0;
+    for (size_t i = threadIdx.x; i < runs; i += kClipThreads) {
+        const Run<T, N> v = ld_run<T, N>(body + i * N);
+#pragma unroll
+        for (int e = 0; e < N; e++) sum = fma((double)Traits<T>::up(v.e[e]), (double)Traits<T>::up(v.e[e]), sum);
+    }
+    return sum;
+}
+
+/**
+ * Squares of one access are added in fp32, and those sums in 64 bits. A square that overflowed shows in the thread's sum for the piece; what got lost below the normal numbers, 2^-150 of
+ * each square, may count where that sum is small without being of zeros alone, as many gradients are. Then the thread adds all of its squares of the piece again, in 64 bits.
+ * (1.1 billion bf16 gradients take 335 us; where each access was looked at 340, where it was decided there 404, and without any of it 330.) Those of fp16 always fit.
+ */
 template <typename T> __device__ __forceinline__ double squares(const T* p, size_t n) {
     constexpr int N = 16 / sizeof(T);
     const size_t head = before_boundary(p, n), runs = (n - head) / N;
     double sum = 0;
-    if (threadIdx.x < head) {
-        const float v = Traits<T>::up(p[threadIdx.x]);
-        sum += (double)v * v;
-    }
+    constexpr bool kMayNotFit = !std::is_same<T, __half>::value;
+    uint32_t bits = 0;
     const T* body = p + head;
     size_t i = threadIdx.x;
     const auto some = [&](auto count) {         // as many at a time, while all of them are there
@@ -87,12 +101,24 @@ template <typename T> __device__ __forceinline__ double squares(const T* p, size
 #pragma unroll
                 for (int e = 0; e < N; e++) s = fmaf(Traits<T>::up(v[u].e[e]), Traits<T>::up(v[u].e[e]), s);
                 sum += s;
+                if constexpr (kMayNotFit) {
+                    const uint32_t* const w = reinterpret_cast<const uint32_t*>(&v[u]);
+                    bits |= w[0] | w[1] | w[2] | w[3];
+                }
             }
         }
     };
     some(std::integral_constant<int, kClipUnroll>{});
     some(std::integral_constant<int, kClipUnroll / 2>{});
     some(std::integral_constant<int, 1>{});
+    if constexpr (kMayNotFit) {
+        constexpr uint32_t sizes = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;         // without the signs
+        if (!(sum < INFINITY) || (sum < 0x1p-80 && (bits & sizes))) sum = squares_exactly(body, runs);
+    }
+    if (threadIdx.x < head) {
+        const float v = Traits<T>::up(p[threadIdx.x]);
+        sum += (double)v * v;
+    }
     for (size_t j = head + runs * N + threadIdx.x; j < n; j += kClipThreads) {
         const float v = Traits<T>::up(p[j]);
         sum += (double)v * v;

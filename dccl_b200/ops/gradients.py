@@ -4,8 +4,8 @@
 
 CUDA tensors of one device are read by one kernel and scaled by a second one (csrc/gradients/grad_norm.cu), up to 512 tensors each, on the device's current
 stream; nothing is read by the host, and the calls can be captured into a graph. CPU tensors take the same formulas in torch.
-Squares are added in fp32 within one access of 16 bytes and in 64 bits from there on, in an order that depends on sizes, types and addresses only: the same
-tensors give the same bits. A square overflows where an element is larger than 1.8e19, and the norm is then infinite.
+Squares are added in fp32 within one access of 16 bytes, or in 64 bits where fp32 does not hold them, and in 64 bits from there on, in an order that depends on sizes, types and
+addresses only: the same tensors give the same bits. The norm is infinite only where an element is, or where it is itself beyond fp32.
 
 Where gradients are split over ranks, each with its own (the slices of a sharded optimizer, experts that live on one rank), `comm` adds up the squares of all of them.
 

@@ -140,6 +140,29 @@ def test_values_that_are_not_finite(device):
     clip_check(t, math.inf)
 
 
+# What the squares of some eight elements are where fp32 cannot hold them, or only with few bits.
+EXTREMES = [6.0e18, 7.0e18, 9.3e18, 3.0e19, 1.0e25, 1.0e33, 1.0e-17, 1.0e-19, 3.0e-21, 1.0e-22, 1.0e-25, 1.0e-33]
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("size", EXTREMES)
+def test_squares_beyond_fp32(device, dtype, size):
+    """The same norm wherever the tensors start."""
+    for off in range(0, 8 if device == "cuda" else 1):
+        for sizes in ([5], [64, 1], [4099, 70, 8]):
+            tensors = [(t / 10.0 ** (-i % 4) * size).clone() for i, t in enumerate(gradients(sizes, [torch.float32], device))]
+            whole = [torch.zeros(t.numel() + off, device=device, dtype=dtype) for t in tensors]
+            moved = [v[off:].copy_(t) for v, t in zip(whole, tensors)]
+            clip_check(moved, 1.0e-3 if size > 1 else size * 1.0e-8)
+    few = torch.zeros(3000, device=device, dtype=dtype)        # among zeros, and beside one element of another size
+    few[7], few[2008] = size, -size
+    clip_check([few], 1.0e-3 if size > 1 else size * 1.0e-8)
+    few[9] = 1.0
+    clip_check([few], 1.0e-3)
+    assert ops.grad_norm([few * 0]).item() == 0.0
+
+
 @pytest.mark.parametrize("device", EACH)
 def test_gradients_of_a_model(device):
     """Parameters without a gradient are left out, and the answer is torch's."""
