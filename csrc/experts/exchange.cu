@@ -196,8 +196,9 @@ template <typename T> __device__ __forceinline__ Token token_of(const RowsArgs& 
     return t;
 }
 
-/** Zeros in those of the rows that stand at this token's places in `to` which nobody uses. */
+/** Zeros in those of the rows that stand at this token's places in `to` which nobody uses, where somebody says how many are used. */
 template <typename T, int N> __device__ __forceinline__ void clear_unused(const RowsArgs& a, T* to, const Token& t) {
+    if (!a.used) return;
     const unsigned used = (unsigned)*a.used;
     if ((t.index + 1) * a.k <= used) return;
     for (unsigned j = 0; j < a.k; j++) {
@@ -386,7 +387,7 @@ extern "C" int dccl_expert_plan(int device, size_t places, int experts, const vo
 extern "C" int dccl_dispatch(int device, int dtype, size_t tokens, int k, size_t width, const void* x, const int* rows, const int* used, void* out, void* stream) {
     const char* who = "dccl_dispatch";
     if (!tokens) return 0;
-    if (!rows_fit(tokens, k, width) || !x || !rows || !used || !out || (dtype != 6 && dtype != 7 && dtype != 9)) return report(who, cudaErrorInvalidValue);
+    if (!rows_fit(tokens, k, width) || !x || !rows || !out || (dtype != 6 && dtype != 7 && dtype != 9)) return report(who, cudaErrorInvalidValue);
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
     RowsArgs a = {};
@@ -448,7 +449,7 @@ extern "C" int dccl_combine_backward(int device, int dtype, size_t tokens, int k
                                      int weights32, void* din, void* dweights, void* stream) {
     const char* who = "dccl_combine_backward";
     if (!tokens || (!din && !dweights)) return 0;
-    if (!rows_fit(tokens, k, width) || !dy || !rows || !used || (dweights && !in) || (dtype != 6 && dtype != 7 && dtype != 9)) return report(who, cudaErrorInvalidValue);
+    if (!rows_fit(tokens, k, width) || !dy || !rows || (dweights && !in) || (dtype != 6 && dtype != 7 && dtype != 9)) return report(who, cudaErrorInvalidValue);
     OnDevice on(device);
     if (on.e != cudaSuccess) return report(who, on.e);
     RowsArgs a = {};

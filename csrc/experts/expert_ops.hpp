@@ -32,13 +32,13 @@ int dccl_route_backward(int device, int dtype, size_t tokens, int experts, const
  *  the number is none of an expert), counts [experts], starts [experts + 1]. */
 int dccl_expert_plan(int device, size_t places, int experts, const void* chosen, int chosen64, int* rows, int* counts, int* starts, void* stream);
 
-/** out[rows[t][j]] = x[t], and zeros in the rows from *used up to tokens * k. */
+/** out[rows[t][j]] = x[t], and zeros in the rows from *used up to tokens * k: each of those before has a place. With a null `used`, rows without a place are left as they are. */
 int dccl_dispatch(int device, int dtype, size_t tokens, int k, size_t width, const void* x, const int* rows, const int* used, void* out, void* stream);
 
 /** y[t] = sum over j of weights[t][j] * in[rows[t][j]], those with a row; weights (null: ones) are fp32, or of dtype. */
 int dccl_combine(int device, int dtype, size_t tokens, int k, size_t width, const void* in, const int* rows, const void* weights, int weights32, void* y, void* stream);
 
-/** Its gradients: din[rows[t][j]] = weights[t][j] * dy[t], zeros in the rows from *used on, and dweights[t][j] = in[rows[t][j]] . dy[t]. Each may be null. */
+/** Its gradients: din[rows[t][j]] = weights[t][j] * dy[t], zeros in the rows from *used on (null: as above), and dweights[t][j] = in[rows[t][j]] . dy[t]. Each may be null. */
 int dccl_combine_backward(int device, int dtype, size_t tokens, int k, size_t width, const void* dy, const void* in, const int* rows, const int* used, const void* weights,
                           int weights32, void* din, void* dweights, void* stream);
 

@@ -160,7 +160,23 @@ bool plan_fits(const Tensor& rows, const Tensor& starts, const Tensor& like) {
 }
 bool width_fits(const Tensor& t) { return t.dim() >= 1 && t.size(-1) >= 1 && t.size(-1) <= DCCL_EXPERTS_MAX_WIDTH; }
 
-const int* used_of(const Tensor& starts) { return ptr<int>(starts) + starts.size(0) - 1; }
+/** Whether each row that a plan uses has a place: said by whoever knows, or because `rows` and `starts` are still the tensors that expert_plan made, as it made them. */
+bool whole_plan(PyObject* made, PyObject* rows, PyObject* starts, bool* whole) {
+    if (made == Py_None) return *whole = false, true;
+    if (!PyTuple_Check(made)) return truth(made, whole);
+    const auto unchanged = [](PyObject* o) {
+        at::TensorImpl* const t = THPVariable_Unpack(o).unsafeGetTensorImpl();
+        return t->is_inference() || t->version_counter().current_version() == 0;
+    };
+    *whole = PyTuple_GET_SIZE(made) == 2 && PyTuple_GET_ITEM(made, 0) == rows && PyTuple_GET_ITEM(made, 1) == starts && unchanged(rows) && unchanged(starts);
+    return true;
+}
+/** How many rows a whole plan uses, each of which has a place. Of another one it is not known which have. */
+const int* used_of(const Tensor& starts, bool whole) { return whole ? ptr<int>(starts) + starts.size(0) - 1 : nullptr; }
+/** What rows are written to that one of the plan's places has: others are zeros. */
+Tensor rows_for(bool whole, at::IntArrayRef sizes, const Tensor& like) {
+    return whole ? fresh(sizes, like.scalar_type(), like) : at::zeros(sizes, at::TensorOptions().dtype(like.scalar_type()).device(like.device()));
+}
 
 Tensor run_combine(const Tensor& in, const Tensor& rows, const Tensor& weights, at::IntArrayRef sizes) {
     const Tensor y = fresh(sizes, in.scalar_type(), in);
@@ -188,12 +204,14 @@ struct DispatchBackward : public Node {
     void release_variables() override { rows.reset_data(); }
 };
 
-/** dispatch(x, rows, starts): x's rows in the order of the experts. */
+/** dispatch(x, rows, starts, whether each row that is used has a place, or what whole_plan tells it by): x's rows in the order of the experts. */
 PyObject* dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(nargs == 3, "dispatch takes three arguments");
+    TORCH_CHECK(nargs == 4, "dispatch takes four arguments");
     Tensor x, rows, starts;
-    if (!tensor_of(args[0], false, &x) || !tensor_of(args[1], false, &rows) || !tensor_of(args[2], false, &starts)) Py_RETURN_NOTIMPLEMENTED;
+    bool whole;
+    if (!tensor_of(args[0], false, &x) || !tensor_of(args[1], false, &rows) || !tensor_of(args[2], false, &starts) || !whole_plan(args[3], args[1], args[2], &whole))
+        Py_RETURN_NOTIMPLEMENTED;
     const int dtype = dtype_of(x);
     if (dtype < 0 || !width_fits(x) || !plan_fits(rows, starts, x) || x.dim() != rows.dim() || x.sizes().slice(0, x.dim() - 1) != rows.sizes().slice(0, x.dim() - 1)) Py_RETURN_NOTIMPLEMENTED;
     if (observed(args, nargs)) Py_RETURN_NONE;
@@ -203,9 +221,9 @@ PyObject* dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         pybind11::gil_scoped_release no_gil;
         x = dense(x), rows = dense(rows), starts = dense(starts);
         const int64_t width = x.size(-1), k = rows.size(-1), tokens = rows.numel() / k;
-        out = fresh({tokens * k, width}, x.scalar_type(), x);
+        out = rows_for(whole, {tokens * k, width}, x);
         if (tokens) {
-            const int rc = entry.dispatch(x.device().index(), dtype, tokens, (int)k, width, ptr(x), ptr<int>(rows), used_of(starts), ptr(out), stream_of(x));
+            const int rc = entry.dispatch(x.device().index(), dtype, tokens, (int)k, width, ptr(x), ptr<int>(rows), used_of(starts, whole), ptr(out), stream_of(x));
             TORCH_CHECK(rc == 0, "dispatch was not launched (see stderr)");
         }
         if (records({&x})) {
@@ -222,15 +240,16 @@ PyObject* dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 struct CombineBackward : public Node {
     SavedVariable in, rows, starts, weights;
+    bool whole = false;
 
     variable_list apply(variable_list&& grads) override {
         const Tensor v = unpacked(in), r = unpacked(rows), s = unpacked(starts), w = unpacked(weights), dy = dense(grads[0]);
         variable_list out(2);
         if (!dy.defined()) return out;
-        const Tensor din = task_should_compute_output(0) ? fresh_like(v) : Tensor(), dw = w.defined() && task_should_compute_output(1) ? fresh_like(w) : Tensor();
+        const Tensor din = task_should_compute_output(0) ? rows_for(whole, v.sizes(), v) : Tensor(), dw = w.defined() && task_should_compute_output(1) ? fresh_like(w) : Tensor();
         const int64_t k = r.size(-1), tokens = r.numel() / k;
         if (tokens && (din.defined() || dw.defined())) {
-            const int rc = entry.combine_backward(v.device().index(), dtype_of(v), tokens, (int)k, v.size(-1), ptr(dy), ptr(v), ptr<int>(r), used_of(s), ptr(w),
+            const int rc = entry.combine_backward(v.device().index(), dtype_of(v), tokens, (int)k, v.size(-1), ptr(dy), ptr(v), ptr<int>(r), used_of(s, whole), ptr(w),
                                                   w.defined() && w.scalar_type() == at::kFloat, ptr(din), ptr(dw), stream_of(v));
             TORCH_CHECK(rc == 0, "combine: the backward pass was not launched (see stderr)");
         }
@@ -243,12 +262,14 @@ struct CombineBackward : public Node {
     }
 };
 
-/** combine(in, rows, starts, weights or None): the weighted sums of each token's rows. */
+/** combine(in, rows, starts, weights or None, whether each row that is used has a place, or likewise): the weighted sums of each token's rows. */
 PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(nargs == 4, "combine takes four arguments");
+    TORCH_CHECK(nargs == 5, "combine takes five arguments");
     Tensor in, rows, starts, weights;
-    if (!tensor_of(args[0], false, &in) || !tensor_of(args[1], false, &rows) || !tensor_of(args[2], false, &starts) || !tensor_of(args[3], true, &weights)) Py_RETURN_NOTIMPLEMENTED;
+    bool whole;
+    if (!tensor_of(args[0], false, &in) || !tensor_of(args[1], false, &rows) || !tensor_of(args[2], false, &starts) || !tensor_of(args[3], true, &weights) || !whole_plan(args[4], args[1], args[2], &whole))
+        Py_RETURN_NOTIMPLEMENTED;
     if (dtype_of(in) < 0 || in.dim() != 2 || !width_fits(in) || !plan_fits(rows, starts, in) || in.size(0) != rows.numel()) Py_RETURN_NOTIMPLEMENTED;
     if (weights.defined() && (weights.sizes() != rows.sizes() || weights.device() != in.device() || (weights.scalar_type() != at::kFloat && weights.scalar_type() != in.scalar_type())))
         Py_RETURN_NOTIMPLEMENTED;
@@ -266,6 +287,7 @@ PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             node->rows = SavedVariable(rows, false);
             node->starts = SavedVariable(starts, false);
             node->weights = SavedVariable(weights, false);
+            node->whole = whole;
             torch::autograd::set_history(y, node);
         }
     }

@@ -65,8 +65,8 @@ def _ext():
 
 _SCHEMAS = {"route": "Tensor logits, int k, bool sigmoid, Tensor? bias, int groups, int top_groups, bool top2, bool renormalize, float scale",
             "expert_plan": "Tensor experts, int num_experts",
-            "dispatch": "Tensor x, Tensor rows, Tensor starts",
-            "combine": "Tensor rows, Tensor places, Tensor starts, Tensor? weights",
+            "dispatch": "Tensor x, Tensor rows, Tensor starts, bool whole",
+            "combine": "Tensor rows, Tensor places, Tensor starts, Tensor? weights, bool whole",
             "expert_linear": "Tensor x, Tensor weight, Tensor starts, int activation"}
 
 
@@ -187,15 +187,31 @@ def route(logits, k, scores="softmax", bias=None, groups=1, top_groups=1, group_
 
 class ExpertPlan:
     """Where the copies of tokens go in the order of the experts: ``rows`` int32 [..., k], the row of each (-1: none), ``counts`` int32 [experts], how many rows each
-    expert has, and ``starts`` int32 [experts + 1], where its rows begin; starts[-1] rows are used."""
-    __slots__ = ("rows", "counts", "starts")
+    expert has, and ``starts`` int32 [experts + 1], where its rows begin; starts[-1] rows are used.
+
+    A plan may also be made of other tensors, or be given others: one from which places over an expert's capacity are dropped has -1 in ``rows`` for them. No two places have the
+    same row, and rows that none has are nobody's, wherever they lie; ``dispatch`` and the gradient of ``combine`` fill all rows of such a plan with zeros first. (The tensors
+    of a plan by ``expert_plan`` are not changed where torch does not count it: in place in inference mode, or through ``.data``.)"""
+    __slots__ = ("rows", "counts", "starts", "_made")
 
     def __init__(self, rows, counts, starts):
-        self.rows, self.counts, self.starts = rows, counts, starts
+        self.rows, self.counts, self.starts, self._made = rows, counts, starts, None
 
     @property
     def num_experts(self):
         return self.counts.shape[0]
+
+    @property
+    def _whole(self):
+        """Whether each of the rows that are used has a place: in what ``expert_plan`` made, as long as nobody changes it."""
+        return (self._made is not None and all(t is m for t, m in zip((self.rows, self.starts), self._made))
+                and all(t.is_inference() or t._version == 0 for t in self._made))
+
+
+def _exchange(name, plan, *args):
+    """As _kernel, with what the host side needs to know of the plan."""
+    out = getattr(_ext(), name)(*args, plan._made)
+    return _registered.call(name, _SCHEMAS[name], _compute, (*args, plan._whole)) if out is None else out
 
 
 def _check_chosen(what, name, t):
@@ -212,7 +228,9 @@ def expert_plan(experts, num_experts):
     if isinstance(experts, torch.Tensor) and experts.is_cuda:
         out = _kernel("expert_plan", experts, num_experts)
         if out is not NotImplemented:
-            return ExpertPlan(*out)
+            plan = ExpertPlan(*out)
+            plan._made = out[::2]
+            return plan
     if not isinstance(experts, torch.Tensor):
         raise TypeError("expert_plan: experts must be a tensor")
     if experts.dtype not in (torch.int32, torch.int64):
@@ -223,7 +241,11 @@ def expert_plan(experts, num_experts):
     _check_chosen("expert_plan", "experts", experts)
     if experts.is_cuda:
         out = _kernel("expert_plan", experts, num_experts)
-        return ExpertPlan(*out) if out is not NotImplemented else _refuse("expert_plan")
+        if out is NotImplemented:
+            _refuse("expert_plan")
+        plan = ExpertPlan(*out)
+        plan._made = out[::2]
+        return plan
     flat = experts.reshape(-1).long()
     there = (flat >= 0) & (flat < num_experts)
     order = torch.where(there, flat, num_experts).argsort(stable=True)
@@ -253,10 +275,10 @@ def _check_width(what, width):
 
 
 def dispatch(x, plan):
-    """x [..., width] copied into the order of the experts: [tokens * k, width]. Rows that nobody has, behind the last expert's, are zeros. The gradient of a token
+    """x [..., width] copied into the order of the experts: [tokens * k, width]. Rows that nobody has, behind the last expert's as a rule, are zeros. The gradient of a token
     is the sum of those of its rows."""
     if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(plan, ExpertPlan):
-        out = _kernel("dispatch", x, plan.rows, plan.starts)
+        out = _exchange("dispatch", plan, x, plan.rows, plan.starts)
         if out is not NotImplemented:
             return out
     _check_activations("dispatch", "x", x, range(1, 65))
@@ -265,7 +287,7 @@ def dispatch(x, plan):
         raise ValueError("dispatch: x has shape %s, and the plan is for tokens [%s]" % (tuple(x.shape), ", ".join(str(s) for s in plan.rows.shape[:-1])))
     _check_width("dispatch", x.shape[-1])
     if x.is_cuda:
-        out = _kernel("dispatch", x, plan.rows, plan.starts)
+        out = _exchange("dispatch", plan, x, plan.rows, plan.starts)
         return out if out is not NotImplemented else _refuse("dispatch")
     flat, k = plan.rows.reshape(-1).long(), plan.rows.shape[-1]
     places = ((flat >= 0) & (flat < flat.numel())).nonzero().squeeze(-1)
@@ -276,7 +298,7 @@ def combine(rows, plan, weights=None):
     """The sum of each token's rows, times `weights` [..., k] (float32, or of the rows' type) where they are given: [..., width] of rows [tokens * k, width]. A place
     without a row adds nothing, whatever its weight, and its weight's gradient is 0; rows that nobody has are not read, and their gradient is 0."""
     if isinstance(rows, torch.Tensor) and rows.is_cuda and isinstance(plan, ExpertPlan):
-        out = _kernel("combine", rows, plan.rows, plan.starts, weights)
+        out = _exchange("combine", plan, rows, plan.rows, plan.starts, weights)
         if out is not NotImplemented:
             return out
     _check_activations("combine", "rows", rows, (2,))
@@ -287,7 +309,7 @@ def combine(rows, plan, weights=None):
     if weights is not None:
         _check_like("combine", "weights", weights, plan.rows.shape, (torch.float32, rows.dtype), rows.device)
     if rows.is_cuda:
-        out = _kernel("combine", rows, plan.rows, plan.starts, weights)
+        out = _exchange("combine", plan, rows, plan.rows, plan.starts, weights)
         return out if out is not NotImplemented else _refuse("combine")
     at = plan.rows.long()
     there = (at >= 0) & (at < at.numel())

@@ -593,6 +593,61 @@ def test_places_of_a_plan_that_is_none_are_not_followed():
     assert ops.combine(out, plan)[:, 3].tolist() == [2, 0, 3]
 
 
+def partial_plans(plan, keep):
+    """Plans of which some places have given up their rows, by each way that there is."""
+    fewer = torch.where(keep, plan.rows, -1)
+    assigned = ops.ExpertPlan(plan.rows, plan.counts, plan.starts)
+    assigned.rows = fewer
+    replaced = ops.expert_plan(torch.where(plan.rows >= 0, 0, -1).int(), 1)
+    replaced.rows, replaced.counts, replaced.starts = fewer, plan.counts, plan.starts
+    changed = ops.expert_plan(torch.where(plan.rows >= 0, 0, -1).int(), 1)
+    changed.rows.copy_(fewer)
+    changed.starts = plan.starts
+    return {"made": ops.ExpertPlan(fewer, plan.counts, plan.starts), "assigned": assigned, "replaced": replaced, "changed": changed}
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("width", [64, 66, 1451])
+def test_rows_that_no_place_of_a_plan_has(device, dtype, width):
+    """Tokens over an expert's capacity are dropped from a plan, which leaves rows among the others' that nobody has: zeros, and so are their gradients."""
+    g = torch.Generator().manual_seed(1)
+    tokens, k = 37, 3
+    plan = ops.expert_plan(chosen_case(tokens, k, 5, device=device), 5)
+    keep = (torch.rand(tokens, k, generator=g) < 0.6).to(device)
+    x, dy = (torch.randn(tokens, width, generator=g).to(dtype).to(device) for _ in range(2))
+    rows = torch.randn(tokens * k, width, generator=g).to(dtype).to(device).requires_grad_(True)
+    w = torch.rand(tokens, k, generator=g).to(device)
+    for how, fewer in partial_plans(plan, keep).items():
+        kept = fewer.rows[fewer.rows >= 0].long()
+        nobody = torch.ones(tokens * k, dtype=torch.bool, device=device)
+        nobody[kept] = False
+        soil(rows)
+        out = ops.dispatch(x, fewer)
+        assert torch.equal(out[kept], x[(fewer.rows >= 0).nonzero()[:, 0]]) and bool((out[nobody] == 0).all()), how
+        y = ops.combine(rows, fewer, w)
+        soil(rows)
+        grad, = torch.autograd.grad(y, rows, dy)
+        want = (w[fewer.rows >= 0].unsqueeze(-1) * dy[(fewer.rows >= 0).nonzero()[:, 0]].float()).to(dtype)
+        assert torch.equal(grad[kept], want) and bool((grad[nobody] == 0).all()), how
+
+
+@gpu
+def test_rows_that_nobody_has_while_a_mode_looks_on():
+    plan = ops.expert_plan(chosen_case(20, 2, 5, device="cuda"), 5)
+    fewer = ops.ExpertPlan(torch.where(torch.arange(40, device="cuda").view(20, 2) % 3 == 0, -1, plan.rows), plan.counts, plan.starts)
+    x = torch.randn(20, 64, device="cuda")
+    rows = torch.randn(40, 64, device="cuda", requires_grad=True)
+    nobody = torch.ones(40, dtype=torch.bool, device="cuda")
+    nobody[fewer.rows[fewer.rows >= 0].long()] = False
+    soil(rows)
+    with SeesDispatch():
+        out = ops.dispatch(x, fewer)
+        soil(rows)
+        ops.combine(rows, fewer).sum().backward()
+    assert bool((out[nobody] == 0).all()) and bool((rows.grad[nobody] == 0).all()) and bool((rows.grad[~nobody] == 1).all())
+
+
 @pytest.mark.parametrize("device", EACH)
 def test_exchange_refusals(device):
     plan = ops.expert_plan(torch.zeros(4, 2, dtype=torch.int32, device=device), 3)
