@@ -194,8 +194,8 @@ class ExpertPlan:
     of a plan by ``expert_plan`` are not changed where torch does not count it: in place in inference mode, or through ``.data``.)"""
     __slots__ = ("rows", "counts", "starts", "_made")
 
-    def __init__(self, rows, counts, starts):
-        self.rows, self.counts, self.starts, self._made = rows, counts, starts, None
+    def __init__(self, rows, counts, starts, _made=None):
+        self.rows, self.counts, self.starts, self._made = rows, counts, starts, _made
 
     @property
     def num_experts(self):
@@ -209,7 +209,7 @@ class ExpertPlan:
 
 
 def _exchange(name, plan, *args):
-    """As _kernel, with what the host side needs to know of the plan."""
+    """_kernel with the plan's rows and starts, and what the host side tells by whether it is whole."""
     out = getattr(_ext(), name)(*args, plan._made)
     return _registered.call(name, _SCHEMAS[name], _compute, (*args, plan._whole)) if out is None else out
 
@@ -228,9 +228,7 @@ def expert_plan(experts, num_experts):
     if isinstance(experts, torch.Tensor) and experts.is_cuda:
         out = _kernel("expert_plan", experts, num_experts)
         if out is not NotImplemented:
-            plan = ExpertPlan(*out)
-            plan._made = out[::2]
-            return plan
+            return ExpertPlan(*out, out[::2])
     if not isinstance(experts, torch.Tensor):
         raise TypeError("expert_plan: experts must be a tensor")
     if experts.dtype not in (torch.int32, torch.int64):
@@ -241,11 +239,7 @@ def expert_plan(experts, num_experts):
     _check_chosen("expert_plan", "experts", experts)
     if experts.is_cuda:
         out = _kernel("expert_plan", experts, num_experts)
-        if out is NotImplemented:
-            _refuse("expert_plan")
-        plan = ExpertPlan(*out)
-        plan._made = out[::2]
-        return plan
+        return ExpertPlan(*out, out[::2]) if out is not NotImplemented else _refuse("expert_plan")
     flat = experts.reshape(-1).long()
     there = (flat >= 0) & (flat < num_experts)
     order = torch.where(there, flat, num_experts).argsort(stable=True)
@@ -278,8 +272,8 @@ def dispatch(x, plan):
     """x [..., width] copied into the order of the experts: [tokens * k, width]. Rows that nobody has, behind the last expert's as a rule, are zeros. The gradient of a token
     is the sum of those of its rows."""
     if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(plan, ExpertPlan):
-        out = _exchange("dispatch", plan, x, plan.rows, plan.starts)
-        if out is not NotImplemented:
+        out = _ext().dispatch(x, plan.rows, plan.starts, plan._made)
+        if out is not None and out is not NotImplemented:
             return out
     _check_activations("dispatch", "x", x, range(1, 65))
     _check_plan("dispatch", plan, x.device)
@@ -298,8 +292,8 @@ def combine(rows, plan, weights=None):
     """The sum of each token's rows, times `weights` [..., k] (float32, or of the rows' type) where they are given: [..., width] of rows [tokens * k, width]. A place
     without a row adds nothing, whatever its weight, and its weight's gradient is 0; rows that nobody has are not read, and their gradient is 0."""
     if isinstance(rows, torch.Tensor) and rows.is_cuda and isinstance(plan, ExpertPlan):
-        out = _exchange("combine", plan, rows, plan.rows, plan.starts, weights)
-        if out is not NotImplemented:
+        out = _ext().combine(rows, plan.rows, plan.starts, weights, plan._made)
+        if out is not None and out is not NotImplemented:
             return out
     _check_activations("combine", "rows", rows, (2,))
     _check_plan("combine", plan, rows.device)
