@@ -126,5 +126,5 @@ def _take_either_form(module, state, prefix, *_):
         one, each = prefix + name, ["%s%s.%d" % (prefix, name, j) for j in range(module.per)]
         if module.fused and each[0] in state and all(k in state for k in each):
             state[one] = torch.stack([state.pop(k) for k in each])
-        elif not module.fused and one in state:
+        elif not module.fused and one in state and len(state[one]) == module.per:       # of other numbers it stays, and is not expected
             state.update(zip(each, state.pop(one)))

@@ -1419,6 +1419,24 @@ def test_the_plain_layer_takes_no_options_of_the_fused_one(dccl_lib):
         comm.finalize()
 
 
+def test_a_layer_loads_no_part_of_other_experts(dccl_lib):
+    """The weights of more experts than the layer has, or fewer, in one tensor or in a list, are refused in either form."""
+    from dccl_b200 import Communicator
+    from dccl_b200.parallel.expert_parallel import ExpertParallelMLP
+    comm = Communicator(rank=0, world=1)
+    try:
+        for other in (2, 6):
+            for had in (True, False):
+                state = ExpertParallelMLP(8, 12, other, comm, seed=1, fused=had).state_dict()
+                for fused in (True, False):
+                    layer = ExpertParallelMLP(8, 12, 4, comm, fused=fused)
+                    state["router"] = layer.router.detach().clone()
+                    with pytest.raises(RuntimeError):
+                        layer.load_state_dict(state)
+    finally:
+        comm.finalize()
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
 def test_the_fused_layer_on_the_gpu(dccl_lib, dtype):
