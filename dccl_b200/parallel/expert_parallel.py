@@ -16,7 +16,7 @@ takes it, tokens put in the experts' order and added up by kernels, and one prod
                             routing=dict(scores="sigmoid", renormalize=True, scale=2.5))
 
 Its experts' weights are one parameter each for all experts of the rank (``w_in`` [experts, h, d], ``w_out`` [experts, d, h]); a state dict of either form loads
-into the other. One rank alone never reads anything back to the host, and can be captured into a graph. (In float32 on the GPU, without autocast, the experts' products are
+into the other. A bias among the keywords of ``routing`` goes with the layer to its device, where it stays fp32, and into its state dict. One rank alone never reads anything back to the host, and can be captured into a graph. (In float32 on the GPU, without autocast, the experts' products are
 the plain layer's, and how many rows each has is read.)
 
 The router is replicated; its gradient on a rank covers that rank's tokens only and is summed with the other
@@ -62,6 +62,20 @@ class ExpertParallelMLP(torch.nn.Module):
             self.w_in = torch.nn.ParameterList([torch.nn.Parameter(w[0]) for w in ws])
             self.w_out = torch.nn.ParameterList([torch.nn.Parameter(w[1]) for w in ws])
         self.register_load_state_dict_pre_hook(_take_either_form)
+
+    def _apply(self, fn, *args, **kw):
+        super()._apply(fn, *args, **kw)
+        bias = self.routing.get("bias")
+        if bias is not None:            # as a buffer would, but for its type, which is not the layer's
+            moved = fn(bias)
+            self.routing["bias"] = moved if moved.dtype is bias.dtype else bias.to(moved.device)
+        return self
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        bias = self.routing.get("bias")
+        if bias is not None:
+            destination[prefix + "routing_bias"] = bias if keep_vars else bias.detach()
 
     def forward(self, x):
         if self.fused:
@@ -120,8 +134,18 @@ class ExpertParallelMLP(torch.nn.Module):
         return ops.expert_linear(ops.expert_linear(rows, w_in, plan, activation="gelu"), w_out, plan)
 
 
-def _take_either_form(module, state, prefix, *_):
-    """Experts' weights in a list or in one tensor, as the module has them."""
+def _take_either_form(module, state, prefix, _metadata, _strict, _missing, _unexpected, errors):
+    """Experts' weights in a list or in one tensor, as the module has them, and the bias of its routing."""
+    bias, key = module.routing.get("bias"), prefix + "routing_bias"
+    if key in state and bias is not None:
+        value = state.pop(key)
+        if value.shape == bias.shape:
+            with torch.no_grad():
+                bias.copy_(value)
+        else:
+            errors.append("size mismatch for %s: %s, and the layer has %s" % (key, tuple(value.shape), tuple(bias.shape)))
+    elif not module.fused:
+        state.pop(key, None)
     for name in ("w_in", "w_out"):
         one, each = prefix + name, ["%s%s.%d" % (prefix, name, j) for j in range(module.per)]
         if module.fused and each[0] in state and all(k in state for k in each):

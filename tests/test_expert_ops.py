@@ -1419,6 +1419,46 @@ def test_the_plain_layer_takes_no_options_of_the_fused_one(dccl_lib):
         comm.finalize()
 
 
+@pytest.mark.parametrize("device", EACH)
+def test_the_routing_bias_goes_with_the_layer(dccl_lib, device):
+    """To other devices, where it stays fp32, and into state dicts: it holds how the load has been balanced."""
+    import copy
+    from dccl_b200 import Communicator
+    from dccl_b200.parallel.expert_parallel import ExpertParallelMLP
+    comm = Communicator(rank=0, world=1, **({"device": 0} if device == "cuda" else {}))
+    try:
+        def layer(bias, **kw):
+            return ExpertParallelMLP(16, 24, 4, comm, fused=True, top_k=2, routing=dict(scores="sigmoid", **({} if bias is None else {"bias": bias})), **kw)
+
+        bias = torch.tensor([0.5, -0.25, 3.0, 0.0])
+        a, b = layer(bias.clone()), layer(torch.zeros(4))
+        mine = a.routing["bias"]
+        assert a.to("cpu").routing["bias"] is mine and a.double().float().routing["bias"] is mine       # whoever balances the load may keep it
+        type_ = torch.bfloat16 if device == "cuda" else torch.float32
+        a, b = a.to(device).to(type_), b.to(device).to(type_)
+        assert a.routing["bias"].dtype is torch.float32 and a.routing["bias"].device.type == device and torch.equal(a.routing["bias"].cpu(), bias)
+        state = copy.deepcopy(a.state_dict())
+        assert torch.equal(state["routing_bias"].cpu(), bias)
+        held = b.routing["bias"]
+        b.load_state_dict(state)
+        assert b.routing["bias"] is held and torch.equal(held.cpu(), bias)
+        x = torch.randn(9, 16, generator=torch.Generator().manual_seed(0)).to(device).to(type_)
+        assert torch.equal(a(x), b(x))
+        held.add_(1.0)
+        del state["routing_bias"]           # of a layer that had none
+        b.load_state_dict(state)
+        assert torch.equal(held.cpu(), bias + 1.0)
+        ExpertParallelMLP(16, 24, 4, comm).load_state_dict(a.state_dict())          # the plain layer has no use for it
+        with pytest.raises(RuntimeError):
+            layer(None).load_state_dict(a.state_dict())
+        state = a.state_dict()
+        state["routing_bias"] = torch.zeros(5)
+        with pytest.raises(RuntimeError, match="routing_bias"):
+            b.load_state_dict(state)
+    finally:
+        comm.finalize()
+
+
 def test_a_layer_loads_no_part_of_other_experts(dccl_lib):
     """The weights of more experts than the layer has, or fewer, in one tensor or in a list, are refused in either form."""
     from dccl_b200 import Communicator
