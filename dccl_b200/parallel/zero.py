@@ -19,6 +19,7 @@ symmetric memory (``symmetric=True``), so that both collectives run zero-copy th
 ``close()`` before the communicator is finalized to give that memory back.
 """
 import ctypes
+import inspect
 import math
 import os
 import warnings
@@ -132,12 +133,22 @@ def _a_mode_is_active():
     return n > 0 and any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))
 
 
+def _takes(function, name):
+    try:
+        return name in inspect.signature(function).parameters
+    except ValueError:          # of a builtin
+        return False
+
+
 class ShardedOptimizer:
     """optimizer_cls(params, **kwargs) is built over ONE tensor per dtype: this rank's fp32 master slice. With `max_norm` a step first cuts the averaged
-    gradients back to that norm, over all parameters and ranks, and leaves the norm before in ``grad_norm`` (a float32 tensor on their device, which the host need not read)."""
+    gradients back to that norm, over all parameters and ranks, and leaves the norm before in ``grad_norm`` (a float32 tensor on their device, which the host need not read). An
+    optimizer that takes a `max_norm` of its own gets it, and clips what it has: this rank's slice."""
 
     def __init__(self, params, comm, optimizer_cls=torch.optim.AdamW, symmetric=True, *, max_norm=None, **kwargs):
         self.comm = comm
+        if max_norm is not None and _takes(optimizer_cls, "max_norm"):
+            kwargs["max_norm"], max_norm = max_norm, None
         self.max_norm, self.grad_norm = max_norm, None
         self._sym = []
         params = [p for p in params if p.requires_grad]

@@ -380,6 +380,36 @@ def test_limits_of_the_sharded_optimizer(dccl_lib):
         comm.finalize()
 
 
+def test_an_optimizer_keeps_a_max_norm_of_its_own(dccl_lib):
+    """One that takes the keyword gets it, as it did before there was one of the sharded optimizer."""
+    from dccl_b200 import Communicator
+    from dccl_b200.parallel.zero import ShardedOptimizer
+    seen = []
+
+    class Clips(torch.optim.SGD):
+        def __init__(self, params, lr=0.1, max_norm=7.0):
+            super().__init__(params, lr=lr)
+            seen.append(max_norm)
+
+    comm = Communicator(rank=0, world=1)
+    try:
+        def step(*args, **kw):
+            p = torch.nn.Parameter(torch.zeros(3))
+            opt = ShardedOptimizer([p], comm, *args, **kw)
+            p.grad.fill_(4.0)
+            opt.step()
+            return p.detach(), opt.grad_norm
+
+        p, norm = step(Clips, max_norm=0.5)
+        assert seen == [0.5] and norm is None and torch.allclose(p, torch.full((3,), -0.4))
+        p, norm = step(Clips, lr=1.0)
+        assert seen == [0.5, 7.0] and norm is None
+        p, norm = step(torch.optim.SGD, lr=1.0, max_norm=0.5)
+        assert abs(norm.item() - 48 ** 0.5) < 1e-5 and torch.allclose(p, torch.full((3,), -0.5 / 3 ** 0.5), atol=1e-5)
+    finally:
+        comm.finalize()
+
+
 @pytest.mark.parametrize("world", [1, 3])
 def test_norms_over_ranks(dccl_lib, world):
     """Gradients of which every rank has its own: grad_norm and clip_grad_norm with a communicator, the sharded optimizer's max_norm and the reducer's clip, against all of
