@@ -23,7 +23,6 @@ The router is replicated; its gradient on a rank covers that rank's tokens only 
 replicated parameters (``tensor_parallel.sync_replicated_grads``) when the ranks hold different tokens.
 """
 import math
-import types
 
 import torch
 
@@ -45,8 +44,6 @@ def router_weight(d_model, num_experts, seed, dtype=torch.float32, device="cpu")
 
 
 class ExpertParallelMLP(torch.nn.Module):
-    fused, routing = False, types.MappingProxyType({})        # of modules that were pickled before they had them
-
     def __init__(self, d_model, d_hidden, num_experts, comm, seed=0, dtype=torch.float32, device="cpu", fused=False, top_k=1, routing=None):
         """routing: keyword arguments of ``ops.route``; without it the weights are the softmax's, as they are without `fused`."""
         super().__init__()

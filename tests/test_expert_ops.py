@@ -1459,23 +1459,6 @@ def test_the_routing_bias_goes_with_the_layer(dccl_lib, device):
         comm.finalize()
 
 
-def test_layers_from_before_there_was_a_fused_form(dccl_lib):
-    """A module that was pickled then has none of the attributes."""
-    from dccl_b200 import Communicator
-    from dccl_b200.parallel.expert_parallel import ExpertParallelMLP
-    comm = Communicator(rank=0, world=1)
-    try:
-        layer = ExpertParallelMLP(8, 12, 4, comm)
-        x = torch.randn(5, 8, generator=torch.Generator().manual_seed(0))
-        want, state = layer(x), layer.state_dict()
-        for name in ("fused", "top_k", "routing"):
-            del layer.__dict__[name]
-        layer.load_state_dict(state)
-        assert torch.equal(layer.to("cpu")(x), want) and set(layer.state_dict()) == set(state)
-    finally:
-        comm.finalize()
-
-
 def test_a_layer_loads_no_part_of_other_experts(dccl_lib):
     """The weights of more experts than the layer has, or fewer, in one tensor or in a list, are refused in either form."""
     from dccl_b200 import Communicator
