@@ -175,7 +175,9 @@ bool whole_plan(PyObject* made, PyObject* rows, PyObject* starts, bool* whole) {
 const int* used_of(const Tensor& starts, bool whole) { return whole ? ptr<int>(starts) + starts.size(0) - 1 : nullptr; }
 /** What rows are written to that one of the plan's places has: others are zeros. */
 Tensor rows_for(bool whole, at::IntArrayRef sizes, const Tensor& like) {
-    return whole ? fresh(sizes, like.scalar_type(), like) : at::zeros(sizes, at::TensorOptions().dtype(like.scalar_type()).device(like.device()));
+    const Tensor t = fresh(sizes, like.scalar_type(), like);
+    if (!whole) t.zero_();
+    return t;
 }
 
 Tensor run_combine(const Tensor& in, const Tensor& rows, const Tensor& weights, at::IntArrayRef sizes) {

@@ -63,9 +63,14 @@ class ExpertParallelMLP(torch.nn.Module):
             self.w_out = torch.nn.ParameterList([torch.nn.Parameter(w[1]) for w in ws])
         self.register_load_state_dict_pre_hook(_take_either_form)
 
+    @property
+    def routing_bias(self):
+        """The bias among the keywords of ``routing``, by the name that it has in a state dict."""
+        return self.routing.get("bias")
+
     def _apply(self, fn, *args, **kw):
         super()._apply(fn, *args, **kw)
-        bias = self.routing.get("bias")
+        bias = self.routing_bias
         if bias is not None:            # as a buffer would, but for its type, which is not the layer's
             moved = fn(bias)
             self.routing["bias"] = moved if moved.dtype is bias.dtype else bias.to(moved.device)
@@ -73,7 +78,7 @@ class ExpertParallelMLP(torch.nn.Module):
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)
-        bias = self.routing.get("bias")
+        bias = self.routing_bias
         if bias is not None:
             destination[prefix + "routing_bias"] = bias if keep_vars else bias.detach()
 
@@ -136,7 +141,7 @@ class ExpertParallelMLP(torch.nn.Module):
 
 def _take_either_form(module, state, prefix, _metadata, _strict, _missing, _unexpected, errors):
     """Experts' weights in a list or in one tensor, as the module has them, and the bias of its routing."""
-    bias, key = module.routing.get("bias"), prefix + "routing_bias"
+    bias, key = module.routing_bias, prefix + "routing_bias"
     if key in state and bias is not None:
         value = state.pop(key)
         if value.shape == bias.shape:

@@ -1440,6 +1440,7 @@ def test_the_routing_bias_goes_with_the_layer(dccl_lib, device):
         state = copy.deepcopy(a.state_dict())
         assert torch.equal(state["routing_bias"].cpu(), bias)
         held = b.routing["bias"]
+        assert all(hasattr(b, name) for name in state)
         b.load_state_dict(state)
         assert b.routing["bias"] is held and torch.equal(held.cpu(), bias)
         x = torch.randn(9, 16, generator=torch.Generator().manual_seed(0)).to(device).to(type_)
