@@ -7,7 +7,8 @@
  *
  * All four go token by token: a token's own row is read or written once, and no two add to the same place, so that sums need no atomics and come in the order of
  * j. HBM bounds them: 16384 tokens of 2048 bf16 by four experts, dispatch 51 us (335 MB, 6.5 TB/s), combine 59 (335 MB, 5.7), its gradient 112 (604 MB, 5.4); by one
- * expert 32 us and 51. Rows of an odd width go one element at a time, as nothing wider starts where they do.
+ * expert 32 us and 51. Rows of an odd width go one element at a time: nothing wider starts where they do, and aligned pieces would have to
+ * be shifted by what the starts of two rows differ.
  */
 #include "expert_ops.hpp"
 #include "../kernels/launch_early.cuh"
@@ -58,7 +59,8 @@ __device__ __forceinline__ unsigned lanes_alike(unsigned e, int bits) {
 /**
  * One launch of one CTA, or of a cluster of eight that exchange their counts through shared memory. Every warp has a run of consecutive places, and counts of its
  * own. Two walks over the places: how many there are of each expert, and where they go; among 32 places one lane of each kind counts on. The chain from one 32
- * places to the next bounds it: 48 places 2.8 us, 1024 of 64 experts 5.6, 16384 by the cluster 6.7, 65536 10.4. More SMs would need a second launch, or a barrier over the device, of 3 us.
+ * places to the next bounds it: 48 places 2.8 us, 1024 of 64 experts 5.6, 16384 by the cluster 6.7, 65536 10.4. More SMs would need a second launch, or a barrier over the device,
+ * of 3 us: nothing to be gained up to some 16384 places, and more and more beyond.
  */
 template <bool MANY> __device__ __forceinline__ void plan(const PlanArgs& a) {
     extern __shared__ unsigned counted[];           // [warps][experts], then [experts] of the CTA, then [32]

@@ -24,7 +24,7 @@ constexpr int kNoActivation = -1;
  * The normal distribution's cdf(z) and e^(-z^2 / 2), which its density needs as well. erfc(x) = t (c1 + ... + c7 t^6) e^(-x^2) with t = 1 / (1 + p x), the form of
  * Abramowitz and Stegun, "Handbook of Mathematical Functions", 7.1.26, with one more term pair and coefficients fitted on [0, 8] for an error that stays small against
  * erfc itself: 2e-8 near 0, 3e-6 of erfc at 4; in fp32 the cdf is off by 1.5e-7 at most. With erff the epilogue of a tile took longer than its
- * products, and k_act_grad, bound by its arithmetic, 177 us for 16384 x 5632 bf16 instead of 124.
+ * products, and k_act_grad, bound by its arithmetic, 177 us for 16384 x 5632 bf16 instead of 124 (each alone; see there).
  */
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     constexpr float root = 0.70710678118654752f;
@@ -153,7 +153,7 @@ template <int LINES> __device__ __forceinline__ void clear_rows(char* at, unsign
  * The loader must never pause: it finds its place in a tile from shared memory and without divisions, and as a load takes it some 60 clocks to give out, one box holds all
  * blocks of an operand where rows allow (dW of single CTAs 333 us with a box per block of 64 columns, 286 with one).
  * Tiles of 128 x 128 and 128 x 256 serve where the larger would leave SMs without work; tiles of 32 x 64, two CTAs of an SM, where experts have few rows and reading the weights
- * takes the time (16 rows of those experts: 41 us, 4.4 TB/s); there, what one thread takes to give products out counts: 60 us with descriptors made anew for each, 44 with
+ * takes the time (two rows of each of those experts: 41 us, 4.5 TB/s; four of each of four: 25); there, what one thread takes to give products out counts: 60 us with descriptors made anew for each, 44 with
  * their low words counted up.
  */
 template <typename T, int FORM, int M, int N> __device__ __forceinline__ void grouped(const GroupedArgs& a) {
@@ -481,7 +481,8 @@ __global__ void __launch_bounds__(kRowCta) k_pad_rows(const __grid_constant__ Pa
 struct ActGradArgs { const void* dh; const float* z; void* dz; const int* starts; size_t z_stride, stride; unsigned rows, experts, n, from, threads; Divisor runs; int act; };
 
 /** dz from dh and the saved products, eight elements per thread; rows behind the last expert's, whose products nobody wrote, are left out. Only the rows of dh may start
- *  anywhere (VEC: they do not). HBM bounds it: 8 bytes per element, 16384 x 5632 in 125 us (5.9 TB/s). */
+ *  anywhere (VEC: they do not). HBM bounds it: 8 bytes per element, 16384 x 5632 in 125 us alone (5.9 TB/s), in 142 between
+ *  the products of a step, which take the clock down. */
 template <typename T, bool VEC> __global__ void __launch_bounds__(kRowCta) k_act_grad(const __grid_constant__ ActGradArgs a) {
     wait_for_stream();
     __shared__ unsigned reach[kRowCta / 32];
