@@ -197,6 +197,11 @@ class ExpertPlan:
     def __init__(self, rows, counts, starts, _made=None):
         self.rows, self.counts, self.starts, self._made = rows, counts, starts, _made
 
+    def __setstate__(self, state):          # of a copy, of which it is not known who changes its tensors; or of a plan from before there was _made
+        for name in ("rows", "counts", "starts"):
+            setattr(self, name, state[1][name])
+        self._made = None
+
     @property
     def num_experts(self):
         return self.counts.shape[0]

@@ -632,6 +632,22 @@ def test_rows_that_no_place_of_a_plan_has(device, dtype, width):
         assert torch.equal(grad[kept], want) and bool((grad[nobody] == 0).all()), how
 
 
+@pytest.mark.parametrize("device", EACH)
+def test_plans_can_be_copied(device):
+    """Pickled, copied, and as they were pickled when they had three tensors and nothing else."""
+    import copy
+    import pickle
+    plan = ops.expert_plan(chosen_case(9, 2, 4, device=device), 4)
+    old = ops.ExpertPlan.__new__(ops.ExpertPlan)
+    old.__setstate__((None, {"rows": plan.rows, "counts": plan.counts, "starts": plan.starts}))
+    x = torch.randn(9, 16, generator=torch.Generator().manual_seed(2)).to(device)
+    want = ops.dispatch(x, plan)
+    for other in (pickle.loads(pickle.dumps(plan)), copy.copy(plan), copy.deepcopy(plan), old):
+        assert torch.equal(ops.dispatch(x, other), want) and torch.equal(ops.combine(want, other), ops.combine(want, plan)) and other.num_experts == 4
+        other.rows = torch.where(other.rows == 0, -1, other.rows)
+        assert bool((ops.dispatch(x, other)[0] == 0).all()) and torch.equal(ops.dispatch(x, other)[1:], want[1:])
+
+
 @gpu
 def test_rows_that_nobody_has_while_a_mode_looks_on():
     plan = ops.expert_plan(chosen_case(20, 2, 5, device="cuda"), 5)
