@@ -78,8 +78,10 @@ template <typename T> __device__ __noinline__ double squares_exactly(const T* bo
 
 /**
  * Squares of one access are added in fp32, and those sums in 64 bits. A square that overflowed shows in the thread's sum for the piece; what got lost below the normal numbers, 2^-150 of
- * each square, may count where that sum is small without being of zeros alone, as many gradients are. Then the thread adds all of its squares of the piece again, in 64 bits.
- * (1.1 billion bf16 gradients take 335 us; where each access was looked at 340, where it was decided there 404, and without any of it 330.) Those of fp16 always fit.
+ * each of at most 64 squares, may count where that sum is below 2^-110 (the 2^34th of it no longer does) without being of zeros alone, as many gradients are. Then the thread adds
+ * all of its squares of the piece again, in 64 bits.
+ * (1.1 billion bf16 gradients take 335 us; where each access was looked at 340, where it was decided there 404, and without any of it 330. Half as many, all of them to be added
+ * again, 258 instead of 169.) Those of fp16 always fit.
  */
 template <typename T> __device__ __forceinline__ double squares(const T* p, size_t n) {
     constexpr int N = 16 / sizeof(T);
@@ -113,7 +115,7 @@ template <typename T> __device__ __forceinline__ double squares(const T* p, size
     some(std::integral_constant<int, 1>{});
     if constexpr (kMayNotFit) {
         constexpr uint32_t sizes = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;         // without the signs
-        if (!(sum < INFINITY) || (sum < 0x1p-80 && (bits & sizes))) sum = squares_exactly(body, runs);
+        if (!(sum < INFINITY) || (sum < 0x1p-110 && (bits & sizes))) sum = squares_exactly(body, runs);
     }
     if (threadIdx.x < head) {
         const float v = Traits<T>::up(p[threadIdx.x]);
