@@ -1207,6 +1207,56 @@ print("OK")
 
 
 @gpu
+@pytest.mark.parametrize("experts", [8, 200])
+def test_dropped_places_and_some_of_the_experts_in_graphs(experts):
+    """Places over a capacity dropped from the plan, the products of some experts, and a table that goes back: captured forward and backward, replayed on other tokens, and on
+    two streams at once."""
+    tokens, width, out, capacity = 300, 64, 72, 2 * 600 // experts
+    g = torch.Generator().manual_seed(experts)
+    w = (torch.randn(experts, out, width, generator=g) / 8).bfloat16().cuda().requires_grad_(True)
+    dy, dh = (torch.randn(n, out, generator=g).bfloat16().cuda() for n in (tokens, 2 * tokens))
+    back = torch.tensor([0, 400, 100] + [100 + 2 * e for e in range(experts - 2)], dtype=torch.int32, device="cuda")
+
+    def step(x, chosen, weights):
+        plan = ops.expert_plan(chosen, experts)
+        place = plan.rows - plan.starts[chosen.long()]
+        fewer = ops.ExpertPlan(torch.where(place < capacity, plan.rows, -1), plan.counts, plan.starts)
+        leaf = x.detach().requires_grad_(True)
+        rows = ops.dispatch(leaf, fewer)
+        h = ops.expert_linear(rows, w, plan, activation="silu")
+        y = ops.combine(h, fewer, weights)
+        part = ops.expert_linear(rows, w[2:5], plan.starts[2:6])
+        odd = ops.expert_linear(rows, w, back, activation="gelu")
+        return [t.detach() for t in (rows, h, y, part, odd)] + list(torch.autograd.grad((y, part, odd), (leaf, w), (dy, dh, dh)))
+
+    cases = [(torch.randn(tokens, width, generator=g).bfloat16().cuda(), torch.randint(0, experts, (tokens, 2), generator=g).int().cuda(), torch.rand(tokens, 2, generator=g).cuda())
+             for _ in range(3)]
+    wants = []
+    for c in cases:
+        soil(cases[0][0], dh, w)
+        wants.append(step(*c))
+    assert all(bool(t.isfinite().all()) for want in wants for t in want)
+    still, stream, graph = [t.clone() for t in cases[0]], torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step(*still)
+    for c, want in zip(cases, wants):
+        for t, v in zip(still, c):
+            t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    streams, both = [stream, torch.cuda.Stream()], [None, None]
+    for _ in range(3):
+        for i, side in enumerate(streams):
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                both[i] = step(*cases[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(2) for a, b in zip(both[i], wants[i]))
+
+
+@gpu
 def test_the_first_call_of_a_process_can_be_captured():
     res = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and res.stdout.strip().endswith("OK"), res.stdout + res.stderr[-2000:]
